@@ -15,7 +15,10 @@ OBJ = os.path.join(HERE, 'build')
 LIB = os.path.join(HERE, 'libn3d.so')
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
 ARCH = 'gfx950'
-CFLAGS = ['-O3', '-std=c++17', '-fPIC', f'--offload-arch={ARCH}', '-Wall', '-Wno-unused-function', '-Wno-unused-variable']
+CFLAGS = ['-O3', '-std=c++17', '-fPIC', f'--offload-arch={ARCH}', '-Wall', '-Wno-unused-function', '-Wno-unused-variable',
+          # no packed float32 instructions (v_pk_add / mul / fma_f32), which the optimiser otherwise forms out of ordinary float code: some of their
+          # forms have given wrong results on this hardware.  (hipcc's host pass does not know the feature and says so: harmless)
+          '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 # raster.hip mirrors the C oracle operation-for-operation: no FMA contraction there (bit-exact face selection)
 PER_FILE = {'raster.hip': ['-ffp-contract=off']}
 
@@ -47,8 +50,9 @@ def build(force=False, verbose=True):
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f'hipcc failed: {" ".join(cmd)}\n{r.stdout}\n{r.stderr}')
-        if verbose and r.stderr.strip():
-            print(r.stderr, file=sys.stderr)
+        said = '\n'.join(line for line in r.stderr.splitlines() if 'packed-fp32-ops' not in line)
+        if verbose and said.strip():
+            print(said, file=sys.stderr)
 
     with ThreadPoolExecutor(max_workers=min(8, max(1, len(jobs)))) as ex:
         list(ex.map(run, jobs))
