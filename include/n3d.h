@@ -23,12 +23,12 @@ extern "C" {
 
 typedef void* n3d_stream_t; /* hipStream_t */
 
-#define N3D_ABI_VERSION 8
+#define N3D_ABI_VERSION 9
 
 /* activation ids = the reference's cuda_idx (torch_utils/ops/bias_act.py:23-33) */
 enum { N3D_ACT_LINEAR = 1, N3D_ACT_RELU = 2, N3D_ACT_LRELU = 3, N3D_ACT_TANH = 4, N3D_ACT_SIGMOID = 5,
        N3D_ACT_ELU = 6, N3D_ACT_SELU = 7, N3D_ACT_SOFTPLUS = 8, N3D_ACT_SWISH = 9 };
-enum { N3D_F32 = 0, N3D_F16 = 1 };
+enum { N3D_F32 = 0, N3D_F16 = 1, N3D_BF16 = 2 /* the token operators only */ };
 /* activation layouts: float32 NCHW; split8 (see n3d_fir4_split8); "c8" = float32 [N][C/8][H][row pitch in pixels][8], one
  * 32-byte unit = 8 consecutive channels of one pixel (what the transposed convolution hands to n3d_fir4_split8) */
 enum { N3D_LAYOUT_NCHW_F32 = 0, N3D_LAYOUT_SPLIT8 = 1, N3D_LAYOUT_C8_F32 = 2,
@@ -44,7 +44,7 @@ enum { N3D_K_BIAS_ACT = 0, N3D_K_UPFIRDN2D = 1, N3D_K_CONV2D = 2, N3D_K_FC = 3, 
        N3D_K_MISC = 6, N3D_K_CONV2D_BF16X3 = 7 /* 3x3 split-bf16 kernels: MFMA-bound */,
        N3D_K_CONV1X1_BF16X3 = 8 /* 1x1 split-bf16 kernels (and the float16 toRGB): HBM-bound */,
        N3D_K_CONV2D_F16 = 9 /* 3x3 float16 kernels of the fp16 blocks (n3d_conv2d_f16): MFMA / HBM */,
-       N3D_K_RENDER_RAYS = 10 /* n3d_render_rays(_ex): depth-bounds pre-pass + render_rays_kernel (texel gathers through L1 / L2 + the decoder) */, N3D_K_COUNT = 11 };
+       N3D_K_RENDER_RAYS = 10 /* n3d_render_rays(_ex): depth-bounds pre-pass + render_rays_kernel (texel gathers through L1 / L2 + the decoder) */, N3D_K_LAYER_NORM = 11, N3D_K_ROTARY = 12, N3D_K_ATTENTION = 13, N3D_K_COUNT = 14 };
 int n3d_prof_enable(int on);
 int n3d_prof_reset(void);
 int n3d_prof_read(int family, double* total_ms, int64_t* launches, double* flops, double* bytes);
@@ -486,6 +486,36 @@ int n3d_resize_aa(const float* src, float* dst, const int* src_box, const int* d
  * super-resolution module, tat/triplane_next3d.py:179-181 — is resized without a copy. */
 int n3d_resize_aa_strided(const float* src, int64_t src_batch_stride, float* dst, const int* src_box, const int* dst_box, int N, int C, int SH, int SW,
                           int DH, int DW, int dst_square, n3d_stream_t stream);
+
+/* ---- token operators: layer norm, rotary positions and attention over rows of channels (w vectors, tri-plane texels, frames of a video).  They have
+ *      no counterpart in the reference.  dtype: N3D_F32 / N3D_F16 / N3D_BF16 as stated; element strides; every scratch buffer is the caller's. */
+
+/* y = (x - mean) / sqrt(var + eps) * w + b over the last dimension: x [rows, C] with row stride x_stride (elements; channels dense) -> y [rows, C] dense.
+ * w / b [C] or NULL, of w_dtype (N3D_F32 or dtype).  mean / rstd [rows] float32 for the gradient, both or neither NULL.  float32 statistics. */
+int n3d_layer_norm(const void* x, const void* w, const void* b, void* y, float* mean, float* rstd, int64_t rows, int C, int64_t x_stride, int dtype,
+                   int w_dtype, float eps, n3d_stream_t stream);
+/* Gradients of n3d_layer_norm: dx [rows, C] dense (type dtype), dw / db [C] (type w_dtype); each may be NULL.  rows > 0.
+ * workspace: n3d_layer_norm_bwd_workspace(rows, C, dtype) floats, needed when dw or db is asked for.  Sums in a fixed order: bitwise reproducible. */
+int64_t n3d_layer_norm_bwd_workspace(int64_t rows, int C, int dtype);
+int n3d_layer_norm_bwd(const void* dy, const void* x, const void* w, const float* mean, const float* rstd, void* dx, void* dw, void* db, float* workspace,
+                       int64_t rows, int C, int64_t x_stride, int64_t dy_stride, int dtype, int w_dtype, n3d_stream_t stream);
+
+/* Rotary positions with 1..4 axes.  Pairs of channels turn by position * base^-e: axis a owns sections[a] / 2 pairs, in order; the remaining
+ * D - sum(sections) channels pass through.  e = 2 i / sections[a] for pair i of axis a, or (shared_ladder) p / P for pair p of all P.  A pair is
+ * (2p, 2p + 1) when interleaved, else channels i and i + half — the halves of the axis's section, or of all rotated channels with shared_ladder.
+ * inverse: turn back (the gradient).  q [B, L, heads_q, D] and k [B, L, heads_k, D] (heads_k 0: none) of one dtype with element strides (batch, token,
+ * head) and dense channels -> out_q / out_k, dense.  positions: pos_type 0 float32, 1 int32, 2 int64; element (b, l, a) at
+ * b * pos_batch_stride + l * pos_token_stride + a.  Angles in 64 bits. */
+typedef struct {
+    const void *q, *k, *positions;
+    void *out_q, *out_k;
+    int64_t q_strides[3], k_strides[3];
+    int64_t pos_batch_stride, pos_token_stride;
+    double base;
+    int B, L, heads_q, heads_k, D, axes, sections[4];
+    int dtype, pos_type, interleaved, shared_ladder, inverse;
+} n3d_rotary_desc;
+int n3d_rotary(const n3d_rotary_desc* desc, n3d_stream_t stream);
 
 #ifdef __cplusplus
 }

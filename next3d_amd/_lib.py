@@ -13,13 +13,14 @@ import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get('N3D_LIB') or os.path.join(_HERE, 'libn3d.so')     # N3D_LIB: A/B-compare two builds on one box
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 c_void_p, c_int, c_int64, c_float, c_double = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_double
 
 ACT_IDS = {'linear': 1, 'relu': 2, 'lrelu': 3, 'tanh': 4, 'sigmoid': 5, 'elu': 6, 'selu': 7, 'softplus': 8, 'swish': 9}
 K_BIAS_ACT, K_UPFIRDN2D, K_CONV2D, K_FC, K_RENDER, K_RASTER, K_MISC, K_CONV2D_BF16X3 = range(8)
-FAMILY_NAMES = ['bias_act', 'upfirdn2d', 'conv2d', 'fc', 'render', 'raster', 'misc', 'conv2d_bf16x3', 'conv1x1_bf16x3', 'conv2d_f16', 'render_rays']
+FAMILY_NAMES = ['bias_act', 'upfirdn2d', 'conv2d', 'fc', 'render', 'raster', 'misc', 'conv2d_bf16x3', 'conv1x1_bf16x3', 'conv2d_f16', 'render_rays',
+                'layer_norm', 'rotary', 'attention']
 
 
 class Epilogue(ctypes.Structure):
@@ -54,6 +55,13 @@ class FcJob(ctypes.Structure):
     _fields_ = [('w', c_void_p), ('b', c_void_p), ('x_off', c_int64), ('x_stride', c_int64), ('y_off', c_int64),
                 ('y_stride', c_int64), ('I', c_int), ('O', c_int), ('wgain', c_float), ('bgain', c_float), ('act', c_int),
                 ('alpha', c_float), ('gain', c_float), ('pre_square', c_int), ('post_rsqrt', c_int)]
+
+
+class RotaryDesc(ctypes.Structure):
+    _fields_ = [('q', c_void_p), ('k', c_void_p), ('positions', c_void_p), ('out_q', c_void_p), ('out_k', c_void_p), ('q_strides', c_int64 * 3),
+                ('k_strides', c_int64 * 3), ('pos_batch_stride', c_int64), ('pos_token_stride', c_int64), ('base', c_double), ('B', c_int), ('L', c_int),
+                ('heads_q', c_int), ('heads_k', c_int), ('D', c_int), ('axes', c_int), ('sections', c_int * 4), ('dtype', c_int), ('pos_type', c_int),
+                ('interleaved', c_int), ('shared_ladder', c_int), ('inverse', c_int)]
 
 
 _SIGNATURES = {
@@ -121,6 +129,10 @@ _SIGNATURES = {
     'n3d_fc_multi': (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p]),
     'n3d_fc': (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_float, c_int, c_float,
                        c_float, c_int, c_int, c_void_p]),
+    'n3d_layer_norm': (c_int, [c_void_p] * 6 + [c_int64, c_int, c_int64, c_int, c_int, c_float, c_void_p]),
+    'n3d_layer_norm_bwd_workspace': (c_int64, [c_int64, c_int, c_int]),
+    'n3d_rotary': (c_int, [ctypes.POINTER(RotaryDesc), c_void_p]),
+    'n3d_layer_norm_bwd': (c_int, [c_void_p] * 9 + [c_int64, c_int, c_int64, c_int64, c_int, c_int, c_void_p]),
 }
 
 _lib = None

@@ -1,0 +1,113 @@
+"""CPU tests of the token operators: what they refuse, before anything reaches a device."""
+import ctypes as C
+import os
+import subprocess
+
+import pytest
+import torch
+
+REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def _raises(match, fn, *args, **kw):
+    with pytest.raises(RuntimeError, match=match):
+        fn(*args, **kw)
+
+
+def test_layer_norm_refusals():
+    from next3d_amd.torch_utils.ops.layer_norm import layer_norm
+    x = torch.zeros(3, 8)
+    _raises('HIP device only', layer_norm, x)
+    _raises('must be', layer_norm, x.double())
+    _raises('must be', layer_norm, x.long())
+    _raises('tensor', layer_norm, [1.0])
+    _raises('last dimension', layer_norm, torch.zeros(()))
+    _raises('last dimension', layer_norm, torch.zeros(3, 0))
+    _raises('7 elements for 8', layer_norm, x, torch.ones(7))
+    _raises('dimensions', layer_norm, x, torch.ones(1, 8))
+    _raises('weight must be', layer_norm, x, torch.ones(8).half())
+    _raises('bias must be', layer_norm, x.half(), None, torch.ones(8).bfloat16())
+    _raises('one dtype', layer_norm, x.half(), torch.ones(8).half(), torch.ones(8))
+    for eps in (-1e-6, float('nan'), float('inf')):
+        _raises('eps', layer_norm, x, eps=eps)
+
+
+def test_rotary_refusals():
+    from next3d_amd.torch_utils.ops.rotary import rotary
+    q, pos = torch.zeros(2, 5, 3, 16), torch.zeros(5, 2, dtype=torch.int32)
+    _raises('HIP device only', rotary, q, pos, (8, 8))
+    _raises('4 dimensions', rotary, q[0], pos, (8, 8))
+    _raises('q must be', rotary, q.double(), pos, (8, 8))
+    _raises('k must be', rotary, q, pos, (8, 8), k=q.half())
+    _raises('does not have', rotary, q, pos, (8, 8), k=q[:, :4])
+    _raises('does not have', rotary, q, pos, (8, 8), k=q[..., :8])
+    _raises('positions must be', rotary, q, pos.short(), (8, 8))
+    _raises('positions must be', rotary, q, pos[:4], (8, 8))
+    _raises('positions must be', rotary, q, pos, (4, 4, 8))
+    _raises('positions must be', rotary, q, pos[None].expand(3, 5, 2), (8, 8))
+    for sections in ((), (3, 5), (8, 16), (-2, 8), (0, 0), (2, 2, 2, 2, 2)):
+        _raises('sections', rotary, q, pos, sections)
+    _raises('pairing', rotary, q, pos, (8, 8), pairing='quarters')
+    _raises('ladder', rotary, q, pos, (8, 8), ladder='rope')
+    for base in (0.0, -1.0, float('inf'), float('nan')):
+        _raises('base', rotary, q, pos, (8, 8), base=base)
+    _raises('no gradient', rotary, q, pos.float().requires_grad_(), (8, 8))
+    _raises('channels', rotary, torch.zeros(1, 5, 1, 1026), pos, (8, 8))
+    _raises('heads', rotary, torch.zeros(1, 5, 4097, 16), pos, (8, 8))
+
+
+def _struct_layout(tmp_path, cname, cls):
+    lines = ['#include <stdio.h>', '#include <stddef.h>', f'#include "{os.path.join(REPO, "include", "n3d.h")}"', 'int main(void) {', f'  printf("size %zu\\n", sizeof({cname}));']
+    lines += [f'  printf("{name} %zu\\n", offsetof({cname}, {name}));' for name, _ in cls._fields_] + ['  return 0;', '}']
+    src, exe = tmp_path / 'layout.c', tmp_path / 'layout'
+    src.write_text('\n'.join(lines))
+    subprocess.run(['gcc', '-std=c11', str(src), '-o', str(exe)], check=True)
+    out = dict(line.split() for line in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.splitlines())
+    assert int(out.pop('size')) == C.sizeof(cls)
+    assert {k: int(v) for k, v in out.items()} == {name: getattr(cls, name).offset for name, _ in cls._fields_}
+
+
+def test_rotary_descriptor_layout(tmp_path):
+    from next3d_amd import _lib
+    _struct_layout(tmp_path, 'n3d_rotary_desc', _lib.RotaryDesc)
+
+
+def test_c_entries_refuse_bad_calls():
+    """The library's own checks (a C caller has no Python in front of it): they return before any launch, so they hold without a device."""
+    from next3d_amd import _lib
+    lib = _lib.lib()
+
+    def err(rc):
+        assert rc != 0
+        return lib.n3d_last_error().decode()
+
+    p = 4096                                                       # never dereferenced: every call below is refused
+    assert 'dtype' in err(lib.n3d_layer_norm(p, None, None, p, None, None, 1, 8, 8, 7, 0, 1e-5, None))
+    assert 'sizes' in err(lib.n3d_layer_norm(p, None, None, p, None, None, 1, 0, 8, 0, 0, 1e-5, None))
+    assert 'null' in err(lib.n3d_layer_norm(None, None, None, p, None, None, 1, 8, 8, 0, 0, 1e-5, None))
+    assert 'null' in err(lib.n3d_layer_norm(p, None, None, p, p, None, 1, 8, 8, 0, 0, 1e-5, None))
+    assert 'weight' in err(lib.n3d_layer_norm(p, p, None, p, None, None, 1, 8, 8, 1, 2, 1e-5, None))
+    assert 'eps' in err(lib.n3d_layer_norm(p, p, None, p, None, None, 1, 8, 8, 1, 1, -1.0, None))
+    assert lib.n3d_layer_norm(None, None, None, None, None, None, 0, 8, 8, 0, 0, 1e-5, None) == 0
+    assert 'rows' in err(lib.n3d_layer_norm_bwd(p, p, None, p, p, p, None, None, None, 0, 8, 8, 8, 0, 0, None))
+    assert 'null' in err(lib.n3d_layer_norm_bwd(p, p, None, p, p, p, p, None, None, 1, 8, 8, 8, 0, 0, None))
+    assert lib.n3d_layer_norm_bwd_workspace(0, 8, 0) == 0
+
+    def rot(**kw):
+        d = _lib.RotaryDesc(q=p, positions=p, out_q=p, pos_token_stride=1, base=1e4, B=1, L=2, heads_q=1, D=16, axes=1, dtype=0)
+        d.sections[0] = 16
+        for k, v in kw.items():
+            if k == 'sections':
+                d.sections[:] = v
+            else:
+                setattr(d, k, v)
+        return lib.n3d_rotary(d, None)
+
+    for kw, word in ((dict(axes=5), 'axes'), (dict(axes=0), 'axes'), (dict(D=1), 'channels'), (dict(D=2048), 'channels'), (dict(dtype=4), 'dtype'),
+                     (dict(pos_type=3), 'positions'), (dict(positions=None), 'positions'), (dict(base=0.0), 'base'), (dict(q=None), 'null'),
+                     (dict(heads_k=1), 'null'), (dict(sections=(3, 0, 0, 0)), 'even'), (dict(sections=(18, 0, 0, 0)), 'even'), (dict(sections=(0, 0, 0, 0)), 'add up'),
+                     (dict(axes=2, sections=(16, 16, 0, 0)), 'add up'), (dict(L=-1), 'negative'),
+                     (dict(B=2 ** 16, L=2 ** 16), 'tokens')):
+        assert word in err(rot(**kw)), kw
+    assert rot(L=0) == 0
+    assert 'null' in err(lib.n3d_rotary(None, None))
