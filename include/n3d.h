@@ -517,6 +517,35 @@ typedef struct {
 } n3d_rotary_desc;
 int n3d_rotary(const n3d_rotary_desc* desc, n3d_stream_t stream);
 
+/* Attention.  q [B, Lq, heads_q, D], k / v [B, Lk, heads_k, D] (dtype N3D_F16 or N3D_BF16; element strides (batch, token, head), multiples of 8, dense
+ * channels; 16-byte aligned; D a multiple of 8 up to 128; heads_q a multiple of heads_k: query head h reads key head h / (heads_q / heads_k)) ->
+ * out [B, Lq, heads_q, D] dense, lse [B, heads_q, Lq] float32 (logarithm of the softmax's sum; may be NULL; needed for the gradient).
+ * With n = lengths[b] (NULL: Lk) keys in use, query i stands at position i + n - Lq (the last query beside the last key):
+ *   t = scale * q.k;   softcap > 0: t = softcap * tanh(t / softcap);   slopes [heads_q] float32: t -= slope * |position - j|
+ *   visible: j < n; causal: j <= position or j < prefix[b] (prefix [B] int32 or NULL); documents (int32, [B, Lq] / [B, Lk] with the given batch strides,
+ *   both or neither NULL): equal and not negative.
+ * A row that sees nothing gives out 0 and lse -inf.  Keys behind n are not read.  float32 softmax and accumulation.
+ * workspace: n3d_attention_workspace(desc) bytes (-1: refused, see n3d_last_error), 16-byte aligned; nothing in it outlives the call. */
+typedef struct {
+    const void *q, *k, *v;
+    void* out;
+    float* lse;
+    const int *prefix, *lengths, *q_documents, *k_documents;
+    const float* slopes;
+    void* workspace;
+    const void* dout;               /* gradient of out (n3d_attention_bwd) */
+    void *dq, *dk, *dv;             /* gradients, dense like q / k / v; dq, or dk and dv together, may be NULL */
+    int64_t q_strides[3], k_strides[3], v_strides[3], dout_strides[3], q_doc_stride, k_doc_stride, workspace_bytes;
+    float scale, softcap;
+    int B, Lq, Lk, heads_q, heads_k, D, dtype, causal;
+} n3d_attention_desc;
+int64_t n3d_attention_workspace(const n3d_attention_desc* desc);
+int n3d_attention(const n3d_attention_desc* desc, n3d_stream_t stream);
+/* Gradients from the forward call's q, k, v, out and lse and from dout.  dk / dv are summed over the query heads of a key head, in a fixed order: the
+ * results are bitwise reproducible.  Rows that see nothing and keys that nobody sees get zeros. */
+int64_t n3d_attention_bwd_workspace(const n3d_attention_desc* desc);
+int n3d_attention_bwd(const n3d_attention_desc* desc, n3d_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

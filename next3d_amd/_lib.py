@@ -64,6 +64,15 @@ class RotaryDesc(ctypes.Structure):
                 ('interleaved', c_int), ('shared_ladder', c_int), ('inverse', c_int)]
 
 
+class AttentionDesc(ctypes.Structure):
+    _fields_ = [('q', c_void_p), ('k', c_void_p), ('v', c_void_p), ('out', c_void_p), ('lse', c_void_p), ('prefix', c_void_p), ('lengths', c_void_p),
+                ('q_documents', c_void_p), ('k_documents', c_void_p), ('slopes', c_void_p), ('workspace', c_void_p), ('dout', c_void_p), ('dq', c_void_p),
+                ('dk', c_void_p), ('dv', c_void_p), ('q_strides', c_int64 * 3), ('k_strides', c_int64 * 3), ('v_strides', c_int64 * 3),
+                ('dout_strides', c_int64 * 3), ('q_doc_stride', c_int64), ('k_doc_stride', c_int64), ('workspace_bytes', c_int64), ('scale', c_float),
+                ('softcap', c_float), ('B', c_int), ('Lq', c_int), ('Lk', c_int), ('heads_q', c_int), ('heads_k', c_int), ('D', c_int), ('dtype', c_int),
+                ('causal', c_int)]
+
+
 _SIGNATURES = {
     'n3d_abi_version': (c_int, []),
     'n3d_last_error': (ctypes.c_char_p, []),
@@ -131,6 +140,10 @@ _SIGNATURES = {
                        c_float, c_int, c_int, c_void_p]),
     'n3d_layer_norm': (c_int, [c_void_p] * 6 + [c_int64, c_int, c_int64, c_int, c_int, c_float, c_void_p]),
     'n3d_layer_norm_bwd_workspace': (c_int64, [c_int64, c_int, c_int]),
+    'n3d_attention_workspace': (c_int64, [ctypes.POINTER(AttentionDesc)]),
+    'n3d_attention': (c_int, [ctypes.POINTER(AttentionDesc), c_void_p]),
+    'n3d_attention_bwd_workspace': (c_int64, [ctypes.POINTER(AttentionDesc)]),
+    'n3d_attention_bwd': (c_int, [ctypes.POINTER(AttentionDesc), c_void_p]),
     'n3d_rotary': (c_int, [ctypes.POINTER(RotaryDesc), c_void_p]),
     'n3d_layer_norm_bwd': (c_int, [c_void_p] * 9 + [c_int64, c_int, c_int64, c_int64, c_int, c_int, c_void_p]),
 }

@@ -1,0 +1,257 @@
+// What the attention kernels share (attention_fwd.hip, attention_bwd.hip): parameters, the visibility rule, matrix fragments and tile staging.
+//
+// Score of query i (of Lq) and key j (of the n in use) of one head:   t = scale * q.k;   t = cap tanh(t / cap);   t -= slope |i + n - Lq - j|
+// visible:  j < n,  and (not causal, or j <= i + n - Lq, or j < prefix),  and (no documents, or doc(i) == doc(j) >= 0).
+// Scores are kept in base 2 (t log2 e), softmax statistics and every accumulator in float32.
+//
+// Matrix layout (v_mfma_f32_32x32x16: operand element e of lane (l31, half) is row / column l31, k = 8 half + e; accumulator register r is row
+// 8 (r / 4) + 4 half + r % 4, column l31).  Products are arranged so that a lane owns ONE column — a query in the forward and dq kernels, a key in the
+// dk / dv kernel — and the 16 scores a lane holds are, in register order, the second operand of the next product: k is only a name for "which row", so
+// that product's first operand is read with the same naming (two transposed LDS reads of four rows each).  Scores never leave their lane.
+#pragma once
+#include "common.h"
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void attn_lds_void;
+
+static constexpr float ATTN_LOG2E = 1.4426950408889634f, ATTN_LN2 = 0.6931471805599453f;
+static constexpr int ATTN_TILE = 64;                 // keys (queries in the dk / dv kernel) of an LDS tile, and of a document range
+
+struct AttnParams {
+    const void *q, *k, *v, *o, *dout;
+    void *out, *dq, *dk, *dv;
+    float* lse;
+    int64_t qs[3], ks[3], vs[3], ds[3];              // element strides (batch, token, head) of q, k, v, dout; out / dq / dk / dv are dense
+    const int *prefix, *lengths, *qdoc, *kdoc;
+    int64_t qdoc_stride, kdoc_stride;
+    const float* slopes;
+    const int2 *ktiles, *qtiles;                     // lowest and highest document of every ATTN_TILE keys / queries, [B][nkt] / [B][nqt]
+    float* delta;                                    // [B][Hq][Lq]
+    float* part;                                     // partial results of split kernels
+    int64_t part_ml;                                 // offset of their statistics in `part`
+    const float* maxima;                             // partial maxima (float16 gradients), see attn_ds_scale
+    int n_maxima;
+    int B, Lq, Lk, Hq, Hk, G, D, nkt, nqt, causal, splits, row_blocks;
+    float scale, softcap;
+};
+
+template <typename T> struct AttnVec;
+template <> struct AttnVec<_Float16> { typedef _Float16 x8 __attribute__((ext_vector_type(8))); typedef _Float16 x4 __attribute__((ext_vector_type(4))); };
+template <> struct AttnVec<__bf16> { typedef __bf16 x8 __attribute__((ext_vector_type(8))); typedef __bf16 x4 __attribute__((ext_vector_type(4))); };
+
+__device__ __forceinline__ f32x16 attn_mfma(AttnVec<_Float16>::x8 a, AttnVec<_Float16>::x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x16 attn_mfma(AttnVec<__bf16>::x8 a, AttnVec<__bf16>::x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+
+// the other half's value (lane ^ 32) folded in
+__device__ __forceinline__ void attn_halves(float x, float& lower, float& upper) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t a = r[0], b = r[1];                       // (a bit cast straight from r[1] reads r[0])
+    lower = __builtin_bit_cast(float, a);
+    upper = __builtin_bit_cast(float, b);
+}
+__device__ __forceinline__ float attn_half_max(float x) {
+    float a, b;
+    attn_halves(x, a, b);
+    return fmaxf(a, b);
+}
+__device__ __forceinline__ float attn_half_sum(float x) {
+    float a, b;
+    attn_halves(x, a, b);
+    return a + b;
+}
+__device__ __forceinline__ int attn_uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// keys in use / last visible key of query i without documents (-1: none)
+__device__ __forceinline__ int attn_keys(const AttnParams& p, int b) {
+    const int n = p.lengths ? p.lengths[b] : p.Lk;
+    return n < 0 ? 0 : n < p.Lk ? n : p.Lk;
+}
+__device__ __forceinline__ int attn_limit(const AttnParams& p, int i, int n, int prefix) {
+    int lim = n - 1;
+    if (p.causal) {
+        int c = i + n - p.Lq;
+        c = c > prefix - 1 ? c : prefix - 1;
+        lim = c < lim ? c : lim;
+    }
+    return lim < -1 ? -1 : lim;
+}
+
+// base-2 score of a raw product, and the factor d t / d (scale q.k) of the cap
+struct AttnScore {
+    float mul, cap_in, cap_out, slope;               // mul: scale log2 e;  cap_in: 2 scale log2 e / cap;  cap_out: cap log2 e;  slope: slope log2 e
+    __device__ AttnScore(const AttnParams& p, int head) {
+        mul = p.scale * ATTN_LOG2E;
+        cap_in = p.softcap > 0.f ? 2.f * ATTN_LOG2E * p.scale / p.softcap : 0.f;
+        cap_out = p.softcap > 0.f ? p.softcap * ATTN_LOG2E : 0.f;
+        slope = p.slopes ? p.slopes[head] * ATTN_LOG2E : 0.f;
+    }
+    // tanh x = 1 - 2 / (1 + e^2x): off by some 2^-23 absolutely, 2^-23 cap of a score
+    __device__ __forceinline__ float tanh_part(float s) const { return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s * cap_in)); }
+};
+
+// ---- LDS tiles: ROW channels of 16 bits a row (64 or 128; channels beyond D are zero), rows of 16-byte chunks.  Chunk c of row r sits at c ^ swizzle(r):
+// 16 rows of one chunk, and 4 rows of 4 neighbouring chunks (a transposed read), each touch every bank once.
+template <int ROW>
+__device__ __forceinline__ int attn_swizzle(int row) {
+    if constexpr (ROW == 128) return ((row & 3) << 2) | ((row >> 2) & 3);
+    else return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+}
+
+// Staging by LDS-DMA: a piece is 1 KB = 64 lanes x 16 bytes; wave w of W takes pieces w, w + W, ...  Rows behind the last and channels behind D are beyond
+// the descriptor's range and arrive as zeros.
+template <int ROW, int ROWS, int WAVES>
+struct AttnStage {
+    static constexpr int CHUNKS = ROW / 8, RPP = 64 / CHUNKS, PIECES = ROWS / RPP / WAVES;
+    static_assert(PIECES >= 1, "a wave stages whole pieces");
+    int voff[PIECES];
+    __device__ __forceinline__ void setup(int wave, int lane, int64_t stride, int D) {
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) {
+            const int row = (wave + i * WAVES) * RPP + lane / CHUNKS, c = (lane % CHUNKS) ^ attn_swizzle<ROW>(row);
+            voff[i] = c * 8 < D ? row * (int)stride * 2 + c * 16 : (int)0x80000000;
+        }
+    }
+    // rows [0, rows) of `base` (rows >= 1) -> lds
+    __device__ __forceinline__ void issue(const void* base, int rows, int64_t stride, int D, char* lds, int wave) const {
+        const uint64_t a = (uint64_t)base;
+        const uint64_t u = ((uint64_t)(uint32_t)attn_uniform((int)(a >> 32)) << 32) | (uint32_t)attn_uniform((int)a);
+        const int n = attn_uniform(((rows < ROWS ? rows : ROWS) - 1) * (int)stride * 2 + D * 2);
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)u, 0, n, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (attn_lds_void*)(lds + (wave + i * WAVES) * 1024), 16, voff[i], 0, 0, 0);
+    }
+};
+
+// first operand, rows = tile rows row0 + l31, k = channels: chunk 2 c + half
+template <typename T, int ROW>
+__device__ __forceinline__ typename AttnVec<T>::x8 attn_row_frag(const char* tile, int row, int chunk) {
+    return *reinterpret_cast<const typename AttnVec<T>::x8*>(tile + row * (ROW * 2) + ((chunk ^ attn_swizzle<ROW>(row)) << 4));
+}
+// first operand, rows = channels 32 db + l31, k = tile rows row0 + {4 half + 0..3, 8 + 4 half + 0..3} (row0 a multiple of 16)
+template <typename T, int ROW>
+__device__ __forceinline__ typename AttnVec<T>::x8 attn_col_frag(const char* tile, int row0, int db, int lane) {
+    const int half = lane >> 5, l16 = lane & 15;
+    const int row = row0 + 4 * half + (l16 >> 2), chunk = 4 * db + ((lane >> 4) & 1) * 2 + ((l16 & 3) >> 1), in = (l16 & 1) * 8;
+    const char* lo = tile + row * (ROW * 2) + ((chunk ^ attn_swizzle<ROW>(row)) << 4) + in;
+    const char* hi = tile + (row + 8) * (ROW * 2) + ((chunk ^ attn_swizzle<ROW>(row + 8)) << 4) + in;
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)lo);
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)hi);
+    typedef short s16x8 __attribute__((ext_vector_type(8)));
+    const s16x8 v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    return __builtin_bit_cast(typename AttnVec<T>::x8, v);
+}
+// second operand from global memory: column = this lane's row of `p` (null: zeros), k = channels 16 c + 8 half + 0..7
+template <typename T>
+__device__ __forceinline__ typename AttnVec<T>::x8 attn_lane_frag(const T* p, int chunk, int D) {
+    typename AttnVec<T>::x8 z = {};
+    return p && chunk * 8 < D ? *reinterpret_cast<const typename AttnVec<T>::x8*>(p + chunk * 8) : z;
+}
+
+// every wave's pieces have landed and every wave is done with what it read: a tile buffer changes hands
+__device__ __forceinline__ void attn_sync() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// ---- which tiles to visit: [t, end) in order; with documents only those whose range [lowest, highest] meets [lo, hi] (64 ranges looked at together)
+struct AttnTiles {
+    const int2* ranges;
+    int t, end, lo, hi;
+    uint64_t bits;
+    int base, kmin, kmax;
+    __device__ void start(const int2* r, int first, int stop, int dlo, int dhi) {
+        ranges = r; t = first; end = stop; lo = dlo; hi = dhi; bits = 0; base = first - 64;
+    }
+    // the next tile or -1
+    __device__ int next(int lane) {
+        if (!ranges) return t < end ? t++ : -1;
+        while (bits == 0) {
+            base += 64;
+            if (base >= end) return -1;
+            const int i = base + lane;
+            const int2 d = i < end ? ranges[i] : make_int2(1, 0);
+            bits = __ballot(i < end && d.y >= lo && d.x <= hi);
+        }
+        const int n = __builtin_ctzll(bits);
+        bits &= bits - 1;
+        return attn_uniform(base + n);
+    }
+};
+
+// visible to a scalar pass over single keys (the repair of rows that a masked NaN or infinity has reached through 0 * NaN in a matrix product)
+__device__ __forceinline__ bool attn_visible(const AttnParams& p, int b, int j, int lim, int qdoc) {
+    return j <= lim && (!p.kdoc || (qdoc >= 0 && p.kdoc[b * p.kdoc_stride + j] == qdoc));
+}
+template <typename T>
+__device__ __forceinline__ float attn_dot(const T* a, const T* c, int D) {
+    float s = 0.f;
+    for (int d = 0; d < D; d += 8) {
+        const auto x = *reinterpret_cast<const typename AttnVec<T>::x8*>(a + d), y = *reinterpret_cast<const typename AttnVec<T>::x8*>(c + d);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s += (float)x[e] * (float)y[e];
+    }
+    return s;
+}
+// base-2 score of raw product s at distance `dist`
+__device__ __forceinline__ float attn_score(const AttnScore& f, float s, int dist) {
+    const float u = f.cap_out > 0.f ? f.cap_out * f.tanh_part(s) : s * f.mul;
+    return u - f.slope * fabsf((float)dist);
+}
+
+// a row's 32 * DB channels spread over lanes l31 and l31 + 32 -> 16-byte stores (the halves trade their 8-byte runs)
+template <typename T, int DB>
+__device__ __forceinline__ void attn_store_row(T* row, const f32x16 (&acc)[DB], float by, int half, int D, bool on) {
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int a = 0; a < 4; a += 2) {
+            typename AttnVec<T>::x4 x, y;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[e] = (T)(acc[db][4 * a + e] * by);
+                y[e] = (T)(acc[db][4 * a + 4 + e] * by);
+            }
+            uint2 u = __builtin_bit_cast(uint2, x), w = __builtin_bit_cast(uint2, y);
+            const auto r0 = __builtin_amdgcn_permlane32_swap(u.x, w.x, false, false);
+            const auto r1 = __builtin_amdgcn_permlane32_swap(u.y, w.y, false, false);
+            const int d = 32 * db + 8 * a + 8 * half;
+            if (on && d < D) *reinterpret_cast<uint4*>(row + d) = make_uint4(r0[0], r1[0], r0[1], r1[1]);
+        }
+}
+
+// ---- host: a checked descriptor as kernel parameters
+static inline const char* attn_params(const n3d_attention_desc* d, AttnParams& p) {
+    if (!d) return "null descriptor";
+    if (d->B < 0 || d->Lq < 0 || d->Lk < 0) return "negative sizes";
+    if (d->dtype != N3D_F16 && d->dtype != N3D_BF16) return "float16 or bfloat16 only";
+    if (d->heads_k < 1 || d->heads_q < 1 || d->heads_q % d->heads_k) return "the query heads must be a multiple of the key heads";
+    if (d->D < 8 || d->D > 128 || d->D % 8) return "head sizes are multiples of 8 from 8 to 128";
+    if ((int64_t)d->B * d->heads_q * ((d->Lq > d->Lk ? d->Lq : d->Lk) / 32 + 1) >= (1 << 28)) return "too many rows for one launch";
+    if (!(d->softcap >= 0.f && d->softcap < INFINITY) || !(d->scale > -INFINITY && d->scale < INFINITY)) return "scale and softcap must be finite, softcap not negative";
+    if (d->prefix && !d->causal) return "a prefix needs causal";
+    if ((!d->q_documents) != (!d->k_documents)) return "documents of the queries and of the keys, or neither";
+    const bool some = d->B > 0 && d->Lq > 0;
+    if (some && (!d->q || !d->out)) return "null tensor";
+    if (some && d->Lk > 0 && (!d->k || !d->v)) return "null tensor";
+    const int64_t* strides[3] = {d->q_strides, d->k_strides, d->v_strides};
+    for (const int64_t* s : strides)
+        for (int i = 0; i < 3; ++i)
+            if (s[i] % 8 || s[i] < 0 || (i == 1 && s[i] > (1 << 23))) return "strides must be multiples of 8 elements, of tokens 2^23 at most";
+    if (((uintptr_t)d->q | (uintptr_t)d->k | (uintptr_t)d->v | (uintptr_t)d->out) % 16) return "tensors must be 16-byte aligned";
+    p = AttnParams{};
+    p.q = d->q; p.k = d->k; p.v = d->v; p.out = d->out; p.o = d->out; p.lse = d->lse;
+    for (int i = 0; i < 3; ++i) {
+        p.qs[i] = d->q_strides[i]; p.ks[i] = d->k_strides[i]; p.vs[i] = d->v_strides[i]; p.ds[i] = d->dout_strides[i];
+    }
+    p.prefix = d->prefix; p.lengths = d->lengths; p.qdoc = d->q_documents; p.kdoc = d->k_documents;
+    p.qdoc_stride = d->q_doc_stride; p.kdoc_stride = d->k_doc_stride; p.slopes = d->slopes;
+    p.B = d->B; p.Lq = d->Lq; p.Lk = d->Lk; p.Hq = d->heads_q; p.Hk = d->heads_k; p.G = d->heads_q / d->heads_k; p.D = d->D;
+    p.nkt = cdiv(d->Lk, ATTN_TILE); p.nqt = cdiv(d->Lq, ATTN_TILE);
+    p.causal = d->causal != 0; p.scale = d->scale; p.softcap = d->softcap;
+    p.splits = 1;
+    return nullptr;
+}
+
+// workspace, in floats: the document ranges come first
+static inline int64_t attn_range_floats(const AttnParams& p) { return p.kdoc ? 2 * (int64_t)p.B * (p.nkt + p.nqt) : 0; }
+void attn_ranges(AttnParams& p, void* workspace, hipStream_t stream);      // attention_fwd.hip

@@ -1,0 +1,553 @@
+// Attention, backward (attention.h):  P = exp2(u - lse),  dP = do v^T,  delta = sum(do o),  dt = P (dP - delta),  ds = dt (1 - tanh^2),
+//   dq = scale ds k,   dk = scale ds^T q,   dv = P^T do,   dk and dv summed over the query heads of a key head.
+// attn_prep_kernel: delta, and for float16 the largest |do| and |v| (attn_ds_scale).
+// attn_dq_kernel: a workgroup owns 128 queries of a head and walks the keys;  attn_dkv_kernel: a workgroup owns 128 keys of a key head and walks the
+// queries of all its heads.  Scores are computed in both (7 products for 5) so that every sum has one owner: no atomics, the same bits every time.
+#include "attention.h"
+
+static constexpr int ATTN_MAXIMA = 256;              // workgroups (= partial maxima) of |do|, and as many of |v|
+// float16 has 5 exponent bits, and P ~ 1 / length and ds ~ P do v leave its range on long rows or with small gradients.  The dk / dv kernel therefore uses
+// P 2^12, and both kernels ds times a power of two taken from the largest |do| and |v| of the call, so that no ds can overflow:
+// |ds| <= |dP - delta| <= 2 D max|do| max|v|.  The accumulators undo both.  bfloat16 has float32's exponents: neither is needed.
+template <typename T> static constexpr float ATTN_P_SHIFT = 0.f;
+template <> constexpr float ATTN_P_SHIFT<_Float16> = 12.f;
+
+template <typename T>
+__global__ __launch_bounds__(256) void attn_prep_kernel(AttnParams p) {
+    // 16 lanes a row, 8 channels a lane
+    const int lane16 = threadIdx.x & 15, D = p.D;
+    float top = 0.f;
+    if (blockIdx.y == 0) {
+        const int64_t rows = (int64_t)p.B * p.Lq * p.Hq;
+        for (int64_t w = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); w < rows; w += (int64_t)gridDim.x * 16) {
+            const int h = (int)(w % p.Hq);
+            const int64_t bi = w / p.Hq;
+            const int b = (int)(bi / p.Lq), i = (int)(bi - (int64_t)b * p.Lq);
+            const int64_t stat = ((int64_t)b * p.Hq + h) * p.Lq + i;
+            float s = 0.f;
+            const bool live = p.lse[stat] != -INFINITY;
+            if (lane16 * 8 < D) {
+                const auto x = *reinterpret_cast<const typename AttnVec<T>::x8*>((const T*)p.dout + b * p.ds[0] + i * p.ds[1] + h * p.ds[2] + lane16 * 8);
+                const auto y = *reinterpret_cast<const typename AttnVec<T>::x8*>((const T*)p.o + w * D + lane16 * 8);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    s += (float)x[e] * (float)y[e];
+                    const float a = fabsf((float)x[e]);
+                    if (live && a < INFINITY) top = fmaxf(top, a);
+                }
+            }
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o);
+            if (lane16 == 0) p.delta[stat] = s;
+        }
+    } else {
+        const int64_t rows = (int64_t)p.B * p.Lk * p.Hk;
+        for (int64_t w = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); w < rows; w += (int64_t)gridDim.x * 16) {
+            const int h = (int)(w % p.Hk);
+            const int64_t bj = w / p.Hk;
+            const int b = (int)(bj / p.Lk), j = (int)(bj - (int64_t)b * p.Lk);
+            if (j >= attn_keys(p, b) || (p.kdoc && p.kdoc[b * p.kdoc_stride + j] < 0) || lane16 * 8 >= D) continue;
+            const auto x = *reinterpret_cast<const typename AttnVec<T>::x8*>((const T*)p.v + b * p.vs[0] + j * p.vs[1] + h * p.vs[2] + lane16 * 8);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float a = fabsf((float)x[e]);
+                if (a < INFINITY) top = fmaxf(top, a);
+            }
+        }
+    }
+    if (!p.maxima) return;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    __shared__ float tops[4];
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) ((float*)p.maxima)[blockIdx.y * ATTN_MAXIMA + blockIdx.x] = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+}
+
+// the exponent of ds's factor (0 without maxima); every wave computes it for itself
+__device__ __forceinline__ int attn_ds_scale(const AttnParams& p, int lane) {
+    if (!p.maxima) return 0;
+    float a = 0.f, c = 0.f;
+#pragma unroll
+    for (int i = 0; i < ATTN_MAXIMA / 64; ++i) {
+        a = fmaxf(a, p.maxima[i * 64 + lane]);
+        c = fmaxf(c, p.maxima[ATTN_MAXIMA + i * 64 + lane]);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        a = fmaxf(a, __shfl_xor(a, o));
+        c = fmaxf(c, __shfl_xor(c, o));
+    }
+    if (a == 0.f || c == 0.f) return 0;
+    // 2 D <= 2^8 and a < 2^(ilogb a + 1): ds 2^e < 2^15
+    const int e = 15 - 8 - (ilogbf(a) + 1) - (ilogbf(c) + 1);
+    return attn_uniform(e);
+}
+
+// raw scores S and dP of 16 (row, column) elements -> P 2^shift and ds 2^e.  lse2 / delta of register r by the functions given; see(r) is asked only if !full
+template <typename FL, typename FD, typename FS, typename FDist>
+__device__ __forceinline__ void attn_ds_step(f32x16& S, f32x16& dP, const AttnScore& f, float ds_by, bool full, FL lse2, FD delta, FS see, FDist dist) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        float u, slope_of_cap = 1.f;
+        if (f.cap_out > 0.f) {
+            const float th = f.tanh_part(S[r]);
+            u = f.cap_out * th;
+            slope_of_cap = 1.f - th * th;
+        } else {
+            u = S[r] * f.mul;
+        }
+        if (f.slope != 0.f) u -= f.slope * fabsf((float)dist(r));
+        const float w = __builtin_amdgcn_exp2f(u - lse2(r));
+        float d = w * (dP[r] - delta(r)) * (slope_of_cap * ds_by);
+        const bool on = full || see(r);
+        S[r] = on ? w : 0.f;
+        dP[r] = on ? d : 0.f;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void attn_pack(const f32x16& x, typename AttnVec<T>::x8 (&out)[2]) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) out[c][e] = (T)x[8 * c + e];
+}
+
+// P and ds / scale of one (query, key) pair, plain arithmetic
+template <typename T>
+__device__ __forceinline__ void attn_pair(const AttnParams& p, const AttnScore& f, const T* q, const T* k, const T* v, const T* dout, float lse2, float delta, int dist,
+                                          float& w, float& ds) {
+    const float s = attn_dot<T>(q, k, p.D);
+    const float th = f.cap_out > 0.f ? f.tanh_part(s) : 0.f;
+    w = __builtin_amdgcn_exp2f(attn_score(f, s, dist) - lse2);
+    ds = w * (attn_dot<T>(dout, v, p.D) - delta) * (1.f - th * th);
+}
+__device__ __forceinline__ float attn_lse2(float lse) { return lse == -INFINITY ? INFINITY : lse * ATTN_LOG2E; }       // (a row that sees nothing: every weight 0)
+
+template <typename T, int DB>
+__global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnParams p) {
+#ifdef __HIP_DEVICE_COMPILE__                            // (hipcc drops the launch stub of a template whose body its host pass cannot read)
+    constexpr int ROW = DB > 2 ? 128 : 64, TILE_BYTES = ATTN_TILE * ROW * 2;
+    __shared__ __align__(16) char smem[4 * TILE_BYTES];
+    __shared__ int sdoc[2][ATTN_TILE];
+    const int wave = attn_uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
+    const int total = p.B * p.Hq * p.row_blocks, per = (total + 7) / 8;
+    const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per || id >= total) return;
+    const int blk = p.row_blocks - 1 - id % p.row_blocks, bh = id / p.row_blocks, h = bh % p.Hq, b = bh / p.Hq, hk = h / p.G;
+    const int n = attn_keys(p, b), prefix = p.prefix ? p.prefix[b] : 0, q0 = blk * 128;
+    const int i = q0 + 32 * wave + l31;
+    const bool row_ok = i < p.Lq;
+    const int qdoc = p.kdoc && row_ok ? p.qdoc[b * p.qdoc_stride + i] : 0;
+    const int lim = !row_ok || qdoc < 0 ? -1 : attn_limit(p, i, n, prefix);
+    const int lim_first = attn_limit(p, q0 + 32 * wave, n, prefix), lim_last = attn_limit(p, min(q0 + 32 * wave + 31, p.Lq - 1), n, prefix);
+    const int key_end = attn_limit(p, min(q0 + 127, p.Lq - 1), n, prefix) + 1;
+    int dlo = 0, dhi = 0;
+    if (p.kdoc) {
+        const int2* r = p.qtiles + (int64_t)b * p.nqt + 2 * blk;
+        const int2 r0 = r[0], r1 = 2 * blk + 1 < p.nqt ? r[1] : r[0];
+        dlo = min(r0.x, r1.x);
+        dhi = max(r0.y, r1.y);
+    }
+    AttnTiles tiles;
+    tiles.start(p.kdoc ? p.ktiles + (int64_t)b * p.nkt : nullptr, 0, (key_end + ATTN_TILE - 1) / ATTN_TILE, max(dlo, 0), dhi);
+    typename AttnVec<T>::x8 qf[2 * DB], df[2 * DB];
+    const T* q = row_ok ? (const T*)p.q + b * p.qs[0] + i * p.qs[1] + h * p.qs[2] : nullptr;
+    const T* dout = row_ok ? (const T*)p.dout + b * p.ds[0] + i * p.ds[1] + h * p.ds[2] : nullptr;
+#pragma unroll
+    for (int c = 0; c < 2 * DB; ++c) {
+        qf[c] = attn_lane_frag<T>(q, 2 * c + half, p.D);
+        df[c] = attn_lane_frag<T>(dout, 2 * c + half, p.D);
+    }
+    const int64_t stat = ((int64_t)b * p.Hq + h) * p.Lq + i;
+    const float lse2 = row_ok ? attn_lse2(p.lse[stat]) : INFINITY, delta = row_ok ? p.delta[stat] : 0.f;
+    const T* k = (const T*)p.k + b * p.ks[0] + hk * p.ks[2];
+    const T* v = (const T*)p.v + b * p.vs[0] + hk * p.vs[2];
+    const int* kdoc = p.kdoc ? p.kdoc + b * p.kdoc_stride : nullptr;
+    const AttnScore f(p, h);
+    const int ds_exp = attn_ds_scale(p, lane);
+    const float ds_by = ldexpf(1.f, ds_exp);
+    AttnStage<ROW, ATTN_TILE, 4> sk, sv;
+    sk.setup(wave, lane, p.ks[1], p.D);
+    sv.setup(wave, lane, p.vs[1], p.D);
+    f32x16 acc[DB] = {};
+    auto stage = [&](int t, int buf) {
+        char* at = smem + buf * 2 * TILE_BYTES;
+        sk.issue(k + (int64_t)t * ATTN_TILE * p.ks[1], n - t * ATTN_TILE, p.ks[1], p.D, at, wave);
+        sv.issue(v + (int64_t)t * ATTN_TILE * p.vs[1], n - t * ATTN_TILE, p.vs[1], p.D, at + TILE_BYTES, wave);
+        if (kdoc && wave == 0) sdoc[buf][lane] = kdoc[min(t * ATTN_TILE + lane, p.Lk - 1)];
+    };
+    int t = tiles.next(lane);
+    if (t >= 0) stage(t, 0);
+    for (int buf = 0; t >= 0; buf ^= 1) {
+        attn_sync();
+        const int t_next = tiles.next(lane);
+        if (t_next >= 0) stage(t_next, buf ^ 1);
+        const int j0 = t * ATTN_TILE;
+        if (j0 <= lim_last) {
+            const char* kt = smem + buf * 2 * TILE_BYTES;
+            const char* vt = kt + TILE_BYTES;
+            bool full = j0 + ATTN_TILE - 1 <= lim_first;
+            if (kdoc) {
+                const int2 r = p.ktiles[(int64_t)b * p.nkt + t];
+                full = full && dlo == dhi && r.x == dlo && r.y == dlo;
+            }
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                f32x16 S = {}, dP = {};
+#pragma unroll
+                for (int c = 0; c < 2 * DB; ++c) {
+                    S = attn_mfma(attn_row_frag<T, ROW>(kt, 32 * kb + l31, 2 * c + half), qf[c], S);
+                    dP = attn_mfma(attn_row_frag<T, ROW>(vt, 32 * kb + l31, 2 * c + half), df[c], dP);
+                }
+                const int at = i + n - p.Lq, jb = j0 + 32 * kb + 4 * half;
+                attn_ds_step(S, dP, f, ds_by, full, [&](int) { return lse2; }, [&](int) { return delta; },
+                             [&](int r) {
+                                 const int j = 8 * (r >> 2) + (r & 3);
+                                 return jb + j <= lim && (!kdoc || sdoc[buf][32 * kb + 4 * half + j] == qdoc);
+                             },
+                             [&](int r) { return at - (jb + 8 * (r >> 2) + (r & 3)); });
+                typename AttnVec<T>::x8 d[2];
+                attn_pack<T>(dP, d);
+#pragma unroll
+                for (int db = 0; db < DB; ++db)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) acc[db] = attn_mfma(attn_col_frag<T, ROW>(kt, 32 * kb + 16 * c, db, lane), d[c], acc[db]);
+            }
+        }
+        t = t_next;
+    }
+    bool nan = false;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) nan = nan || acc[db][r] != acc[db][r];
+    uint64_t redo = __ballot(nan && row_ok && lse2 == lse2);
+    redo = (redo | (redo >> 32)) & 0xffffffffu;
+    T* out = (T*)p.dq + ((int64_t)(b * (int64_t)p.Lq + i) * p.Hq + h) * p.D;
+    attn_store_row<T, DB>(out, acc, ldexpf(p.scale, -ds_exp), half, p.D, row_ok && !((redo >> l31) & 1));
+    while (redo) {                                                      // a NaN behind the mask may have come in through 0 * NaN: these rows key by key
+        const int e = __builtin_ctzll(redo);
+        redo &= redo - 1;
+        const int ie = q0 + 32 * wave + e, lime = __shfl(lim, e), doce = __shfl(qdoc, e);
+        const float le = __shfl(lse2, e), de = __shfl(delta, e);
+        const T* qe = (const T*)p.q + b * p.qs[0] + ie * p.qs[1] + h * p.qs[2];
+        const T* doe = (const T*)p.dout + b * p.ds[0] + ie * p.ds[1] + h * p.ds[2];
+        float x[2] = {0.f, 0.f};
+        for (int j0 = 0; j0 <= lime; j0 += 64) {
+            const int j = j0 + lane;
+            const bool see = j <= lime && attn_visible(p, b, j, lime, doce);
+            float w, ds = 0.f;
+            if (see) attn_pair<T>(p, f, qe, k + j * p.ks[1], v + j * p.vs[1], doe, le, de, ie + n - p.Lq - j, w, ds);
+            uint64_t todo = __ballot(see);
+            while (todo) {
+                const int s = __builtin_ctzll(todo);
+                todo &= todo - 1;
+                const float d = __shfl(ds, s);
+                const T* kj = k + (int64_t)(j0 + s) * p.ks[1];
+                if (lane < p.D) x[0] += d * (float)kj[lane];
+                if (lane + 64 < p.D) x[1] += d * (float)kj[lane + 64];
+            }
+        }
+        T* o = (T*)p.dq + ((int64_t)(b * (int64_t)p.Lq + ie) * p.Hq + h) * p.D;
+        if (lane < p.D) o[lane] = (T)(x[0] * p.scale);
+        if (lane + 64 < p.D) o[lane + 64] = (T)(x[1] * p.scale);
+    }
+#endif
+}
+
+template <typename T, int DB>
+__global__ __launch_bounds__(256, DB > 2 ? 1 : 2) void attn_dkv_kernel(AttnParams p) {
+#ifdef __HIP_DEVICE_COMPILE__                            // (hipcc drops the launch stub of a template whose body its host pass cannot read)
+    constexpr int ROW = DB > 2 ? 128 : 64, TILE_BYTES = ATTN_TILE * ROW * 2;
+    constexpr float SHIFT = ATTN_P_SHIFT<T>;
+    __shared__ __align__(16) char smem[4 * TILE_BYTES];                 // [buffer][q, do]
+    __shared__ __align__(16) float slse[2][ATTN_TILE], sdelta[2][ATTN_TILE];
+    __shared__ __align__(16) int sdoc[2][ATTN_TILE];
+    const int wave = attn_uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
+    // p.splits: 1 (a workgroup adds up all heads of the group) or G (one head a workgroup, float32 parts that attn_parts_kernel adds in order)
+    const int total = p.B * p.Hk * p.splits * p.row_blocks, per = (total + 7) / 8;
+    const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per || id >= total) return;
+    const int blk = id % p.row_blocks, split = id / p.row_blocks % p.splits, bh = id / p.row_blocks / p.splits, hk = bh % p.Hk, b = bh / p.Hk;
+    const int g0 = p.splits > 1 ? split : 0, g1 = p.splits > 1 ? split + 1 : p.G;
+    const int n = attn_keys(p, b), prefix = p.prefix ? p.prefix[b] : 0, k0 = blk * 128, off = n - p.Lq;
+    const int j = k0 + 32 * wave + l31;
+    const int kdoc = p.kdoc && j < p.Lk ? p.kdoc[b * p.kdoc_stride + j] : 0;
+    const bool key_ok = j < n && kdoc >= 0;
+    // first query that sees key x
+    auto first_query = [&](int x) { return !p.causal || x < prefix ? 0 : max(x - off, 0); };
+    const int qmin = key_ok ? first_query(j) : 0x7fffffff;
+    const int last_key = min(k0 + 32 * wave + 31, n - 1);
+    const int wave_first = first_query(k0 + 32 * wave), wave_full = first_query(last_key);
+    const bool wave_on = k0 + 32 * wave < n;
+    int dlo = 0, dhi = 0;
+    if (p.kdoc) {
+        const int2* r = p.ktiles + (int64_t)b * p.nkt + 2 * blk;
+        const int2 r0 = r[0], r1 = 2 * blk + 1 < p.nkt ? r[1] : r[0];
+        dlo = min(r0.x, r1.x);
+        dhi = max(r0.y, r1.y);
+    }
+    const int2* ranges = p.kdoc ? p.qtiles + (int64_t)b * p.nqt : nullptr;
+    const int t_first = first_query(k0) / ATTN_TILE, t_end = k0 < n ? p.nqt : 0;
+    AttnTiles tiles;
+    int g = g0;
+    tiles.start(ranges, t_first, t_end, max(dlo, 0), dhi);
+    auto next = [&](int& gn) {
+        int t = tiles.next(lane);
+        while (t < 0 && gn + 1 < g1) {
+            ++gn;
+            tiles.start(ranges, t_first, t_end, max(dlo, 0), dhi);
+            t = tiles.next(lane);
+        }
+        return t;
+    };
+    typename AttnVec<T>::x8 kf[2 * DB], vf[2 * DB];
+    const T* k = j < n ? (const T*)p.k + b * p.ks[0] + j * p.ks[1] + hk * p.ks[2] : nullptr;
+    const T* v = j < n ? (const T*)p.v + b * p.vs[0] + j * p.vs[1] + hk * p.vs[2] : nullptr;
+#pragma unroll
+    for (int c = 0; c < 2 * DB; ++c) {
+        kf[c] = attn_lane_frag<T>(k, 2 * c + half, p.D);
+        vf[c] = attn_lane_frag<T>(v, 2 * c + half, p.D);
+    }
+    AttnStage<ROW, ATTN_TILE, 4> sq, sd;
+    sq.setup(wave, lane, p.qs[1], p.D);
+    sd.setup(wave, lane, p.ds[1], p.D);
+    const int ds_exp = attn_ds_scale(p, lane);
+    const float ds_by = ldexpf(1.f, ds_exp - (int)SHIFT);
+    auto stage = [&](int t, int gt, int buf) {
+        const int h = hk * p.G + gt, i0 = t * ATTN_TILE;
+        char* at = smem + buf * 2 * TILE_BYTES;
+        sq.issue((const T*)p.q + b * p.qs[0] + i0 * p.qs[1] + h * p.qs[2], p.Lq - i0, p.qs[1], p.D, at, wave);
+        sd.issue((const T*)p.dout + b * p.ds[0] + i0 * p.ds[1] + h * p.ds[2], p.Lq - i0, p.ds[1], p.D, at + TILE_BYTES, wave);
+        const int i = i0 + lane;
+        const int64_t stat = ((int64_t)b * p.Hq + h) * p.Lq + i;
+        if (wave == 0) slse[buf][lane] = i < p.Lq ? attn_lse2(p.lse[stat]) - SHIFT : INFINITY;      // (queries behind the last: every weight 0)
+        if (wave == 1) sdelta[buf][lane] = i < p.Lq ? p.delta[stat] : 0.f;
+        if (wave == 2 && p.kdoc) sdoc[buf][lane] = i < p.Lq ? p.qdoc[b * p.qdoc_stride + i] : -1;
+    };
+    f32x16 dk[DB] = {}, dv[DB] = {};
+    int t = next(g);
+    if (t >= 0) stage(t, g, 0);
+    for (int buf = 0; t >= 0; buf ^= 1) {
+        attn_sync();
+        int g_next = g;
+        const int t_next = next(g_next);
+        if (t_next >= 0) stage(t_next, g_next, buf ^ 1);
+        const int i0 = t * ATTN_TILE;
+        if (wave_on && i0 + ATTN_TILE - 1 >= wave_first) {
+            const char* qt = smem + buf * 2 * TILE_BYTES;
+            const char* dt = qt + TILE_BYTES;
+            const AttnScore f(p, hk * p.G + g);
+            bool full = i0 >= wave_full;
+            if (p.kdoc) {
+                const int2 r = ranges[t];
+                full = full && dlo == dhi && r.x == dlo && r.y == dlo;
+            }
+#pragma unroll
+            for (int qb = 0; qb < 2; ++qb) {
+                f32x16 S = {}, dP = {};
+#pragma unroll
+                for (int c = 0; c < 2 * DB; ++c) {
+                    S = attn_mfma(attn_row_frag<T, ROW>(qt, 32 * qb + l31, 2 * c + half), kf[c], S);
+                    dP = attn_mfma(attn_row_frag<T, ROW>(dt, 32 * qb + l31, 2 * c + half), vf[c], dP);
+                }
+                const int ib = 32 * qb + 4 * half;
+                attn_ds_step(S, dP, f, ds_by, full, [&](int r) { return slse[buf][ib + 8 * (r >> 2) + (r & 3)]; },
+                             [&](int r) { return sdelta[buf][ib + 8 * (r >> 2) + (r & 3)]; },
+                             [&](int r) {
+                                 const int i = ib + 8 * (r >> 2) + (r & 3);
+                                 return i0 + i >= qmin && (!p.kdoc || sdoc[buf][i] == kdoc);
+                             },
+                             [&](int r) { return i0 + ib + 8 * (r >> 2) + (r & 3) + off - j; });
+                typename AttnVec<T>::x8 w[2], d[2];
+                attn_pack<T>(S, w);
+                attn_pack<T>(dP, d);
+#pragma unroll
+                for (int db = 0; db < DB; ++db)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        dv[db] = attn_mfma(attn_col_frag<T, ROW>(dt, 32 * qb + 16 * c, db, lane), w[c], dv[db]);
+                        dk[db] = attn_mfma(attn_col_frag<T, ROW>(qt, 32 * qb + 16 * c, db, lane), d[c], dk[db]);
+                    }
+            }
+        }
+        t = t_next;
+        g = g_next;
+    }
+    bool nan = false;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) nan = nan || dk[db][r] != dk[db][r] || dv[db][r] != dv[db][r];
+    uint64_t redo = __ballot(nan && key_ok);
+    redo = (redo | (redo >> 32)) & 0xffffffffu;
+    const float k_by = ldexpf(p.scale, -ds_exp), v_by = ldexpf(1.f, -(int)SHIFT);
+    const bool store = j < p.Lk && !((redo >> l31) & 1);
+    if (!key_ok)                                                        // keys that nobody sees (their lanes held something else)
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dk[db][r] = dv[db][r] = 0.f;
+    const int64_t row = ((int64_t)b * p.Lk + j) * p.Hk + hk, all = (int64_t)p.B * p.Lk * p.Hk;
+    if (p.splits > 1) {
+        float* pk = p.part + (2 * split * all + row) * p.D;
+        float* pv = p.part + ((2 * split + 1) * all + row) * p.D;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+                const int d = 32 * db + 8 * a + 4 * half;
+                if (store && d < p.D) {
+                    *reinterpret_cast<float4*>(pk + d) = make_float4(dk[db][4 * a] * k_by, dk[db][4 * a + 1] * k_by, dk[db][4 * a + 2] * k_by, dk[db][4 * a + 3] * k_by);
+                    *reinterpret_cast<float4*>(pv + d) = make_float4(dv[db][4 * a] * v_by, dv[db][4 * a + 1] * v_by, dv[db][4 * a + 2] * v_by, dv[db][4 * a + 3] * v_by);
+                }
+            }
+    } else {
+        attn_store_row<T, DB>((T*)p.dk + row * p.D, dk, k_by, half, p.D, store);
+        attn_store_row<T, DB>((T*)p.dv + row * p.D, dv, v_by, half, p.D, store);
+    }
+    while (redo) {
+        const int e = __builtin_ctzll(redo);
+        redo &= redo - 1;
+        const int je = k0 + 32 * wave + e, doce = __shfl(kdoc, e);
+        const T* ke = (const T*)p.k + b * p.ks[0] + je * p.ks[1] + hk * p.ks[2];
+        const T* ve = (const T*)p.v + b * p.vs[0] + je * p.vs[1] + hk * p.vs[2];
+        float xk[2] = {0.f, 0.f}, xv[2] = {0.f, 0.f};
+        for (int ge = g0; ge < g1; ++ge) {
+            const int h = hk * p.G + ge;
+            const AttnScore f(p, h);
+            const T* q = (const T*)p.q + b * p.qs[0] + h * p.qs[2];
+            const T* dout = (const T*)p.dout + b * p.ds[0] + h * p.ds[2];
+            const int64_t stat = ((int64_t)b * p.Hq + h) * p.Lq;
+            for (int i0 = first_query(je); i0 < p.Lq; i0 += 64) {
+                const int i = i0 + lane;
+                const bool see = i < p.Lq && (!p.kdoc || p.qdoc[b * p.qdoc_stride + i] == doce);
+                float w = 0.f, ds = 0.f;
+                if (see) attn_pair<T>(p, f, q + i * p.qs[1], ke, ve, dout + i * p.ds[1], attn_lse2(p.lse[stat + i]), p.delta[stat + i], i + off - je, w, ds);
+                uint64_t todo = __ballot(see);
+                while (todo) {
+                    const int s = __builtin_ctzll(todo);
+                    todo &= todo - 1;
+                    const float we = __shfl(w, s), de = __shfl(ds, s);
+                    const T* qi = q + (int64_t)(i0 + s) * p.qs[1];
+                    const T* di = dout + (int64_t)(i0 + s) * p.ds[1];
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+                        if (lane + 64 * c < p.D) {
+                            xk[c] += de * (float)qi[lane + 64 * c];
+                            xv[c] += we * (float)di[lane + 64 * c];
+                        }
+                }
+            }
+        }
+        const int64_t re = ((int64_t)b * p.Lk + je) * p.Hk + hk;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int d = lane + 64 * c;
+            if (d >= p.D) continue;
+            if (p.splits > 1) {
+                p.part[(2 * split * all + re) * p.D + d] = xk[c] * p.scale;
+                p.part[((2 * split + 1) * all + re) * p.D + d] = xv[c];
+            } else {
+                ((T*)p.dk)[re * p.D + d] = (T)(xk[c] * p.scale);
+                ((T*)p.dv)[re * p.D + d] = (T)xv[c];
+            }
+        }
+    }
+#endif
+}
+
+// part [split][dk, dv][elements] -> dk, dv; eight elements a thread
+template <typename T>
+__global__ __launch_bounds__(256) void attn_parts_kernel(AttnParams p) {
+    const int64_t all = (int64_t)p.B * p.Lk * p.Hk * p.D;
+    const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+    if (at >= all) return;
+    float x[8] = {};
+    for (int s = 0; s < p.splits; ++s) {
+        const float4* a = reinterpret_cast<const float4*>(p.part + (2 * s + blockIdx.y) * all + at);
+        const float4 u = a[0], w = a[1];
+        x[0] += u.x; x[1] += u.y; x[2] += u.z; x[3] += u.w;
+        x[4] += w.x; x[5] += w.y; x[6] += w.z; x[7] += w.w;
+    }
+    typename AttnVec<T>::x8 o;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = (T)x[e];
+    *reinterpret_cast<typename AttnVec<T>::x8*>((T*)(blockIdx.y ? p.dv : p.dk) + at) = o;
+}
+
+template <typename T, int DB>
+static void attn_bwd_launch(AttnParams& p, int splits, hipStream_t stream) {
+    const int prep = p.maxima ? ATTN_MAXIMA : (int)(cdiv64((int64_t)p.B * p.Lq * p.Hq, 16) < 2048 ? cdiv64((int64_t)p.B * p.Lq * p.Hq, 16) : 2048);
+    hipLaunchKernelGGL((attn_prep_kernel<T>), dim3(prep, p.maxima ? 2 : 1), dim3(256), 0, stream, p);
+    if (p.dq) {
+        p.splits = 1;
+        p.row_blocks = cdiv(p.Lq, 128);
+        hipLaunchKernelGGL((attn_dq_kernel<T, DB>), dim3(8 * cdiv(p.B * p.Hq * p.row_blocks, 8)), dim3(256), 0, stream, p);
+    }
+    if (p.dk && p.Lk > 0) {
+        p.splits = splits;
+        p.row_blocks = cdiv(p.Lk, 128);
+        hipLaunchKernelGGL((attn_dkv_kernel<T, DB>), dim3(8 * cdiv(p.B * p.Hk * p.splits * p.row_blocks, 8)), dim3(256), 0, stream, p);
+        if (splits > 1)
+            hipLaunchKernelGGL((attn_parts_kernel<T>), dim3((unsigned)cdiv64((int64_t)p.B * p.Lk * p.Hk * p.D, 2048), 2), dim3(256), 0, stream, p);
+    }
+}
+
+// floats behind the document ranges: delta, maxima (float16), parts of the heads
+static int64_t attn_bwd_floats(const AttnParams& p, int dtype, int& splits, int64_t& maxima_at, int64_t& parts_at) {
+    const int64_t ranges = (attn_range_floats(p) + 3) / 4 * 4, delta = ((int64_t)p.B * p.Hq * p.Lq + 3) / 4 * 4;
+    maxima_at = ranges + delta;
+    parts_at = maxima_at + (dtype == N3D_F16 ? 2 * ATTN_MAXIMA : 0);
+    // one head of a group a workgroup where whole groups would leave workgroups for less than two rounds of the chip
+    splits = p.G > 1 && (int64_t)p.B * p.Hk * cdiv(p.Lk, 128) < 1024 ? p.G : 1;
+    return parts_at + (splits > 1 ? 2 * (int64_t)splits * p.B * p.Lk * p.Hk * p.D : 0);
+}
+
+extern "C" int64_t n3d_attention_bwd_workspace(const n3d_attention_desc* d) {
+    AttnParams p;
+    const char* bad = attn_params(d, p);
+    N3D_CHECK(!bad, "attention_bwd: %s", bad);
+    int splits;
+    int64_t m, s;
+    return 4 * attn_bwd_floats(p, d->dtype, splits, m, s);
+}
+
+extern "C" int n3d_attention_bwd(const n3d_attention_desc* d, n3d_stream_t stream_) {
+    hipStream_t stream = (hipStream_t)stream_;
+    AttnParams p;
+    const char* bad = attn_params(d, p);
+    N3D_CHECK(!bad, "attention_bwd: %s", bad);
+    N3D_CHECK(p.B > 0 && p.Lq > 0, "attention_bwd: no queries");
+    N3D_CHECK(d->lse && d->dout && (!d->dk) == (!d->dv) && (d->dq || d->dk || p.Lk == 0), "attention_bwd: null tensor");
+    for (int i = 0; i < 3; ++i)
+        N3D_CHECK(d->dout_strides[i] % 8 == 0 && d->dout_strides[i] >= 0 && (i != 1 || d->dout_strides[i] <= (1 << 23)), "attention_bwd: strides must be multiples of 8 elements, of tokens 2^23 at most");
+    N3D_CHECK(((uintptr_t)d->dout | (uintptr_t)d->dq | (uintptr_t)d->dk | (uintptr_t)d->dv) % 16 == 0, "attention_bwd: tensors must be 16-byte aligned");
+    int splits;
+    int64_t maxima_at, parts_at;
+    const int64_t need = 4 * attn_bwd_floats(p, d->dtype, splits, maxima_at, parts_at);
+    N3D_CHECK(d->workspace && d->workspace_bytes >= need && (uintptr_t)d->workspace % 16 == 0, "attention_bwd: a workspace of %lld bytes is needed (16-byte aligned)", (long long)need);
+    float* ws = (float*)d->workspace;
+    p.dout = d->dout; p.dq = d->dq; p.dk = d->dk; p.dv = d->dv;
+    p.delta = ws + (attn_range_floats(p) + 3) / 4 * 4;
+    p.maxima = d->dtype == N3D_F16 ? ws + maxima_at : nullptr;
+    p.part = ws + parts_at;
+    const double pairs = (double)p.B * p.Hq * p.Lq * p.Lk * p.D;
+    N3dProfScope prof(N3D_K_ATTENTION, stream, 10.0 * pairs, 8.0 * ((double)p.B * p.Lq * p.Hq * p.D + (double)p.B * p.Lk * p.Hk * p.D));
+    attn_ranges(p, ws, stream);
+    auto go = [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        switch (cdiv(p.D, 32)) {
+            case 1: attn_bwd_launch<T, 1>(p, splits, stream); break;
+            case 2: attn_bwd_launch<T, 2>(p, splits, stream); break;
+            case 3: attn_bwd_launch<T, 3>(p, splits, stream); break;
+            default: attn_bwd_launch<T, 4>(p, splits, stream); break;
+        }
+    };
+    if (d->dtype == N3D_F16) go((_Float16*)nullptr);
+    else go((__bf16*)nullptr);
+    N3D_LAUNCH_CHECK();
+    return 0;
+}

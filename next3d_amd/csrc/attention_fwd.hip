@@ -1,0 +1,455 @@
+// Attention, forward (attention.h): o = softmax(t) v over the visible keys, and the logarithm of the softmax's sum.
+// attn_fwd_kernel: a workgroup owns 128 queries of one head, a wave 32 of them; tiles of 64 keys pass through the LDS once, double-buffered by LDS-DMA, with
+//   the running maximum and sum of every query in its lane.  The accumulators are rescaled only when a maximum grows by more than 2^8 since they were last.
+// attn_token_kernel: few queries over many keys.  The rows of a wave are (query, head) pairs that share a key head, so a key is read once for all of
+//   them; every wave walks its own tiles of 32 keys through its own LDS (no barriers), the keys are split over `splits` workgroups, and
+//   attn_combine_kernel joins their (maximum, sum, accumulator).
+#include "attention.h"
+
+// lowest and highest document of every ATTN_TILE tokens
+__global__ __launch_bounds__(256) void attn_ranges_kernel(const int* __restrict__ doc, int64_t stride, int L, int tiles, int2* __restrict__ out) {
+    const int t = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, b = blockIdx.y;
+    if (t >= tiles) return;
+    const int j = t * ATTN_TILE + lane;
+    const int d = doc[b * stride + (j < L ? j : L - 1)];
+    int lo = d, hi = d;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        lo = min(lo, __shfl_xor(lo, o));
+        hi = max(hi, __shfl_xor(hi, o));
+    }
+    if (lane == 0) out[(int64_t)b * tiles + t] = make_int2(lo, hi);
+}
+
+// accumulator [DB] of one row += sum over visible keys j in [k0, k1) of exp2(u - m) v_j, one wave, plain arithmetic: acc[e] belongs to channel lane + 64 e
+template <typename T>
+__device__ void attn_exact_row(const AttnParams& p, int b, int i, int h, int k0, int k1, float m, int lane, float (&acc)[2]) {
+    const AttnScore f(p, h);
+    const int hk = h / p.G, n = attn_keys(p, b), lim = attn_limit(p, i, n, p.prefix ? p.prefix[b] : 0);
+    const int qdoc = p.kdoc ? p.qdoc[b * p.qdoc_stride + i] : 0;
+    const T* q = (const T*)p.q + b * p.qs[0] + i * p.qs[1] + h * p.qs[2];
+    const T* k = (const T*)p.k + b * p.ks[0] + hk * p.ks[2];
+    const T* v = (const T*)p.v + b * p.vs[0] + hk * p.vs[2];
+    acc[0] = acc[1] = 0.f;
+    const int end = min(k1, lim + 1);
+    for (int j0 = k0; j0 < end; j0 += 64) {
+        const int j = j0 + lane;
+        const bool see = j < end && attn_visible(p, b, j, lim, qdoc);
+        float w = 0.f;
+        if (see) w = __builtin_amdgcn_exp2f(attn_score(f, attn_dot<T>(q, k + j * p.ks[1], p.D), i + n - p.Lq - j) - m);
+        uint64_t todo = __ballot(see);
+        while (todo) {
+            const int e = __builtin_ctzll(todo);
+            todo &= todo - 1;
+            const float we = __shfl(w, e);
+            const T* vj = v + (int64_t)(j0 + e) * p.vs[1];
+            if (lane < p.D) acc[0] += we * (float)vj[lane];
+            if (lane + 64 < p.D) acc[1] += we * (float)vj[lane + 64];
+        }
+    }
+}
+
+// one wave's softmax step over the 32 queries of its lanes: S (raw products of KB blocks of 32 keys) -> P as second operands; rescales acc, sum and m
+template <typename T, int KB, int DB>
+__device__ __forceinline__ void attn_softmax_step(f32x16 (&S)[KB], typename AttnVec<T>::x8 (&P)[KB][2], f32x16 (&acc)[DB], float& m, float& sum,
+                                                  const AttnScore& f, bool full, int lim, int at, int j0, int half, const int* docs, int qdoc) {
+    float mul = f.mul;
+    if (f.cap_out > 0.f || f.slope != 0.f || !(mul > 0.f)) {         // (uniform) the score itself instead of a multiple of it
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) S[kb][r] = f.cap_out > 0.f ? f.cap_out * f.tanh_part(S[kb][r]) : S[kb][r] * f.mul;
+        if (f.slope != 0.f)
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) S[kb][r] -= f.slope * fabsf((float)(at - (j0 + 32 * kb + 8 * (r >> 2) + 4 * half + (r & 3))));
+        mul = 1.f;
+    }
+    if (!full) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int at_tile = 32 * kb + 8 * (r >> 2) + 4 * half + (r & 3);
+                bool see = j0 + at_tile <= lim;
+                if (docs) see = see && docs[at_tile] == qdoc;
+                S[kb][r] = see ? S[kb][r] : -INFINITY;
+            }
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, S[kb][r]);
+    top = attn_half_max(top) * mul;                                     // (mul > 0; -inf stays -inf)
+    if (__ballot(top > m + 8.f || (m == -INFINITY && top > m))) {
+        const float now = fmaxf(m, top);
+        const float shrink = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - now);
+        m = now;
+        sum *= shrink;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[db][r] *= shrink;
+    }
+    const float sub = m == -INFINITY ? 0.f : m;
+    float add = 0.f;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            S[kb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[kb][r], mul, -sub));
+            add += S[kb][r];
+        }
+        // weights to 16 bits (half a step of the inputs' own type, each on its own: their sum above is of the unrounded ones)
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) P[kb][c][e] = (T)S[kb][8 * c + e];
+    }
+    sum += add;
+}
+
+template <typename T, int DB>
+__global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnParams p) {
+#ifdef __HIP_DEVICE_COMPILE__                            // (hipcc drops the launch stub of a template whose body its host pass cannot read)
+    constexpr int ROW = DB > 2 ? 128 : 64, TILE_BYTES = ATTN_TILE * ROW * 2;
+    __shared__ __align__(16) char smem[4 * TILE_BYTES];                 // [buffer][k, v]
+    __shared__ int sdoc[2][ATTN_TILE];
+    const int wave = attn_uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
+    // consecutive workgroups go to different XCDs: give each XCD whole heads, so that its L2 serves their keys, and the longest rows first
+    const int total = p.B * p.Hq * p.row_blocks, per = (total + 7) / 8;
+    const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per || id >= total) return;
+    const int blk = p.row_blocks - 1 - id % p.row_blocks, bh = id / p.row_blocks, h = bh % p.Hq, b = bh / p.Hq, hk = h / p.G;
+    const int n = attn_keys(p, b), prefix = p.prefix ? p.prefix[b] : 0, q0 = blk * 128;
+    const int i = q0 + 32 * wave + l31;
+    const bool row_ok = i < p.Lq;
+    const int qdoc = p.kdoc && row_ok ? p.qdoc[b * p.qdoc_stride + i] : 0;
+    const int lim = !row_ok || qdoc < 0 ? -1 : attn_limit(p, i, n, prefix);
+    const int lim_first = attn_limit(p, q0 + 32 * wave, n, prefix), lim_last = attn_limit(p, min(q0 + 32 * wave + 31, p.Lq - 1), n, prefix);
+    const int key_end = attn_limit(p, min(q0 + 127, p.Lq - 1), n, prefix) + 1;
+    int dlo = 0, dhi = 0;
+    if (p.kdoc) {                                                       // documents of this workgroup's queries: two ranges of ATTN_TILE queries
+        const int2* r = p.qtiles + (int64_t)b * p.nqt + 2 * blk;
+        const int2 r0 = r[0], r1 = 2 * blk + 1 < p.nqt ? r[1] : r[0];
+        dlo = min(r0.x, r1.x);
+        dhi = max(r0.y, r1.y);
+    }
+    AttnTiles tiles;
+    tiles.start(p.kdoc ? p.ktiles + (int64_t)b * p.nkt : nullptr, 0, (key_end + ATTN_TILE - 1) / ATTN_TILE, max(dlo, 0), dhi);
+
+    typename AttnVec<T>::x8 qf[2 * DB];
+    const T* q = row_ok ? (const T*)p.q + b * p.qs[0] + i * p.qs[1] + h * p.qs[2] : nullptr;
+#pragma unroll
+    for (int c = 0; c < 2 * DB; ++c) qf[c] = attn_lane_frag<T>(q, 2 * c + half, p.D);
+    const T* k = (const T*)p.k + b * p.ks[0] + hk * p.ks[2];
+    const T* v = (const T*)p.v + b * p.vs[0] + hk * p.vs[2];
+    const int* kdoc = p.kdoc ? p.kdoc + b * p.kdoc_stride : nullptr;
+    const AttnScore f(p, h);
+    AttnStage<ROW, ATTN_TILE, 4> sk, sv;
+    sk.setup(wave, lane, p.ks[1], p.D);
+    sv.setup(wave, lane, p.vs[1], p.D);
+
+    f32x16 acc[DB] = {};
+    float m = -INFINITY, sum = 0.f;
+    auto stage = [&](int t, int buf) {
+        char* at = smem + buf * 2 * TILE_BYTES;
+        sk.issue(k + (int64_t)t * ATTN_TILE * p.ks[1], n - t * ATTN_TILE, p.ks[1], p.D, at, wave);
+        sv.issue(v + (int64_t)t * ATTN_TILE * p.vs[1], n - t * ATTN_TILE, p.vs[1], p.D, at + TILE_BYTES, wave);
+        if (kdoc && wave == 0) sdoc[buf][lane] = kdoc[min(t * ATTN_TILE + lane, p.Lk - 1)];
+    };
+    int t = tiles.next(lane);
+    if (t >= 0) stage(t, 0);
+    for (int buf = 0; t >= 0; buf ^= 1) {
+        attn_sync();
+        const int t_next = tiles.next(lane);
+        if (t_next >= 0) stage(t_next, buf ^ 1);
+        const int j0 = t * ATTN_TILE;
+        if (j0 <= lim_last) {
+            const char* kt = smem + buf * 2 * TILE_BYTES;
+            const char* vt = kt + TILE_BYTES;
+            f32x16 S[2] = {};
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int c = 0; c < 2 * DB; ++c) S[kb] = attn_mfma(attn_row_frag<T, ROW>(kt, 32 * kb + l31, 2 * c + half), qf[c], S[kb]);
+            bool full = j0 + ATTN_TILE - 1 <= lim_first;
+            if (kdoc) {
+                const int2 r = p.ktiles[(int64_t)b * p.nkt + t];
+                full = full && dlo == dhi && r.x == dlo && r.y == dlo;
+            }
+            typename AttnVec<T>::x8 P[2][2];
+            attn_softmax_step<T, 2, DB>(S, P, acc, m, sum, f, full, lim, i + n - p.Lq, j0, half, kdoc ? sdoc[buf] : nullptr, qdoc);
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) acc[db] = attn_mfma(attn_col_frag<T, ROW>(vt, 32 * kb + 16 * c, db, lane), P[kb][c], acc[db]);
+        }
+        t = t_next;
+    }
+    sum = attn_half_sum(sum);
+    const float by = sum == 0.f ? 0.f : 1.f / sum;
+    bool nan = false;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) nan = nan || acc[db][r] != acc[db][r];
+    uint64_t redo = __ballot(nan && sum == sum && row_ok);
+    redo = (redo | (redo >> 32)) & 0xffffffffu;
+    T* out = (T*)p.out + ((int64_t)(b * (int64_t)p.Lq + i) * p.Hq + h) * p.D;
+    attn_store_row<T, DB>(out, acc, by, half, p.D, row_ok && !((redo >> l31) & 1));
+    if (p.lse && row_ok && half == 0) p.lse[((int64_t)b * p.Hq + h) * p.Lq + i] = sum == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(sum)) * ATTN_LN2;
+    while (redo) {
+        const int e = __builtin_ctzll(redo);
+        redo &= redo - 1;
+        const int ie = q0 + 32 * wave + e;
+        const float me = __shfl(m, e), bye = __shfl(by, e);
+        float row[2];
+        attn_exact_row<T>(p, b, ie, h, 0, n, me, lane, row);
+        T* o = (T*)p.out + ((int64_t)(b * (int64_t)p.Lq + ie) * p.Hq + h) * p.D;
+        if (lane < p.D) o[lane] = (T)(row[0] * bye);
+        if (lane + 64 < p.D) o[lane + 64] = (T)(row[1] * bye);
+    }
+#endif
+}
+
+// ---- few queries: rows r = query * G + head of the group, 32 a workgroup
+template <typename T, int DB>
+__global__ __launch_bounds__(256) void attn_token_kernel(AttnParams p) {
+#ifdef __HIP_DEVICE_COMPILE__                            // (hipcc drops the launch stub of a template whose body its host pass cannot read)
+    constexpr int ROW = DB > 2 ? 128 : 64, KEYS = 32, TILE_BYTES = KEYS * ROW * 2, WAVES = 4;
+    extern __shared__ __align__(16) char smem[];                        // [wave][buffer][k, v], then the waves' results
+    __shared__ float sm[WAVES][32], ssum[WAVES][32];
+    __shared__ int sdoc[WAVES][2][KEYS];
+    const int wave = attn_uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
+    const int split = blockIdx.x % p.splits, blk = blockIdx.x / p.splits % p.row_blocks, bh = blockIdx.x / (p.splits * p.row_blocks);
+    const int hk = bh % p.Hk, b = bh / p.Hk, rows = p.Lq * p.G;
+    const int n = attn_keys(p, b), prefix = p.prefix ? p.prefix[b] : 0;
+    const int r = blk * 32 + l31, i = r / p.G, h = hk * p.G + r - i * p.G;
+    const bool row_ok = r < rows;
+    const int qdoc = p.kdoc && row_ok ? p.qdoc[b * p.qdoc_stride + i] : 0;
+    const int lim = !row_ok || qdoc < 0 ? -1 : attn_limit(p, i, n, prefix);
+    const int lim_first = attn_limit(p, blk * 32 / p.G, n, prefix), lim_last = attn_limit(p, min(blk * 32 + 31, rows - 1) / p.G, n, prefix);
+    // this workgroup's share of the keys, in whole rounds of the four waves' tiles
+    const int rounds = (lim_last + WAVES * KEYS) / (WAVES * KEYS), per = (rounds + p.splits - 1) / p.splits;
+    const int k0 = split * per * WAVES * KEYS, k1 = min(lim_last + 1, (split + 1) * per * WAVES * KEYS);
+    typename AttnVec<T>::x8 qf[2 * DB];
+    const T* q = row_ok ? (const T*)p.q + b * p.qs[0] + i * p.qs[1] + h * p.qs[2] : nullptr;
+#pragma unroll
+    for (int c = 0; c < 2 * DB; ++c) qf[c] = attn_lane_frag<T>(q, 2 * c + half, p.D);
+    const T* k = (const T*)p.k + b * p.ks[0] + hk * p.ks[2];
+    const T* v = (const T*)p.v + b * p.vs[0] + hk * p.vs[2];
+    const int* kdoc = p.kdoc ? p.kdoc + b * p.kdoc_stride : nullptr;
+    AttnScore f(p, row_ok ? h : hk * p.G);
+    const bool same_slope = !p.slopes;
+    AttnStage<ROW, KEYS, 1> sk, sv;
+    sk.setup(0, lane, p.ks[1], p.D);
+    sv.setup(0, lane, p.vs[1], p.D);
+    char* mine = smem + wave * 4 * TILE_BYTES;
+    auto stage = [&](int j0, int buf) {
+        sk.issue(k + (int64_t)j0 * p.ks[1], n - j0, p.ks[1], p.D, mine + buf * 2 * TILE_BYTES, 0);
+        sv.issue(v + (int64_t)j0 * p.vs[1], n - j0, p.vs[1], p.D, mine + buf * 2 * TILE_BYTES + TILE_BYTES, 0);
+        if (kdoc && lane < KEYS) sdoc[wave][buf][lane] = kdoc[min(j0 + lane, p.Lk - 1)];
+    };
+    f32x16 acc[DB] = {};
+    float m = -INFINITY, sum = 0.f;
+    int j0 = k0 + wave * KEYS;
+    if (j0 < k1) stage(j0, 0);
+    for (int buf = 0; j0 < k1; buf ^= 1, j0 += WAVES * KEYS) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");    // the wave's own pieces: no other wave touches this LDS
+        if (j0 + WAVES * KEYS < k1) stage(j0 + WAVES * KEYS, buf ^ 1);
+        const char* kt = mine + buf * 2 * TILE_BYTES;
+        f32x16 S[1] = {};
+#pragma unroll
+        for (int c = 0; c < 2 * DB; ++c) S[0] = attn_mfma(attn_row_frag<T, ROW>(kt, l31, 2 * c + half), qf[c], S[0]);
+        const bool full = j0 + KEYS - 1 <= lim_first && !kdoc;
+        typename AttnVec<T>::x8 P[1][2];
+        attn_softmax_step<T, 1, DB>(S, P, acc, m, sum, f, full, lim, i + n - p.Lq, j0, half, kdoc ? sdoc[wave][buf] : nullptr, qdoc);
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) acc[db] = attn_mfma(attn_col_frag<T, ROW>(kt + TILE_BYTES, 16 * c, db, lane), P[0][c], acc[db]);
+    }
+    (void)same_slope;
+    // join the four waves: common maximum, then the accumulators through the LDS, one [32 rows][32 * DB + 1] float image a wave
+    constexpr int PITCH = 32 * DB + 1;
+    sum = attn_half_sum(sum);
+    if (half == 0) {
+        sm[wave][l31] = m;
+        ssum[wave][l31] = sum;
+    }
+    __syncthreads();                                                    // (also: every wave is done with its tiles)
+    float top = -INFINITY, all = 0.f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) top = fmaxf(top, sm[w][l31]);
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) all += ssum[w][l31] == 0.f ? 0.f : ssum[w][l31] * __builtin_amdgcn_exp2f(sm[w][l31] - top);
+    const float shrink = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+    float* img = reinterpret_cast<float*>(smem) + wave * 32 * PITCH;
+    bool nan = false;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int rr = 0; rr < 16; ++rr) {
+            const float x = m == -INFINITY ? 0.f : acc[db][rr] * shrink;
+            nan = nan || x != x;
+            img[l31 * PITCH + 32 * db + 8 * (rr >> 2) + 4 * half + (rr & 3)] = x;
+        }
+    __shared__ uint32_t bad[WAVES];
+    uint64_t any = __ballot(nan && all == all && row_ok);
+    if (lane == 0) bad[wave] = (uint32_t)(any | (any >> 32));
+    __syncthreads();
+    const uint32_t redo = bad[0] | bad[1] | bad[2] | bad[3];
+    const bool direct = p.splits == 1;
+    for (int e = wave * 8; e < wave * 8 + 8; ++e) {                     // eight rows a wave
+        const int re = blk * 32 + e;
+        if (re >= rows) break;
+        const int ie = re / p.G, he = hk * p.G + re - ie * p.G;
+        const float te = __shfl(top, e), ae = __shfl(all, e);
+        float x[2];
+        if ((redo >> e) & 1) {
+            attn_exact_row<T>(p, b, ie, he, k0, k1, te, lane, x);
+        } else {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                x[c] = 0.f;
+                if (lane + 64 * c < 32 * DB)
+#pragma unroll
+                    for (int w = 0; w < WAVES; ++w) x[c] += reinterpret_cast<float*>(smem)[(w * 32 + e) * PITCH + lane + 64 * c];
+            }
+        }
+        if (direct) {
+            T* o = (T*)p.out + ((int64_t)(b * (int64_t)p.Lq + ie) * p.Hq + he) * p.D;
+            const float by = ae == 0.f ? 0.f : 1.f / ae;
+            if (lane < p.D) o[lane] = (T)(x[0] * by);
+            if (lane + 64 < p.D) o[lane + 64] = (T)(x[1] * by);
+            if (p.lse && lane == 0) p.lse[((int64_t)b * p.Hq + he) * p.Lq + ie] = ae == 0.f ? -INFINITY : (te + __builtin_amdgcn_logf(ae)) * ATTN_LN2;
+        } else {
+            const int64_t at = (int64_t)(bh * (int64_t)rows + re) * p.splits + split;
+            if (lane < p.D) p.part[at * p.D + lane] = x[0];
+            if (lane + 64 < p.D) p.part[at * p.D + lane + 64] = x[1];
+            if (lane == 0) {
+                p.part[p.part_ml + 2 * at] = te;
+                p.part[p.part_ml + 2 * at + 1] = ae;
+            }
+        }
+    }
+#endif
+}
+
+// one wave a row: the splits' accumulators, in order
+template <typename T>
+__global__ __launch_bounds__(256) void attn_combine_kernel(AttnParams p) {
+    const int rows = p.Lq * p.G, lane = threadIdx.x & 63;
+    const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (w >= (int64_t)p.B * p.Hk * rows) return;
+    const int r = (int)(w % rows), bh = (int)(w / rows), hk = bh % p.Hk, b = bh / p.Hk, i = r / p.G, h = hk * p.G + r - i * p.G;
+    const float* ml = p.part + p.part_ml + 2 * w * p.splits;
+    float top = -INFINITY;
+    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, ml[2 * s]);
+    float all = 0.f, x[2] = {0.f, 0.f};
+    for (int s = 0; s < p.splits; ++s) {
+        if (ml[2 * s + 1] == 0.f) continue;                             // nothing visible in this share
+        const float by = __builtin_amdgcn_exp2f(ml[2 * s] - top);
+        all += by * ml[2 * s + 1];
+        const float* a = p.part + (w * p.splits + s) * p.D;
+        if (lane < p.D) x[0] += by * a[lane];
+        if (lane + 64 < p.D) x[1] += by * a[lane + 64];
+    }
+    const float by = all == 0.f ? 0.f : 1.f / all;
+    T* o = (T*)p.out + ((int64_t)(b * (int64_t)p.Lq + i) * p.Hq + h) * p.D;
+    if (lane < p.D) o[lane] = (T)(x[0] * by);
+    if (lane + 64 < p.D) o[lane + 64] = (T)(x[1] * by);
+    if (p.lse && lane == 0) p.lse[((int64_t)b * p.Hq + h) * p.Lq + i] = all == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(all)) * ATTN_LN2;
+}
+
+void attn_ranges(AttnParams& p, void* workspace, hipStream_t stream) {
+    if (!p.kdoc) return;
+    int2* kt = (int2*)workspace;
+    int2* qt = kt + (int64_t)p.B * p.nkt;
+    if (p.nkt) hipLaunchKernelGGL(attn_ranges_kernel, dim3(cdiv(p.nkt, 4), p.B), dim3(256), 0, stream, p.kdoc, p.kdoc_stride, p.Lk, p.nkt, kt);
+    if (p.qdoc == p.kdoc && p.qdoc_stride == p.kdoc_stride && p.Lq == p.Lk) qt = kt;
+    else hipLaunchKernelGGL(attn_ranges_kernel, dim3(cdiv(p.nqt, 4), p.B), dim3(256), 0, stream, p.qdoc, p.qdoc_stride, p.Lq, p.nqt, qt);
+    p.ktiles = kt;
+    p.qtiles = qt;
+}
+
+// The token kernel where its rows (queries x heads of a group) fill two 32-row blocks at most; its keys go to enough workgroups to fill the chip twice.
+static bool attn_token_plan(AttnParams& p) {
+    const int64_t rows = (int64_t)p.Lq * p.G;
+    if (rows > 64) return false;
+    p.row_blocks = (int)cdiv64(rows, 32);
+    const int64_t groups = (int64_t)p.B * p.Hk * p.row_blocks;
+    int64_t s = 512 / groups, most = cdiv64(p.Lk, 256);                 // (256 keys: two rounds of the four waves)
+    if (s > most) s = most;
+    p.splits = s < 1 ? 1 : s > 64 ? 64 : (int)s;
+    return true;
+}
+
+template <typename T, int DB>
+static hipError_t attn_fwd_launch(AttnParams& p, bool token, hipStream_t stream) {
+    if (!token) {
+        p.row_blocks = cdiv(p.Lq, 128);
+        const int total = p.B * p.Hq * p.row_blocks;
+        hipLaunchKernelGGL((attn_fwd_kernel<T, DB>), dim3(8 * cdiv(total, 8)), dim3(256), 0, stream, p);
+        return hipSuccess;
+    }
+    constexpr int lds = 4 * 4 * 32 * (DB > 2 ? 128 : 64) * 2;
+    const hipError_t e = hipFuncSetAttribute((const void*)attn_token_kernel<T, DB>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((attn_token_kernel<T, DB>), dim3(p.B * p.Hk * p.row_blocks * p.splits), dim3(256), lds, stream, p);
+    if (p.splits > 1) hipLaunchKernelGGL((attn_combine_kernel<T>), dim3((unsigned)cdiv64((int64_t)p.B * p.Hk * p.Lq * p.G, 4)), dim3(256), 0, stream, p);
+    return hipSuccess;
+}
+
+static int64_t attn_fwd_floats(AttnParams& p) {
+    int64_t n = attn_range_floats(p);
+    if (attn_token_plan(p) && p.splits > 1) {
+        const int64_t parts = (int64_t)p.B * p.Hk * p.Lq * p.G * p.splits;
+        p.part_ml = parts * p.D;
+        n += parts * (p.D + 2);
+    }
+    return n;
+}
+
+extern "C" int64_t n3d_attention_workspace(const n3d_attention_desc* d) {
+    AttnParams p;
+    const char* bad = attn_params(d, p);
+    N3D_CHECK(!bad, "attention: %s", bad);
+    return attn_fwd_floats(p) * 4;
+}
+
+extern "C" int n3d_attention(const n3d_attention_desc* d, n3d_stream_t stream_) {
+    hipStream_t stream = (hipStream_t)stream_;
+    AttnParams p;
+    const char* bad = attn_params(d, p);
+    N3D_CHECK(!bad, "attention: %s", bad);
+    if (p.B == 0 || p.Lq == 0) return 0;
+    const int64_t need = attn_fwd_floats(p) * 4;
+    N3D_CHECK(need == 0 || (d->workspace && d->workspace_bytes >= need && (uintptr_t)d->workspace % 16 == 0), "attention: a workspace of %lld bytes is needed (16-byte aligned)",
+              (long long)need);
+    const double pairs = (double)p.B * p.Hq * p.Lq * p.Lk * p.D;
+    N3dProfScope prof(N3D_K_ATTENTION, stream, 4.0 * pairs, 4.0 * ((double)p.B * p.Lq * p.Hq * p.D + (double)p.B * p.Lk * p.Hk * p.D));
+    attn_ranges(p, d->workspace, stream);
+    p.part = (float*)d->workspace + attn_range_floats(p);
+    const bool token = attn_token_plan(p);
+    hipError_t e = hipSuccess;
+    auto go = [&](auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        switch (cdiv(p.D, 32)) {
+            case 1: e = attn_fwd_launch<T, 1>(p, token, stream); break;
+            case 2: e = attn_fwd_launch<T, 2>(p, token, stream); break;
+            case 3: e = attn_fwd_launch<T, 3>(p, token, stream); break;
+            default: e = attn_fwd_launch<T, 4>(p, token, stream); break;
+        }
+    };
+    if (d->dtype == N3D_F16) go((_Float16*)nullptr);
+    else go((__bf16*)nullptr);
+    N3D_CHECK(e == hipSuccess, "attention: %s", hipGetErrorString(e));
+    N3D_LAUNCH_CHECK();
+    return 0;
+}

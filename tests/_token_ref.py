@@ -78,3 +78,92 @@ def rotary(x, positions, sections, base, pairing, ladder, inverse=False):
     tol = tol + HALF[dt] * y.abs() + TINY[dt]
     tol[..., rest] = 0                                                                          # channels that pass through: the same bits
     return y, tol
+
+
+# ----------------------------------------------------------------------------------------------------------------------------- attention
+def attention(q, k, v, do=None, scale=None, causal=False, prefix=None, documents=None, key_documents=None, lengths=None, softcap=0.0, slopes=None):
+    """(values, bounds) of out, lse [, dq, dk, dv].  Masked places are left out of every sum (a NaN there reaches nothing).
+
+    Bounds.  A score is a float32 sum of D exact products (D + 2 roundings), a multiplication into base 2 and, with a cap, 1 - 2 / (1 + e^2x), which is off
+    by 2^-22 of the cap; the weight of a score off by e is off by e relatively, plus 2^-21 for the exponential.  Weights, dscores and results are each
+    rounded once to the inputs' type: HALF of themselves, or half of its smallest step.  What falls below 2^-126, the smallest normal number of float32
+    and bfloat16, may become zero: a weight (exp2's result; then its 16-bit form) is off by 2 * 2^-126 more, a dscore by as much times |dP| + |delta|."""
+    flush = 2.0 ** -125
+    dt = q.dtype
+    u, n_q, n_k, d = HALF[dt], q.shape[1], k.shape[1], q.shape[3]
+    group, scale = q.shape[2] // k.shape[2], d ** -0.5 if scale is None else scale
+    step = 2.0 ** -25 if dt == torch.float16 else 0.0                                       # half the smallest step of float16 (bfloat16: 2^-134)
+    if documents is not None and key_documents is None:
+        key_documents = documents
+    heads = lambda t: t.double().transpose(1, 2)                                            # [B, H, L, D]
+    spread = lambda t: heads(t).repeat_interleave(group, dim=1)
+    q_, k_, v_ = heads(q), spread(k), spread(v)
+    b = q.shape[0]
+    n = torch.full((b,), n_k) if lengths is None else lengths.long().clamp(0, n_k)
+    pos = torch.arange(n_q)[None, :, None] + n[:, None, None] - n_q
+    j = torch.arange(n_k)[None, None, :]
+    see = (j < n[:, None, None]).expand(b, n_q, n_k).clone()
+    if causal:
+        see &= (j <= pos) | (j < (prefix.long() if prefix is not None else torch.zeros(b).long())[:, None, None])
+    if documents is not None:
+        see &= (documents[:, :, None] == key_documents[:, None, :]) & (documents[:, :, None] >= 0)
+    see = see[:, None].expand(b, q.shape[2], n_q, n_k)
+    clean = lambda t, keep: torch.where(keep, t, torch.zeros_like(t))
+    any_q, any_k = see.any(3)[..., None], see.any(2)[..., None]
+    q_, k_, v_ = clean(q_, any_q), clean(k_, any_k), clean(v_, any_k)
+
+    raw = q_ @ k_.transpose(2, 3)
+    e_s = abs(scale) * (d + 4) * U32 * (q_.abs() @ k_.abs().transpose(2, 3))
+    t = raw * scale
+    th = torch.tanh(t / softcap) if softcap else torch.zeros_like(t)
+    if softcap:
+        t = softcap * th
+        e_s = e_s + 2.0 ** -21 * softcap
+    if slopes is not None:
+        bias = slopes.double()[None, :, None, None] * (pos - j).abs()[:, None]
+        t = t - bias
+        e_s = e_s + 4 * U32 * bias.abs()
+    e_s = e_s + 8 * U32 * t.abs() + 2.0 ** -21
+    low = torch.full_like(t, float('-inf'))
+    t = torch.where(see, t, low)
+    top = t.amax(3, keepdim=True)
+    top = torch.where(top == float('-inf'), torch.zeros_like(top), top)
+    w = torch.exp(t - top)
+    total = w.sum(3, keepdim=True)
+    p = w / torch.where(total == 0, torch.ones_like(total), total)
+    lse = torch.log(total.squeeze(3)) + top.squeeze(3)
+    e_p = torch.where(see, e_s, torch.zeros_like(e_s)).amax(3, keepdim=True)                # relative error of a row's weights, and of their sum
+    chain = (n_k + 64) * U32
+    pv = p @ v_.abs()
+    o = p @ v_
+    e_o = (u + 2 * e_p + chain) * pv + (step + flush) * clean(v_.abs(), any_k).sum(2, keepdim=True) * any_q + u * o.abs() + TINY[dt]
+    vals = dict(out=o.transpose(1, 2), lse=lse)
+    tols = dict(out=e_o.transpose(1, 2), lse=(e_p.squeeze(3) + chain + 4 * U32 * (lse.abs().nan_to_num(0.0, 0.0, 0.0) + 1)))
+    if do is None:
+        return vals, tols
+    do_ = clean(heads(do), any_q)
+    e_w = 2 * e_p + e_s + chain + 8 * U32 * lse.abs().nan_to_num(0.0, 0.0, 0.0)[..., None]  # weights again, from the stored lse
+    fold = lambda t: t.reshape(b, k.shape[2], group, *t.shape[2:]).sum(2)
+    dv = p.transpose(2, 3) @ do_
+    e_dv = ((p * (u + e_w + (group * n_q + 64) * U32)).transpose(2, 3) @ do_.abs()) + (step * 2.0 ** -12 + flush) * do_.abs().sum(2, keepdim=True)
+    delta = (do_ * o).sum(3, keepdim=True)
+    dp = do_ @ v_.transpose(2, 3)
+    e_d = (do_.abs() * e_o).sum(3, keepdim=True) + (d + 4) * U32 * (do_.abs() @ v_.abs().transpose(2, 3) + (do_ * o).abs().sum(3, keepdim=True))
+    cap = 1 - th * th
+    dt_ = p * (dp - delta)
+    ds = torch.where(see, dt_ * cap * scale, torch.zeros_like(dt_))
+    e_ds = torch.where(see, abs(scale) * (p * (e_d + (dp - delta).abs() * (e_w + 2.0 ** -20))) + u * ds.abs() + abs(scale) * flush * (dp.abs() + delta.abs() + 1), torch.zeros_like(ds))
+    if dt == torch.float16:                                                                 # ds 2^e in float16: e as the kernels choose it
+        a, c = float(do_.abs().max()), float(v_.abs().max())
+        if a and c:
+            import math
+            e = 7 - math.frexp(a)[1] - math.frexp(c)[1]
+            e_ds = e_ds + torch.where(see, torch.full_like(ds, step * 2.0 ** -e * abs(scale)), torch.zeros_like(ds))
+    dq, dk = ds @ k_, ds.transpose(2, 3) @ q_
+    e_dq = e_ds @ k_.abs() + chain * (ds.abs() @ k_.abs())
+    e_dk = e_ds.transpose(2, 3) @ q_.abs() + (group * n_q + 64) * U32 * (ds.abs().transpose(2, 3) @ q_.abs())
+    out = lambda val, err: (val.transpose(1, 2), (err + u * val.abs() + TINY[dt]).transpose(1, 2))
+    vals['dq'], tols['dq'] = out(dq, e_dq)
+    vals['dk'], tols['dk'] = out(fold(dk), fold(e_dk))
+    vals['dv'], tols['dv'] = out(fold(dv), fold(e_dv))
+    return vals, tols

@@ -1,0 +1,319 @@
+"""-m gpu tests of `attention` against its definition in float64 (tests/_token_ref.py, bounds derived there)."""
+import pytest
+import torch
+
+import _token_ref as R
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+def _randn(shape, seed, dtype, scale=1.0):
+    return (torch.randn(shape, generator=torch.Generator().manual_seed(seed)) * scale).to(dtype)
+
+
+def _inputs(b, lq, lk, hq, hk, d, dtype, seed=0):
+    return (_randn((b, lq, hq, d), seed, dtype), _randn((b, lk, hk, d), seed + 1, dtype), _randn((b, lk, hk, d), seed + 2, dtype),
+            _randn((b, lq, hq, d), seed + 3, dtype))
+
+
+def _docs(b, n, count, seed=0, pad=0):
+    cuts = torch.randint(0, max(n - pad, 1), (b, count - 1), generator=torch.Generator().manual_seed(seed)).sort(dim=1).values
+    ids = (torch.arange(n)[None, :, None] >= cuts[:, None, :]).sum(2).to(torch.int32)
+    if pad:
+        ids[:, n - pad:] = -1
+    return ids
+
+
+def _to(dev, kw):
+    return {name: t.to(dev) if isinstance(t, torch.Tensor) else t for name, t in kw.items()}
+
+
+def _check(dev, q, k, v, do=None, what='', **kw):
+    """Forward (with lse) and, with `do`, the gradients; returns what came out."""
+    from next3d_amd.torch_utils.ops import attention
+    leaves = [t.to(dev).requires_grad_(do is not None) for t in (q, k, v)]
+    out, lse = attention.attention(*leaves, return_lse=True, **_to(dev, kw))
+    got = dict(out=out, lse=lse)
+    if do is not None:
+        got.update(zip(('dq', 'dk', 'dv'), torch.autograd.grad(out, leaves, do.to(dev))))
+    vals, tols = R.attention(q, k, v, do, **kw)
+    for name, t in got.items():
+        want, tol = vals[name], tols[name]
+        if name == 'lse':
+            empty = want == float('-inf')
+            assert torch.equal(t.cpu() == float('-inf'), empty), what
+            t, want, tol = t.cpu()[~empty], want[~empty], tol[~empty]
+        R.assert_within(t, want, tol, f'{what} {name}')
+    return {name: t.detach() for name, t in got.items()}
+
+
+SIZES = [  # B, Lq, Lk, Hq, Hk, D
+    (1, 1, 1, 1, 1, 64), (2, 1, 77, 4, 2, 128), (1, 3, 200, 2, 2, 32), (2, 65, 65, 2, 1, 64), (1, 129, 300, 3, 3, 72), (1, 300, 129, 4, 1, 128), (2, 128, 128, 2, 2, 96),
+    (1, 257, 191, 2, 1, 8), (1, 66, 1000, 1, 1, 80), (1, 200, 64, 6, 2, 40)]
+
+
+@pytest.mark.parametrize('causal', [False, True])
+@pytest.mark.parametrize('dtype', [F16, BF16])
+@pytest.mark.parametrize('size', SIZES, ids=str)
+def test_attention(dev, size, dtype, causal):
+    q, k, v, do = _inputs(*size, dtype)
+    _check(dev, q, k, v, do, causal=causal)
+
+
+@pytest.mark.parametrize('dtype', [F16, BF16])
+@pytest.mark.parametrize('d', [64, 128])
+def test_attention_score_forms(dev, d, dtype):
+    b, n, hq, hk = 2, 150, 4, 2
+    q, k, v, do = _inputs(b, n, n, hq, hk, d, dtype, 7)
+    slopes = 2.0 ** -torch.arange(1.0, hq + 1)
+    prefix = torch.tensor([0, 70], dtype=torch.int32)
+    docs = _docs(b, n, 5, 1, pad=20)
+    for kw in (dict(softcap=4.0), dict(slopes=slopes), dict(causal=True, prefix=prefix), dict(documents=docs), dict(documents=docs, causal=True),
+               dict(causal=True, prefix=prefix, documents=docs, softcap=10.0, slopes=slopes), dict(scale=0.0), dict(scale=-0.3), dict(scale=0.7, softcap=1.0)):
+        _check(dev, q, k, v, do, what=str(sorted(kw)), **kw)
+
+
+@pytest.mark.parametrize('dtype', [F16, BF16])
+def test_attention_lengths(dev, dtype):
+    """A cache filled to different lengths, zero and full among them: few queries (keys split over the chip), and many."""
+    lengths = torch.tensor([0, 1, 63, 64, 65, 700, 1500, 5000], dtype=torch.int32)         # (5000: more than there are, all 1500)
+    for lq, hq, hk, d in ((1, 4, 1, 128), (5, 2, 2, 64), (40, 2, 1, 80), (100, 1, 1, 64)):
+        q, k, v, do = _inputs(8, lq, 1500, hq, hk, d, dtype, 3)
+        for kw in (dict(), dict(causal=True), dict(causal=True, prefix=torch.tensor([9, 0, 100, 3, 65, 1, 1500, 2000], dtype=torch.int32))):
+            _check(dev, q, k, v, do if lq in (5, 100) else None, what=f'{lq} {sorted(kw)}', lengths=lengths, **kw)
+    q, k, v, do = _inputs(1, 3, 9, 1, 1, 16, dtype, 3)
+    _check(dev, q, k, v, do, lengths=torch.tensor([-4], dtype=torch.int32))
+
+
+def test_attention_never_reads_behind_the_length(dev):
+    """NaN behind the last key in use reaches nothing, and the gradients there are zero."""
+    for lq in (1, 33, 200):
+        q, k, v, do = _inputs(2, lq, 300, 2, 1, 64, BF16, 5)
+        k[:, 250:], v[:, 250:] = float('nan'), float('inf')
+        got = _check(dev, q, k, v, do, lengths=torch.tensor([250, 100], dtype=torch.int32))
+        assert int(got['dk'][:, 250:].abs().sum()) == 0 and int(got['dv'][1, 100:].abs().sum()) == 0
+
+
+@pytest.mark.parametrize('bad', [float('nan'), float('inf'), -float('inf')])
+def test_attention_masked_nonfinite_stays_away(dev, bad):
+    """NaN or infinity in tokens of another document, behind the diagonal or in padding does not reach the rows that do not see them — forward (tiles with
+    matrix products over masked keys) and in every gradient."""
+    b, n, d = 1, 190, 64
+    for dtype, hq, hk in ((F16, 2, 2), (BF16, 4, 1)):
+        q, k, v, do = _inputs(b, n, n, hq, hk, d, dtype, 11)
+        docs = _docs(b, n, 3, 2, pad=30)
+        pad = docs[0] < 0
+        for t in (q, k, v, do):                                             # padding: seen by nobody, sees nothing
+            t[:, pad] = bad
+        _check(dev, q, k, v, do, what='padding', documents=docs)
+        q, k, v, do = _inputs(b, n, n, hq, hk, d, dtype, 12)
+        docs = _docs(b, n, 2, 3)
+        cut = int((docs[0] == 0).sum())
+        for t, name in ((k, 'k'), (v, 'v'), (q, 'q'), (do, 'do')):
+            spoiled = dict(q=q, k=k, v=v, do=do)
+            spoiled[name] = t.clone()
+            spoiled[name][:, cut + 5] = bad                                 # in the second document: the first must not notice
+            clean = _run(dev, q, k, v, do, documents=docs)
+            got = _run(dev, *(spoiled[x] for x in ('q', 'k', 'v', 'do')), documents=docs)
+            for key in ('out', 'dq', 'dk', 'dv'):
+                assert bool(torch.isfinite(got[key][:, :cut]).all()), (name, key)
+                assert float((got[key][:, :cut].float() - clean[key][:, :cut].float()).abs().max()) <= 0.05, (name, key)
+        q, k, v, do = _inputs(b, n, n, hq, hk, d, dtype, 13)
+        v[:, 100] = bad                                                     # causal: queries before 100 do not see it
+        got = _run(dev, q, k, v, do, causal=True)
+        vals, tols = R.attention(q[:, :100], k[:, :100], v[:, :100], do[:, :100], causal=True)
+        R.assert_within(got['out'][:, :100], vals['out'], tols['out'], 'before the bad key')
+        R.assert_within(got['dq'][:, :100], vals['dq'], tols['dq'], 'before the bad key')
+        assert not bool(torch.isfinite(got['out'][:, 100:]).any())
+        for lq in (1, 4):                                                   # few queries over a cache
+            q, k, v, _ = _inputs(2, lq, 600, hq, hk, d, dtype, 14)
+            kd = _docs(2, 600, 2, 4)
+            qd = torch.zeros(2, lq, dtype=torch.int32)
+            for x in range(2):
+                v[x, kd[x] == 1], k[x, kd[x] == 1] = bad, bad
+            _check(dev, q, k, v, what='cache', documents=qd, key_documents=kd)
+
+
+def _run(dev, q, k, v, do, **kw):
+    from next3d_amd.torch_utils.ops import attention
+    leaves = [t.to(dev).requires_grad_() for t in (q, k, v)]
+    out = attention.attention(*leaves, **_to(dev, kw))
+    return dict(zip(('out', 'dq', 'dk', 'dv'), (out.detach(), *torch.autograd.grad(out, leaves, do.to(dev)))))
+
+
+def test_attention_documents_out_of_order(dev):
+    """Documents need not be sorted, and queries and keys may carry different ones."""
+    g = torch.Generator().manual_seed(1)
+    for lq, lk in ((150, 270), (3, 900)):
+        q, k, v, do = _inputs(2, lq, lk, 2, 1, 64, F16, 21)
+        qd = torch.randint(-1, 6, (2, lq), generator=g).to(torch.int32)
+        kd = torch.randint(-1, 7, (2, lk), generator=g).to(torch.int32)
+        _check(dev, q, k, v, do, documents=qd, key_documents=kd)
+        _check(dev, q, k, v, do, documents=torch.full_like(qd, -1), key_documents=kd)
+
+
+def test_attention_small_and_large_gradients_float16(dev):
+    """float16 gradients of any size keep their relative accuracy (the dscores get a power of two of their own)."""
+    for size in (1e-6, 1e-3, 300.0):
+        q, k, v, do = _inputs(1, 200, 200, 2, 1, 64, F16, 31)
+        _check(dev, q, k, v, (do.float() * size).to(F16), causal=True, what=f'{size}')
+    q, k, v, do = _inputs(1, 150, 150, 1, 1, 32, F16, 32)
+    _check(dev, q, k, (v.float() * 100).to(F16), (do.float() * 100).to(F16))
+
+
+def test_attention_extreme_scores(dev):
+    """Scores far apart: one key takes all; the running maximum rises tile after tile, or falls."""
+    b, n, d = 1, 400, 64
+    q, k, v, do = _inputs(b, n, n, 1, 1, d, BF16, 41)
+    ramp = torch.linspace(-1, 1, n)[None, :, None, None]
+    for sign in (1, -1):
+        for size in (1.0, 8.0):
+            qq = (q.float().abs() * size).to(BF16)
+            kk = (k.float().abs() * ramp * sign * size).to(BF16)
+            _check(dev, qq, kk, v, do, what=f'{sign} {size}')
+
+
+def test_attention_strides(dev):
+    """Heads-first tensors, slices of one projection, broadcast keys, odd offsets; gradients that are expanded."""
+    from next3d_amd.torch_utils.ops import attention
+    fused = _randn((2, 90, 12, 64), 51, F16).to(dev)
+    heads_first = fused.transpose(1, 2).contiguous().transpose(1, 2)
+    odd = _randn((2, 90, 12, 67), 52, F16).to(dev)[..., 3:]
+    flat = torch.empty(2 * 90 * 12 * 64 + 4, dtype=F16, device=dev)[4:].view(2, 90, 12, 64).copy_(fused)
+    wide = _randn((2, 90, 12, 128), 53, F16).to(dev)
+    for src in (fused, heads_first, odd, flat, wide[..., ::2], wide[..., 32:96], fused[:1].expand(2, 90, 12, 64), fused[:, :1].expand(2, 90, 12, 64)):
+        parts = [src[:, :, :6], src[:, :, 6:9], src[:, :, 9:]]
+        results = []
+        for ts in (parts, [t.clone(memory_format=torch.contiguous_format) for t in parts]):
+            leaves = [t.detach().requires_grad_() for t in ts]
+            out = attention.attention(*leaves, causal=True)
+            one = torch.full((), 0.5, dtype=F16, device=dev).expand(out.shape)
+            results.append([out, *torch.autograd.grad(out, leaves, one)])
+        assert all(torch.equal(a, c) for a, c in zip(*results))
+
+
+def test_attention_empty(dev):
+    from next3d_amd.torch_utils.ops import attention
+    for b, lq, lk in ((0, 4, 4), (2, 0, 5), (2, 5, 0)):
+        q, k, v, do = (t.to(dev) for t in _inputs(b, lq, lk, 2, 1, 16, F16))
+        leaves = [t.requires_grad_() for t in (q, k, v)]
+        out, lse = attention.attention(*leaves, return_lse=True)
+        grads = torch.autograd.grad(out, leaves, do)
+        assert out.shape == q.shape and not bool(out.abs().sum()) and bool((lse == float('-inf')).all())
+        assert [g.shape for g in grads] == [t.shape for t in leaves] and not any(bool(g.abs().sum()) for g in grads)
+
+
+def test_attention_partial_gradients_and_differences(dev):
+    from next3d_amd.torch_utils.ops import attention
+    q, k, v, do = _inputs(1, 70, 70, 2, 1, 64, F16, 61)
+    kw = dict(causal=True, softcap=5.0, slopes=torch.tensor([0.1, 0.02]))
+    full = _run(dev, q, k, v, do, **kw)
+    for which, name in enumerate(('dq', 'dk', 'dv')):
+        leaves = [t.to(dev).requires_grad_(i == which) for i, t in enumerate((q, k, v))]
+        got, = torch.autograd.grad(attention.attention(*leaves, **_to(dev, kw)), leaves[which], do.to(dev))
+        assert torch.equal(got, full[name])
+    h = 1e-4
+    _, tols = R.attention(q, k, v, do, **kw)
+    for i, name in enumerate(('dq', 'dk', 'dv')):
+        step = _randn((q, k, v)[i].shape, 62 + i, torch.float64)
+        vary = lambda s: [t.double() + s * h * step if x == i else t.double() for x, t in enumerate((q, k, v))]
+        f = [float((_out64(*vary(s), **kw) * do.double()).sum()) for s in (1, -1)]
+        analytic = float((full[name].cpu().double() * step).sum())
+        # the float64 differences are exact to h^2 ~ 1e-8 of their terms; the kernel's gradient is within its bound, element by element
+        assert abs((f[0] - f[1]) / (2 * h) - analytic) <= float((tols[name] * step.abs()).sum()) + 1e-5 * float((full[name].cpu().double() * step).abs().sum())
+
+
+def _out64(q, k, v, causal, softcap, slopes):
+    group = q.shape[2] // k.shape[2]
+    q, k, v = q.transpose(1, 2), k.transpose(1, 2).repeat_interleave(group, 1), v.transpose(1, 2).repeat_interleave(group, 1)
+    t = softcap * torch.tanh(q @ k.transpose(2, 3) * q.shape[3] ** -0.5 / softcap)
+    n = q.shape[2]
+    dist = (torch.arange(n)[:, None] - torch.arange(n)[None]).double()
+    t = (t - slopes.double()[None, :, None, None] * dist.abs()).masked_fill(dist < 0, float('-inf'))
+    return (torch.softmax(t, 3) @ v).transpose(1, 2)
+
+
+def test_attention_reproducible_on_another_stream_and_in_graphs(dev):
+    from next3d_amd.torch_utils.ops import attention
+    cases = [(_inputs(2, 200, 200, 4, 2, 64, F16, 71), dict(documents=_docs(2, 200, 4), causal=True)), (_inputs(3, 1, 2000, 8, 2, 128, F16, 72), dict(causal=True, lengths=torch.tensor([1, 700, 2000], dtype=torch.int32)))]
+    for tensors, kw in cases:
+        q, k, v, do = (t.to(dev) for t in tensors)
+        kw = _to(dev, kw)
+
+        def step():
+            leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+            out = attention.attention(*leaves, **kw)
+            return [out.detach(), *torch.autograd.grad(out, leaves, do)]
+
+        want = [t.clone() for t in step()]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            again = step()
+        torch.cuda.current_stream().wait_stream(side)
+        assert all(torch.equal(a, c) for a, c in zip(want, again))
+        graphs = []
+        for _ in range(2):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                out = step()
+            graphs.append((g, out))
+        for seed in range(3):
+            q.copy_(_randn(tuple(q.shape), 80 + seed, F16))
+            want = [t.clone() for t in step()]
+            side.wait_stream(torch.cuda.current_stream())
+            graphs[0][0].replay()
+            with torch.cuda.stream(side):
+                graphs[1][0].replay()
+            torch.cuda.current_stream().wait_stream(side)
+            torch.cuda.synchronize()
+            for _, out in graphs:
+                assert all(torch.equal(a, c) for a, c in zip(want, out))
+
+
+def test_token_block(dev):
+    """The three operators as a block uses them — normalise, project, turn, attend, add — forward and gradients, against the same block in float64."""
+    from next3d_amd.torch_utils.ops import attention, layer_norm, rotary
+    b, t, h, w, heads, kv, d = 1, 2, 5, 7, 4, 2, 32
+    n, c = t * h * w, heads * d
+    pos = torch.stack(torch.meshgrid(torch.arange(t), torch.arange(h), torch.arange(w), indexing='ij'), -1).reshape(n, 3).to(torch.int32)
+    x, weight, bias, g = _randn((b, n, c), 91, F16), 1 + 0.1 * torch.randn(c, generator=torch.Generator().manual_seed(92)), _randn((c,), 93, torch.float32, 0.1), _randn((b, n, c), 94, F16)
+    proj = _randn((c, (heads + 2 * kv) * d), 95, F16, c ** -0.5)
+
+    def block(x, weight, bias, proj, norm, turn, attend):
+        y = norm(x, weight, bias) @ proj
+        q, k, v = y.reshape(b, n, heads + 2 * kv, d).split([heads, kv, kv], dim=2)
+        q, k = turn(q, k)
+        return x + attend(q, k, v).reshape(b, n, c)
+
+    leaves = [p.to(dev).requires_grad_() for p in (x, weight, bias, proj)]
+    out = block(*leaves, layer_norm.layer_norm, lambda q, k: rotary.rotary(q, pos.to(dev), (8, 12, 12), k=k, pairing='half'),
+                lambda q, k, v: attention.attention(q, k, v, softcap=20.0))
+    got = [out, *torch.autograd.grad(out, leaves, g.to(dev))]
+
+    def norm64(x, weight, bias):
+        z = x - x.mean(-1, keepdim=True)
+        return z / (z.square().mean(-1, keepdim=True) + 1e-5).sqrt() * weight + bias
+
+    def turn64(q, k):
+        ang = torch.cat([pos[:, a, None].double() * 10000.0 ** (-torch.arange(0, s, 2).double() / s) for a, s in enumerate((8, 12, 12))], 1)
+        lo = torch.cat([torch.arange(o, o + s // 2) for o, s in ((0, 8), (8, 12), (20, 12))])
+        hi = torch.cat([torch.arange(o + s // 2, o + s) for o, s in ((0, 8), (8, 12), (20, 12))])
+        order = torch.argsort(torch.cat([lo, hi]))
+        cos, sin = ang.cos()[None, :, None], ang.sin()[None, :, None]
+        return [torch.cat([z[..., lo] * cos - z[..., hi] * sin, z[..., lo] * sin + z[..., hi] * cos], -1)[..., order] for z in (q, k)]
+
+    def attend64(q, k, v):
+        q, k, v = q.transpose(1, 2), k.transpose(1, 2).repeat_interleave(heads // kv, 1), v.transpose(1, 2).repeat_interleave(heads // kv, 1)
+        return (torch.softmax(20 * torch.tanh(q @ k.transpose(2, 3) * d ** -0.5 / 20), 3) @ v).transpose(1, 2)
+
+    leaves64 = [p.double().requires_grad_() for p in (x, weight, bias, proj)]
+    out64 = block(*leaves64, norm64, turn64, attend64)
+    want = [out64, *torch.autograd.grad(out64, leaves64, g.double())]
+    # six roundings to float16 one behind the other (norm, projection, rotation, weights, output, sum), each 2^-11 of the largest value it meets; gradients
+    # pass the same chain and back: twelve, and are sums over the tokens of terms that may cancel, so 2^-11 of the largest magnitude bounds each
+    for name, a, ref, roundings in zip(('out', 'x', 'weight', 'bias', 'proj'), got, want, (6, 12, 12, 12, 12)):
+        err = float((a.detach().cpu().double() - ref.detach()).abs().max())
+        assert err <= roundings * 2.0 ** -11 * float(ref.detach().abs().max()) * 2, (name, err, float(ref.detach().abs().max()))

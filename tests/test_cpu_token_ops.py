@@ -111,3 +111,72 @@ def test_c_entries_refuse_bad_calls():
         assert word in err(rot(**kw)), kw
     assert rot(L=0) == 0
     assert 'null' in err(lib.n3d_rotary(None, None))
+
+
+def test_attention_refusals():
+    from next3d_amd.torch_utils.ops.attention import attention
+    q, k = torch.zeros(2, 5, 4, 16).half(), torch.zeros(2, 7, 2, 16).half()
+    i32 = lambda *shape: torch.zeros(shape, dtype=torch.int32)
+    _raises('HIP device only', attention, q, k, k)
+    _raises('4 dimensions', attention, q[0], k, k)
+    _raises('q must be', attention, q.float(), k, k)
+    _raises('k must be', attention, q, k.bfloat16(), k)
+    _raises('v must be', attention, q, k, k.float())
+    _raises('do not match', attention, q, k, k[:, :6])
+    _raises('do not match', attention, q, k[:1], k[:1])
+    _raises('do not match', attention, q[..., :8], k, k)
+    _raises('multiple of', attention, q[:, :, :3], k, k)
+    _raises('multiple of', attention, q, k[:, :, :0], k[:, :, :0])
+    _raises('head sizes', attention, q[..., :12], k[..., :12], k[..., :12])
+    _raises('head sizes', attention, torch.zeros(1, 2, 1, 136).half(), torch.zeros(1, 2, 1, 136).half(), torch.zeros(1, 2, 1, 136).half())
+    for kw in (dict(scale=float('nan')), dict(scale=float('inf')), dict(softcap=-1.0), dict(softcap=float('inf'))):
+        _raises('finite', attention, q, k, k, **kw)
+    _raises('causal', attention, q, k, k, prefix=i32(2))
+    _raises('prefix must be', attention, q, k, k, prefix=i32(3), causal=True)
+    _raises('prefix must be', attention, q, k, k, prefix=i32(2).long(), causal=True)
+    _raises('lengths must', attention, q, k, k, lengths=i32(2, 1))
+    _raises('key_documents', attention, q, k, k, documents=i32(2, 5))
+    _raises('documents must be', attention, q, k, k, documents=i32(2, 7), key_documents=i32(2, 7))
+    _raises('key_documents must be', attention, q, k, k, documents=i32(2, 5), key_documents=i32(2, 5))
+    _raises('need documents', attention, q, k, k, key_documents=i32(2, 7))
+    _raises('slopes for', attention, q, k, k, slopes=torch.zeros(2))
+    _raises('slopes must', attention, q, k, k, slopes=torch.zeros(4).half())
+    _raises('no gradient', attention, q, k, k, slopes=torch.zeros(4, requires_grad=True))
+
+
+def test_attention_descriptor_layout(tmp_path):
+    from next3d_amd import _lib
+    _struct_layout(tmp_path, 'n3d_attention_desc', _lib.AttentionDesc)
+
+
+def test_attention_c_entries_refuse_bad_calls():
+    from next3d_amd import _lib
+    lib = _lib.lib()
+
+    def desc(**kw):
+        p = 4096                                                   # never dereferenced: every call below is refused
+        d = _lib.AttentionDesc(q=p, k=p, v=p, out=p, lse=p, dout=p, dq=p, dk=p, dv=p, scale=1.0, B=1, Lq=4, Lk=300, heads_q=2, heads_k=1, D=16, dtype=1)
+        for name, value in dict(dict(q_strides=(128, 32, 16), k_strides=(4800, 16, 16), v_strides=(4800, 16, 16), dout_strides=(128, 32, 16)), **kw).items():
+            if name.endswith('_strides'):
+                getattr(d, name)[:] = value
+            else:
+                setattr(d, name, value)
+        return d
+
+    shared = ((dict(dtype=0), 'float16'), (dict(D=12), 'head sizes'), (dict(D=136), 'head sizes'), (dict(heads_q=3, heads_k=2), 'multiple'), (dict(heads_k=0), 'multiple'),
+              (dict(B=-1), 'negative'), (dict(softcap=-1.0), 'softcap'), (dict(scale=float('nan')), 'scale'), (dict(prefix=4096), 'causal'), (dict(q_documents=4096), 'documents'),
+              (dict(q=None), 'null'), (dict(v=None), 'null'), (dict(k_strides=(4800, 15, 16)), 'strides'), (dict(v_strides=(4800, 1 << 24, 16)), 'strides'),
+              (dict(q_strides=(128, 32, -16)), 'strides'), (dict(k=4100), 'aligned'), (dict(B=1 << 20, Lq=1 << 14), 'rows'))
+    for entry, size in ((lib.n3d_attention, lib.n3d_attention_workspace), (lib.n3d_attention_bwd, lib.n3d_attention_bwd_workspace)):
+        for kw, word in shared:
+            assert entry(desc(**kw), None) != 0 and word in lib.n3d_last_error().decode(), (kw, lib.n3d_last_error())
+            assert size(desc(**kw)) == -1 and word in lib.n3d_last_error().decode(), kw
+        need = size(desc())
+        assert need > 0
+        for kw in (dict(), dict(workspace=4096, workspace_bytes=need - 1), dict(workspace=4104, workspace_bytes=need)):
+            assert entry(desc(**kw), None) != 0 and 'workspace' in lib.n3d_last_error().decode()
+        assert entry(None, None) != 0
+    assert lib.n3d_attention(desc(Lq=0), None) == 0 and lib.n3d_attention(desc(B=0), None) == 0
+    for kw, word in ((dict(Lq=0), 'queries'), (dict(lse=None), 'null'), (dict(dout=None), 'null'), (dict(dk=None), 'null'), (dict(dq=None, dk=None, dv=None), 'null'),
+                     (dict(dout_strides=(128, 33, 16)), 'strides'), (dict(dout=4100), 'aligned'), (dict(dv=4100), 'aligned')):
+        assert lib.n3d_attention_bwd(desc(workspace=4096, workspace_bytes=1 << 30, **kw), None) != 0 and word in lib.n3d_last_error().decode(), kw
