@@ -99,6 +99,14 @@ __device__ __forceinline__ int attn_swizzle(int row) {
     else return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
 }
 
+// One piece: 16 bytes a lane from voff of the buffer to lds + 16 lane (zeros beyond the range).  In asm because the compiler, which sees LDS behind the
+// builtin, would wait for every piece in flight before the next LDS read of any buffer.  It has no register result; attn_sync / attn_landed wait for it, and
+// the compiler's own vmcnt waits, which do not count it, can only be longer than needed (loads return in order).  (m0 has no other use in these kernels.)
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void attn_piece(i32x4 rsrc, int voff, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(lds), "v"(voff), "s"(rsrc) : "memory");
+}
+
 // Staging by LDS-DMA: a piece is 1 KB = 64 lanes x 16 bytes; wave w of W takes pieces w, w + W, ...  Rows behind the last and channels behind D are beyond
 // the descriptor's range and arrive as zeros.
 template <int ROW, int ROWS, int WAVES>
@@ -116,12 +124,11 @@ struct AttnStage {
     // rows [0, rows) of `base` (rows >= 1) -> lds
     __device__ __forceinline__ void issue(const void* base, int rows, int64_t stride, int D, char* lds, int wave) const {
         const uint64_t a = (uint64_t)base;
-        const uint64_t u = ((uint64_t)(uint32_t)attn_uniform((int)(a >> 32)) << 32) | (uint32_t)attn_uniform((int)a);
-        const int n = attn_uniform(((rows < ROWS ? rows : ROWS) - 1) * (int)stride * 2 + D * 2);
-        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)u, 0, n, 0x00020000);
+        const int n = ((rows < ROWS ? rows : ROWS) - 1) * (int)stride * 2 + D * 2;
+        const i32x4 r = {attn_uniform((int)a), attn_uniform((int)(a >> 32) & 0xffff), attn_uniform(n), 0x00020000};
+        const uint32_t to = (uint32_t)(uintptr_t)(attn_lds_void*)lds + wave * 1024;
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (attn_lds_void*)(lds + (wave + i * WAVES) * 1024), 16, voff[i], 0, 0, 0);
+        for (int i = 0; i < PIECES; ++i) attn_piece(r, voff[i], attn_uniform(to + i * WAVES * 1024));
     }
 };
 
@@ -150,30 +157,41 @@ __device__ __forceinline__ typename AttnVec<T>::x8 attn_lane_frag(const T* p, in
     return p && chunk * 8 < D ? *reinterpret_cast<const typename AttnVec<T>::x8*>(p + chunk * 8) : z;
 }
 
-// every wave's pieces have landed and every wave is done with what it read: a tile buffer changes hands
-__device__ __forceinline__ void attn_sync() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// this wave's pieces have landed and its LDS accesses are done (the asm for the hardware, the builtin for the compiler's own book-keeping)
+__device__ __forceinline__ void attn_landed() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070);
+}
+// ... and every other wave's: a tile buffer changes hands
+__device__ __forceinline__ void attn_sync() {
+    attn_landed();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" : : : "memory");
+}
 
 // ---- which tiles to visit: [t, end) in order; with documents only those whose range [lowest, highest] meets [lo, hi] (64 ranges looked at together)
 struct AttnTiles {
     const int2* ranges;
-    int t, end, lo, hi;
+    int t, end, lo, hi, base, low, high;                     // low, high: documents of the tile last returned
     uint64_t bits;
-    int base, kmin, kmax;
-    __device__ void start(const int2* r, int first, int stop, int dlo, int dhi) {
-        ranges = r; t = first; end = stop; lo = dlo; hi = dhi; bits = 0; base = first - 64;
+    int2 mine;
+    __device__ __forceinline__ void start(const int2* r, int first, int stop, int dlo, int dhi) {
+        ranges = r; t = first; end = stop; lo = dlo; hi = dhi; bits = 0; base = first - 64; low = high = 0;
     }
     // the next tile or -1
-    __device__ int next(int lane) {
+    __device__ __forceinline__ int next(int lane) {
         if (!ranges) return t < end ? t++ : -1;
         while (bits == 0) {
             base += 64;
             if (base >= end) return -1;
             const int i = base + lane;
-            const int2 d = i < end ? ranges[i] : make_int2(1, 0);
-            bits = __ballot(i < end && d.y >= lo && d.x <= hi);
+            mine = i < end ? ranges[i] : make_int2(1, 0);
+            bits = __ballot((i < end) & (mine.y >= lo) & (mine.x <= hi));
         }
         const int n = __builtin_ctzll(bits);
         bits &= bits - 1;
+        low = __builtin_amdgcn_readlane(mine.x, n);
+        high = __builtin_amdgcn_readlane(mine.y, n);
         return attn_uniform(base + n);
     }
 };

@@ -84,26 +84,36 @@ __device__ __forceinline__ int attn_ds_scale(const AttnParams& p, int lane) {
     return attn_uniform(e);
 }
 
-// raw scores S and dP of 16 (row, column) elements -> P 2^shift and ds 2^e.  lse2 / delta of register r by the functions given; see(r) is asked only if !full
-template <typename FL, typename FD, typename FS, typename FDist>
-__device__ __forceinline__ void attn_ds_step(f32x16& S, f32x16& dP, const AttnScore& f, float ds_by, bool full, FL lse2, FD delta, FS see, FDist dist) {
+// Raw scores S and dP of 16 (row, column) elements -> P 2^shift and ds 2^e.  lse2(a) / delta(a): of the four registers 4 a .. 4 a + 3; dist + step * row:
+// the element's distance; visible(S, dP) zeroes what is masked (asked only if !full).
+template <bool CAP, typename FL, typename FD>
+__device__ __forceinline__ void attn_ds_form(f32x16& S, f32x16& dP, const AttnScore& f, float ds_by, FL lse2, FD delta, float dist, float step) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        float u, slope_of_cap = 1.f;
-        if (f.cap_out > 0.f) {
-            const float th = f.tanh_part(S[r]);
-            u = f.cap_out * th;
-            slope_of_cap = 1.f - th * th;
-        } else {
-            u = S[r] * f.mul;
+    for (int a = 0; a < 4; ++a) {
+        const float4 l = lse2(a), d = delta(a);
+        const float la[4] = {l.x, l.y, l.z, l.w}, da[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int r = 4 * a + e;
+            float u, by = ds_by;
+            if constexpr (CAP) {
+                const float th = f.tanh_part(S[r]);
+                u = f.cap_out * th;
+                by = ds_by - ds_by * th * th;
+            } else {
+                u = S[r] * f.mul;
+            }
+            u -= f.slope * fabsf(dist + step * (float)(8 * a + e)) + la[e];
+            S[r] = __builtin_amdgcn_exp2f(u);
+            dP[r] = S[r] * (dP[r] - da[e]) * by;
         }
-        if (f.slope != 0.f) u -= f.slope * fabsf((float)dist(r));
-        const float w = __builtin_amdgcn_exp2f(u - lse2(r));
-        float d = w * (dP[r] - delta(r)) * (slope_of_cap * ds_by);
-        const bool on = full || see(r);
-        S[r] = on ? w : 0.f;
-        dP[r] = on ? d : 0.f;
     }
+}
+template <typename FL, typename FD, typename FV>
+__device__ __forceinline__ void attn_ds_step(f32x16& S, f32x16& dP, const AttnScore& f, float ds_by, bool full, FL lse2, FD delta, FV visible, float dist, float step) {
+    if (f.cap_out > 0.f) attn_ds_form<true>(S, dP, f, ds_by, lse2, delta, dist, step);
+    else attn_ds_form<false>(S, dP, f, ds_by, lse2, delta, dist, step);
+    if (!full) visible(S, dP);
 }
 
 template <typename T>
@@ -130,7 +140,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnParams p) {
 #ifdef __HIP_DEVICE_COMPILE__                            // (hipcc drops the launch stub of a template whose body its host pass cannot read)
     constexpr int ROW = DB > 2 ? 128 : 64, TILE_BYTES = ATTN_TILE * ROW * 2;
     __shared__ __align__(16) char smem[4 * TILE_BYTES];
-    __shared__ int sdoc[2][ATTN_TILE];
+    __shared__ __align__(16) int sdoc[2][ATTN_TILE];
     const int wave = attn_uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
     const int total = p.B * p.Hq * p.row_blocks, per = (total + 7) / 8;
     const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
@@ -172,27 +182,26 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnParams p) {
     sk.setup(wave, lane, p.ks[1], p.D);
     sv.setup(wave, lane, p.vs[1], p.D);
     f32x16 acc[DB] = {};
+    int doc_next = 0;                                                   // of the tile being staged: loaded ahead of its pieces, written behind the products
     auto stage = [&](int t, int buf) {
         char* at = smem + buf * 2 * TILE_BYTES;
+        if (kdoc && wave == 0) doc_next = kdoc[min(t * ATTN_TILE + lane, p.Lk - 1)];
         sk.issue(k + (int64_t)t * ATTN_TILE * p.ks[1], n - t * ATTN_TILE, p.ks[1], p.D, at, wave);
         sv.issue(v + (int64_t)t * ATTN_TILE * p.vs[1], n - t * ATTN_TILE, p.vs[1], p.D, at + TILE_BYTES, wave);
-        if (kdoc && wave == 0) sdoc[buf][lane] = kdoc[min(t * ATTN_TILE + lane, p.Lk - 1)];
     };
     int t = tiles.next(lane);
     if (t >= 0) stage(t, 0);
+    if (kdoc && wave == 0) sdoc[0][lane] = doc_next;
     for (int buf = 0; t >= 0; buf ^= 1) {
         attn_sync();
+        const bool one_doc = (dlo == dhi) & (tiles.low == dlo) & (tiles.high == dlo);
         const int t_next = tiles.next(lane);
         if (t_next >= 0) stage(t_next, buf ^ 1);
         const int j0 = t * ATTN_TILE;
         if (j0 <= lim_last) {
             const char* kt = smem + buf * 2 * TILE_BYTES;
             const char* vt = kt + TILE_BYTES;
-            bool full = j0 + ATTN_TILE - 1 <= lim_first;
-            if (kdoc) {
-                const int2 r = p.ktiles[(int64_t)b * p.nkt + t];
-                full = full && dlo == dhi && r.x == dlo && r.y == dlo;
-            }
+            const bool full = (j0 + ATTN_TILE - 1 <= lim_first) & one_doc;
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
                 f32x16 S = {}, dP = {};
@@ -201,13 +210,23 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnParams p) {
                     S = attn_mfma(attn_row_frag<T, ROW>(kt, 32 * kb + l31, 2 * c + half), qf[c], S);
                     dP = attn_mfma(attn_row_frag<T, ROW>(vt, 32 * kb + l31, 2 * c + half), df[c], dP);
                 }
-                const int at = i + n - p.Lq, jb = j0 + 32 * kb + 4 * half;
-                attn_ds_step(S, dP, f, ds_by, full, [&](int) { return lse2; }, [&](int) { return delta; },
-                             [&](int r) {
-                                 const int j = 8 * (r >> 2) + (r & 3);
-                                 return jb + j <= lim && (!kdoc || sdoc[buf][32 * kb + 4 * half + j] == qdoc);
+                const int jb = j0 + 32 * kb + 4 * half;
+                attn_ds_step(S, dP, f, ds_by, full, [&](int) { return make_float4(lse2, lse2, lse2, lse2); }, [&](int) { return make_float4(delta, delta, delta, delta); },
+                             [&](f32x16&, f32x16& x) {
+                                 const int last = lim - jb;
+#pragma unroll
+                                 for (int r = 0; r < 16; ++r) x[r] = 8 * (r >> 2) + (r & 3) <= last ? x[r] : 0.f;
+                                 if (kdoc)
+#pragma unroll
+                                     for (int a = 0; a < 4; ++a) {
+                                         const int4 o = *reinterpret_cast<const int4*>(&sdoc[buf][32 * kb + 8 * a + 4 * half]);
+                                         x[4 * a] = o.x == qdoc ? x[4 * a] : 0.f;
+                                         x[4 * a + 1] = o.y == qdoc ? x[4 * a + 1] : 0.f;
+                                         x[4 * a + 2] = o.z == qdoc ? x[4 * a + 2] : 0.f;
+                                         x[4 * a + 3] = o.w == qdoc ? x[4 * a + 3] : 0.f;
+                                     }
                              },
-                             [&](int r) { return at - (jb + 8 * (r >> 2) + (r & 3)); });
+                             (float)(i + n - p.Lq - jb), -1.f);
                 typename AttnVec<T>::x8 d[2];
                 attn_pack<T>(dP, d);
 #pragma unroll
@@ -216,6 +235,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnParams p) {
                     for (int c = 0; c < 2; ++c) acc[db] = attn_mfma(attn_col_frag<T, ROW>(kt, 32 * kb + 16 * c, db, lane), d[c], acc[db]);
             }
         }
+        if (kdoc && wave == 0) sdoc[buf ^ 1][lane] = doc_next;
         t = t_next;
     }
     bool nan = false;
@@ -316,22 +336,31 @@ __global__ __launch_bounds__(256, DB > 2 ? 1 : 2) void attn_dkv_kernel(AttnParam
     sd.setup(wave, lane, p.ds[1], p.D);
     const int ds_exp = attn_ds_scale(p, lane);
     const float ds_by = ldexpf(1.f, ds_exp - (int)SHIFT);
+    float row_next = 0.f;
     auto stage = [&](int t, int gt, int buf) {
         const int h = hk * p.G + gt, i0 = t * ATTN_TILE;
         char* at = smem + buf * 2 * TILE_BYTES;
-        sq.issue((const T*)p.q + b * p.qs[0] + i0 * p.qs[1] + h * p.qs[2], p.Lq - i0, p.qs[1], p.D, at, wave);
-        sd.issue((const T*)p.dout + b * p.ds[0] + i0 * p.ds[1] + h * p.ds[2], p.Lq - i0, p.ds[1], p.D, at + TILE_BYTES, wave);
+        // the rows' statistics: loaded ahead of the pieces (one of the three a wave), written to the LDS behind the products of the tile before
         const int i = i0 + lane;
         const int64_t stat = ((int64_t)b * p.Hq + h) * p.Lq + i;
-        if (wave == 0) slse[buf][lane] = i < p.Lq ? attn_lse2(p.lse[stat]) - SHIFT : INFINITY;      // (queries behind the last: every weight 0)
-        if (wave == 1) sdelta[buf][lane] = i < p.Lq ? p.delta[stat] : 0.f;
-        if (wave == 2 && p.kdoc) sdoc[buf][lane] = i < p.Lq ? p.qdoc[b * p.qdoc_stride + i] : -1;
+        if (wave == 0) row_next = i < p.Lq ? attn_lse2(p.lse[stat]) - SHIFT : INFINITY;            // (queries behind the last: every weight 0)
+        if (wave == 1) row_next = i < p.Lq ? p.delta[stat] : 0.f;
+        if (wave == 2 && p.kdoc) row_next = __builtin_bit_cast(float, i < p.Lq ? p.qdoc[b * p.qdoc_stride + i] : -1);
+        sq.issue((const T*)p.q + b * p.qs[0] + i0 * p.qs[1] + h * p.qs[2], p.Lq - i0, p.qs[1], p.D, at, wave);
+        sd.issue((const T*)p.dout + b * p.ds[0] + i0 * p.ds[1] + h * p.ds[2], p.Lq - i0, p.ds[1], p.D, at + TILE_BYTES, wave);
+    };
+    auto commit = [&](int buf) {
+        if (wave == 0) slse[buf][lane] = row_next;
+        if (wave == 1) sdelta[buf][lane] = row_next;
+        if (wave == 2) sdoc[buf][lane] = __builtin_bit_cast(int, row_next);
     };
     f32x16 dk[DB] = {}, dv[DB] = {};
     int t = next(g);
     if (t >= 0) stage(t, g, 0);
+    commit(0);
     for (int buf = 0; t >= 0; buf ^= 1) {
         attn_sync();
+        const bool one_doc = (dlo == dhi) & (tiles.low == dlo) & (tiles.high == dlo);
         int g_next = g;
         const int t_next = next(g_next);
         if (t_next >= 0) stage(t_next, g_next, buf ^ 1);
@@ -340,11 +369,7 @@ __global__ __launch_bounds__(256, DB > 2 ? 1 : 2) void attn_dkv_kernel(AttnParam
             const char* qt = smem + buf * 2 * TILE_BYTES;
             const char* dt = qt + TILE_BYTES;
             const AttnScore f(p, hk * p.G + g);
-            bool full = i0 >= wave_full;
-            if (p.kdoc) {
-                const int2 r = ranges[t];
-                full = full && dlo == dhi && r.x == dlo && r.y == dlo;
-            }
+            const bool full = (i0 >= wave_full) & one_doc;
 #pragma unroll
             for (int qb = 0; qb < 2; ++qb) {
                 f32x16 S = {}, dP = {};
@@ -354,13 +379,30 @@ __global__ __launch_bounds__(256, DB > 2 ? 1 : 2) void attn_dkv_kernel(AttnParam
                     dP = attn_mfma(attn_row_frag<T, ROW>(dt, 32 * qb + l31, 2 * c + half), vf[c], dP);
                 }
                 const int ib = 32 * qb + 4 * half;
-                attn_ds_step(S, dP, f, ds_by, full, [&](int r) { return slse[buf][ib + 8 * (r >> 2) + (r & 3)]; },
-                             [&](int r) { return sdelta[buf][ib + 8 * (r >> 2) + (r & 3)]; },
-                             [&](int r) {
-                                 const int i = ib + 8 * (r >> 2) + (r & 3);
-                                 return i0 + i >= qmin && (!p.kdoc || sdoc[buf][i] == kdoc);
+                attn_ds_step(S, dP, f, ds_by, full, [&](int a) { return *reinterpret_cast<const float4*>(&slse[buf][ib + 8 * a]); },
+                             [&](int a) { return *reinterpret_cast<const float4*>(&sdelta[buf][ib + 8 * a]); },
+                             [&](f32x16& w, f32x16& x) {
+                                 const int first = qmin - i0 - ib;
+#pragma unroll
+                                 for (int r = 0; r < 16; ++r) {
+                                     const bool see = 8 * (r >> 2) + (r & 3) >= first;
+                                     w[r] = see ? w[r] : 0.f;
+                                     x[r] = see ? x[r] : 0.f;
+                                 }
+                                 if (p.kdoc)
+#pragma unroll
+                                     for (int a = 0; a < 4; ++a) {
+                                         const int4 o4 = *reinterpret_cast<const int4*>(&sdoc[buf][ib + 8 * a]);
+                                         const int o[4] = {o4.x, o4.y, o4.z, o4.w};
+#pragma unroll
+                                         for (int e = 0; e < 4; ++e) {
+                                             const bool see = o[e] == kdoc;
+                                             w[4 * a + e] = see ? w[4 * a + e] : 0.f;
+                                             x[4 * a + e] = see ? x[4 * a + e] : 0.f;
+                                         }
+                                     }
                              },
-                             [&](int r) { return i0 + ib + 8 * (r >> 2) + (r & 3) + off - j; });
+                             (float)(i0 + ib + off - j), 1.f);
                 typename AttnVec<T>::x8 w[2], d[2];
                 attn_pack<T>(S, w);
                 attn_pack<T>(dP, d);
@@ -373,6 +415,7 @@ __global__ __launch_bounds__(256, DB > 2 ? 1 : 2) void attn_dkv_kernel(AttnParam
                     }
             }
         }
+        commit(buf ^ 1);
         t = t_next;
         g = g_next;
     }

@@ -54,28 +54,43 @@ template <typename T, int KB, int DB>
 __device__ __forceinline__ void attn_softmax_step(f32x16 (&S)[KB], typename AttnVec<T>::x8 (&P)[KB][2], f32x16 (&acc)[DB], float& m, float& sum,
                                                   const AttnScore& f, bool full, int lim, int at, int j0, int half, const int* docs, int qdoc) {
     float mul = f.mul;
-    if (f.cap_out > 0.f || f.slope != 0.f || !(mul > 0.f)) {         // (uniform) the score itself instead of a multiple of it
+    if (f.cap_out > 0.f) {                                              // the score itself instead of a multiple of it
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) S[kb][r] = f.cap_out > 0.f ? f.cap_out * f.tanh_part(S[kb][r]) : S[kb][r] * f.mul;
-        if (f.slope != 0.f)
+            for (int r = 0; r < 16; ++r) S[kb][r] = f.cap_out * f.tanh_part(S[kb][r]);
+        mul = 1.f;
+    } else if (f.slope != 0.f || !(mul > 0.f)) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) S[kb][r] *= f.mul;
+        mul = 1.f;
+    }
+    if (f.slope != 0.f) {
+        const float dist = (float)(at - j0 - 4 * half);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) S[kb][r] -= f.slope * fabsf(dist - (float)(32 * kb + 8 * (r >> 2) + (r & 3)));
+    }
+    if (!full) {
+        const int last = lim - j0 - 4 * half;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) S[kb][r] = 32 * kb + 8 * (r >> 2) + (r & 3) <= last ? S[kb][r] : -INFINITY;
+        if (docs)
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) S[kb][r] -= f.slope * fabsf((float)(at - (j0 + 32 * kb + 8 * (r >> 2) + 4 * half + (r & 3))));
-        mul = 1.f;
-    }
-    if (!full) {
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int at_tile = 32 * kb + 8 * (r >> 2) + 4 * half + (r & 3);
-                bool see = j0 + at_tile <= lim;
-                if (docs) see = see && docs[at_tile] == qdoc;
-                S[kb][r] = see ? S[kb][r] : -INFINITY;
-            }
+                for (int a = 0; a < 4; ++a) {
+                    const int4 d = *reinterpret_cast<const int4*>(docs + 32 * kb + 8 * a + 4 * half);
+                    S[kb][4 * a] = d.x == qdoc ? S[kb][4 * a] : -INFINITY;
+                    S[kb][4 * a + 1] = d.y == qdoc ? S[kb][4 * a + 1] : -INFINITY;
+                    S[kb][4 * a + 2] = d.z == qdoc ? S[kb][4 * a + 2] : -INFINITY;
+                    S[kb][4 * a + 3] = d.w == qdoc ? S[kb][4 * a + 3] : -INFINITY;
+                }
     }
     float top = -INFINITY;
 #pragma unroll
@@ -83,7 +98,7 @@ __device__ __forceinline__ void attn_softmax_step(f32x16 (&S)[KB], typename Attn
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, S[kb][r]);
     top = attn_half_max(top) * mul;                                     // (mul > 0; -inf stays -inf)
-    if (__ballot(top > m + 8.f || (m == -INFINITY && top > m))) {
+    if (__ballot((top > m + 8.f) | ((m == -INFINITY) & (top > m)))) {
         const float now = fmaxf(m, top);
         const float shrink = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - now);
         m = now;
@@ -116,7 +131,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnParams p) {
 #ifdef __HIP_DEVICE_COMPILE__                            // (hipcc drops the launch stub of a template whose body its host pass cannot read)
     constexpr int ROW = DB > 2 ? 128 : 64, TILE_BYTES = ATTN_TILE * ROW * 2;
     __shared__ __align__(16) char smem[4 * TILE_BYTES];                 // [buffer][k, v]
-    __shared__ int sdoc[2][ATTN_TILE];
+    __shared__ __align__(16) int sdoc[2][ATTN_TILE];
     const int wave = attn_uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
     // consecutive workgroups go to different XCDs: give each XCD whole heads, so that its L2 serves their keys, and the longest rows first
     const int total = p.B * p.Hq * p.row_blocks, per = (total + 7) / 8;
@@ -154,19 +169,21 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnParams p) {
 
     f32x16 acc[DB] = {};
     float m = -INFINITY, sum = 0.f;
-    auto stage = [&](int t, int buf) {
-        char* at = smem + buf * 2 * TILE_BYTES;
+    int doc_next = 0;                                                   // of the tile being staged: loaded ahead of its pieces, written behind the products
+    auto stage = [&](int t, char* at) {
+        if (kdoc && wave == 0) doc_next = kdoc[min(t * ATTN_TILE + lane, p.Lk - 1)];
         sk.issue(k + (int64_t)t * ATTN_TILE * p.ks[1], n - t * ATTN_TILE, p.ks[1], p.D, at, wave);
         sv.issue(v + (int64_t)t * ATTN_TILE * p.vs[1], n - t * ATTN_TILE, p.vs[1], p.D, at + TILE_BYTES, wave);
-        if (kdoc && wave == 0) sdoc[buf][lane] = kdoc[min(t * ATTN_TILE + lane, p.Lk - 1)];
     };
     int t = tiles.next(lane);
-    if (t >= 0) stage(t, 0);
+    if (t >= 0) stage(t, smem);
+    if (kdoc && wave == 0) sdoc[0][lane] = doc_next;
     for (int buf = 0; t >= 0; buf ^= 1) {
         attn_sync();
-        const int t_next = tiles.next(lane);
-        if (t_next >= 0) stage(t_next, buf ^ 1);
+        const bool one_doc = (dlo == dhi) & (tiles.low == dlo) & (tiles.high == dlo);
         const int j0 = t * ATTN_TILE;
+        t = tiles.next(lane);
+        if (t >= 0) stage(t, smem + (buf ^ 1) * 2 * TILE_BYTES);
         if (j0 <= lim_last) {
             const char* kt = smem + buf * 2 * TILE_BYTES;
             const char* vt = kt + TILE_BYTES;
@@ -175,11 +192,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnParams p) {
             for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                 for (int c = 0; c < 2 * DB; ++c) S[kb] = attn_mfma(attn_row_frag<T, ROW>(kt, 32 * kb + l31, 2 * c + half), qf[c], S[kb]);
-            bool full = j0 + ATTN_TILE - 1 <= lim_first;
-            if (kdoc) {
-                const int2 r = p.ktiles[(int64_t)b * p.nkt + t];
-                full = full && dlo == dhi && r.x == dlo && r.y == dlo;
-            }
+            const bool full = (j0 + ATTN_TILE - 1 <= lim_first) & one_doc;
             typename AttnVec<T>::x8 P[2][2];
             attn_softmax_step<T, 2, DB>(S, P, acc, m, sum, f, full, lim, i + n - p.Lq, j0, half, kdoc ? sdoc[buf] : nullptr, qdoc);
 #pragma unroll
@@ -189,7 +202,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnParams p) {
 #pragma unroll
                     for (int c = 0; c < 2; ++c) acc[db] = attn_mfma(attn_col_frag<T, ROW>(vt, 32 * kb + 16 * c, db, lane), P[kb][c], acc[db]);
         }
-        t = t_next;
+        if (kdoc && wave == 0) sdoc[buf ^ 1][lane] = doc_next;
     }
     sum = attn_half_sum(sum);
     const float by = sum == 0.f ? 0.f : 1.f / sum;
@@ -224,7 +237,7 @@ __global__ __launch_bounds__(256) void attn_token_kernel(AttnParams p) {
     constexpr int ROW = DB > 2 ? 128 : 64, KEYS = 32, TILE_BYTES = KEYS * ROW * 2, WAVES = 4;
     extern __shared__ __align__(16) char smem[];                        // [wave][buffer][k, v], then the waves' results
     __shared__ float sm[WAVES][32], ssum[WAVES][32];
-    __shared__ int sdoc[WAVES][2][KEYS];
+    __shared__ __align__(16) int sdoc[WAVES][2][KEYS];
     const int wave = attn_uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
     const int split = blockIdx.x % p.splits, blk = blockIdx.x / p.splits % p.row_blocks, bh = blockIdx.x / (p.splits * p.row_blocks);
     const int hk = bh % p.Hk, b = bh / p.Hk, rows = p.Lq * p.G;
@@ -245,22 +258,24 @@ __global__ __launch_bounds__(256) void attn_token_kernel(AttnParams p) {
     const T* v = (const T*)p.v + b * p.vs[0] + hk * p.vs[2];
     const int* kdoc = p.kdoc ? p.kdoc + b * p.kdoc_stride : nullptr;
     AttnScore f(p, row_ok ? h : hk * p.G);
-    const bool same_slope = !p.slopes;
     AttnStage<ROW, KEYS, 1> sk, sv;
     sk.setup(0, lane, p.ks[1], p.D);
     sv.setup(0, lane, p.vs[1], p.D);
     char* mine = smem + wave * 4 * TILE_BYTES;
+    int doc_next = 0;
     auto stage = [&](int j0, int buf) {
+        if (kdoc && lane < KEYS) doc_next = kdoc[min(j0 + lane, p.Lk - 1)];
         sk.issue(k + (int64_t)j0 * p.ks[1], n - j0, p.ks[1], p.D, mine + buf * 2 * TILE_BYTES, 0);
         sv.issue(v + (int64_t)j0 * p.vs[1], n - j0, p.vs[1], p.D, mine + buf * 2 * TILE_BYTES + TILE_BYTES, 0);
-        if (kdoc && lane < KEYS) sdoc[wave][buf][lane] = kdoc[min(j0 + lane, p.Lk - 1)];
     };
     f32x16 acc[DB] = {};
     float m = -INFINITY, sum = 0.f;
     int j0 = k0 + wave * KEYS;
     if (j0 < k1) stage(j0, 0);
+    if (kdoc && lane < KEYS) sdoc[wave][0][lane] = doc_next;
     for (int buf = 0; j0 < k1; buf ^= 1, j0 += WAVES * KEYS) {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");    // the wave's own pieces: no other wave touches this LDS
+        asm volatile("" ::: "memory");
+        attn_landed();                                                  // the wave's own pieces: no other wave touches this LDS
         if (j0 + WAVES * KEYS < k1) stage(j0 + WAVES * KEYS, buf ^ 1);
         const char* kt = mine + buf * 2 * TILE_BYTES;
         f32x16 S[1] = {};
@@ -273,8 +288,8 @@ __global__ __launch_bounds__(256) void attn_token_kernel(AttnParams p) {
         for (int db = 0; db < DB; ++db)
 #pragma unroll
             for (int c = 0; c < 2; ++c) acc[db] = attn_mfma(attn_col_frag<T, ROW>(kt + TILE_BYTES, 16 * c, db, lane), P[0][c], acc[db]);
+        if (kdoc && lane < KEYS) sdoc[wave][buf ^ 1][lane] = doc_next;
     }
-    (void)same_slope;
     // join the four waves: common maximum, then the accumulators through the LDS, one [32 rows][32 * DB + 1] float image a wave
     constexpr int PITCH = 32 * DB + 1;
     sum = attn_half_sum(sum);
