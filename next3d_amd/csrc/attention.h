@@ -121,31 +121,52 @@ struct AttnStage {
             voff[i] = c * 8 < D ? row * (int)stride * 2 + c * 16 : (int)0x80000000;
         }
     }
-    // rows [0, rows) of `base` (rows >= 1) -> lds
-    __device__ __forceinline__ void issue(const void* base, int rows, int64_t stride, int D, char* lds, int wave) const {
-        const uint64_t a = (uint64_t)base;
-        const int n = ((rows < ROWS ? rows : ROWS) - 1) * (int)stride * 2 + D * 2;
-        const i32x4 r = {attn_uniform((int)a), attn_uniform((int)(a >> 32) & 0xffff), attn_uniform(n), 0x00020000};
-        const uint32_t to = (uint32_t)(uintptr_t)(attn_lds_void*)lds + wave * 1024;
+    // rows [t ROWS, ...) of the `rows` rows at `base` -> lds (t ROWS < rows)
+    __device__ __forceinline__ void issue(uint64_t base, int t, int rows, int stride, int D, uint32_t lds, int wave) const {
+        const int left = rows - t * ROWS;
+        const uint64_t a = base + (uint64_t)(uint32_t)t * (uint32_t)(ROWS * 2 * stride);
+        const int n = ((left < ROWS ? left : ROWS) - 1) * stride * 2 + D * 2;
+        const i32x4 r = {attn_uniform((int)a), attn_uniform((int)(a >> 32)), attn_uniform(n), 0x00020000};
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) attn_piece(r, voff[i], attn_uniform(to + i * WAVES * 1024));
+        for (int i = 0; i < PIECES; ++i) attn_piece(r, voff[i], attn_uniform(lds + (wave + i * WAVES) * 1024));
     }
 };
+__device__ __forceinline__ uint32_t attn_lds(const void* p) { return (uint32_t)(uintptr_t)(attn_lds_void*)p; }
+__device__ __forceinline__ uint64_t attn_addr(const void* p) { return (uint64_t)p & 0xffffffffffffull; }       // (48 bits: the descriptor's upper 16 are 0)
 
-// first operand, rows = tile rows row0 + l31, k = channels: chunk 2 c + half
+// Where a lane reads its fragments of a tile at LDS address `tile` (a multiple of 256).  The compiler would keep every fragment's address in a register of its own across the
+// loop; the empty asm makes the two bases new in each iteration, and an exclusive or (chunks) and the instruction's offset (rows) give the rest.
+template <int ROW>
+struct AttnLane {
+    uint32_t row0, col0;
+    __device__ __forceinline__ AttnLane(int lane) {
+        const int l31 = lane & 31, half = lane >> 5, l16 = lane & 15, r = 4 * half + (l16 >> 2);
+        row0 = l31 * (ROW * 2) + ((half ^ attn_swizzle<ROW>(l31)) << 4);
+        col0 = r * (ROW * 2) + (((((lane >> 4) & 1) * 2 + ((l16 & 3) >> 1)) ^ attn_swizzle<ROW>(r)) << 4) + (l16 & 1) * 8;
+    }
+    __device__ __forceinline__ uint32_t rows(uint32_t tile) const {
+        uint32_t a = row0 + tile;
+        asm volatile("" : "+v"(a));
+        return a;
+    }
+    __device__ __forceinline__ uint32_t cols(uint32_t tile) const {
+        uint32_t a = col0 + tile;
+        asm volatile("" : "+v"(a));
+        return a;
+    }
+};
+// first operand, rows = tile rows 32 block + l31, k = channels 16 c + 8 half + 0..7
 template <typename T, int ROW>
-__device__ __forceinline__ typename AttnVec<T>::x8 attn_row_frag(const char* tile, int row, int chunk) {
-    return *reinterpret_cast<const typename AttnVec<T>::x8*>(tile + row * (ROW * 2) + ((chunk ^ attn_swizzle<ROW>(row)) << 4));
+__device__ __forceinline__ typename AttnVec<T>::x8 attn_row_frag(uint32_t rows, int block, int c) {
+    typedef __attribute__((address_space(3))) const typename AttnVec<T>::x8* ptr;
+    return *(ptr)(uintptr_t)((rows ^ (c << 5)) + block * 32 * ROW * 2);
 }
-// first operand, rows = channels 32 db + l31, k = tile rows row0 + {4 half + 0..3, 8 + 4 half + 0..3} (row0 a multiple of 16)
+// first operand, rows = channels 32 db + l31, k = tile rows 16 block + {4 half + 0..3, 8 + 4 half + 0..3}; eight rows on, bit 1 of the swizzle differs
 template <typename T, int ROW>
-__device__ __forceinline__ typename AttnVec<T>::x8 attn_col_frag(const char* tile, int row0, int db, int lane) {
-    const int half = lane >> 5, l16 = lane & 15;
-    const int row = row0 + 4 * half + (l16 >> 2), chunk = 4 * db + ((lane >> 4) & 1) * 2 + ((l16 & 3) >> 1), in = (l16 & 1) * 8;
-    const char* lo = tile + row * (ROW * 2) + ((chunk ^ attn_swizzle<ROW>(row)) << 4) + in;
-    const char* hi = tile + (row + 8) * (ROW * 2) + ((chunk ^ attn_swizzle<ROW>(row + 8)) << 4) + in;
-    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)lo);
-    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)hi);
+__device__ __forceinline__ typename AttnVec<T>::x8 attn_col_frag(uint32_t cols, int block, int db) {
+    typedef __attribute__((address_space(3))) s16x4* ptr;
+    const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(uintptr_t)((cols ^ (db << 6)) + block * 16 * ROW * 2));
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(uintptr_t)((cols ^ (db << 6) ^ 32) + block * 16 * ROW * 2 + 8 * ROW * 2));
     typedef short s16x8 __attribute__((ext_vector_type(8)));
     const s16x8 v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     return __builtin_bit_cast(typename AttnVec<T>::x8, v);
@@ -170,17 +191,18 @@ __device__ __forceinline__ void attn_sync() {
 }
 
 // ---- which tiles to visit: [t, end) in order; with documents only those whose range [lowest, highest] meets [lo, hi] (64 ranges looked at together)
+template <bool DOCS>
 struct AttnTiles {
     const int2* ranges;
-    int t, end, lo, hi, base, low, high;                     // low, high: documents of the tile last returned
+    int t, end, lo, hi, base, low = 0, high = 0;             // low, high: documents of the tile last returned
     uint64_t bits;
     int2 mine;
     __device__ __forceinline__ void start(const int2* r, int first, int stop, int dlo, int dhi) {
-        ranges = r; t = first; end = stop; lo = dlo; hi = dhi; bits = 0; base = first - 64; low = high = 0;
+        ranges = r; t = first; end = stop; lo = dlo; hi = dhi; bits = 0; base = first - 64;
     }
     // the next tile or -1
     __device__ __forceinline__ int next(int lane) {
-        if (!ranges) return t < end ? t++ : -1;
+        if (!DOCS || !ranges) return t < end ? t++ : -1;
         while (bits == 0) {
             base += 64;
             if (base >= end) return -1;
@@ -268,6 +290,26 @@ static inline const char* attn_params(const n3d_attention_desc* d, AttnParams& p
     p.causal = d->causal != 0; p.scale = d->scale; p.softcap = d->softcap;
     p.splits = 1;
     return nullptr;
+}
+
+// f(element type, 32-channel blocks, FORM: the score is not a positive multiple of the raw product)
+template <typename F>
+static inline void attn_dispatch(int dtype, const AttnParams& p, F&& f) {
+    const bool form = p.softcap > 0.f || p.slopes || !(p.scale > 0.f);
+    auto with = [&](auto* t, auto db) {
+        if (form) f(t, db, std::true_type());
+        else f(t, db, std::false_type());
+    };
+    auto typed = [&](auto* t) {
+        switch (cdiv(p.D, 32)) {
+            case 1: with(t, std::integral_constant<int, 1>()); break;
+            case 2: with(t, std::integral_constant<int, 2>()); break;
+            case 3: with(t, std::integral_constant<int, 3>()); break;
+            default: with(t, std::integral_constant<int, 4>()); break;
+        }
+    };
+    if (dtype == N3D_F16) typed((_Float16*)nullptr);
+    else typed((__bf16*)nullptr);
 }
 
 // workspace, in floats: the document ranges come first

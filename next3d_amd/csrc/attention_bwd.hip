@@ -139,7 +139,7 @@ template <typename T, int DB>
 __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnParams p) {
 #ifdef __HIP_DEVICE_COMPILE__                            // (hipcc drops the launch stub of a template whose body its host pass cannot read)
     constexpr int ROW = DB > 2 ? 128 : 64, TILE_BYTES = ATTN_TILE * ROW * 2;
-    __shared__ __align__(16) char smem[4 * TILE_BYTES];
+    __shared__ __align__(1024) char smem[4 * TILE_BYTES];
     __shared__ __align__(16) int sdoc[2][ATTN_TILE];
     const int wave = attn_uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
     const int total = p.B * p.Hq * p.row_blocks, per = (total + 7) / 8;
@@ -160,7 +160,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnParams p) {
         dlo = min(r0.x, r1.x);
         dhi = max(r0.y, r1.y);
     }
-    AttnTiles tiles;
+    AttnTiles<true> tiles;
     tiles.start(p.kdoc ? p.ktiles + (int64_t)b * p.nkt : nullptr, 0, (key_end + ATTN_TILE - 1) / ATTN_TILE, max(dlo, 0), dhi);
     typename AttnVec<T>::x8 qf[2 * DB], df[2 * DB];
     const T* q = row_ok ? (const T*)p.q + b * p.qs[0] + i * p.qs[1] + h * p.qs[2] : nullptr;
@@ -182,12 +182,16 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnParams p) {
     sk.setup(wave, lane, p.ks[1], p.D);
     sv.setup(wave, lane, p.vs[1], p.D);
     f32x16 acc[DB] = {};
+    const uint64_t k_at = attn_addr(k), v_at = attn_addr(v);
+    const int k_row = (int)p.ks[1], v_row = (int)p.vs[1];
+    const AttnLane<ROW> at_lane(lane);
+    const uint32_t lds = attn_lds(smem);
     int doc_next = 0;                                                   // of the tile being staged: loaded ahead of its pieces, written behind the products
     auto stage = [&](int t, int buf) {
-        char* at = smem + buf * 2 * TILE_BYTES;
+        const uint32_t at = lds + buf * 2 * TILE_BYTES;
         if (kdoc && wave == 0) doc_next = kdoc[min(t * ATTN_TILE + lane, p.Lk - 1)];
-        sk.issue(k + (int64_t)t * ATTN_TILE * p.ks[1], n - t * ATTN_TILE, p.ks[1], p.D, at, wave);
-        sv.issue(v + (int64_t)t * ATTN_TILE * p.vs[1], n - t * ATTN_TILE, p.vs[1], p.D, at + TILE_BYTES, wave);
+        sk.issue(k_at, t, n, k_row, p.D, at, wave);
+        sv.issue(v_at, t, n, v_row, p.D, at + TILE_BYTES, wave);
     };
     int t = tiles.next(lane);
     if (t >= 0) stage(t, 0);
@@ -199,16 +203,16 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnParams p) {
         if (t_next >= 0) stage(t_next, buf ^ 1);
         const int j0 = t * ATTN_TILE;
         if (j0 <= lim_last) {
-            const char* kt = smem + buf * 2 * TILE_BYTES;
-            const char* vt = kt + TILE_BYTES;
+            const uint32_t k_lds = at_lane.rows(lds + buf * 2 * TILE_BYTES), v_lds = at_lane.rows(lds + buf * 2 * TILE_BYTES + TILE_BYTES);
+            const uint32_t kc_lds = at_lane.cols(lds + buf * 2 * TILE_BYTES);
             const bool full = (j0 + ATTN_TILE - 1 <= lim_first) & one_doc;
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
                 f32x16 S = {}, dP = {};
 #pragma unroll
                 for (int c = 0; c < 2 * DB; ++c) {
-                    S = attn_mfma(attn_row_frag<T, ROW>(kt, 32 * kb + l31, 2 * c + half), qf[c], S);
-                    dP = attn_mfma(attn_row_frag<T, ROW>(vt, 32 * kb + l31, 2 * c + half), df[c], dP);
+                    S = attn_mfma(attn_row_frag<T, ROW>(k_lds, kb, c), qf[c], S);
+                    dP = attn_mfma(attn_row_frag<T, ROW>(v_lds, kb, c), df[c], dP);
                 }
                 const int jb = j0 + 32 * kb + 4 * half;
                 attn_ds_step(S, dP, f, ds_by, full, [&](int) { return make_float4(lse2, lse2, lse2, lse2); }, [&](int) { return make_float4(delta, delta, delta, delta); },
@@ -232,7 +236,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnParams p) {
 #pragma unroll
                 for (int db = 0; db < DB; ++db)
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) acc[db] = attn_mfma(attn_col_frag<T, ROW>(kt, 32 * kb + 16 * c, db, lane), d[c], acc[db]);
+                    for (int c = 0; c < 2; ++c) acc[db] = attn_mfma(attn_col_frag<T, ROW>(kc_lds, 2 * kb + c, db), d[c], acc[db]);
             }
         }
         if (kdoc && wave == 0) sdoc[buf ^ 1][lane] = doc_next;
@@ -282,7 +286,7 @@ __global__ __launch_bounds__(256, DB > 2 ? 1 : 2) void attn_dkv_kernel(AttnParam
 #ifdef __HIP_DEVICE_COMPILE__                            // (hipcc drops the launch stub of a template whose body its host pass cannot read)
     constexpr int ROW = DB > 2 ? 128 : 64, TILE_BYTES = ATTN_TILE * ROW * 2;
     constexpr float SHIFT = ATTN_P_SHIFT<T>;
-    __shared__ __align__(16) char smem[4 * TILE_BYTES];                 // [buffer][q, do]
+    __shared__ __align__(1024) char smem[4 * TILE_BYTES];                 // [buffer][q, do]
     __shared__ __align__(16) float slse[2][ATTN_TILE], sdelta[2][ATTN_TILE];
     __shared__ __align__(16) int sdoc[2][ATTN_TILE];
     const int wave = attn_uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
@@ -311,7 +315,7 @@ __global__ __launch_bounds__(256, DB > 2 ? 1 : 2) void attn_dkv_kernel(AttnParam
     }
     const int2* ranges = p.kdoc ? p.qtiles + (int64_t)b * p.nqt : nullptr;
     const int t_first = first_query(k0) / ATTN_TILE, t_end = k0 < n ? p.nqt : 0;
-    AttnTiles tiles;
+    AttnTiles<true> tiles;
     int g = g0;
     tiles.start(ranges, t_first, t_end, max(dlo, 0), dhi);
     auto next = [&](int& gn) {
@@ -336,18 +340,20 @@ __global__ __launch_bounds__(256, DB > 2 ? 1 : 2) void attn_dkv_kernel(AttnParam
     sd.setup(wave, lane, p.ds[1], p.D);
     const int ds_exp = attn_ds_scale(p, lane);
     const float ds_by = ldexpf(1.f, ds_exp - (int)SHIFT);
+    const AttnLane<ROW> at_lane(lane);
+    const uint32_t lds = attn_lds(smem);
     float row_next = 0.f;
     auto stage = [&](int t, int gt, int buf) {
         const int h = hk * p.G + gt, i0 = t * ATTN_TILE;
-        char* at = smem + buf * 2 * TILE_BYTES;
+        const uint32_t at = lds + buf * 2 * TILE_BYTES;
         // the rows' statistics: loaded ahead of the pieces (one of the three a wave), written to the LDS behind the products of the tile before
         const int i = i0 + lane;
         const int64_t stat = ((int64_t)b * p.Hq + h) * p.Lq + i;
         if (wave == 0) row_next = i < p.Lq ? attn_lse2(p.lse[stat]) - SHIFT : INFINITY;            // (queries behind the last: every weight 0)
         if (wave == 1) row_next = i < p.Lq ? p.delta[stat] : 0.f;
         if (wave == 2 && p.kdoc) row_next = __builtin_bit_cast(float, i < p.Lq ? p.qdoc[b * p.qdoc_stride + i] : -1);
-        sq.issue((const T*)p.q + b * p.qs[0] + i0 * p.qs[1] + h * p.qs[2], p.Lq - i0, p.qs[1], p.D, at, wave);
-        sd.issue((const T*)p.dout + b * p.ds[0] + i0 * p.ds[1] + h * p.ds[2], p.Lq - i0, p.ds[1], p.D, at + TILE_BYTES, wave);
+        sq.issue(attn_addr((const T*)p.q + b * p.qs[0] + h * p.qs[2]), t, p.Lq, (int)p.qs[1], p.D, at, wave);
+        sd.issue(attn_addr((const T*)p.dout + b * p.ds[0] + h * p.ds[2]), t, p.Lq, (int)p.ds[1], p.D, at + TILE_BYTES, wave);
     };
     auto commit = [&](int buf) {
         if (wave == 0) slse[buf][lane] = row_next;
@@ -366,8 +372,8 @@ __global__ __launch_bounds__(256, DB > 2 ? 1 : 2) void attn_dkv_kernel(AttnParam
         if (t_next >= 0) stage(t_next, g_next, buf ^ 1);
         const int i0 = t * ATTN_TILE;
         if (wave_on && i0 + ATTN_TILE - 1 >= wave_first) {
-            const char* qt = smem + buf * 2 * TILE_BYTES;
-            const char* dt = qt + TILE_BYTES;
+            const uint32_t q_lds = at_lane.rows(lds + buf * 2 * TILE_BYTES), d_lds = at_lane.rows(lds + buf * 2 * TILE_BYTES + TILE_BYTES);
+            const uint32_t qc_lds = at_lane.cols(lds + buf * 2 * TILE_BYTES), dc_lds = at_lane.cols(lds + buf * 2 * TILE_BYTES + TILE_BYTES);
             const AttnScore f(p, hk * p.G + g);
             const bool full = (i0 >= wave_full) & one_doc;
 #pragma unroll
@@ -375,8 +381,8 @@ __global__ __launch_bounds__(256, DB > 2 ? 1 : 2) void attn_dkv_kernel(AttnParam
                 f32x16 S = {}, dP = {};
 #pragma unroll
                 for (int c = 0; c < 2 * DB; ++c) {
-                    S = attn_mfma(attn_row_frag<T, ROW>(qt, 32 * qb + l31, 2 * c + half), kf[c], S);
-                    dP = attn_mfma(attn_row_frag<T, ROW>(dt, 32 * qb + l31, 2 * c + half), vf[c], dP);
+                    S = attn_mfma(attn_row_frag<T, ROW>(q_lds, qb, c), kf[c], S);
+                    dP = attn_mfma(attn_row_frag<T, ROW>(d_lds, qb, c), vf[c], dP);
                 }
                 const int ib = 32 * qb + 4 * half;
                 attn_ds_step(S, dP, f, ds_by, full, [&](int a) { return *reinterpret_cast<const float4*>(&slse[buf][ib + 8 * a]); },
@@ -410,8 +416,8 @@ __global__ __launch_bounds__(256, DB > 2 ? 1 : 2) void attn_dkv_kernel(AttnParam
                 for (int db = 0; db < DB; ++db)
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        dv[db] = attn_mfma(attn_col_frag<T, ROW>(dt, 32 * qb + 16 * c, db, lane), w[c], dv[db]);
-                        dk[db] = attn_mfma(attn_col_frag<T, ROW>(qt, 32 * qb + 16 * c, db, lane), d[c], dk[db]);
+                        dv[db] = attn_mfma(attn_col_frag<T, ROW>(dc_lds, 2 * qb + c, db), w[c], dv[db]);
+                        dk[db] = attn_mfma(attn_col_frag<T, ROW>(qc_lds, 2 * qb + c, db), d[c], dk[db]);
                     }
             }
         }

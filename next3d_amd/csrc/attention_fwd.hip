@@ -49,32 +49,31 @@ __device__ void attn_exact_row(const AttnParams& p, int b, int i, int h, int k0,
     }
 }
 
-// one wave's softmax step over the 32 queries of its lanes: S (raw products of KB blocks of 32 keys) -> P as second operands; rescales acc, sum and m
-template <typename T, int KB, int DB>
-__device__ __forceinline__ void attn_softmax_step(f32x16 (&S)[KB], typename AttnVec<T>::x8 (&P)[KB][2], f32x16 (&acc)[DB], float& m, float& sum,
-                                                  const AttnScore& f, bool full, int lim, int at, int j0, int half, const int* docs, int qdoc) {
-    float mul = f.mul;
-    if (f.cap_out > 0.f) {                                              // the score itself instead of a multiple of it
+// One wave's softmax step over the 32 queries of its lanes: S (raw products of KB blocks of 32 keys) -> P as second operands; rescales acc, sum and m.
+// FORM: the score is not a positive multiple of the raw product (a cap, a slope, a scale <= 0).  MASK: not every key of the tile is visible to every query.
+// (Each combination is straight code of its own: values that pass through a branch in place cost a register copy each.)
+template <typename T, int KB, int DB, bool FORM, bool MASK>
+__device__ __forceinline__ void attn_softmax_form(f32x16 (&S)[KB], typename AttnVec<T>::x8 (&P)[KB][2], f32x16 (&acc)[DB], float& m, float& sum, const AttnScore& f,
+                                                  int lim, int at, int j0, int half, const int* docs, int qdoc) {
+    if constexpr (FORM) {
+        if (f.cap_out > 0.f) {
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
+            for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) S[kb][r] = f.cap_out * f.tanh_part(S[kb][r]);
-        mul = 1.f;
-    } else if (f.slope != 0.f || !(mul > 0.f)) {
+                for (int r = 0; r < 16; ++r) S[kb][r] = f.cap_out * f.tanh_part(S[kb][r]);
+        } else {
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
+            for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) S[kb][r] *= f.mul;
-        mul = 1.f;
-    }
-    if (f.slope != 0.f) {
+                for (int r = 0; r < 16; ++r) S[kb][r] *= f.mul;
+        }
         const float dist = (float)(at - j0 - 4 * half);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int r = 0; r < 16; ++r) S[kb][r] -= f.slope * fabsf(dist - (float)(32 * kb + 8 * (r >> 2) + (r & 3)));
     }
-    if (!full) {
+    if constexpr (MASK) {
         const int last = lim - j0 - 4 * half;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
@@ -90,14 +89,16 @@ __device__ __forceinline__ void attn_softmax_step(f32x16 (&S)[KB], typename Attn
                     S[kb][4 * a + 1] = d.y == qdoc ? S[kb][4 * a + 1] : -INFINITY;
                     S[kb][4 * a + 2] = d.z == qdoc ? S[kb][4 * a + 2] : -INFINITY;
                     S[kb][4 * a + 3] = d.w == qdoc ? S[kb][4 * a + 3] : -INFINITY;
+                    if (a & 1) __builtin_amdgcn_sched_barrier(0);     // (two loads at a time: registers)
                 }
     }
-    float top = -INFINITY;
+    float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, S[kb][r]);
-    top = attn_half_max(top) * mul;                                     // (mul > 0; -inf stays -inf)
+        for (int r = 0; r < 16; ++r) tops[r & 3] = fmaxf(tops[r & 3], S[kb][r]);
+    const float mul = FORM ? 1.f : f.mul;
+    const float top = attn_half_max(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]))) * mul;          // (mul > 0; -inf stays -inf)
     if (__ballot((top > m + 8.f) | ((m == -INFINITY) & (top > m)))) {
         const float now = fmaxf(m, top);
         const float shrink = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - now);
@@ -109,13 +110,13 @@ __device__ __forceinline__ void attn_softmax_step(f32x16 (&S)[KB], typename Attn
             for (int r = 0; r < 16; ++r) acc[db][r] *= shrink;
     }
     const float sub = m == -INFINITY ? 0.f : m;
-    float add = 0.f;
+    float add[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             S[kb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[kb][r], mul, -sub));
-            add += S[kb][r];
+            add[r & 3] += S[kb][r];
         }
         // weights to 16 bits (half a step of the inputs' own type, each on its own: their sum above is of the unrounded ones)
 #pragma unroll
@@ -123,14 +124,20 @@ __device__ __forceinline__ void attn_softmax_step(f32x16 (&S)[KB], typename Attn
 #pragma unroll
             for (int e = 0; e < 8; ++e) P[kb][c][e] = (T)S[kb][8 * c + e];
     }
-    sum += add;
+    sum += (add[0] + add[1]) + (add[2] + add[3]);
+}
+template <typename T, int KB, int DB, bool FORM>
+__device__ __forceinline__ void attn_softmax_step(f32x16 (&S)[KB], typename AttnVec<T>::x8 (&P)[KB][2], f32x16 (&acc)[DB], float& m, float& sum, const AttnScore& f,
+                                                  bool full, int lim, int at, int j0, int half, const int* docs, int qdoc) {
+    if (full) attn_softmax_form<T, KB, DB, FORM, false>(S, P, acc, m, sum, f, lim, at, j0, half, docs, qdoc);
+    else attn_softmax_form<T, KB, DB, FORM, true>(S, P, acc, m, sum, f, lim, at, j0, half, docs, qdoc);
 }
 
-template <typename T, int DB>
+template <typename T, int DB, bool FORM, bool DOCS>
 __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnParams p) {
 #ifdef __HIP_DEVICE_COMPILE__                            // (hipcc drops the launch stub of a template whose body its host pass cannot read)
     constexpr int ROW = DB > 2 ? 128 : 64, TILE_BYTES = ATTN_TILE * ROW * 2;
-    __shared__ __align__(16) char smem[4 * TILE_BYTES];                 // [buffer][k, v]
+    __shared__ __align__(1024) char smem[4 * TILE_BYTES];                 // [buffer][k, v]
     __shared__ __align__(16) int sdoc[2][ATTN_TILE];
     const int wave = attn_uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
     // consecutive workgroups go to different XCDs: give each XCD whole heads, so that its L2 serves their keys, and the longest rows first
@@ -141,19 +148,19 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnParams p) {
     const int n = attn_keys(p, b), prefix = p.prefix ? p.prefix[b] : 0, q0 = blk * 128;
     const int i = q0 + 32 * wave + l31;
     const bool row_ok = i < p.Lq;
-    const int qdoc = p.kdoc && row_ok ? p.qdoc[b * p.qdoc_stride + i] : 0;
+    const int qdoc = DOCS && row_ok ? p.qdoc[b * p.qdoc_stride + i] : 0;
     const int lim = !row_ok || qdoc < 0 ? -1 : attn_limit(p, i, n, prefix);
-    const int lim_first = attn_limit(p, q0 + 32 * wave, n, prefix), lim_last = attn_limit(p, min(q0 + 32 * wave + 31, p.Lq - 1), n, prefix);
+    const int lim_last = attn_limit(p, min(q0 + 32 * wave + 31, p.Lq - 1), n, prefix);
     const int key_end = attn_limit(p, min(q0 + 127, p.Lq - 1), n, prefix) + 1;
     int dlo = 0, dhi = 0;
-    if (p.kdoc) {                                                       // documents of this workgroup's queries: two ranges of ATTN_TILE queries
+    if constexpr (DOCS) {                                                       // documents of this workgroup's queries: two ranges of ATTN_TILE queries
         const int2* r = p.qtiles + (int64_t)b * p.nqt + 2 * blk;
         const int2 r0 = r[0], r1 = 2 * blk + 1 < p.nqt ? r[1] : r[0];
         dlo = min(r0.x, r1.x);
         dhi = max(r0.y, r1.y);
     }
-    AttnTiles tiles;
-    tiles.start(p.kdoc ? p.ktiles + (int64_t)b * p.nkt : nullptr, 0, (key_end + ATTN_TILE - 1) / ATTN_TILE, max(dlo, 0), dhi);
+    AttnTiles<DOCS> tiles;
+    tiles.start(DOCS ? p.ktiles + (int64_t)b * p.nkt : nullptr, 0, (key_end + ATTN_TILE - 1) / ATTN_TILE, max(dlo, 0), dhi);
 
     typename AttnVec<T>::x8 qf[2 * DB];
     const T* q = row_ok ? (const T*)p.q + b * p.qs[0] + i * p.qs[1] + h * p.qs[2] : nullptr;
@@ -161,7 +168,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnParams p) {
     for (int c = 0; c < 2 * DB; ++c) qf[c] = attn_lane_frag<T>(q, 2 * c + half, p.D);
     const T* k = (const T*)p.k + b * p.ks[0] + hk * p.ks[2];
     const T* v = (const T*)p.v + b * p.vs[0] + hk * p.vs[2];
-    const int* kdoc = p.kdoc ? p.kdoc + b * p.kdoc_stride : nullptr;
+    const int* kdoc = DOCS ? p.kdoc + b * p.kdoc_stride : nullptr;
     const AttnScore f(p, h);
     AttnStage<ROW, ATTN_TILE, 4> sk, sv;
     sk.setup(wave, lane, p.ks[1], p.D);
@@ -170,39 +177,72 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnParams p) {
     f32x16 acc[DB] = {};
     float m = -INFINITY, sum = 0.f;
     int doc_next = 0;                                                   // of the tile being staged: loaded ahead of its pieces, written behind the products
-    auto stage = [&](int t, char* at) {
-        if (kdoc && wave == 0) doc_next = kdoc[min(t * ATTN_TILE + lane, p.Lk - 1)];
-        sk.issue(k + (int64_t)t * ATTN_TILE * p.ks[1], n - t * ATTN_TILE, p.ks[1], p.D, at, wave);
-        sv.issue(v + (int64_t)t * ATTN_TILE * p.vs[1], n - t * ATTN_TILE, p.vs[1], p.D, at + TILE_BYTES, wave);
+    const uint64_t k_at = attn_addr(k), v_at = attn_addr(v);
+    const int k_row = (int)p.ks[1], v_row = (int)p.vs[1];
+    const AttnLane<ROW> at_lane(lane);
+    const uint32_t lds = attn_lds(smem);
+    auto stage = [&](int t, int buf) {
+        if (DOCS && wave == 0) doc_next = kdoc[min(t * ATTN_TILE + lane, p.Lk - 1)];
+        sk.issue(k_at, t, n, k_row, p.D, lds + buf * 2 * TILE_BYTES, wave);
+        sv.issue(v_at, t, n, v_row, p.D, lds + buf * 2 * TILE_BYTES + TILE_BYTES, wave);
     };
-    int t = tiles.next(lane);
-    if (t >= 0) stage(t, smem);
-    if (kdoc && wave == 0) sdoc[0][lane] = doc_next;
-    for (int buf = 0; t >= 0; buf ^= 1) {
+    int t = tiles.next(lane), buf = 0;
+    if (t >= 0) stage(t, 0);
+    if (DOCS && wave == 0) sdoc[0][lane] = doc_next;
+    // every key of tile t visible to every query of the workgroup
+    const int full_end = DOCS && dlo != dhi ? 0 : attn_limit(p, q0, n, prefix) + 1;
+    auto full = [&] { return (t + 1) * ATTN_TILE <= full_end && (!DOCS || ((tiles.low == dlo) & (tiles.high == dlo))); };
+    auto visit = [&](auto mask) {
+        const int j0 = t * ATTN_TILE, now = buf;
         attn_sync();
-        const bool one_doc = (dlo == dhi) & (tiles.low == dlo) & (tiles.high == dlo);
-        const int j0 = t * ATTN_TILE;
         t = tiles.next(lane);
-        if (t >= 0) stage(t, smem + (buf ^ 1) * 2 * TILE_BYTES);
-        if (j0 <= lim_last) {
-            const char* kt = smem + buf * 2 * TILE_BYTES;
-            const char* vt = kt + TILE_BYTES;
+        buf ^= 1;
+        if (t >= 0) stage(t, buf);
+        if (!mask.value || j0 <= lim_last) {
+            const uint32_t k_lds = at_lane.rows(lds + now * 2 * TILE_BYTES), v_lds = at_lane.cols(lds + now * 2 * TILE_BYTES + TILE_BYTES);
+            // every fragment is on its way before the first product that needs one: keys ahead of the scores, values (their first half, where registers
+            // are short) ahead of the softmax
+            constexpr int AHEAD = DB > 2 ? 1 : 2;
+            typename AttnVec<T>::x8 kf[2][2 * DB], vf[DB][2][2], P[2][2];
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int c = 0; c < 2 * DB; ++c) kf[kb][c] = attn_row_frag<T, ROW>(k_lds, kb, c);
+            __builtin_amdgcn_sched_barrier(0);
             f32x16 S[2] = {};
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-                for (int c = 0; c < 2 * DB; ++c) S[kb] = attn_mfma(attn_row_frag<T, ROW>(kt, 32 * kb + l31, 2 * c + half), qf[c], S[kb]);
-            const bool full = (j0 + ATTN_TILE - 1 <= lim_first) & one_doc;
-            typename AttnVec<T>::x8 P[2][2];
-            attn_softmax_step<T, 2, DB>(S, P, acc, m, sum, f, full, lim, i + n - p.Lq, j0, half, kdoc ? sdoc[buf] : nullptr, qdoc);
+                for (int c = 0; c < 2 * DB; ++c) S[kb] = attn_mfma(kf[kb][c], qf[c], S[kb]);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int db = 0; db < DB; ++db)
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
+                for (int kb = 0; kb < AHEAD; ++kb)
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) acc[db] = attn_mfma(attn_col_frag<T, ROW>(vt, 32 * kb + 16 * c, db, lane), P[kb][c], acc[db]);
+                    for (int c = 0; c < 2; ++c) vf[db][kb][c] = attn_col_frag<T, ROW>(v_lds, 2 * kb + c, db);
+            __builtin_amdgcn_sched_barrier(0);
+            attn_softmax_form<T, 2, DB, FORM, mask.value>(S, P, acc, m, sum, f, lim, i + n - p.Lq, j0, half, DOCS ? sdoc[now] : nullptr, qdoc);
+#pragma unroll
+            for (int kb = AHEAD; kb < 2; ++kb)
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) vf[db][kb][c] = attn_col_frag<T, ROW>(v_lds, 2 * kb + c, db);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) acc[db] = attn_mfma(vf[db][kb][c], P[kb][c], acc[db]);
         }
-        if (kdoc && wave == 0) sdoc[buf ^ 1][lane] = doc_next;
+        if (DOCS && wave == 0) sdoc[buf][lane] = doc_next;
+    };
+    // (two loops, not one with a branch inside: the accumulators keep their registers)
+    while (t >= 0) {
+        while (t >= 0 && full()) visit(std::false_type());
+        while (t >= 0 && !full()) visit(std::true_type());
     }
     sum = attn_half_sum(sum);
     const float by = sum == 0.f ? 0.f : 1.f / sum;
@@ -231,11 +271,11 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnParams p) {
 }
 
 // ---- few queries: rows r = query * G + head of the group, 32 a workgroup
-template <typename T, int DB>
+template <typename T, int DB, bool FORM>
 __global__ __launch_bounds__(256) void attn_token_kernel(AttnParams p) {
 #ifdef __HIP_DEVICE_COMPILE__                            // (hipcc drops the launch stub of a template whose body its host pass cannot read)
     constexpr int ROW = DB > 2 ? 128 : 64, KEYS = 32, TILE_BYTES = KEYS * ROW * 2, WAVES = 4;
-    extern __shared__ __align__(16) char smem[];                        // [wave][buffer][k, v], then the waves' results
+    extern __shared__ __align__(1024) char smem[];                        // [wave][buffer][k, v], then the waves' results
     __shared__ float sm[WAVES][32], ssum[WAVES][32];
     __shared__ __align__(16) int sdoc[WAVES][2][KEYS];
     const int wave = attn_uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
@@ -262,11 +302,15 @@ __global__ __launch_bounds__(256) void attn_token_kernel(AttnParams p) {
     sk.setup(0, lane, p.ks[1], p.D);
     sv.setup(0, lane, p.vs[1], p.D);
     char* mine = smem + wave * 4 * TILE_BYTES;
+    const uint64_t k_at = attn_addr(k), v_at = attn_addr(v);
+    const int k_row = (int)p.ks[1], v_row = (int)p.vs[1];
+    const AttnLane<ROW> at_lane(lane);
+    const uint32_t lds = attn_lds(mine);
     int doc_next = 0;
     auto stage = [&](int j0, int buf) {
         if (kdoc && lane < KEYS) doc_next = kdoc[min(j0 + lane, p.Lk - 1)];
-        sk.issue(k + (int64_t)j0 * p.ks[1], n - j0, p.ks[1], p.D, mine + buf * 2 * TILE_BYTES, 0);
-        sv.issue(v + (int64_t)j0 * p.vs[1], n - j0, p.vs[1], p.D, mine + buf * 2 * TILE_BYTES + TILE_BYTES, 0);
+        sk.issue(k_at, j0 / KEYS, n, k_row, p.D, lds + buf * 2 * TILE_BYTES, 0);
+        sv.issue(v_at, j0 / KEYS, n, v_row, p.D, lds + buf * 2 * TILE_BYTES + TILE_BYTES, 0);
     };
     f32x16 acc[DB] = {};
     float m = -INFINITY, sum = 0.f;
@@ -277,17 +321,17 @@ __global__ __launch_bounds__(256) void attn_token_kernel(AttnParams p) {
         asm volatile("" ::: "memory");
         attn_landed();                                                  // the wave's own pieces: no other wave touches this LDS
         if (j0 + WAVES * KEYS < k1) stage(j0 + WAVES * KEYS, buf ^ 1);
-        const char* kt = mine + buf * 2 * TILE_BYTES;
+        const uint32_t k_lds = at_lane.rows(lds + buf * 2 * TILE_BYTES), v_lds = at_lane.cols(lds + buf * 2 * TILE_BYTES + TILE_BYTES);
         f32x16 S[1] = {};
 #pragma unroll
-        for (int c = 0; c < 2 * DB; ++c) S[0] = attn_mfma(attn_row_frag<T, ROW>(kt, l31, 2 * c + half), qf[c], S[0]);
+        for (int c = 0; c < 2 * DB; ++c) S[0] = attn_mfma(attn_row_frag<T, ROW>(k_lds, 0, c), qf[c], S[0]);
         const bool full = j0 + KEYS - 1 <= lim_first && !kdoc;
         typename AttnVec<T>::x8 P[1][2];
-        attn_softmax_step<T, 1, DB>(S, P, acc, m, sum, f, full, lim, i + n - p.Lq, j0, half, kdoc ? sdoc[wave][buf] : nullptr, qdoc);
+        attn_softmax_step<T, 1, DB, FORM>(S, P, acc, m, sum, f, full, lim, i + n - p.Lq, j0, half, kdoc ? sdoc[wave][buf] : nullptr, qdoc);
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
-            for (int c = 0; c < 2; ++c) acc[db] = attn_mfma(attn_col_frag<T, ROW>(kt + TILE_BYTES, 16 * c, db, lane), P[0][c], acc[db]);
+            for (int c = 0; c < 2; ++c) acc[db] = attn_mfma(attn_col_frag<T, ROW>(v_lds, c, db), P[0][c], acc[db]);
         if (kdoc && lane < KEYS) sdoc[wave][buf ^ 1][lane] = doc_next;
     }
     // join the four waves: common maximum, then the accumulators through the LDS, one [32 rows][32 * DB + 1] float image a wave
@@ -405,18 +449,19 @@ static bool attn_token_plan(AttnParams& p) {
     return true;
 }
 
-template <typename T, int DB>
+template <typename T, int DB, bool FORM>
 static hipError_t attn_fwd_launch(AttnParams& p, bool token, hipStream_t stream) {
     if (!token) {
         p.row_blocks = cdiv(p.Lq, 128);
-        const int total = p.B * p.Hq * p.row_blocks;
-        hipLaunchKernelGGL((attn_fwd_kernel<T, DB>), dim3(8 * cdiv(total, 8)), dim3(256), 0, stream, p);
+        const dim3 grid(8 * cdiv(p.B * p.Hq * p.row_blocks, 8));
+        if (p.kdoc) hipLaunchKernelGGL((attn_fwd_kernel<T, DB, FORM, true>), grid, dim3(256), 0, stream, p);
+        else hipLaunchKernelGGL((attn_fwd_kernel<T, DB, FORM, false>), grid, dim3(256), 0, stream, p);
         return hipSuccess;
     }
     constexpr int lds = 4 * 4 * 32 * (DB > 2 ? 128 : 64) * 2;
-    const hipError_t e = hipFuncSetAttribute((const void*)attn_token_kernel<T, DB>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    const hipError_t e = hipFuncSetAttribute((const void*)attn_token_kernel<T, DB, FORM>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((attn_token_kernel<T, DB>), dim3(p.B * p.Hk * p.row_blocks * p.splits), dim3(256), lds, stream, p);
+    hipLaunchKernelGGL((attn_token_kernel<T, DB, FORM>), dim3(p.B * p.Hk * p.row_blocks * p.splits), dim3(256), lds, stream, p);
     if (p.splits > 1) hipLaunchKernelGGL((attn_combine_kernel<T>), dim3((unsigned)cdiv64((int64_t)p.B * p.Hk * p.Lq * p.G, 4)), dim3(256), 0, stream, p);
     return hipSuccess;
 }
@@ -453,17 +498,7 @@ extern "C" int n3d_attention(const n3d_attention_desc* d, n3d_stream_t stream_) 
     p.part = (float*)d->workspace + attn_range_floats(p);
     const bool token = attn_token_plan(p);
     hipError_t e = hipSuccess;
-    auto go = [&](auto* t) {
-        using T = std::remove_pointer_t<decltype(t)>;
-        switch (cdiv(p.D, 32)) {
-            case 1: e = attn_fwd_launch<T, 1>(p, token, stream); break;
-            case 2: e = attn_fwd_launch<T, 2>(p, token, stream); break;
-            case 3: e = attn_fwd_launch<T, 3>(p, token, stream); break;
-            default: e = attn_fwd_launch<T, 4>(p, token, stream); break;
-        }
-    };
-    if (d->dtype == N3D_F16) go((_Float16*)nullptr);
-    else go((__bf16*)nullptr);
+    attn_dispatch(d->dtype, p, [&](auto* t, auto db, auto form) { e = attn_fwd_launch<std::remove_pointer_t<decltype(t)>, db.value, form.value>(p, token, stream); });
     N3D_CHECK(e == hipSuccess, "attention: %s", hipGetErrorString(e));
     N3D_LAUNCH_CHECK();
     return 0;
