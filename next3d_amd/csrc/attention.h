@@ -202,7 +202,7 @@ struct AttnTiles {
     }
     // the next tile or -1
     __device__ __forceinline__ int next(int lane) {
-        if (!DOCS || !ranges) return t < end ? t++ : -1;
+        if constexpr (!DOCS) return t < end ? t++ : -1;
         while (bits == 0) {
             base += 64;
             if (base >= end) return -1;
@@ -292,20 +292,27 @@ static inline const char* attn_params(const n3d_attention_desc* d, AttnParams& p
     return nullptr;
 }
 
-// f(element type, 32-channel blocks, FORM: the score is not a positive multiple of the raw product)
+// How a score comes out of the raw product: 0 a positive multiple of it, 1 any multiple and a distance, 2 a cap (and a distance).  Each is straight code of
+// its own in the kernels: values that pass through a branch in place cost a register copy each, and no product is scheduled across it.
+enum { ATTN_PLAIN = 0, ATTN_BIAS = 1, ATTN_CAP = 2 };
+// f(element type, 32-channel blocks, mode, documents)
 template <typename F>
 static inline void attn_dispatch(int dtype, const AttnParams& p, F&& f) {
-    const bool form = p.softcap > 0.f || p.slopes || !(p.scale > 0.f);
-    auto with = [&](auto* t, auto db) {
-        if (form) f(t, db, std::true_type());
-        else f(t, db, std::false_type());
+    auto doc = [&](auto* t, auto db, auto mode) {
+        if (p.kdoc) f(t, db, mode, std::true_type());
+        else f(t, db, mode, std::false_type());
+    };
+    auto form = [&](auto* t, auto db) {
+        if (p.softcap > 0.f) doc(t, db, std::integral_constant<int, ATTN_CAP>());
+        else if (p.slopes || !(p.scale > 0.f)) doc(t, db, std::integral_constant<int, ATTN_BIAS>());
+        else doc(t, db, std::integral_constant<int, ATTN_PLAIN>());
     };
     auto typed = [&](auto* t) {
         switch (cdiv(p.D, 32)) {
-            case 1: with(t, std::integral_constant<int, 1>()); break;
-            case 2: with(t, std::integral_constant<int, 2>()); break;
-            case 3: with(t, std::integral_constant<int, 3>()); break;
-            default: with(t, std::integral_constant<int, 4>()); break;
+            case 1: form(t, std::integral_constant<int, 1>()); break;
+            case 2: form(t, std::integral_constant<int, 2>()); break;
+            case 3: form(t, std::integral_constant<int, 3>()); break;
+            default: form(t, std::integral_constant<int, 4>()); break;
         }
     };
     if (dtype == N3D_F16) typed((_Float16*)nullptr);

@@ -84,36 +84,22 @@ __device__ __forceinline__ int attn_ds_scale(const AttnParams& p, int lane) {
     return attn_uniform(e);
 }
 
-// Raw scores S and dP of 16 (row, column) elements -> P 2^shift and ds 2^e.  lse2(a) / delta(a): of the four registers 4 a .. 4 a + 3; dist + step * row:
-// the element's distance; visible(S, dP) zeroes what is masked (asked only if !full).
-template <bool CAP, typename FL, typename FD>
-__device__ __forceinline__ void attn_ds_form(f32x16& S, f32x16& dP, const AttnScore& f, float ds_by, FL lse2, FD delta, float dist, float step) {
-#pragma unroll
-    for (int a = 0; a < 4; ++a) {
-        const float4 l = lse2(a), d = delta(a);
-        const float la[4] = {l.x, l.y, l.z, l.w}, da[4] = {d.x, d.y, d.z, d.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int r = 4 * a + e;
-            float u, by = ds_by;
-            if constexpr (CAP) {
-                const float th = f.tanh_part(S[r]);
-                u = f.cap_out * th;
-                by = ds_by - ds_by * th * th;
-            } else {
-                u = S[r] * f.mul;
-            }
-            u -= f.slope * fabsf(dist + step * (float)(8 * a + e)) + la[e];
-            S[r] = __builtin_amdgcn_exp2f(u);
-            dP[r] = S[r] * (dP[r] - da[e]) * by;
-        }
+// Raw score and dP of one element -> P 2^shift and ds 2^e (ds_by 1 where T needs no scaling: no multiplication then)
+template <typename T, int MODE>
+__device__ __forceinline__ void attn_ds(f32x16& S, f32x16& dP, int r, const AttnScore& f, float ds_by, float lse2, float delta, float dist) {
+    float w, d = dP[r] - delta;
+    if constexpr (MODE == ATTN_CAP) {
+        const float th = f.tanh_part(S[r]);
+        w = __builtin_amdgcn_exp2f(__builtin_fmaf(f.cap_out, th, -lse2) - f.slope * fabsf(dist));
+        d *= 1.f - th * th;
+    } else if constexpr (MODE == ATTN_BIAS) {
+        w = __builtin_amdgcn_exp2f(__builtin_fmaf(S[r], f.mul, -lse2) - f.slope * fabsf(dist));
+    } else {
+        w = __builtin_amdgcn_exp2f(__builtin_fmaf(S[r], f.mul, -lse2));
     }
-}
-template <typename FL, typename FD, typename FV>
-__device__ __forceinline__ void attn_ds_step(f32x16& S, f32x16& dP, const AttnScore& f, float ds_by, bool full, FL lse2, FD delta, FV visible, float dist, float step) {
-    if (f.cap_out > 0.f) attn_ds_form<true>(S, dP, f, ds_by, lse2, delta, dist, step);
-    else attn_ds_form<false>(S, dP, f, ds_by, lse2, delta, dist, step);
-    if (!full) visible(S, dP);
+    S[r] = w;
+    if constexpr (ATTN_P_SHIFT<T> != 0.f) d *= ds_by;
+    dP[r] = w * d;
 }
 
 template <typename T>
@@ -135,7 +121,7 @@ __device__ __forceinline__ void attn_pair(const AttnParams& p, const AttnScore& 
 }
 __device__ __forceinline__ float attn_lse2(float lse) { return lse == -INFINITY ? INFINITY : lse * ATTN_LOG2E; }       // (a row that sees nothing: every weight 0)
 
-template <typename T, int DB>
+template <typename T, int DB, int MODE, bool DOCS>
 __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnParams p) {
 #ifdef __HIP_DEVICE_COMPILE__                            // (hipcc drops the launch stub of a template whose body its host pass cannot read)
     constexpr int ROW = DB > 2 ? 128 : 64, TILE_BYTES = ATTN_TILE * ROW * 2;
@@ -149,19 +135,19 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnParams p) {
     const int n = attn_keys(p, b), prefix = p.prefix ? p.prefix[b] : 0, q0 = blk * 128;
     const int i = q0 + 32 * wave + l31;
     const bool row_ok = i < p.Lq;
-    const int qdoc = p.kdoc && row_ok ? p.qdoc[b * p.qdoc_stride + i] : 0;
+    const int qdoc = DOCS && row_ok ? p.qdoc[b * p.qdoc_stride + i] : 0;
     const int lim = !row_ok || qdoc < 0 ? -1 : attn_limit(p, i, n, prefix);
-    const int lim_first = attn_limit(p, q0 + 32 * wave, n, prefix), lim_last = attn_limit(p, min(q0 + 32 * wave + 31, p.Lq - 1), n, prefix);
+    const int lim_last = attn_limit(p, min(q0 + 32 * wave + 31, p.Lq - 1), n, prefix);
     const int key_end = attn_limit(p, min(q0 + 127, p.Lq - 1), n, prefix) + 1;
     int dlo = 0, dhi = 0;
-    if (p.kdoc) {
+    if constexpr (DOCS) {
         const int2* r = p.qtiles + (int64_t)b * p.nqt + 2 * blk;
         const int2 r0 = r[0], r1 = 2 * blk + 1 < p.nqt ? r[1] : r[0];
         dlo = min(r0.x, r1.x);
         dhi = max(r0.y, r1.y);
     }
-    AttnTiles<true> tiles;
-    tiles.start(p.kdoc ? p.ktiles + (int64_t)b * p.nkt : nullptr, 0, (key_end + ATTN_TILE - 1) / ATTN_TILE, max(dlo, 0), dhi);
+    AttnTiles<DOCS> tiles;
+    tiles.start(DOCS ? p.ktiles + (int64_t)b * p.nkt : nullptr, 0, (key_end + ATTN_TILE - 1) / ATTN_TILE, max(dlo, 0), dhi);
     typename AttnVec<T>::x8 qf[2 * DB], df[2 * DB];
     const T* q = row_ok ? (const T*)p.q + b * p.qs[0] + i * p.qs[1] + h * p.qs[2] : nullptr;
     const T* dout = row_ok ? (const T*)p.dout + b * p.ds[0] + i * p.ds[1] + h * p.ds[2] : nullptr;
@@ -174,7 +160,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnParams p) {
     const float lse2 = row_ok ? attn_lse2(p.lse[stat]) : INFINITY, delta = row_ok ? p.delta[stat] : 0.f;
     const T* k = (const T*)p.k + b * p.ks[0] + hk * p.ks[2];
     const T* v = (const T*)p.v + b * p.vs[0] + hk * p.vs[2];
-    const int* kdoc = p.kdoc ? p.kdoc + b * p.kdoc_stride : nullptr;
+    const int* kdoc = DOCS ? p.kdoc + b * p.kdoc_stride : nullptr;
     const AttnScore f(p, h);
     const int ds_exp = attn_ds_scale(p, lane);
     const float ds_by = ldexpf(1.f, ds_exp);
@@ -189,58 +175,80 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnParams p) {
     int doc_next = 0;                                                   // of the tile being staged: loaded ahead of its pieces, written behind the products
     auto stage = [&](int t, int buf) {
         const uint32_t at = lds + buf * 2 * TILE_BYTES;
-        if (kdoc && wave == 0) doc_next = kdoc[min(t * ATTN_TILE + lane, p.Lk - 1)];
+        if (DOCS && wave == 0) doc_next = kdoc[min(t * ATTN_TILE + lane, p.Lk - 1)];
         sk.issue(k_at, t, n, k_row, p.D, at, wave);
         sv.issue(v_at, t, n, v_row, p.D, at + TILE_BYTES, wave);
     };
-    int t = tiles.next(lane);
+    int t = tiles.next(lane), buf = 0;
     if (t >= 0) stage(t, 0);
-    if (kdoc && wave == 0) sdoc[0][lane] = doc_next;
-    for (int buf = 0; t >= 0; buf ^= 1) {
+    if (DOCS && wave == 0) sdoc[0][lane] = doc_next;
+    // every key of tile t visible to every query of the workgroup
+    const int full_end = DOCS && dlo != dhi ? 0 : attn_limit(p, q0, n, prefix) + 1;
+    auto full = [&] { return (t + 1) * ATTN_TILE <= full_end && (!DOCS || ((tiles.low == dlo) & (tiles.high == dlo))); };
+    auto visit = [&](auto mask) {
+        const int j0 = t * ATTN_TILE, now = buf;
         attn_sync();
-        const bool one_doc = (dlo == dhi) & (tiles.low == dlo) & (tiles.high == dlo);
-        const int t_next = tiles.next(lane);
-        if (t_next >= 0) stage(t_next, buf ^ 1);
-        const int j0 = t * ATTN_TILE;
-        if (j0 <= lim_last) {
-            const uint32_t k_lds = at_lane.rows(lds + buf * 2 * TILE_BYTES), v_lds = at_lane.rows(lds + buf * 2 * TILE_BYTES + TILE_BYTES);
-            const uint32_t kc_lds = at_lane.cols(lds + buf * 2 * TILE_BYTES);
-            const bool full = (j0 + ATTN_TILE - 1 <= lim_first) & one_doc;
+        t = tiles.next(lane);
+        buf ^= 1;
+        if (t >= 0) stage(t, buf);
+        if (!mask.value || j0 <= lim_last) {
+            const uint32_t k_lds = at_lane.rows(lds + now * 2 * TILE_BYTES), v_lds = at_lane.rows(lds + now * 2 * TILE_BYTES + TILE_BYTES);
+            const uint32_t kc_lds = at_lane.cols(lds + now * 2 * TILE_BYTES);
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
+                typename AttnVec<T>::x8 kf[2 * DB], vf[2 * DB], cf[DB][2], d[2];
+#pragma unroll
+                for (int c = 0; c < 2 * DB; ++c) kf[c] = attn_row_frag<T, ROW>(k_lds, kb, c);
+                // (values behind the first products where registers are short: half of the keys' are free again by then)
+                constexpr int FIRST = DB > 2 ? DB : 0;
                 f32x16 S = {}, dP = {};
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int c = 0; c < 2 * DB; ++c) {
-                    S = attn_mfma(attn_row_frag<T, ROW>(k_lds, kb, c), qf[c], S);
-                    dP = attn_mfma(attn_row_frag<T, ROW>(v_lds, kb, c), df[c], dP);
-                }
-                const int jb = j0 + 32 * kb + 4 * half;
-                attn_ds_step(S, dP, f, ds_by, full, [&](int) { return make_float4(lse2, lse2, lse2, lse2); }, [&](int) { return make_float4(delta, delta, delta, delta); },
-                             [&](f32x16&, f32x16& x) {
-                                 const int last = lim - jb;
+                for (int c = 0; c < FIRST; ++c) S = attn_mfma(kf[c], qf[c], S);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                                 for (int r = 0; r < 16; ++r) x[r] = 8 * (r >> 2) + (r & 3) <= last ? x[r] : 0.f;
-                                 if (kdoc)
+                for (int c = 0; c < 2 * DB; ++c) vf[c] = attn_row_frag<T, ROW>(v_lds, kb, c);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                                     for (int a = 0; a < 4; ++a) {
-                                         const int4 o = *reinterpret_cast<const int4*>(&sdoc[buf][32 * kb + 8 * a + 4 * half]);
-                                         x[4 * a] = o.x == qdoc ? x[4 * a] : 0.f;
-                                         x[4 * a + 1] = o.y == qdoc ? x[4 * a + 1] : 0.f;
-                                         x[4 * a + 2] = o.z == qdoc ? x[4 * a + 2] : 0.f;
-                                         x[4 * a + 3] = o.w == qdoc ? x[4 * a + 3] : 0.f;
-                                     }
-                             },
-                             (float)(i + n - p.Lq - jb), -1.f);
-                typename AttnVec<T>::x8 d[2];
-                attn_pack<T>(dP, d);
+                for (int c = FIRST; c < 2 * DB; ++c) S = attn_mfma(kf[c], qf[c], S);
+#pragma unroll
+                for (int c = 0; c < 2 * DB; ++c) dP = attn_mfma(vf[c], df[c], dP);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int db = 0; db < DB; ++db)
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) acc[db] = attn_mfma(attn_col_frag<T, ROW>(kc_lds, 2 * kb + c, db), d[c], acc[db]);
+                    for (int c = 0; c < 2; ++c) cf[db][c] = attn_col_frag<T, ROW>(kc_lds, 2 * kb + c, db);
+                __builtin_amdgcn_sched_barrier(0);
+                const int jb = j0 + 32 * kb + 4 * half;
+                const float dist = (float)(i + n - p.Lq - jb);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) attn_ds<T, MODE>(S, dP, r, f, ds_by, lse2, delta, dist - (float)(8 * (r >> 2) + (r & 3)));
+                if constexpr (mask.value) {
+                    const int last = lim - jb;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) dP[r] = 8 * (r >> 2) + (r & 3) <= last ? dP[r] : 0.f;
+                    if constexpr (DOCS)
+#pragma unroll
+                        for (int a = 0; a < 4; ++a) {
+                            const int4 o = *reinterpret_cast<const int4*>(&sdoc[now][32 * kb + 8 * a + 4 * half]);
+                            dP[4 * a] = o.x == qdoc ? dP[4 * a] : 0.f;
+                            dP[4 * a + 1] = o.y == qdoc ? dP[4 * a + 1] : 0.f;
+                            dP[4 * a + 2] = o.z == qdoc ? dP[4 * a + 2] : 0.f;
+                            dP[4 * a + 3] = o.w == qdoc ? dP[4 * a + 3] : 0.f;
+                        }
+                }
+                attn_pack<T>(dP, d);
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) acc[db] = attn_mfma(cf[db][c], d[c], acc[db]);
             }
         }
-        if (kdoc && wave == 0) sdoc[buf ^ 1][lane] = doc_next;
-        t = t_next;
+        if (DOCS && wave == 0) sdoc[buf][lane] = doc_next;
+    };
+    while (t >= 0) {
+        while (t >= 0 && full()) visit(std::false_type());
+        while (t >= 0 && !full()) visit(std::true_type());
     }
     bool nan = false;
 #pragma unroll
@@ -281,7 +289,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnParams p) {
 #endif
 }
 
-template <typename T, int DB>
+template <typename T, int DB, int MODE, bool DOCS>
 __global__ __launch_bounds__(256, DB > 2 ? 1 : 2) void attn_dkv_kernel(AttnParams p) {
 #ifdef __HIP_DEVICE_COMPILE__                            // (hipcc drops the launch stub of a template whose body its host pass cannot read)
     constexpr int ROW = DB > 2 ? 128 : 64, TILE_BYTES = ATTN_TILE * ROW * 2;
@@ -298,24 +306,23 @@ __global__ __launch_bounds__(256, DB > 2 ? 1 : 2) void attn_dkv_kernel(AttnParam
     const int g0 = p.splits > 1 ? split : 0, g1 = p.splits > 1 ? split + 1 : p.G;
     const int n = attn_keys(p, b), prefix = p.prefix ? p.prefix[b] : 0, k0 = blk * 128, off = n - p.Lq;
     const int j = k0 + 32 * wave + l31;
-    const int kdoc = p.kdoc && j < p.Lk ? p.kdoc[b * p.kdoc_stride + j] : 0;
+    const int kdoc = DOCS && j < p.Lk ? p.kdoc[b * p.kdoc_stride + j] : 0;
     const bool key_ok = j < n && kdoc >= 0;
     // first query that sees key x
     auto first_query = [&](int x) { return !p.causal || x < prefix ? 0 : max(x - off, 0); };
     const int qmin = key_ok ? first_query(j) : 0x7fffffff;
-    const int last_key = min(k0 + 32 * wave + 31, n - 1);
-    const int wave_first = first_query(k0 + 32 * wave), wave_full = first_query(last_key);
+    const int wave_first = first_query(k0 + 32 * wave);
     const bool wave_on = k0 + 32 * wave < n;
     int dlo = 0, dhi = 0;
-    if (p.kdoc) {
+    if constexpr (DOCS) {
         const int2* r = p.ktiles + (int64_t)b * p.nkt + 2 * blk;
         const int2 r0 = r[0], r1 = 2 * blk + 1 < p.nkt ? r[1] : r[0];
         dlo = min(r0.x, r1.x);
         dhi = max(r0.y, r1.y);
     }
-    const int2* ranges = p.kdoc ? p.qtiles + (int64_t)b * p.nqt : nullptr;
+    const int2* ranges = DOCS ? p.qtiles + (int64_t)b * p.nqt : nullptr;
     const int t_first = first_query(k0) / ATTN_TILE, t_end = k0 < n ? p.nqt : 0;
-    AttnTiles<true> tiles;
+    AttnTiles<DOCS> tiles;
     int g = g0;
     tiles.start(ranges, t_first, t_end, max(dlo, 0), dhi);
     auto next = [&](int& gn) {
@@ -351,79 +358,104 @@ __global__ __launch_bounds__(256, DB > 2 ? 1 : 2) void attn_dkv_kernel(AttnParam
         const int64_t stat = ((int64_t)b * p.Hq + h) * p.Lq + i;
         if (wave == 0) row_next = i < p.Lq ? attn_lse2(p.lse[stat]) - SHIFT : INFINITY;            // (queries behind the last: every weight 0)
         if (wave == 1) row_next = i < p.Lq ? p.delta[stat] : 0.f;
-        if (wave == 2 && p.kdoc) row_next = __builtin_bit_cast(float, i < p.Lq ? p.qdoc[b * p.qdoc_stride + i] : -1);
+        if (DOCS && wave == 2) row_next = __builtin_bit_cast(float, i < p.Lq ? p.qdoc[b * p.qdoc_stride + i] : -1);
         sq.issue(attn_addr((const T*)p.q + b * p.qs[0] + h * p.qs[2]), t, p.Lq, (int)p.qs[1], p.D, at, wave);
         sd.issue(attn_addr((const T*)p.dout + b * p.ds[0] + h * p.ds[2]), t, p.Lq, (int)p.ds[1], p.D, at + TILE_BYTES, wave);
     };
     auto commit = [&](int buf) {
         if (wave == 0) slse[buf][lane] = row_next;
         if (wave == 1) sdelta[buf][lane] = row_next;
-        if (wave == 2) sdoc[buf][lane] = __builtin_bit_cast(int, row_next);
+        if (DOCS && wave == 2) sdoc[buf][lane] = __builtin_bit_cast(int, row_next);
     };
     f32x16 dk[DB] = {}, dv[DB] = {};
-    int t = next(g);
+    AttnScore f(p, hk * p.G);
+    int t = next(g), buf = 0;
     if (t >= 0) stage(t, g, 0);
     commit(0);
-    for (int buf = 0; t >= 0; buf ^= 1) {
+    // every query of tile t sees every key of the workgroup (but those behind the last, whose lanes are not stored)
+    const int full_first = DOCS && dlo != dhi ? 0x7fffffff : first_query(min(k0 + 127, n - 1));
+    auto full = [&] { return t * ATTN_TILE >= full_first && (!DOCS || ((tiles.low == dlo) & (tiles.high == dlo))); };
+    auto visit = [&](auto mask) {
+        const int i0 = t * ATTN_TILE, now = buf;
+        const float slope = MODE != ATTN_PLAIN && p.slopes ? p.slopes[hk * p.G + g] * ATTN_LOG2E : 0.f;
         attn_sync();
-        const bool one_doc = (dlo == dhi) & (tiles.low == dlo) & (tiles.high == dlo);
-        int g_next = g;
-        const int t_next = next(g_next);
-        if (t_next >= 0) stage(t_next, g_next, buf ^ 1);
-        const int i0 = t * ATTN_TILE;
-        if (wave_on && i0 + ATTN_TILE - 1 >= wave_first) {
-            const uint32_t q_lds = at_lane.rows(lds + buf * 2 * TILE_BYTES), d_lds = at_lane.rows(lds + buf * 2 * TILE_BYTES + TILE_BYTES);
-            const uint32_t qc_lds = at_lane.cols(lds + buf * 2 * TILE_BYTES), dc_lds = at_lane.cols(lds + buf * 2 * TILE_BYTES + TILE_BYTES);
-            const AttnScore f(p, hk * p.G + g);
-            const bool full = (i0 >= wave_full) & one_doc;
+        t = next(g);
+        buf ^= 1;
+        if (t >= 0) stage(t, g, buf);
+        if (wave_on && (!mask.value || i0 + ATTN_TILE - 1 >= wave_first)) {
+            f.slope = slope;
+            const uint32_t q_lds = at_lane.rows(lds + now * 2 * TILE_BYTES), d_lds = at_lane.rows(lds + now * 2 * TILE_BYTES + TILE_BYTES);
+            const uint32_t qc_lds = at_lane.cols(lds + now * 2 * TILE_BYTES), dc_lds = at_lane.cols(lds + now * 2 * TILE_BYTES + TILE_BYTES);
 #pragma unroll
             for (int qb = 0; qb < 2; ++qb) {
+                typename AttnVec<T>::x8 qf[2 * DB], df[2 * DB], qc[DB][2], dc[DB][2], w[2], d[2];
+#pragma unroll
+                for (int c = 0; c < 2 * DB; ++c) {
+                    qf[c] = attn_row_frag<T, ROW>(q_lds, qb, c);
+                    df[c] = attn_row_frag<T, ROW>(d_lds, qb, c);
+                }
+                __builtin_amdgcn_sched_barrier(0);
                 f32x16 S = {}, dP = {};
 #pragma unroll
                 for (int c = 0; c < 2 * DB; ++c) {
-                    S = attn_mfma(attn_row_frag<T, ROW>(q_lds, qb, c), kf[c], S);
-                    dP = attn_mfma(attn_row_frag<T, ROW>(d_lds, qb, c), vf[c], dP);
+                    S = attn_mfma(qf[c], kf[c], S);
+                    dP = attn_mfma(df[c], vf[c], dP);
                 }
-                const int ib = 32 * qb + 4 * half;
-                attn_ds_step(S, dP, f, ds_by, full, [&](int a) { return *reinterpret_cast<const float4*>(&slse[buf][ib + 8 * a]); },
-                             [&](int a) { return *reinterpret_cast<const float4*>(&sdelta[buf][ib + 8 * a]); },
-                             [&](f32x16& w, f32x16& x) {
-                                 const int first = qmin - i0 - ib;
-#pragma unroll
-                                 for (int r = 0; r < 16; ++r) {
-                                     const bool see = 8 * (r >> 2) + (r & 3) >= first;
-                                     w[r] = see ? w[r] : 0.f;
-                                     x[r] = see ? x[r] : 0.f;
-                                 }
-                                 if (p.kdoc)
-#pragma unroll
-                                     for (int a = 0; a < 4; ++a) {
-                                         const int4 o4 = *reinterpret_cast<const int4*>(&sdoc[buf][ib + 8 * a]);
-                                         const int o[4] = {o4.x, o4.y, o4.z, o4.w};
-#pragma unroll
-                                         for (int e = 0; e < 4; ++e) {
-                                             const bool see = o[e] == kdoc;
-                                             w[4 * a + e] = see ? w[4 * a + e] : 0.f;
-                                             x[4 * a + e] = see ? x[4 * a + e] : 0.f;
-                                         }
-                                     }
-                             },
-                             (float)(i0 + ib + off - j), 1.f);
-                typename AttnVec<T>::x8 w[2], d[2];
-                attn_pack<T>(S, w);
-                attn_pack<T>(dP, d);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int db = 0; db < DB; ++db)
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        dv[db] = attn_mfma(attn_col_frag<T, ROW>(dc_lds, 2 * qb + c, db), w[c], dv[db]);
-                        dk[db] = attn_mfma(attn_col_frag<T, ROW>(qc_lds, 2 * qb + c, db), d[c], dk[db]);
+                        dc[db][c] = attn_col_frag<T, ROW>(dc_lds, 2 * qb + c, db);
+                        qc[db][c] = attn_col_frag<T, ROW>(qc_lds, 2 * qb + c, db);
+                    }
+                __builtin_amdgcn_sched_barrier(0);
+                const int ib = 32 * qb + 4 * half;
+                const float dist = (float)(i0 + ib + off - j);
+#pragma unroll
+                for (int a = 0; a < 4; ++a) {
+                    const float4 l4 = *reinterpret_cast<const float4*>(&slse[now][ib + 8 * a]), e4 = *reinterpret_cast<const float4*>(&sdelta[now][ib + 8 * a]);
+                    const float l[4] = {l4.x, l4.y, l4.z, l4.w}, de[4] = {e4.x, e4.y, e4.z, e4.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) attn_ds<T, MODE>(S, dP, 4 * a + e, f, ds_by, l[e], de[e], dist + (float)(8 * a + e));
+                }
+                if constexpr (mask.value) {
+                    const int first = qmin - i0 - ib;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const bool see = 8 * (r >> 2) + (r & 3) >= first;
+                        S[r] = see ? S[r] : 0.f;
+                        dP[r] = see ? dP[r] : 0.f;
+                    }
+                    if constexpr (DOCS)
+#pragma unroll
+                        for (int a = 0; a < 4; ++a) {
+                            const int4 o4 = *reinterpret_cast<const int4*>(&sdoc[now][ib + 8 * a]);
+                            const int o[4] = {o4.x, o4.y, o4.z, o4.w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const bool see = o[e] == kdoc;
+                                S[4 * a + e] = see ? S[4 * a + e] : 0.f;
+                                dP[4 * a + e] = see ? dP[4 * a + e] : 0.f;
+                            }
+                        }
+                }
+                attn_pack<T>(S, w);
+                attn_pack<T>(dP, d);
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) {
+                        dv[db] = attn_mfma(dc[db][c], w[c], dv[db]);
+                        dk[db] = attn_mfma(qc[db][c], d[c], dk[db]);
                     }
             }
         }
-        commit(buf ^ 1);
-        t = t_next;
-        g = g_next;
+        commit(buf);
+    };
+    while (t >= 0) {
+        while (t >= 0 && full()) visit(std::false_type());
+        while (t >= 0 && !full()) visit(std::true_type());
     }
     bool nan = false;
 #pragma unroll
@@ -527,19 +559,19 @@ __global__ __launch_bounds__(256) void attn_parts_kernel(AttnParams p) {
     *reinterpret_cast<typename AttnVec<T>::x8*>((T*)(blockIdx.y ? p.dv : p.dk) + at) = o;
 }
 
-template <typename T, int DB>
+template <typename T, int DB, int MODE, bool DOCS>
 static void attn_bwd_launch(AttnParams& p, int splits, hipStream_t stream) {
     const int prep = p.maxima ? ATTN_MAXIMA : (int)(cdiv64((int64_t)p.B * p.Lq * p.Hq, 16) < 2048 ? cdiv64((int64_t)p.B * p.Lq * p.Hq, 16) : 2048);
     hipLaunchKernelGGL((attn_prep_kernel<T>), dim3(prep, p.maxima ? 2 : 1), dim3(256), 0, stream, p);
     if (p.dq) {
         p.splits = 1;
         p.row_blocks = cdiv(p.Lq, 128);
-        hipLaunchKernelGGL((attn_dq_kernel<T, DB>), dim3(8 * cdiv(p.B * p.Hq * p.row_blocks, 8)), dim3(256), 0, stream, p);
+        hipLaunchKernelGGL((attn_dq_kernel<T, DB, MODE, DOCS>), dim3(8 * cdiv(p.B * p.Hq * p.row_blocks, 8)), dim3(256), 0, stream, p);
     }
     if (p.dk && p.Lk > 0) {
         p.splits = splits;
         p.row_blocks = cdiv(p.Lk, 128);
-        hipLaunchKernelGGL((attn_dkv_kernel<T, DB>), dim3(8 * cdiv(p.B * p.Hk * p.splits * p.row_blocks, 8)), dim3(256), 0, stream, p);
+        hipLaunchKernelGGL((attn_dkv_kernel<T, DB, MODE, DOCS>), dim3(8 * cdiv(p.B * p.Hk * p.splits * p.row_blocks, 8)), dim3(256), 0, stream, p);
         if (splits > 1)
             hipLaunchKernelGGL((attn_parts_kernel<T>), dim3((unsigned)cdiv64((int64_t)p.B * p.Lk * p.Hk * p.D, 2048), 2), dim3(256), 0, stream, p);
     }
@@ -586,17 +618,9 @@ extern "C" int n3d_attention_bwd(const n3d_attention_desc* d, n3d_stream_t strea
     const double pairs = (double)p.B * p.Hq * p.Lq * p.Lk * p.D;
     N3dProfScope prof(N3D_K_ATTENTION, stream, 10.0 * pairs, 8.0 * ((double)p.B * p.Lq * p.Hq * p.D + (double)p.B * p.Lk * p.Hk * p.D));
     attn_ranges(p, ws, stream);
-    auto go = [&](auto* t) {
-        using T = std::remove_pointer_t<decltype(t)>;
-        switch (cdiv(p.D, 32)) {
-            case 1: attn_bwd_launch<T, 1>(p, splits, stream); break;
-            case 2: attn_bwd_launch<T, 2>(p, splits, stream); break;
-            case 3: attn_bwd_launch<T, 3>(p, splits, stream); break;
-            default: attn_bwd_launch<T, 4>(p, splits, stream); break;
-        }
-    };
-    if (d->dtype == N3D_F16) go((_Float16*)nullptr);
-    else go((__bf16*)nullptr);
+    attn_dispatch(d->dtype, p, [&](auto* t, auto db, auto mode, auto docs) {
+        attn_bwd_launch<std::remove_pointer_t<decltype(t)>, db.value, mode.value, docs.value>(p, splits, stream);
+    });
     N3D_LAUNCH_CHECK();
     return 0;
 }

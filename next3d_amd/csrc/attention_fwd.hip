@@ -50,28 +50,19 @@ __device__ void attn_exact_row(const AttnParams& p, int b, int i, int h, int k0,
 }
 
 // One wave's softmax step over the 32 queries of its lanes: S (raw products of KB blocks of 32 keys) -> P as second operands; rescales acc, sum and m.
-// FORM: the score is not a positive multiple of the raw product (a cap, a slope, a scale <= 0).  MASK: not every key of the tile is visible to every query.
-// (Each combination is straight code of its own: values that pass through a branch in place cost a register copy each.)
-template <typename T, int KB, int DB, bool FORM, bool MASK>
+// MASK: not every key of the tile is visible to every query.
+template <typename T, int KB, int DB, int MODE, bool MASK>
 __device__ __forceinline__ void attn_softmax_form(f32x16 (&S)[KB], typename AttnVec<T>::x8 (&P)[KB][2], f32x16 (&acc)[DB], float& m, float& sum, const AttnScore& f,
                                                   int lim, int at, int j0, int half, const int* docs, int qdoc) {
-    if constexpr (FORM) {
-        if (f.cap_out > 0.f) {
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) S[kb][r] = f.cap_out * f.tanh_part(S[kb][r]);
-        } else {
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) S[kb][r] *= f.mul;
-        }
+    if constexpr (MODE != ATTN_PLAIN) {
         const float dist = (float)(at - j0 - 4 * half);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) S[kb][r] -= f.slope * fabsf(dist - (float)(32 * kb + 8 * (r >> 2) + (r & 3)));
+            for (int r = 0; r < 16; ++r) {
+                const float u = MODE == ATTN_CAP ? f.cap_out * f.tanh_part(S[kb][r]) : S[kb][r] * f.mul;
+                S[kb][r] = u - f.slope * fabsf(dist - (float)(32 * kb + 8 * (r >> 2) + (r & 3)));
+            }
     }
     if constexpr (MASK) {
         const int last = lim - j0 - 4 * half;
@@ -97,7 +88,7 @@ __device__ __forceinline__ void attn_softmax_form(f32x16 (&S)[KB], typename Attn
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int r = 0; r < 16; ++r) tops[r & 3] = fmaxf(tops[r & 3], S[kb][r]);
-    const float mul = FORM ? 1.f : f.mul;
+    const float mul = MODE == ATTN_PLAIN ? f.mul : 1.f;
     const float top = attn_half_max(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]))) * mul;          // (mul > 0; -inf stays -inf)
     if (__ballot((top > m + 8.f) | ((m == -INFINITY) & (top > m)))) {
         const float now = fmaxf(m, top);
@@ -126,14 +117,14 @@ __device__ __forceinline__ void attn_softmax_form(f32x16 (&S)[KB], typename Attn
     }
     sum += (add[0] + add[1]) + (add[2] + add[3]);
 }
-template <typename T, int KB, int DB, bool FORM>
+template <typename T, int KB, int DB, int MODE>
 __device__ __forceinline__ void attn_softmax_step(f32x16 (&S)[KB], typename AttnVec<T>::x8 (&P)[KB][2], f32x16 (&acc)[DB], float& m, float& sum, const AttnScore& f,
                                                   bool full, int lim, int at, int j0, int half, const int* docs, int qdoc) {
-    if (full) attn_softmax_form<T, KB, DB, FORM, false>(S, P, acc, m, sum, f, lim, at, j0, half, docs, qdoc);
-    else attn_softmax_form<T, KB, DB, FORM, true>(S, P, acc, m, sum, f, lim, at, j0, half, docs, qdoc);
+    if (full) attn_softmax_form<T, KB, DB, MODE, false>(S, P, acc, m, sum, f, lim, at, j0, half, docs, qdoc);
+    else attn_softmax_form<T, KB, DB, MODE, true>(S, P, acc, m, sum, f, lim, at, j0, half, docs, qdoc);
 }
 
-template <typename T, int DB, bool FORM, bool DOCS>
+template <typename T, int DB, int MODE, bool DOCS>
 __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnParams p) {
 #ifdef __HIP_DEVICE_COMPILE__                            // (hipcc drops the launch stub of a template whose body its host pass cannot read)
     constexpr int ROW = DB > 2 ? 128 : 64, TILE_BYTES = ATTN_TILE * ROW * 2;
@@ -222,7 +213,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnParams p) {
 #pragma unroll
                     for (int c = 0; c < 2; ++c) vf[db][kb][c] = attn_col_frag<T, ROW>(v_lds, 2 * kb + c, db);
             __builtin_amdgcn_sched_barrier(0);
-            attn_softmax_form<T, 2, DB, FORM, mask.value>(S, P, acc, m, sum, f, lim, i + n - p.Lq, j0, half, DOCS ? sdoc[now] : nullptr, qdoc);
+            attn_softmax_form<T, 2, DB, MODE, mask.value>(S, P, acc, m, sum, f, lim, i + n - p.Lq, j0, half, DOCS ? sdoc[now] : nullptr, qdoc);
 #pragma unroll
             for (int kb = AHEAD; kb < 2; ++kb)
 #pragma unroll
@@ -271,7 +262,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnParams p) {
 }
 
 // ---- few queries: rows r = query * G + head of the group, 32 a workgroup
-template <typename T, int DB, bool FORM>
+template <typename T, int DB, int MODE>
 __global__ __launch_bounds__(256) void attn_token_kernel(AttnParams p) {
 #ifdef __HIP_DEVICE_COMPILE__                            // (hipcc drops the launch stub of a template whose body its host pass cannot read)
     constexpr int ROW = DB > 2 ? 128 : 64, KEYS = 32, TILE_BYTES = KEYS * ROW * 2, WAVES = 4;
@@ -327,7 +318,7 @@ __global__ __launch_bounds__(256) void attn_token_kernel(AttnParams p) {
         for (int c = 0; c < 2 * DB; ++c) S[0] = attn_mfma(attn_row_frag<T, ROW>(k_lds, 0, c), qf[c], S[0]);
         const bool full = j0 + KEYS - 1 <= lim_first && !kdoc;
         typename AttnVec<T>::x8 P[1][2];
-        attn_softmax_step<T, 1, DB, FORM>(S, P, acc, m, sum, f, full, lim, i + n - p.Lq, j0, half, kdoc ? sdoc[wave][buf] : nullptr, qdoc);
+        attn_softmax_step<T, 1, DB, MODE>(S, P, acc, m, sum, f, full, lim, i + n - p.Lq, j0, half, kdoc ? sdoc[wave][buf] : nullptr, qdoc);
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
@@ -449,19 +440,17 @@ static bool attn_token_plan(AttnParams& p) {
     return true;
 }
 
-template <typename T, int DB, bool FORM>
+template <typename T, int DB, int MODE, bool DOCS>
 static hipError_t attn_fwd_launch(AttnParams& p, bool token, hipStream_t stream) {
     if (!token) {
         p.row_blocks = cdiv(p.Lq, 128);
-        const dim3 grid(8 * cdiv(p.B * p.Hq * p.row_blocks, 8));
-        if (p.kdoc) hipLaunchKernelGGL((attn_fwd_kernel<T, DB, FORM, true>), grid, dim3(256), 0, stream, p);
-        else hipLaunchKernelGGL((attn_fwd_kernel<T, DB, FORM, false>), grid, dim3(256), 0, stream, p);
+        hipLaunchKernelGGL((attn_fwd_kernel<T, DB, MODE, DOCS>), dim3(8 * cdiv(p.B * p.Hq * p.row_blocks, 8)), dim3(256), 0, stream, p);
         return hipSuccess;
     }
     constexpr int lds = 4 * 4 * 32 * (DB > 2 ? 128 : 64) * 2;
-    const hipError_t e = hipFuncSetAttribute((const void*)attn_token_kernel<T, DB, FORM>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    const hipError_t e = hipFuncSetAttribute((const void*)attn_token_kernel<T, DB, MODE>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((attn_token_kernel<T, DB, FORM>), dim3(p.B * p.Hk * p.row_blocks * p.splits), dim3(256), lds, stream, p);
+    hipLaunchKernelGGL((attn_token_kernel<T, DB, MODE>), dim3(p.B * p.Hk * p.row_blocks * p.splits), dim3(256), lds, stream, p);
     if (p.splits > 1) hipLaunchKernelGGL((attn_combine_kernel<T>), dim3((unsigned)cdiv64((int64_t)p.B * p.Hk * p.Lq * p.G, 4)), dim3(256), 0, stream, p);
     return hipSuccess;
 }
@@ -498,7 +487,9 @@ extern "C" int n3d_attention(const n3d_attention_desc* d, n3d_stream_t stream_) 
     p.part = (float*)d->workspace + attn_range_floats(p);
     const bool token = attn_token_plan(p);
     hipError_t e = hipSuccess;
-    attn_dispatch(d->dtype, p, [&](auto* t, auto db, auto form) { e = attn_fwd_launch<std::remove_pointer_t<decltype(t)>, db.value, form.value>(p, token, stream); });
+    attn_dispatch(d->dtype, p, [&](auto* t, auto db, auto mode, auto docs) {
+        e = attn_fwd_launch<std::remove_pointer_t<decltype(t)>, db.value, mode.value, docs.value>(p, token, stream);
+    });
     N3D_CHECK(e == hipSuccess, "attention: %s", hipGetErrorString(e));
     N3D_LAUNCH_CHECK();
     return 0;
