@@ -1,6 +1,7 @@
-"""What the token operators (layer_norm, rotary, attention) share: element types, argument checks, the device their launches go to."""
-import contextlib
+"""What the token operators (layer_norm, rotary, attention) share: element types, argument checks, the device their launches go to.
 
+A call's host time matters here — a block runs these operators on small tensors too, and a Python autograd node already costs some 20 us — so the checks are
+flat, buffers are allocated together, and the descriptors are packed in one call."""
 import torch
 
 from ... import _lib
@@ -18,19 +19,46 @@ def require_tensor(op, name, t, dtypes, ndim=None):
         raise RuntimeError(f'{op}: {name} must have {ndim} dimensions (got {t.ndim})')
 
 
-def require_same_device(op, *tensors):
-    _lib.require_device(*tensors)
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) > 1:
-        raise RuntimeError(f'{op}: all tensors must be on one device (got {", ".join(sorted(str(d) for d in devices))})')
+def require_same_device(op, first, *others):
+    """RuntimeError unless all (that are not None) lie on one HIP device."""
+    device = first.device
+    if device.type != 'cuda':
+        _lib.require_device(first)
+    for t in others:
+        if t is not None and t.device != device:
+            _lib.require_device(t)
+            raise RuntimeError(f'{op}: all tensors must be on one device (got {device} and {t.device})')
 
 
-def on_device(t):
-    """Launches inside go to the device of `t` and to torch's current stream there, whatever the current device is."""
-    if t.device.index is None or t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+def launch(t, fn, *args):
+    """fn(*args, stream) on the device of `t`, on torch's current stream there, whatever the current device is.  The caller's locals keep every tensor of the
+    call alive until it returns: by then the work is enqueued, and the allocator's stream order protects the memory."""
+    if t.get_device() == _lib._get_device():
+        rc = fn(*args, _lib._stream_handle())
+    else:
+        with torch.cuda.device(t.device):
+            rc = fn(*args, _lib._stream_handle())
+    if rc != 0:
+        _lib.check(rc)
+
+
+def pointer(t):
+    return 0 if t is None else t.data_ptr()
 
 
 def wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def once(backward):
+    """Marks a Function's `backward` as differentiable once: under create_graph its results refuse a second derivative (torch's once_differentiable); without
+    it — every ordinary step — the wrapper's bookkeeping is skipped."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return staticmethod(run)

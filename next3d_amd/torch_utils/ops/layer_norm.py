@@ -2,62 +2,70 @@
 
 Not an operator of the reference's layer (whose only norm is `normalize_2nd_moment`): it stands beside the others for models over tokens — w vectors,
 tri-plane texels, frames — together with `rotary` and `attention`."""
-import math
+import functools
 
 import torch
 
 from ... import _lib
-from ._tokens import DTYPES, on_device, require_same_device, require_tensor, wants_grad
+from ._tokens import DTYPES, launch, once, pointer, require_same_device, require_tensor, wants_grad
 
 
 def _rows(x):
     """[rows, C] with dense channels: a view where the strides allow it."""
     c = x.shape[-1]
-    x = x.reshape(x.numel() // c, c)
+    if x.ndim != 2:
+        x = x.reshape(x.numel() // c, c)
     return x if c == 1 or x.stride(1) == 1 else x.contiguous()
 
 
-def _affine_dtype(x, weight, bias):
-    return next((t.dtype for t in (weight, bias) if t is not None), torch.float32 if x is None else x.dtype)
+def _new(x):
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace(rows, c, dtype):
+    return _lib.lib().n3d_layer_norm_bwd_workspace(rows, c, dtype)
 
 
 def _forward(x, weight, bias, eps, want_stats):
     x2 = _rows(x)
     rows, c = x2.shape
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean = torch.empty(rows, dtype=torch.float32, device=x.device) if want_stats else None
-    rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if want_stats else None
-    with on_device(x):
-        _lib.check(_lib.lib().n3d_layer_norm(_lib.ptr(x2), _lib.ptr(weight), _lib.ptr(bias), _lib.ptr(y), _lib.ptr(mean), _lib.ptr(rstd), rows, c, x2.stride(0),
-                                             DTYPES[x.dtype], DTYPES[_affine_dtype(x, weight, bias)], eps, _lib.stream()))
-    return y, mean, rstd
+    y = _new(x)
+    affine = bias if weight is None else weight
+    stats, at = None, 0
+    if want_stats:
+        stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)                 # mean, rstd
+        at = stats.data_ptr()
+    launch(x, _lib.lib().n3d_layer_norm, x2.data_ptr(), pointer(weight), pointer(bias), y.data_ptr(), at, at and at + 4 * rows, rows, c, x2.stride(0), DTYPES[x.dtype],
+           0 if affine is None else DTYPES[affine.dtype], eps)
+    return y, stats
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = _forward(x, weight, bias, eps, True)
-        ctx.save_for_backward(x, weight, mean, rstd)
-        ctx.affine_dtype = _affine_dtype(x, weight, bias)
+        y, stats = _forward(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, stats)
+        ctx.bias_dtype = None if bias is None else bias.dtype
         return y
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once
     def backward(ctx, dy):
-        x, weight, mean, rstd = ctx.saved_tensors
+        x, weight, stats = ctx.saved_tensors
+        want_x, want_w, want_b, _ = ctx.needs_input_grad
         x2, dy2 = _rows(x), _rows(dy)
         rows, c = x2.shape
-        want_x, want_w, want_b = ctx.needs_input_grad[:3]
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_x else None
+        dtype = DTYPES[x.dtype]
+        affine = ctx.bias_dtype if weight is None else weight.dtype
+        dx = _new(x) if want_x else None
         make = torch.empty if rows else torch.zeros
-        dw = make(c, dtype=ctx.affine_dtype, device=x.device) if want_w else None
-        db = make(c, dtype=ctx.affine_dtype, device=x.device) if want_b else None
+        dw = make(c, dtype=affine, device=x.device) if want_w else None
+        db = make(c, dtype=affine, device=x.device) if want_b else None
         if rows:
-            lib, code = _lib.lib(), DTYPES[x.dtype]
-            with on_device(x):
-                ws = torch.empty(lib.n3d_layer_norm_bwd_workspace(rows, c, code), dtype=torch.float32, device=x.device) if want_w or want_b else None
-                _lib.check(lib.n3d_layer_norm_bwd(_lib.ptr(dy2), _lib.ptr(x2), _lib.ptr(weight), _lib.ptr(mean), _lib.ptr(rstd), _lib.ptr(dx), _lib.ptr(dw),
-                                                  _lib.ptr(db), _lib.ptr(ws), rows, c, x2.stride(0), dy2.stride(0), code, DTYPES[ctx.affine_dtype], _lib.stream()))
+            ws = torch.empty(_workspace(rows, c, dtype), dtype=torch.float32, device=x.device) if want_w or want_b else None
+            at = stats.data_ptr()
+            launch(x, _lib.lib().n3d_layer_norm_bwd, dy2.data_ptr(), x2.data_ptr(), pointer(weight), at, at + 4 * rows, pointer(dx), pointer(dw), pointer(db),
+                   pointer(ws), rows, c, x2.stride(0), dy2.stride(0), dtype, 0 if affine is None else DTYPES[affine])
         return dx, dw, db, None
 
 
@@ -77,7 +85,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise RuntimeError('layer_norm: weight and bias must have one dtype')
     eps = float(eps)
-    if not (eps >= 0 and math.isfinite(eps)):
+    if not 0 <= eps < float('inf'):
         raise RuntimeError('layer_norm: eps must be a finite number that is not negative')
     require_same_device('layer_norm', x, weight, bias)
     weight = weight if weight is None else weight.contiguous()

@@ -1,44 +1,40 @@
 """rotary — rotary positions with several axes (time, height, width) for tokens of images and videos, on libn3d.so (csrc/rotary.hip).
 
 Not an operator of the reference's layer; it turns the queries and keys of `attention`."""
-import math
+import struct
 
 import torch
 
 from ... import _lib
-from ._tokens import DTYPES, on_device, require_same_device, require_tensor, wants_grad
+from ._tokens import DTYPES, launch, once, pointer, require_same_device, require_tensor, wants_grad
 
 _POSITIONS = {torch.float32: 0, torch.int32: 1, torch.int64: 2}
+_PACK = struct.Struct('=5Q8qd15i4x')                                     # n3d_rotary_desc, field by field
 
 
 def _turn(q, k, positions, plan, inverse):
     sections, base, interleaved, shared = plan
-    first = q if q is not None else k
+    first = k if q is None else q
     b, l, _, d = first.shape
-    desc = _lib.RotaryDesc()
-    outs = []
-    with on_device(first):
-        for name, t in (('q', q), ('k', k)):
-            if t is None:
-                outs.append(None)
-                continue
-            if t.stride(3) != 1:
-                t = t.contiguous()
-            y = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-            setattr(desc, name, _lib.ptr(t))
-            setattr(desc, 'out_' + name, _lib.ptr(y))
-            setattr(desc, 'heads_' + name, t.shape[2])
-            getattr(desc, name + '_strides')[:] = t.stride()[:3]
-            outs.append(y)
-        desc.positions = _lib.ptr(positions)
-        desc.pos_batch_stride = positions.stride(0) if positions.ndim == 3 and positions.shape[0] > 1 else 0
-        desc.pos_token_stride = positions.stride(-2)
-        desc.base, desc.B, desc.L, desc.D, desc.axes = base, b, l, d, len(sections)
-        desc.sections[:len(sections)] = sections
-        desc.dtype, desc.pos_type = DTYPES[first.dtype], _POSITIONS[positions.dtype]
-        desc.interleaved, desc.shared_ladder, desc.inverse = int(interleaved), int(shared), int(inverse)
-        _lib.check(_lib.lib().n3d_rotary(desc, _lib.stream()))
-    return outs
+    yq = yk = None
+    q_strides = k_strides = (0, 0, 0)
+    if q is not None:
+        if q.stride(3) != 1:
+            q = q.contiguous()
+        yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        q_strides = q.stride()[:3]
+    if k is not None:
+        if k.stride(3) != 1:
+            k = k.contiguous()
+        yk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        k_strides = k.stride()[:3]
+    desc = _lib.RotaryDesc.from_buffer_copy(_PACK.pack(
+        pointer(q), pointer(k), positions.data_ptr(), pointer(yq), pointer(yk), *q_strides, *k_strides,
+        positions.stride(0) if positions.ndim == 3 and positions.shape[0] > 1 else 0, positions.stride(-2), base, b, l, 0 if q is None else q.shape[2],
+        0 if k is None else k.shape[2], d, len(sections), *sections, *(0,) * (4 - len(sections)), DTYPES[first.dtype], _POSITIONS[positions.dtype], interleaved,
+        shared, inverse))
+    launch(first, _lib.lib().n3d_rotary, desc)
+    return yq, yk
 
 
 class _Rotary(torch.autograd.Function):
@@ -50,8 +46,7 @@ class _Rotary(torch.autograd.Function):
         yq, yk = _turn(q, k, positions, plan, False)
         return yq if k is None else (yq, yk)
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @once
     def backward(ctx, dq, dk=None):
         positions, = ctx.saved_tensors
         dq = dq if ctx.needs_input_grad[0] else None
@@ -89,7 +84,7 @@ def rotary(q, positions, sections, k=None, base=10000.0, pairing='interleaved', 
     if pairing not in ('interleaved', 'half') or ladder not in ('axis', 'shared'):
         raise RuntimeError(f"rotary: pairing is 'interleaved' or 'half', ladder 'axis' or 'shared' (got {pairing!r}, {ladder!r})")
     base = float(base)
-    if not (base > 0 and math.isfinite(base)):
+    if not 0 < base < float('inf'):
         raise RuntimeError('rotary: base must be a positive finite number')
     if positions.requires_grad:
         raise RuntimeError('rotary: positions have no gradient')

@@ -180,3 +180,18 @@ def test_attention_c_entries_refuse_bad_calls():
     for kw, word in ((dict(Lq=0), 'queries'), (dict(lse=None), 'null'), (dict(dout=None), 'null'), (dict(dk=None), 'null'), (dict(dq=None, dk=None, dv=None), 'null'),
                      (dict(dout_strides=(128, 33, 16)), 'strides'), (dict(dout=4100), 'aligned'), (dict(dv=4100), 'aligned')):
         assert lib.n3d_attention_bwd(desc(workspace=4096, workspace_bytes=1 << 30, **kw), None) != 0 and word in lib.n3d_last_error().decode(), kw
+
+
+def test_descriptors_are_packed_as_they_are_laid_out():
+    """rotary and attention fill their descriptors with one struct.pack: every field must arrive where the structure has it."""
+    from next3d_amd import _lib
+    from next3d_amd.torch_utils.ops import attention, rotary
+    for pack, cls in ((rotary._PACK, _lib.RotaryDesc), (attention._PACK, _lib.AttentionDesc)):
+        assert pack.size == C.sizeof(cls)
+        count = sum(getattr(kind, '_length_', 1) for _, kind in cls._fields_)
+        d = cls.from_buffer_copy(pack.pack(*range(1, count + 1)))
+        got = []
+        for name, kind in cls._fields_:
+            value = getattr(d, name)
+            got += list(value) if hasattr(kind, '_length_') else [value]
+        assert got == list(range(1, count + 1))
