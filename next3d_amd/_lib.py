@@ -180,6 +180,25 @@ def _handle():
     return _lib
 
 
+_token_ext = None
+
+
+def token_ext():
+    """The C++ host side of the token operators (csrc/token_ext.cpp), bound to this library's entry points.  Like the library: no fallback."""
+    global _token_ext
+    if _token_ext is None:
+        handle = lib()
+        try:
+            from . import _token_ext as ext
+        except ImportError as e:
+            raise RuntimeError(f'{_HERE}/_token_ext.so cannot be loaded ({e}): build it with `python -m next3d_amd.build`') from e
+        names = ('n3d_last_error', 'n3d_layer_norm', 'n3d_layer_norm_bwd_workspace', 'n3d_layer_norm_bwd', 'n3d_rotary', 'n3d_attention_workspace',
+                 'n3d_attention', 'n3d_attention_bwd_workspace', 'n3d_attention_bwd')
+        ext.bind([ctypes.cast(getattr(handle, name), c_void_p).value for name in names])
+        _token_ext = ext
+    return _token_ext
+
+
 _tls = threading.local()
 
 

@@ -1,4 +1,4 @@
-"""Ahead-of-time build of libn3d.so (HIP, gfx950 only) and of the oracle's C helper.
+"""Ahead-of-time build of libn3d.so (HIP, gfx950 only) and of _token_ext.so, the C++ host side of the token operators (against torch's headers).
 
     python -m next3d_amd.build [--force]
 
@@ -13,6 +13,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 OBJ = os.path.join(HERE, 'build')
 LIB = os.path.join(HERE, 'libn3d.so')
+EXT = os.path.join(HERE, '_token_ext.so')
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
 ARCH = 'gfx950'
 CFLAGS = ['-O3', '-std=c++17', '-fPIC', f'--offload-arch={ARCH}', '-Wall', '-Wno-unused-function', '-Wno-unused-variable',
@@ -34,6 +35,22 @@ def _stale(target, deps):
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _ext_commands():
+    """Compile and link commands of _token_ext.so: host code only, linked against the torch that will load it."""
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    src, obj = os.path.join(CSRC, 'token_ext.cpp'), os.path.join(OBJ, 'token_ext.o')
+    includes = [os.path.join(root, 'include'), os.path.join(root, 'include', 'torch', 'csrc', 'api', 'include'), '/opt/rocm/include',
+                sysconfig.get_paths()['include']]
+    compile_ = ['g++', '-O2', '-std=c++17', '-fPIC', '-Wall', '-D__HIP_PLATFORM_AMD__=1', '-DUSE_ROCM=1',
+                f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}']
+    compile_ += [a for i in includes for a in ('-isystem', i)] + ['-c', src, '-o', obj]
+    link = ['g++', '-shared', '-fPIC', '-o', EXT, obj, '-L' + os.path.join(root, 'lib'), '-ltorch_python', '-ltorch', '-ltorch_cpu', '-ltorch_hip', '-lc10', '-lc10_hip']
+    return src, obj, compile_, link
+
+
 def build(force=False, verbose=True):
     os.makedirs(OBJ, exist_ok=True)
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith('.h')]
@@ -44,12 +61,16 @@ def build(force=False, verbose=True):
         if force or _stale(obj, [os.path.join(CSRC, src)] + headers):
             jobs.append([HIPCC] + CFLAGS + PER_FILE.get(src, []) + ['-c', os.path.join(CSRC, src), '-o', obj])
 
+    ext_src, ext_obj, ext_compile, ext_link = _ext_commands()
+    if force or _stale(ext_obj, [ext_src, os.path.join(HERE, '..', 'include', 'n3d.h')]):
+        jobs.insert(0, ext_compile)                    # (the longest job first)
+
     def run(cmd):
         if verbose:
             print('[n3d build]', ' '.join(cmd[-3:]), flush=True)
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
-            raise RuntimeError(f'hipcc failed: {" ".join(cmd)}\n{r.stdout}\n{r.stderr}')
+            raise RuntimeError(f'build failed: {" ".join(cmd)}\n{r.stdout}\n{r.stderr}')
         said = '\n'.join(line for line in r.stderr.splitlines() if 'packed-fp32-ops' not in line)
         if verbose and said.strip():
             print(said, file=sys.stderr)
@@ -57,7 +78,7 @@ def build(force=False, verbose=True):
     with ThreadPoolExecutor(max_workers=min(8, max(1, len(jobs)))) as ex:
         list(ex.map(run, jobs))
     objs = [os.path.join(OBJ, s.replace('.hip', '.o')) for s in _sources()]
-    if force or jobs or _stale(LIB, objs):
+    if force or _stale(LIB, objs):
         run([HIPCC, '-shared', '-fPIC', f'--offload-arch={ARCH}', '-Wl,--no-undefined', '-o', LIB] + objs)
         # a library that links but cannot be loaded (hipcc's host pass silently drops the launch stub of some __global__ templates:
         # an undefined __device_stub__ symbol) must fail HERE, on the build machine, not on the GPU box
@@ -67,6 +88,10 @@ def build(force=False, verbose=True):
         except ImportError:
             pass
         ctypes.CDLL(LIB)
+    if force or _stale(EXT, [ext_obj]):
+        run(ext_link)
+        subprocess.run([sys.executable, '-c', 'import torch; import importlib.util as u; '
+                        f's = u.spec_from_file_location("_token_ext", {EXT!r}); s.loader.exec_module(u.module_from_spec(s))'], check=True)
     return LIB
 
 

@@ -1,7 +1,5 @@
-"""What the token operators (layer_norm, rotary, attention) share: element types, argument checks, the device their launches go to.
-
-A call's host time matters here — a block runs these operators on small tensors too, and a Python autograd node already costs some 20 us — so the checks are
-flat, buffers are allocated together, and the descriptors are packed in one call."""
+"""What the token operators (layer_norm, rotary, attention) share: element types and argument checks.  Buffers, launches and autograd nodes are in
+csrc/token_ext.cpp."""
 import torch
 
 from ... import _lib
@@ -28,37 +26,3 @@ def require_same_device(op, first, *others):
         if t is not None and t.device != device:
             _lib.require_device(t)
             raise RuntimeError(f'{op}: all tensors must be on one device (got {device} and {t.device})')
-
-
-def launch(t, fn, *args):
-    """fn(*args, stream) on the device of `t`, on torch's current stream there, whatever the current device is.  The caller's locals keep every tensor of the
-    call alive until it returns: by then the work is enqueued, and the allocator's stream order protects the memory."""
-    if t.get_device() == _lib._get_device():
-        rc = fn(*args, _lib._stream_handle())
-    else:
-        with torch.cuda.device(t.device):
-            rc = fn(*args, _lib._stream_handle())
-    if rc != 0:
-        _lib.check(rc)
-
-
-def pointer(t):
-    return 0 if t is None else t.data_ptr()
-
-
-def wants_grad(*tensors):
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                return True
-    return False
-
-
-def once(backward):
-    """Marks a Function's `backward` as differentiable once: under create_graph its results refuse a second derivative (torch's once_differentiable); without
-    it — every ordinary step — the wrapper's bookkeeping is skipped."""
-    guarded = torch.autograd.function.once_differentiable(backward)
-
-    def run(ctx, *grads):
-        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
-    return staticmethod(run)

@@ -1,59 +1,12 @@
 """rotary — rotary positions with several axes (time, height, width) for tokens of images and videos, on libn3d.so (csrc/rotary.hip).
 
 Not an operator of the reference's layer; it turns the queries and keys of `attention`."""
-import struct
-
 import torch
 
 from ... import _lib
-from ._tokens import DTYPES, launch, once, pointer, require_same_device, require_tensor, wants_grad
+from ._tokens import DTYPES, require_same_device, require_tensor
 
-_POSITIONS = {torch.float32: 0, torch.int32: 1, torch.int64: 2}
-_PACK = struct.Struct('=5Q8qd15i4x')                                     # n3d_rotary_desc, field by field
-
-
-def _turn(q, k, positions, plan, inverse):
-    sections, base, interleaved, shared = plan
-    first = k if q is None else q
-    b, l, _, d = first.shape
-    yq = yk = None
-    q_strides = k_strides = (0, 0, 0)
-    if q is not None:
-        if q.stride(3) != 1:
-            q = q.contiguous()
-        yq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        q_strides = q.stride()[:3]
-    if k is not None:
-        if k.stride(3) != 1:
-            k = k.contiguous()
-        yk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        k_strides = k.stride()[:3]
-    desc = _lib.RotaryDesc.from_buffer_copy(_PACK.pack(
-        pointer(q), pointer(k), positions.data_ptr(), pointer(yq), pointer(yk), *q_strides, *k_strides,
-        positions.stride(0) if positions.ndim == 3 and positions.shape[0] > 1 else 0, positions.stride(-2), base, b, l, 0 if q is None else q.shape[2],
-        0 if k is None else k.shape[2], d, len(sections), *sections, *(0,) * (4 - len(sections)), DTYPES[first.dtype], _POSITIONS[positions.dtype], interleaved,
-        shared, inverse))
-    launch(first, _lib.lib().n3d_rotary, desc)
-    return yq, yk
-
-
-class _Rotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, positions, plan):
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(positions)
-        ctx.plan = plan
-        yq, yk = _turn(q, k, positions, plan, False)
-        return yq if k is None else (yq, yk)
-
-    @once
-    def backward(ctx, dq, dk=None):
-        positions, = ctx.saved_tensors
-        dq = dq if ctx.needs_input_grad[0] else None
-        dk = dk if ctx.needs_input_grad[1] else None
-        if dq is None and dk is None:
-            return None, None, None, None
-        return (*_turn(dq, dk, positions, ctx.plan, True), None, None)
+_POSITIONS = (torch.float32, torch.int32, torch.int64)
 
 
 def rotary(q, positions, sections, k=None, base=10000.0, pairing='interleaved', ladder='axis'):
@@ -89,10 +42,5 @@ def rotary(q, positions, sections, k=None, base=10000.0, pairing='interleaved', 
     if positions.requires_grad:
         raise RuntimeError('rotary: positions have no gradient')
     require_same_device('rotary', q, k, positions)
-    if positions.stride(-1) != 1:
-        positions = positions.contiguous()
-    plan = (sections, base, pairing == 'interleaved', ladder == 'shared')
-    if wants_grad(q, k):
-        return _Rotary.apply(q, k, positions, plan)
-    yq, yk = _turn(q, k, positions, plan, False)
+    yq, yk = _lib.token_ext().rotary(q, k, positions, sections, base, pairing == 'interleaved', ladder == 'shared')
     return yq if k is None else (yq, yk)

@@ -227,3 +227,17 @@ def test_rotary_only_one_gradient_and_differences(dev):
     analytic = (gk.cpu().double() * step)
     assert abs((f[0] - f[1]) / (2 * h) - float(analytic.sum())) <= 2.0 ** -20 * float(analytic.abs().sum()) + 1e-9      # linear: no truncation
 
+
+
+def test_token_ops_refuse_second_derivatives(dev):
+    """Under create_graph the gradients come out as ever, and differentiating them again raises."""
+    from next3d_amd.torch_utils.ops import attention, layer_norm, rotary
+    x = _randn((3, 64), 1).to(dev).requires_grad_()
+    q, k, v = (_randn((1, 5, 2, 16), s, F16).to(dev).requires_grad_() for s in (2, 3, 4))
+    pos = torch.arange(5, device=dev).reshape(5, 1)
+    for leaves, f in (((x,), lambda: layer_norm.layer_norm(x)), ((q,), lambda: rotary.rotary(q, pos, (16,))), ((q, k, v), lambda: attention.attention(q, k, v))):
+        plain = torch.autograd.grad(f().sum(), leaves)
+        graph = torch.autograd.grad(f().sum(), leaves, create_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(plain, graph))
+        with pytest.raises(RuntimeError, match='differentiable once'):
+            torch.autograd.grad(graph[0].float().square().sum(), leaves)
