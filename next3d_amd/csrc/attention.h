@@ -87,8 +87,10 @@ struct AttnScore {
         cap_out = p.softcap > 0.f ? p.softcap * ATTN_LOG2E : 0.f;
         slope = p.slopes ? p.slopes[head] * ATTN_LOG2E : 0.f;
     }
-    // tanh x = 1 - 2 / (1 + e^2x): off by some 2^-23 absolutely, 2^-23 cap of a score
-    __device__ __forceinline__ float tanh_part(float s) const { return 1.f - 2.f * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s * cap_in)); }
+    // tanh x = 1 - 2 r with r = 1 / (1 + e^2x), off by some 2^-23 absolutely, 2^-23 cap of a score;  1 - tanh^2 = 4 (r - r^2)
+    __device__ __forceinline__ float cap_r(float s) const { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s * cap_in)); }
+    // the capped score less `sub`
+    __device__ __forceinline__ float capped(float r, float sub) const { return __builtin_fmaf(-2.f * cap_out, r, cap_out - sub); }
 };
 
 // ---- LDS tiles: ROW channels of 16 bits a row (64 or 128; channels beyond D are zero), rows of 16-byte chunks.  Chunk c of row r sits at c ^ swizzle(r):
@@ -234,7 +236,7 @@ __device__ __forceinline__ float attn_dot(const T* a, const T* c, int D) {
 }
 // base-2 score of raw product s at distance `dist`
 __device__ __forceinline__ float attn_score(const AttnScore& f, float s, int dist) {
-    const float u = f.cap_out > 0.f ? f.cap_out * f.tanh_part(s) : s * f.mul;
+    const float u = f.cap_out > 0.f ? f.capped(f.cap_r(s), 0.f) : s * f.mul;
     return u - f.slope * fabsf((float)dist);
 }
 
@@ -292,9 +294,9 @@ static inline const char* attn_params(const n3d_attention_desc* d, AttnParams& p
     return nullptr;
 }
 
-// How a score comes out of the raw product: 0 a positive multiple of it, 1 any multiple and a distance, 2 a cap (and a distance).  Each is straight code of
+// How a score comes out of the raw product: a positive multiple of it; any multiple and a distance; a cap; a cap and a distance.  Each is straight code of
 // its own in the kernels: values that pass through a branch in place cost a register copy each, and no product is scheduled across it.
-enum { ATTN_PLAIN = 0, ATTN_BIAS = 1, ATTN_CAP = 2 };
+enum { ATTN_PLAIN = 0, ATTN_BIAS = 1, ATTN_CAP = 2, ATTN_CAP_BIAS = 3 };
 // f(element type, 32-channel blocks, mode, documents)
 template <typename F>
 static inline void attn_dispatch(int dtype, const AttnParams& p, F&& f) {
@@ -303,9 +305,13 @@ static inline void attn_dispatch(int dtype, const AttnParams& p, F&& f) {
         else f(t, db, mode, std::false_type());
     };
     auto form = [&](auto* t, auto db) {
-        if (p.softcap > 0.f) doc(t, db, std::integral_constant<int, ATTN_CAP>());
-        else if (p.slopes || !(p.scale > 0.f)) doc(t, db, std::integral_constant<int, ATTN_BIAS>());
-        else doc(t, db, std::integral_constant<int, ATTN_PLAIN>());
+        if (p.softcap > 0.f) {
+            if (p.slopes) doc(t, db, std::integral_constant<int, ATTN_CAP_BIAS>());
+            else doc(t, db, std::integral_constant<int, ATTN_CAP>());
+        } else {
+            if (p.slopes || !(p.scale > 0.f)) doc(t, db, std::integral_constant<int, ATTN_BIAS>());
+            else doc(t, db, std::integral_constant<int, ATTN_PLAIN>());
+        }
     };
     auto typed = [&](auto* t) {
         switch (cdiv(p.D, 32)) {

@@ -87,20 +87,20 @@ __device__ __forceinline__ int attn_ds_scale(const AttnParams& p, int lane) {
 // Raw score and dP of one element -> P 2^shift and ds 2^e (ds_by 1 where T needs no scaling: no multiplication then)
 template <typename T, int MODE>
 __device__ __forceinline__ void attn_ds(f32x16& S, f32x16& dP, int r, const AttnScore& f, float ds_by, float lse2, float delta, float dist) {
-    float w, d = dP[r] - delta;
-    if constexpr (MODE == ATTN_CAP) {
-        const float th = f.tanh_part(S[r]);
-        w = __builtin_amdgcn_exp2f(__builtin_fmaf(f.cap_out, th, -lse2) - f.slope * fabsf(dist));
-        d *= 1.f - th * th;
-    } else if constexpr (MODE == ATTN_BIAS) {
-        w = __builtin_amdgcn_exp2f(__builtin_fmaf(S[r], f.mul, -lse2) - f.slope * fabsf(dist));
+    float u, d = dP[r] - delta;
+    if constexpr (MODE == ATTN_CAP || MODE == ATTN_CAP_BIAS) {
+        const float x = f.cap_r(S[r]);
+        u = f.capped(x, lse2);
+        d *= __builtin_fmaf(-x, x, x);                       // a quarter of 1 - tanh^2: attn_ds_unit
     } else {
-        w = __builtin_amdgcn_exp2f(__builtin_fmaf(S[r], f.mul, -lse2));
+        u = __builtin_fmaf(S[r], f.mul, -lse2);
     }
-    S[r] = w;
+    if constexpr (MODE == ATTN_BIAS || MODE == ATTN_CAP_BIAS) u -= f.slope * fabsf(dist);
+    S[r] = __builtin_amdgcn_exp2f(u);
     if constexpr (ATTN_P_SHIFT<T> != 0.f) d *= ds_by;
-    dP[r] = w * d;
+    dP[r] = S[r] * d;
 }
+template <int MODE> static constexpr float attn_ds_unit() { return MODE == ATTN_CAP || MODE == ATTN_CAP_BIAS ? 4.f : 1.f; }
 
 template <typename T>
 __device__ __forceinline__ void attn_pack(const f32x16& x, typename AttnVec<T>::x8 (&out)[2]) {
@@ -115,9 +115,9 @@ template <typename T>
 __device__ __forceinline__ void attn_pair(const AttnParams& p, const AttnScore& f, const T* q, const T* k, const T* v, const T* dout, float lse2, float delta, int dist,
                                           float& w, float& ds) {
     const float s = attn_dot<T>(q, k, p.D);
-    const float th = f.cap_out > 0.f ? f.tanh_part(s) : 0.f;
+    const float x = f.cap_out > 0.f ? f.cap_r(s) : 0.5f;
     w = __builtin_amdgcn_exp2f(attn_score(f, s, dist) - lse2);
-    ds = w * (attn_dot<T>(dout, v, p.D) - delta) * (1.f - th * th);
+    ds = w * (attn_dot<T>(dout, v, p.D) - delta) * 4.f * (x - x * x);
 }
 __device__ __forceinline__ float attn_lse2(float lse) { return lse == -INFINITY ? INFINITY : lse * ATTN_LOG2E; }       // (a row that sees nothing: every weight 0)
 
@@ -258,7 +258,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnParams p) {
     uint64_t redo = __ballot(nan && row_ok && lse2 == lse2);
     redo = (redo | (redo >> 32)) & 0xffffffffu;
     T* out = (T*)p.dq + ((int64_t)(b * (int64_t)p.Lq + i) * p.Hq + h) * p.D;
-    attn_store_row<T, DB>(out, acc, ldexpf(p.scale, -ds_exp), half, p.D, row_ok && !((redo >> l31) & 1));
+    attn_store_row<T, DB>(out, acc, ldexpf(p.scale * attn_ds_unit<MODE>(), -ds_exp), half, p.D, row_ok && !((redo >> l31) & 1));
     while (redo) {                                                      // a NaN behind the mask may have come in through 0 * NaN: these rows key by key
         const int e = __builtin_ctzll(redo);
         redo &= redo - 1;
@@ -464,7 +464,7 @@ __global__ __launch_bounds__(256, DB > 2 ? 1 : 2) void attn_dkv_kernel(AttnParam
         for (int r = 0; r < 16; ++r) nan = nan || dk[db][r] != dk[db][r] || dv[db][r] != dv[db][r];
     uint64_t redo = __ballot(nan && key_ok);
     redo = (redo | (redo >> 32)) & 0xffffffffu;
-    const float k_by = ldexpf(p.scale, -ds_exp), v_by = ldexpf(1.f, -(int)SHIFT);
+    const float k_by = ldexpf(p.scale * attn_ds_unit<MODE>(), -ds_exp), v_by = ldexpf(1.f, -(int)SHIFT);
     const bool store = j < p.Lk && !((redo >> l31) & 1);
     if (!key_ok)                                                        // keys that nobody sees (their lanes held something else)
 #pragma unroll

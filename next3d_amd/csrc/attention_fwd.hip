@@ -60,8 +60,8 @@ __device__ __forceinline__ void attn_softmax_form(f32x16 (&S)[KB], typename Attn
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const float u = MODE == ATTN_CAP ? f.cap_out * f.tanh_part(S[kb][r]) : S[kb][r] * f.mul;
-                S[kb][r] = u - f.slope * fabsf(dist - (float)(32 * kb + 8 * (r >> 2) + (r & 3)));
+                S[kb][r] = MODE == ATTN_BIAS ? S[kb][r] * f.mul : f.capped(f.cap_r(S[kb][r]), 0.f);
+                if constexpr (MODE != ATTN_CAP) S[kb][r] -= f.slope * fabsf(dist - (float)(32 * kb + 8 * (r >> 2) + (r & 3)));
             }
     }
     if constexpr (MASK) {
