@@ -528,7 +528,8 @@ int n3d_rotary(const n3d_rotary_desc* desc, n3d_stream_t stream);
  * workspace: n3d_attention_workspace(desc) bytes (-1: refused, see n3d_last_error), 16-byte aligned; nothing in it outlives the call. */
 typedef struct {
     const void *q, *k, *v;
-    void* out;
+    void *out, *out_rest;           /* out_rest: what rounding out to dtype left over, again in dtype, or NULL; given back to n3d_attention_bwd it keeps
+                                       sum(dout * out), from which every gradient subtracts, accurate (it may be NULL there too) */
     float* lse;
     const int *prefix, *lengths, *q_documents, *k_documents;
     const float* slopes;

@@ -65,7 +65,7 @@ class RotaryDesc(ctypes.Structure):
 
 
 class AttentionDesc(ctypes.Structure):
-    _fields_ = [('q', c_void_p), ('k', c_void_p), ('v', c_void_p), ('out', c_void_p), ('lse', c_void_p), ('prefix', c_void_p), ('lengths', c_void_p),
+    _fields_ = [('q', c_void_p), ('k', c_void_p), ('v', c_void_p), ('out', c_void_p), ('out_rest', c_void_p), ('lse', c_void_p), ('prefix', c_void_p), ('lengths', c_void_p),
                 ('q_documents', c_void_p), ('k_documents', c_void_p), ('slopes', c_void_p), ('workspace', c_void_p), ('dout', c_void_p), ('dq', c_void_p),
                 ('dk', c_void_p), ('dv', c_void_p), ('q_strides', c_int64 * 3), ('k_strides', c_int64 * 3), ('v_strides', c_int64 * 3),
                 ('dout_strides', c_int64 * 3), ('q_doc_stride', c_int64), ('k_doc_stride', c_int64), ('workspace_bytes', c_int64), ('scale', c_float),

@@ -20,7 +20,7 @@ static constexpr int ATTN_TILE = 64;                 // keys (queries in the dk 
 
 struct AttnParams {
     const void *q, *k, *v, *o, *dout;
-    void *out, *dq, *dk, *dv;
+    void *out, *rest, *dq, *dk, *dv;
     float* lse;
     int64_t qs[3], ks[3], vs[3], ds[3];              // element strides (batch, token, head) of q, k, v, dout; out / dq / dk / dv are dense
     const int *prefix, *lengths, *qdoc, *kdoc;
@@ -240,8 +240,8 @@ __device__ __forceinline__ float attn_score(const AttnScore& f, float s, int dis
     return u - f.slope * fabsf((float)dist);
 }
 
-// a row's 32 * DB channels spread over lanes l31 and l31 + 32 -> 16-byte stores (the halves trade their 8-byte runs)
-template <typename T, int DB>
+// a row's 32 * DB channels spread over lanes l31 and l31 + 32 -> 16-byte stores (the halves trade their 8-byte runs).  REST: what the rounding left over
+template <typename T, int DB, bool REST = false>
 __device__ __forceinline__ void attn_store_row(T* row, const f32x16 (&acc)[DB], float by, int half, int D, bool on) {
 #pragma unroll
     for (int db = 0; db < DB; ++db)
@@ -250,8 +250,9 @@ __device__ __forceinline__ void attn_store_row(T* row, const f32x16 (&acc)[DB], 
             typename AttnVec<T>::x4 x, y;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                x[e] = (T)(acc[db][4 * a + e] * by);
-                y[e] = (T)(acc[db][4 * a + 4 + e] * by);
+                const float u = acc[db][4 * a + e] * by, w = acc[db][4 * a + 4 + e] * by;
+                x[e] = REST ? (T)(u - (float)(T)u) : (T)u;
+                y[e] = REST ? (T)(w - (float)(T)w) : (T)w;
             }
             uint2 u = __builtin_bit_cast(uint2, x), w = __builtin_bit_cast(uint2, y);
             const auto r0 = __builtin_amdgcn_permlane32_swap(u.x, w.x, false, false);
@@ -259,6 +260,18 @@ __device__ __forceinline__ void attn_store_row(T* row, const f32x16 (&acc)[DB], 
             const int d = 32 * db + 8 * a + 8 * half;
             if (on && d < D) *reinterpret_cast<uint4*>(row + d) = make_uint4(r0[0], r1[0], r0[1], r1[1]);
         }
+}
+// channels lane and lane + 64 of a finished row -> out (and rest)
+template <typename T>
+__device__ __forceinline__ void attn_store_pair(const AttnParams& p, int64_t at, const float (&x)[2], float by, int lane) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        const int d = lane + 64 * c;
+        if (d >= p.D) continue;
+        const T t = (T)(x[c] * by);
+        ((T*)p.out)[at + d] = t;
+        if (p.rest) ((T*)p.rest)[at + d] = (T)(x[c] * by - (float)t);
+    }
 }
 
 // ---- host: a checked descriptor as kernel parameters
@@ -279,9 +292,9 @@ static inline const char* attn_params(const n3d_attention_desc* d, AttnParams& p
     for (const int64_t* s : strides)
         for (int i = 0; i < 3; ++i)
             if (s[i] % 8 || s[i] < 0 || (i == 1 && s[i] > (1 << 23))) return "strides must be multiples of 8 elements, of tokens 2^23 at most";
-    if (((uintptr_t)d->q | (uintptr_t)d->k | (uintptr_t)d->v | (uintptr_t)d->out) % 16) return "tensors must be 16-byte aligned";
+    if (((uintptr_t)d->q | (uintptr_t)d->k | (uintptr_t)d->v | (uintptr_t)d->out | (uintptr_t)d->out_rest) % 16) return "tensors must be 16-byte aligned";
     p = AttnParams{};
-    p.q = d->q; p.k = d->k; p.v = d->v; p.out = d->out; p.o = d->out; p.lse = d->lse;
+    p.q = d->q; p.k = d->k; p.v = d->v; p.out = d->out; p.o = d->out; p.rest = d->out_rest; p.lse = d->lse;
     for (int i = 0; i < 3; ++i) {
         p.qs[i] = d->q_strides[i]; p.ks[i] = d->k_strides[i]; p.vs[i] = d->v_strides[i]; p.ds[i] = d->dout_strides[i];
     }

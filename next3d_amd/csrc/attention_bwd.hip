@@ -29,9 +29,11 @@ __global__ __launch_bounds__(256) void attn_prep_kernel(AttnParams p) {
             if (lane16 * 8 < D) {
                 const auto x = *reinterpret_cast<const typename AttnVec<T>::x8*>((const T*)p.dout + b * p.ds[0] + i * p.ds[1] + h * p.ds[2] + lane16 * 8);
                 const auto y = *reinterpret_cast<const typename AttnVec<T>::x8*>((const T*)p.o + w * D + lane16 * 8);
+                typename AttnVec<T>::x8 z = {};
+                if (p.rest) z = *reinterpret_cast<const typename AttnVec<T>::x8*>((const T*)p.rest + w * D + lane16 * 8);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    s += (float)x[e] * (float)y[e];
+                    s += (float)x[e] * ((float)y[e] + (float)z[e]);
                     const float a = fabsf((float)x[e]);
                     if (live && a < INFINITY) top = fmaxf(top, a);
                 }

@@ -244,8 +244,10 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnParams p) {
         for (int r = 0; r < 16; ++r) nan = nan || acc[db][r] != acc[db][r];
     uint64_t redo = __ballot(nan && sum == sum && row_ok);
     redo = (redo | (redo >> 32)) & 0xffffffffu;
-    T* out = (T*)p.out + ((int64_t)(b * (int64_t)p.Lq + i) * p.Hq + h) * p.D;
-    attn_store_row<T, DB>(out, acc, by, half, p.D, row_ok && !((redo >> l31) & 1));
+    const int64_t row_at = ((int64_t)(b * (int64_t)p.Lq + i) * p.Hq + h) * p.D;
+    const bool store = row_ok && !((redo >> l31) & 1);
+    attn_store_row<T, DB>((T*)p.out + row_at, acc, by, half, p.D, store);
+    if (p.rest) attn_store_row<T, DB, true>((T*)p.rest + row_at, acc, by, half, p.D, store);
     if (p.lse && row_ok && half == 0) p.lse[((int64_t)b * p.Hq + h) * p.Lq + i] = sum == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(sum)) * ATTN_LN2;
     while (redo) {
         const int e = __builtin_ctzll(redo);
@@ -254,9 +256,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnParams p) {
         const float me = __shfl(m, e), bye = __shfl(by, e);
         float row[2];
         attn_exact_row<T>(p, b, ie, h, 0, n, me, lane, row);
-        T* o = (T*)p.out + ((int64_t)(b * (int64_t)p.Lq + ie) * p.Hq + h) * p.D;
-        if (lane < p.D) o[lane] = (T)(row[0] * bye);
-        if (lane + 64 < p.D) o[lane + 64] = (T)(row[1] * bye);
+        attn_store_pair<T>(p, ((int64_t)(b * (int64_t)p.Lq + ie) * p.Hq + h) * p.D, row, bye, lane);
     }
 #endif
 }
@@ -373,10 +373,7 @@ __global__ __launch_bounds__(256) void attn_token_kernel(AttnParams p) {
             }
         }
         if (direct) {
-            T* o = (T*)p.out + ((int64_t)(b * (int64_t)p.Lq + ie) * p.Hq + he) * p.D;
-            const float by = ae == 0.f ? 0.f : 1.f / ae;
-            if (lane < p.D) o[lane] = (T)(x[0] * by);
-            if (lane + 64 < p.D) o[lane + 64] = (T)(x[1] * by);
+            attn_store_pair<T>(p, ((int64_t)(b * (int64_t)p.Lq + ie) * p.Hq + he) * p.D, x, ae == 0.f ? 0.f : 1.f / ae, lane);
             if (p.lse && lane == 0) p.lse[((int64_t)b * p.Hq + he) * p.Lq + ie] = ae == 0.f ? -INFINITY : (te + __builtin_amdgcn_logf(ae)) * ATTN_LN2;
         } else {
             const int64_t at = (int64_t)(bh * (int64_t)rows + re) * p.splits + split;
@@ -410,10 +407,7 @@ __global__ __launch_bounds__(256) void attn_combine_kernel(AttnParams p) {
         if (lane < p.D) x[0] += by * a[lane];
         if (lane + 64 < p.D) x[1] += by * a[lane + 64];
     }
-    const float by = all == 0.f ? 0.f : 1.f / all;
-    T* o = (T*)p.out + ((int64_t)(b * (int64_t)p.Lq + i) * p.Hq + h) * p.D;
-    if (lane < p.D) o[lane] = (T)(x[0] * by);
-    if (lane + 64 < p.D) o[lane + 64] = (T)(x[1] * by);
+    attn_store_pair<T>(p, ((int64_t)(b * (int64_t)p.Lq + i) * p.Hq + h) * p.D, x, all == 0.f ? 0.f : 1.f / all, lane);
     if (p.lse && lane == 0) p.lse[((int64_t)b * p.Hq + h) * p.Lq + i] = all == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(all)) * ATTN_LN2;
 }
 

@@ -248,7 +248,7 @@ struct Attention : torch::autograd::Function<Attention> {
         bool causal;
     };
     // one call of the library; the operands' dense copies live until the work is enqueued
-    static void call(const Tensor& q, const Tensor& k, const Tensor& v, const Masks& m, const Tensor& out, const Tensor& lse, const Tensor& dout, const Tensor& dq,
+    static void call(const Tensor& q, const Tensor& k, const Tensor& v, const Masks& m, const Tensor& out, const Tensor& rest, const Tensor& lse, const Tensor& dout, const Tensor& dq,
                      const Tensor& dk, const Tensor& dv, n3d_stream_t stream) {
         n3d_attention_desc d = {};
         const Tensor q_ = operand(q, d.q_strides), k_ = operand(k, d.k_strides), v_ = operand(v, d.v_strides);
@@ -257,6 +257,7 @@ struct Attention : torch::autograd::Function<Attention> {
         d.k = k_.data_ptr();
         d.v = v_.data_ptr();
         d.out = out.data_ptr();
+        d.out_rest = ptr(rest);
         d.lse = (float*)ptr(lse);
         d.prefix = (const int*)ptr(m.prefix);
         d.lengths = (const int*)ptr(m.lengths);
@@ -290,16 +291,18 @@ struct Attention : torch::autograd::Function<Attention> {
         }
         check(dout.defined() ? lib.attention_bwd(&d, stream) : lib.attention(&d, stream));
     }
-    static std::pair<Tensor, Tensor> run(const Tensor& q, const Tensor& k, const Tensor& v, const Masks& m, bool want_lse) {
+    // out, lse, and (for a gradient) what rounding out left over
+    static std::tuple<Tensor, Tensor, Tensor> run(const Tensor& q, const Tensor& k, const Tensor& v, const Masks& m, bool want_lse, bool want_rest) {
         Scope scope(q);
         const Tensor out = dense(q), none;
         const Tensor lse = want_lse ? at::empty({q.size(0), q.size(2), q.size(1)}, q.options().dtype(at::kFloat)) : Tensor();
-        if (q.numel()) call(q, k, v, m, out, lse, none, none, none, none, scope.stream);
-        return {out, lse};
+        const Tensor rest = want_rest ? dense(q) : Tensor();
+        if (q.numel()) call(q, k, v, m, out, rest, lse, none, none, none, none, scope.stream);
+        return {out, lse, rest};
     }
     static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Masks& m) {
-        const auto [out, lse] = run(q, k, v, m, true);
-        ctx->save_for_backward({q, k, v, out, lse, m.prefix, m.documents, m.key_documents, m.lengths, m.slopes});
+        const auto [out, lse, rest] = run(q, k, v, m, true, true);
+        ctx->save_for_backward({q, k, v, out, lse, rest, m.prefix, m.documents, m.key_documents, m.lengths, m.slopes});
         ctx->saved_data["scale"] = m.scale;
         ctx->saved_data["softcap"] = m.softcap;
         ctx->saved_data["causal"] = m.causal;
@@ -312,7 +315,7 @@ struct Attention : torch::autograd::Function<Attention> {
         const Tensor &q = s[0], &k = s[1], &v = s[2];
         Tensor dq, dk, dv;
         if (grads[0].defined()) {
-            const Masks m = {s[5], s[6], s[7], s[8], s[9], ctx->saved_data["scale"].toDouble(), ctx->saved_data["softcap"].toDouble(), ctx->saved_data["causal"].toBool()};
+            const Masks m = {s[6], s[7], s[8], s[9], s[10], ctx->saved_data["scale"].toDouble(), ctx->saved_data["softcap"].toDouble(), ctx->saved_data["causal"].toBool()};
             const bool want_k = ctx->needs_input_grad(1), want_v = ctx->needs_input_grad(2);
             Scope scope(q);
             if (ctx->needs_input_grad(0)) dq = dense(q);
@@ -321,7 +324,7 @@ struct Attention : torch::autograd::Function<Attention> {
                 dv = dense(v);
             }
             if (q.numel()) {
-                call(q, k, v, m, s[3], s[4], grads[0], dq, dk, dv, scope.stream);
+                call(q, k, v, m, s[3], s[5], s[4], grads[0], dq, dk, dv, scope.stream);
             } else if (dk.defined()) {                                            // no queries: nothing flows
                 dk.zero_();
                 dv.zero_();
@@ -340,7 +343,7 @@ std::tuple<Tensor, Opt> attention(const Tensor& q, const Tensor& k, const Tensor
         variable_list r = Attention::apply(q, k, v, m);
         return {r[0], r[1]};
     }
-    auto [out, lse] = Attention::run(q, k, v, m, want_lse);
+    auto [out, lse, rest] = Attention::run(q, k, v, m, want_lse, false);
     return {out, lse.defined() ? Opt(lse) : Opt()};
 }
 

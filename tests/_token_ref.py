@@ -148,7 +148,8 @@ def attention(q, k, v, do=None, scale=None, causal=False, prefix=None, documents
     e_dv = ((p * (u + e_w + (group * n_q + 64) * U32)).transpose(2, 3) @ do_.abs()) + (step * 2.0 ** -12 + flush) * do_.abs().sum(2, keepdim=True)
     delta = (do_ * o).sum(3, keepdim=True)
     dp = do_ @ v_.transpose(2, 3)
-    e_d = (do_.abs() * e_o).sum(3, keepdim=True) + (d + 4) * U32 * (do_.abs() @ v_.abs().transpose(2, 3) + (do_ * o).abs().sum(3, keepdim=True))
+    e_oo = e_o - u * (1 - 2 * u) * o.abs()                                                  # (what out's rounding left over is kept, and rounded itself)
+    e_d = (do_.abs() * e_oo).sum(3, keepdim=True) + (d + 4) * U32 * (do_.abs() @ v_.abs().transpose(2, 3) + (do_ * o).abs().sum(3, keepdim=True))
     cap = 1 - th * th
     dt_ = p * (dp - delta)
     ds = torch.where(see, dt_ * cap * scale, torch.zeros_like(dt_))
