@@ -192,6 +192,14 @@ __device__ __forceinline__ void attn_sync() {
     asm volatile("" : : : "memory");
 }
 
+// LDS stores of all waves are visible; pieces stay in flight
+__device__ __forceinline__ void attn_traded() {
+    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" : : : "memory");
+}
+
 // ---- which tiles to visit: [t, end) in order; with documents only those whose range [lowest, highest] meets [lo, hi] (64 ranges looked at together)
 template <bool DOCS>
 struct AttnTiles {

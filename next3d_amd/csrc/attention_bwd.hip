@@ -291,15 +291,24 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnParams p) {
 #endif
 }
 
+// A wave owns 32 keys: their K and V as operands and their dk and dv as accumulators.  Beyond 96 channels that is more than half of a SIMD's registers, so
+// one wave a SIMD, whose vector work and products would wait for each other (537 us at 2 x 4096 x 16 heads x 128, causal with caps; two loops interleaved by
+// hand: 555).  There two waves share 32 keys (attn_dkv_pair): each takes the scores of half of a tile's queries, they trade the 16-bit weights through the
+// LDS, and each adds up half of the channels over all of the queries.
+template <int DB> static constexpr bool attn_dkv_pair() { return DB > 3; }
 template <typename T, int DB, int MODE, bool DOCS>
-__global__ __launch_bounds__(256, DB > 2 ? 1 : 2) void attn_dkv_kernel(AttnParams p) {
+__global__ __launch_bounds__(attn_dkv_pair<DB>() ? 512 : 256, 2) void attn_dkv_kernel(AttnParams p) {
 #ifdef __HIP_DEVICE_COMPILE__                            // (hipcc drops the launch stub of a template whose body its host pass cannot read)
     constexpr int ROW = DB > 2 ? 128 : 64, TILE_BYTES = ATTN_TILE * ROW * 2;
     constexpr float SHIFT = ATTN_P_SHIFT<T>;
+    constexpr bool PAIR = attn_dkv_pair<DB>();
+    constexpr int NB = PAIR ? DB / 2 : DB;                              // blocks of 32 channels a wave adds up
+    typedef typename AttnVec<T>::x8 frag;
     __shared__ __align__(1024) char smem[4 * TILE_BYTES];                 // [buffer][q, do]
     __shared__ __align__(16) float slse[2][ATTN_TILE], sdelta[2][ATTN_TILE];
     __shared__ __align__(16) int sdoc[2][ATTN_TILE];
-    const int wave = attn_uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
+    __shared__ __align__(16) char traded[PAIR ? 4 * 2 * 4 * 1024 : 16];   // [key group][half of the queries][w, w, d, d][lane] fragments
+    const int wave = attn_uniform(threadIdx.x >> 6), keys = PAIR ? wave & 3 : wave, part = PAIR ? wave >> 2 : 0, lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
     // p.splits: 1 (a workgroup adds up all heads of the group) or G (one head a workgroup, float32 parts that attn_parts_kernel adds in order)
     const int total = p.B * p.Hk * p.splits * p.row_blocks, per = (total + 7) / 8;
     const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
@@ -307,14 +316,14 @@ __global__ __launch_bounds__(256, DB > 2 ? 1 : 2) void attn_dkv_kernel(AttnParam
     const int blk = id % p.row_blocks, split = id / p.row_blocks % p.splits, bh = id / p.row_blocks / p.splits, hk = bh % p.Hk, b = bh / p.Hk;
     const int g0 = p.splits > 1 ? split : 0, g1 = p.splits > 1 ? split + 1 : p.G;
     const int n = attn_keys(p, b), prefix = p.prefix ? p.prefix[b] : 0, k0 = blk * 128, off = n - p.Lq;
-    const int j = k0 + 32 * wave + l31;
+    const int j = k0 + 32 * keys + l31;
     const int kdoc = DOCS && j < p.Lk ? p.kdoc[b * p.kdoc_stride + j] : 0;
     const bool key_ok = j < n && kdoc >= 0;
     // first query that sees key x
     auto first_query = [&](int x) { return !p.causal || x < prefix ? 0 : max(x - off, 0); };
     const int qmin = key_ok ? first_query(j) : 0x7fffffff;
-    const int wave_first = first_query(k0 + 32 * wave);
-    const bool wave_on = k0 + 32 * wave < n;
+    const int wave_first = first_query(k0 + 32 * keys);
+    const bool wave_on = k0 + 32 * keys < n;
     int dlo = 0, dhi = 0;
     if constexpr (DOCS) {
         const int2* r = p.ktiles + (int64_t)b * p.nkt + 2 * blk;
@@ -336,7 +345,7 @@ __global__ __launch_bounds__(256, DB > 2 ? 1 : 2) void attn_dkv_kernel(AttnParam
         }
         return t;
     };
-    typename AttnVec<T>::x8 kf[2 * DB], vf[2 * DB];
+    frag kf[2 * DB], vf[2 * DB];
     const T* k = j < n ? (const T*)p.k + b * p.ks[0] + j * p.ks[1] + hk * p.ks[2] : nullptr;
     const T* v = j < n ? (const T*)p.v + b * p.vs[0] + j * p.vs[1] + hk * p.vs[2] : nullptr;
 #pragma unroll
@@ -344,7 +353,7 @@ __global__ __launch_bounds__(256, DB > 2 ? 1 : 2) void attn_dkv_kernel(AttnParam
         kf[c] = attn_lane_frag<T>(k, 2 * c + half, p.D);
         vf[c] = attn_lane_frag<T>(v, 2 * c + half, p.D);
     }
-    AttnStage<ROW, ATTN_TILE, 4> sq, sd;
+    AttnStage<ROW, ATTN_TILE, PAIR ? 8 : 4> sq, sd;
     sq.setup(wave, lane, p.qs[1], p.D);
     sd.setup(wave, lane, p.ds[1], p.D);
     const int ds_exp = attn_ds_scale(p, lane);
@@ -369,7 +378,7 @@ __global__ __launch_bounds__(256, DB > 2 ? 1 : 2) void attn_dkv_kernel(AttnParam
         if (wave == 1) sdelta[buf][lane] = row_next;
         if (DOCS && wave == 2) sdoc[buf][lane] = __builtin_bit_cast(int, row_next);
     };
-    f32x16 dk[DB] = {}, dv[DB] = {};
+    f32x16 dk[NB] = {}, dv[NB] = {};
     AttnScore f(p, hk * p.G);
     int t = next(g), buf = 0;
     if (t >= 0) stage(t, g, 0);
@@ -384,73 +393,114 @@ __global__ __launch_bounds__(256, DB > 2 ? 1 : 2) void attn_dkv_kernel(AttnParam
         t = next(g);
         buf ^= 1;
         if (t >= 0) stage(t, g, buf);
-        if (wave_on && (!mask.value || i0 + ATTN_TILE - 1 >= wave_first)) {
-            f.slope = slope;
-            const uint32_t q_lds = at_lane.rows(lds + now * 2 * TILE_BYTES), d_lds = at_lane.rows(lds + now * 2 * TILE_BYTES + TILE_BYTES);
-            const uint32_t qc_lds = at_lane.cols(lds + now * 2 * TILE_BYTES), dc_lds = at_lane.cols(lds + now * 2 * TILE_BYTES + TILE_BYTES);
+        const bool on = wave_on && (!mask.value || i0 + ATTN_TILE - 1 >= wave_first);
+        f.slope = slope;
+        constexpr int BLOCK = 32 * ROW * 2;                             // bytes of half a tile
+        const uint32_t tile = lds + now * 2 * TILE_BYTES;
+        // weights and dscores of the 32 queries of half a tile as second operands
+        auto weights = [&](int qb, frag (&w)[2], frag (&d)[2]) {
+            const uint32_t q_lds = at_lane.rows(tile + qb * BLOCK), d_lds = at_lane.rows(tile + TILE_BYTES + qb * BLOCK);
+            frag qf[2 * DB], df[2 * DB];
+            constexpr int FIRST = DB > 2 ? DB : 0;                      // (as in attn_dq_kernel)
+            f32x16 S = {}, dP = {};
+#pragma unroll
+            for (int c = 0; c < 2 * DB; ++c) qf[c] = attn_row_frag<T, ROW>(q_lds, 0, c);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int c = 0; c < FIRST; ++c) S = attn_mfma(qf[c], kf[c], S);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int c = 0; c < 2 * DB; ++c) df[c] = attn_row_frag<T, ROW>(d_lds, 0, c);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int c = FIRST; c < 2 * DB; ++c) S = attn_mfma(qf[c], kf[c], S);
+#pragma unroll
+            for (int c = 0; c < 2 * DB; ++c) dP = attn_mfma(df[c], vf[c], dP);
+            __builtin_amdgcn_sched_barrier(0);
+            const int ib = 32 * qb + 4 * half;
+            const float dist = (float)(i0 + ib + off - j);
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+                const float4 l4 = *reinterpret_cast<const float4*>(&slse[now][ib + 8 * a]), e4 = *reinterpret_cast<const float4*>(&sdelta[now][ib + 8 * a]);
+                const float l[4] = {l4.x, l4.y, l4.z, l4.w}, de[4] = {e4.x, e4.y, e4.z, e4.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) attn_ds<T, MODE>(S, dP, 4 * a + e, f, ds_by, l[e], de[e], dist + (float)(8 * a + e));
+            }
+            if constexpr (mask.value) {
+                const int first = qmin - i0 - ib;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const bool see = 8 * (r >> 2) + (r & 3) >= first;
+                    S[r] = see ? S[r] : 0.f;
+                    dP[r] = see ? dP[r] : 0.f;
+                }
+                if constexpr (DOCS)
+#pragma unroll
+                    for (int a = 0; a < 4; ++a) {
+                        const int4 o4 = *reinterpret_cast<const int4*>(&sdoc[now][ib + 8 * a]);
+                        const int o[4] = {o4.x, o4.y, o4.z, o4.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const bool see = o[e] == kdoc;
+                            S[4 * a + e] = see ? S[4 * a + e] : 0.f;
+                            dP[4 * a + e] = see ? dP[4 * a + e] : 0.f;
+                        }
+                    }
+            }
+            attn_pack<T>(S, w);
+            attn_pack<T>(dP, d);
+        };
+        // first operands of half a tile, this wave's channels
+        auto columns = [&](int qb, frag (&qc)[NB][2], frag (&dc)[NB][2]) {
+            const uint32_t qc_lds = at_lane.cols(tile + qb * BLOCK) ^ (part << 7), dc_lds = at_lane.cols(tile + TILE_BYTES + qb * BLOCK) ^ (part << 7);
+#pragma unroll
+            for (int db = 0; db < NB; ++db)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    dc[db][c] = attn_col_frag<T, ROW>(dc_lds, c, db);
+                    qc[db][c] = attn_col_frag<T, ROW>(qc_lds, c, db);
+                }
+        };
+        auto products = [&](const frag (&w)[2], const frag (&d)[2], const frag (&qc)[NB][2], const frag (&dc)[NB][2]) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int db = 0; db < NB; ++db) {
+                    dv[db] = attn_mfma(dc[db][c], w[c], dv[db]);
+                    dk[db] = attn_mfma(qc[db][c], d[c], dk[db]);
+                }
+        };
+        if constexpr (PAIR) {
+            frag w[2], d[2], qc[NB][2], dc[NB][2];
+            frag* mine = reinterpret_cast<frag*>(traded) + (keys * 2 + part) * 4 * 64 + lane;
+            const frag* theirs = reinterpret_cast<const frag*>(traded) + (keys * 2 + (part ^ 1)) * 4 * 64 + lane;
+            if (on) {
+                weights(part, w, d);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    mine[c * 64] = w[c];
+                    mine[(2 + c) * 64] = d[c];
+                }
+                columns(part, qc, dc);
+                products(w, d, qc, dc);
+            }
+            attn_traded();
+            if (on) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    w[c] = theirs[c * 64];
+                    d[c] = theirs[(2 + c) * 64];
+                }
+                columns(part ^ 1, qc, dc);
+                products(w, d, qc, dc);
+            }
+        } else if (on) {
 #pragma unroll
             for (int qb = 0; qb < 2; ++qb) {
-                typename AttnVec<T>::x8 qf[2 * DB], df[2 * DB], qc[DB][2], dc[DB][2], w[2], d[2];
-#pragma unroll
-                for (int c = 0; c < 2 * DB; ++c) {
-                    qf[c] = attn_row_frag<T, ROW>(q_lds, qb, c);
-                    df[c] = attn_row_frag<T, ROW>(d_lds, qb, c);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-                f32x16 S = {}, dP = {};
-#pragma unroll
-                for (int c = 0; c < 2 * DB; ++c) {
-                    S = attn_mfma(qf[c], kf[c], S);
-                    dP = attn_mfma(df[c], vf[c], dP);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int db = 0; db < DB; ++db)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        dc[db][c] = attn_col_frag<T, ROW>(dc_lds, 2 * qb + c, db);
-                        qc[db][c] = attn_col_frag<T, ROW>(qc_lds, 2 * qb + c, db);
-                    }
-                __builtin_amdgcn_sched_barrier(0);
-                const int ib = 32 * qb + 4 * half;
-                const float dist = (float)(i0 + ib + off - j);
-#pragma unroll
-                for (int a = 0; a < 4; ++a) {
-                    const float4 l4 = *reinterpret_cast<const float4*>(&slse[now][ib + 8 * a]), e4 = *reinterpret_cast<const float4*>(&sdelta[now][ib + 8 * a]);
-                    const float l[4] = {l4.x, l4.y, l4.z, l4.w}, de[4] = {e4.x, e4.y, e4.z, e4.w};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) attn_ds<T, MODE>(S, dP, 4 * a + e, f, ds_by, l[e], de[e], dist + (float)(8 * a + e));
-                }
-                if constexpr (mask.value) {
-                    const int first = qmin - i0 - ib;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const bool see = 8 * (r >> 2) + (r & 3) >= first;
-                        S[r] = see ? S[r] : 0.f;
-                        dP[r] = see ? dP[r] : 0.f;
-                    }
-                    if constexpr (DOCS)
-#pragma unroll
-                        for (int a = 0; a < 4; ++a) {
-                            const int4 o4 = *reinterpret_cast<const int4*>(&sdoc[now][ib + 8 * a]);
-                            const int o[4] = {o4.x, o4.y, o4.z, o4.w};
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const bool see = o[e] == kdoc;
-                                S[4 * a + e] = see ? S[4 * a + e] : 0.f;
-                                dP[4 * a + e] = see ? dP[4 * a + e] : 0.f;
-                            }
-                        }
-                }
-                attn_pack<T>(S, w);
-                attn_pack<T>(dP, d);
-#pragma unroll
-                for (int c = 0; c < 2; ++c)
-#pragma unroll
-                    for (int db = 0; db < DB; ++db) {
-                        dv[db] = attn_mfma(dc[db][c], w[c], dv[db]);
-                        dk[db] = attn_mfma(qc[db][c], d[c], dk[db]);
-                    }
+                frag w[2], d[2], qc[NB][2], dc[NB][2];
+                weights(qb, w, d);
+                columns(qb, qc, dc);
+                products(w, d, qc, dc);
             }
         }
         commit(buf);
@@ -461,7 +511,7 @@ __global__ __launch_bounds__(256, DB > 2 ? 1 : 2) void attn_dkv_kernel(AttnParam
     }
     bool nan = false;
 #pragma unroll
-    for (int db = 0; db < DB; ++db)
+    for (int db = 0; db < NB; ++db)
 #pragma unroll
         for (int r = 0; r < 16; ++r) nan = nan || dk[db][r] != dk[db][r] || dv[db][r] != dv[db][r];
     uint64_t redo = __ballot(nan && key_ok);
@@ -470,7 +520,7 @@ __global__ __launch_bounds__(256, DB > 2 ? 1 : 2) void attn_dkv_kernel(AttnParam
     const bool store = j < p.Lk && !((redo >> l31) & 1);
     if (!key_ok)                                                        // keys that nobody sees (their lanes held something else)
 #pragma unroll
-        for (int db = 0; db < DB; ++db)
+        for (int db = 0; db < NB; ++db)
 #pragma unroll
             for (int r = 0; r < 16; ++r) dk[db][r] = dv[db][r] = 0.f;
     const int64_t row = ((int64_t)b * p.Lk + j) * p.Hk + hk, all = (int64_t)p.B * p.Lk * p.Hk;
@@ -478,23 +528,23 @@ __global__ __launch_bounds__(256, DB > 2 ? 1 : 2) void attn_dkv_kernel(AttnParam
         float* pk = p.part + (2 * split * all + row) * p.D;
         float* pv = p.part + ((2 * split + 1) * all + row) * p.D;
 #pragma unroll
-        for (int db = 0; db < DB; ++db)
+        for (int db = 0; db < NB; ++db)
 #pragma unroll
             for (int a = 0; a < 4; ++a) {
-                const int d = 32 * db + 8 * a + 4 * half;
+                const int d = 64 * part + 32 * db + 8 * a + 4 * half;
                 if (store && d < p.D) {
                     *reinterpret_cast<float4*>(pk + d) = make_float4(dk[db][4 * a] * k_by, dk[db][4 * a + 1] * k_by, dk[db][4 * a + 2] * k_by, dk[db][4 * a + 3] * k_by);
                     *reinterpret_cast<float4*>(pv + d) = make_float4(dv[db][4 * a] * v_by, dv[db][4 * a + 1] * v_by, dv[db][4 * a + 2] * v_by, dv[db][4 * a + 3] * v_by);
                 }
             }
     } else {
-        attn_store_row<T, DB>((T*)p.dk + row * p.D, dk, k_by, half, p.D, store);
-        attn_store_row<T, DB>((T*)p.dv + row * p.D, dv, v_by, half, p.D, store);
+        attn_store_row<T, NB>((T*)p.dk + row * p.D + 64 * part, dk, k_by, half, p.D - 64 * part, store);
+        attn_store_row<T, NB>((T*)p.dv + row * p.D + 64 * part, dv, v_by, half, p.D - 64 * part, store);
     }
     while (redo) {
         const int e = __builtin_ctzll(redo);
         redo &= redo - 1;
-        const int je = k0 + 32 * wave + e, doce = __shfl(kdoc, e);
+        const int je = k0 + 32 * keys + e, doce = __shfl(kdoc, e);
         const T* ke = (const T*)p.k + b * p.ks[0] + je * p.ks[1] + hk * p.ks[2];
         const T* ve = (const T*)p.v + b * p.vs[0] + je * p.vs[1] + hk * p.vs[2];
         float xk[2] = {0.f, 0.f}, xv[2] = {0.f, 0.f};
@@ -529,7 +579,7 @@ __global__ __launch_bounds__(256, DB > 2 ? 1 : 2) void attn_dkv_kernel(AttnParam
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             const int d = lane + 64 * c;
-            if (d >= p.D) continue;
+            if (d >= p.D || (PAIR && c != part)) continue;
             if (p.splits > 1) {
                 p.part[(2 * split * all + re) * p.D + d] = xk[c] * p.scale;
                 p.part[((2 * split + 1) * all + re) * p.D + d] = xv[c];
@@ -573,7 +623,8 @@ static void attn_bwd_launch(AttnParams& p, int splits, hipStream_t stream) {
     if (p.dk && p.Lk > 0) {
         p.splits = splits;
         p.row_blocks = cdiv(p.Lk, 128);
-        hipLaunchKernelGGL((attn_dkv_kernel<T, DB, MODE, DOCS>), dim3(8 * cdiv(p.B * p.Hk * p.splits * p.row_blocks, 8)), dim3(256), 0, stream, p);
+        hipLaunchKernelGGL((attn_dkv_kernel<T, DB, MODE, DOCS>), dim3(8 * cdiv(p.B * p.Hk * p.splits * p.row_blocks, 8)),
+                           dim3(attn_dkv_pair<DB>() ? 512 : 256), 0, stream, p);
         if (splits > 1)
             hipLaunchKernelGGL((attn_parts_kernel<T>), dim3((unsigned)cdiv64((int64_t)p.B * p.Lk * p.Hk * p.D, 2048), 2), dim3(256), 0, stream, p);
     }
