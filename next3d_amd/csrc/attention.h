@@ -32,7 +32,8 @@ struct AttnParams {
     int64_t part_ml;                                 // offset of their statistics in `part`
     const float* maxima;                             // partial maxima (float16 gradients), see attn_ds_scale
     int n_maxima;
-    int B, Lq, Lk, Hq, Hk, G, D, nkt, nqt, causal, splits, row_blocks;
+    int B, Lq, Lk, Hq, Hk, G, D, nkt, nqt, causal, row_blocks;
+    int splits, chunks;                              // workgroups a row block's work is split over; of them over the long axis (dk / dv: per head)
     float scale, softcap;
 };
 
@@ -269,6 +270,17 @@ __device__ __forceinline__ void attn_store_row(T* row, const f32x16 (&acc)[DB], 
             if (on && d < D) *reinterpret_cast<uint4*>(row + d) = make_uint4(r0[0], r1[0], r0[1], r1[1]);
         }
 }
+// ... as float32
+template <int DB>
+__device__ __forceinline__ void attn_store_part(float* row, const f32x16 (&acc)[DB], float by, int half, int D, bool on) {
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            const int d = 32 * db + 8 * a + 4 * half;
+            if (on && d < D) *reinterpret_cast<float4*>(row + d) = make_float4(acc[db][4 * a] * by, acc[db][4 * a + 1] * by, acc[db][4 * a + 2] * by, acc[db][4 * a + 3] * by);
+        }
+}
 // channels lane and lane + 64 of a finished row -> out (and rest)
 template <typename T>
 __device__ __forceinline__ void attn_store_pair(const AttnParams& p, int64_t at, const float (&x)[2], float by, int lane) {
@@ -311,7 +323,7 @@ static inline const char* attn_params(const n3d_attention_desc* d, AttnParams& p
     p.B = d->B; p.Lq = d->Lq; p.Lk = d->Lk; p.Hq = d->heads_q; p.Hk = d->heads_k; p.G = d->heads_q / d->heads_k; p.D = d->D;
     p.nkt = cdiv(d->Lk, ATTN_TILE); p.nqt = cdiv(d->Lq, ATTN_TILE);
     p.causal = d->causal != 0; p.scale = d->scale; p.softcap = d->softcap;
-    p.splits = 1;
+    p.splits = p.chunks = 1;
     return nullptr;
 }
 

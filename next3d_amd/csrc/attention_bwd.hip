@@ -130,10 +130,11 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnParams p) {
     __shared__ __align__(1024) char smem[4 * TILE_BYTES];
     __shared__ __align__(16) int sdoc[2][ATTN_TILE];
     const int wave = attn_uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
-    const int total = p.B * p.Hq * p.row_blocks, per = (total + 7) / 8;
+    // p.splits > 1: the keys in that many runs of whole tiles, float32 parts that attn_parts_kernel adds in order
+    const int total = p.B * p.Hq * p.row_blocks * p.splits, per = (total + 7) / 8;
     const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
     if ((int)(blockIdx.x >> 3) >= per || id >= total) return;
-    const int blk = p.row_blocks - 1 - id % p.row_blocks, bh = id / p.row_blocks, h = bh % p.Hq, b = bh / p.Hq, hk = h / p.G;
+    const int split = id % p.splits, blk = p.row_blocks - 1 - id / p.splits % p.row_blocks, bh = id / p.splits / p.row_blocks, h = bh % p.Hq, b = bh / p.Hq, hk = h / p.G;
     const int n = attn_keys(p, b), prefix = p.prefix ? p.prefix[b] : 0, q0 = blk * 128;
     const int i = q0 + 32 * wave + l31;
     const bool row_ok = i < p.Lq;
@@ -149,7 +150,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnParams p) {
         dhi = max(r0.y, r1.y);
     }
     AttnTiles<DOCS> tiles;
-    tiles.start(DOCS ? p.ktiles + (int64_t)b * p.nkt : nullptr, 0, (key_end + ATTN_TILE - 1) / ATTN_TILE, max(dlo, 0), dhi);
+    const int run = (p.nkt + p.splits - 1) / p.splits, run_first = split * run, run_end = min((key_end + ATTN_TILE - 1) / ATTN_TILE, run_first + run);
+    tiles.start(DOCS ? p.ktiles + (int64_t)b * p.nkt : nullptr, run_first, run_end, max(dlo, 0), dhi);
     typename AttnVec<T>::x8 qf[2 * DB], df[2 * DB];
     const T* q = row_ok ? (const T*)p.q + b * p.qs[0] + i * p.qs[1] + h * p.qs[2] : nullptr;
     const T* dout = row_ok ? (const T*)p.dout + b * p.ds[0] + i * p.ds[1] + h * p.ds[2] : nullptr;
@@ -259,8 +261,11 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnParams p) {
         for (int r = 0; r < 16; ++r) nan = nan || acc[db][r] != acc[db][r];
     uint64_t redo = __ballot(nan && row_ok && lse2 == lse2);
     redo = (redo | (redo >> 32)) & 0xffffffffu;
-    T* out = (T*)p.dq + ((int64_t)(b * (int64_t)p.Lq + i) * p.Hq + h) * p.D;
-    attn_store_row<T, DB>(out, acc, ldexpf(p.scale * attn_ds_unit<MODE>(), -ds_exp), half, p.D, row_ok && !((redo >> l31) & 1));
+    const float by = ldexpf(p.scale * attn_ds_unit<MODE>(), -ds_exp);
+    const int64_t row_at = ((int64_t)(b * (int64_t)p.Lq + i) * p.Hq + h) * p.D, all = (int64_t)p.B * p.Lq * p.Hq * p.D;
+    const bool store = row_ok && !((redo >> l31) & 1);
+    if (p.splits > 1) attn_store_part<DB>(p.part + split * all + row_at, acc, by, half, p.D, store);
+    else attn_store_row<T, DB>((T*)p.dq + row_at, acc, by, half, p.D, store);
     while (redo) {                                                      // a NaN behind the mask may have come in through 0 * NaN: these rows key by key
         const int e = __builtin_ctzll(redo);
         redo &= redo - 1;
@@ -269,9 +274,10 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnParams p) {
         const T* qe = (const T*)p.q + b * p.qs[0] + ie * p.qs[1] + h * p.qs[2];
         const T* doe = (const T*)p.dout + b * p.ds[0] + ie * p.ds[1] + h * p.ds[2];
         float x[2] = {0.f, 0.f};
-        for (int j0 = 0; j0 <= lime; j0 += 64) {
+        const int last = min(lime, run_end * ATTN_TILE - 1);
+        for (int j0 = run_first * ATTN_TILE; j0 <= last; j0 += 64) {
             const int j = j0 + lane;
-            const bool see = j <= lime && attn_visible(p, b, j, lime, doce);
+            const bool see = j <= last && attn_visible(p, b, j, lime, doce);
             float w, ds = 0.f;
             if (see) attn_pair<T>(p, f, qe, k + j * p.ks[1], v + j * p.vs[1], doe, le, de, ie + n - p.Lq - j, w, ds);
             uint64_t todo = __ballot(see);
@@ -284,9 +290,14 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnParams p) {
                 if (lane + 64 < p.D) x[1] += d * (float)kj[lane + 64];
             }
         }
-        T* o = (T*)p.dq + ((int64_t)(b * (int64_t)p.Lq + ie) * p.Hq + h) * p.D;
-        if (lane < p.D) o[lane] = (T)(x[0] * p.scale);
-        if (lane + 64 < p.D) o[lane + 64] = (T)(x[1] * p.scale);
+        const int64_t at = ((int64_t)(b * (int64_t)p.Lq + ie) * p.Hq + h) * p.D;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int d = lane + 64 * c;
+            if (d >= p.D) continue;
+            if (p.splits > 1) p.part[split * all + at + d] = x[c] * p.scale;
+            else ((T*)p.dq)[at + d] = (T)(x[c] * p.scale);
+        }
     }
 #endif
 }
@@ -309,12 +320,13 @@ __global__ __launch_bounds__(attn_dkv_pair<DB>() ? 512 : 256, 2) void attn_dkv_k
     __shared__ __align__(16) int sdoc[2][ATTN_TILE];
     __shared__ __align__(16) char traded[PAIR ? 4 * 2 * 4 * 1024 : 16];   // [key group][half of the queries][w, w, d, d][lane] fragments
     const int wave = attn_uniform(threadIdx.x >> 6), keys = PAIR ? wave & 3 : wave, part = PAIR ? wave >> 2 : 0, lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
-    // p.splits: 1 (a workgroup adds up all heads of the group) or G (one head a workgroup, float32 parts that attn_parts_kernel adds in order)
+    // p.splits: 1 (a workgroup adds up all heads of the group), or float32 parts that attn_parts_kernel adds in order: one head of the group a workgroup
+    // (G > 1), its queries in p.chunks runs of whole tiles
     const int total = p.B * p.Hk * p.splits * p.row_blocks, per = (total + 7) / 8;
     const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
     if ((int)(blockIdx.x >> 3) >= per || id >= total) return;
     const int blk = id % p.row_blocks, split = id / p.row_blocks % p.splits, bh = id / p.row_blocks / p.splits, hk = bh % p.Hk, b = bh / p.Hk;
-    const int g0 = p.splits > 1 ? split : 0, g1 = p.splits > 1 ? split + 1 : p.G;
+    const int g0 = p.splits >= p.G * p.chunks ? split / p.chunks : 0, g1 = p.splits >= p.G * p.chunks ? g0 + 1 : p.G;
     const int n = attn_keys(p, b), prefix = p.prefix ? p.prefix[b] : 0, k0 = blk * 128, off = n - p.Lq;
     const int j = k0 + 32 * keys + l31;
     const int kdoc = DOCS && j < p.Lk ? p.kdoc[b * p.kdoc_stride + j] : 0;
@@ -332,7 +344,8 @@ __global__ __launch_bounds__(attn_dkv_pair<DB>() ? 512 : 256, 2) void attn_dkv_k
         dhi = max(r0.y, r1.y);
     }
     const int2* ranges = DOCS ? p.qtiles + (int64_t)b * p.nqt : nullptr;
-    const int t_first = first_query(k0) / ATTN_TILE, t_end = k0 < n ? p.nqt : 0;
+    const int run = (p.nqt + p.chunks - 1) / p.chunks, run_first = split % p.chunks * run, run_end = min(p.nqt, run_first + run);
+    const int t_first = max(first_query(k0) / ATTN_TILE, run_first), t_end = k0 < n ? run_end : 0;
     AttnTiles<DOCS> tiles;
     int g = g0;
     tiles.start(ranges, t_first, t_end, max(dlo, 0), dhi);
@@ -527,16 +540,8 @@ __global__ __launch_bounds__(attn_dkv_pair<DB>() ? 512 : 256, 2) void attn_dkv_k
     if (p.splits > 1) {
         float* pk = p.part + (2 * split * all + row) * p.D;
         float* pv = p.part + ((2 * split + 1) * all + row) * p.D;
-#pragma unroll
-        for (int db = 0; db < NB; ++db)
-#pragma unroll
-            for (int a = 0; a < 4; ++a) {
-                const int d = 64 * part + 32 * db + 8 * a + 4 * half;
-                if (store && d < p.D) {
-                    *reinterpret_cast<float4*>(pk + d) = make_float4(dk[db][4 * a] * k_by, dk[db][4 * a + 1] * k_by, dk[db][4 * a + 2] * k_by, dk[db][4 * a + 3] * k_by);
-                    *reinterpret_cast<float4*>(pv + d) = make_float4(dv[db][4 * a] * v_by, dv[db][4 * a + 1] * v_by, dv[db][4 * a + 2] * v_by, dv[db][4 * a + 3] * v_by);
-                }
-            }
+        attn_store_part<NB>(pk + 64 * part, dk, k_by, half, p.D - 64 * part, store);
+        attn_store_part<NB>(pv + 64 * part, dv, v_by, half, p.D - 64 * part, store);
     } else {
         attn_store_row<T, NB>((T*)p.dk + row * p.D + 64 * part, dk, k_by, half, p.D - 64 * part, store);
         attn_store_row<T, NB>((T*)p.dv + row * p.D + 64 * part, dv, v_by, half, p.D - 64 * part, store);
@@ -554,9 +559,10 @@ __global__ __launch_bounds__(attn_dkv_pair<DB>() ? 512 : 256, 2) void attn_dkv_k
             const T* q = (const T*)p.q + b * p.qs[0] + h * p.qs[2];
             const T* dout = (const T*)p.dout + b * p.ds[0] + h * p.ds[2];
             const int64_t stat = ((int64_t)b * p.Hq + h) * p.Lq;
-            for (int i0 = first_query(je); i0 < p.Lq; i0 += 64) {
+            const int end = min(p.Lq, run_end * ATTN_TILE);
+            for (int i0 = max(first_query(je), run_first * ATTN_TILE); i0 < end; i0 += 64) {
                 const int i = i0 + lane;
-                const bool see = i < p.Lq && (!p.kdoc || p.qdoc[b * p.qdoc_stride + i] == doce);
+                const bool see = i < end && (!p.kdoc || p.qdoc[b * p.qdoc_stride + i] == doce);
                 float w = 0.f, ds = 0.f;
                 if (see) attn_pair<T>(p, f, q + i * p.qs[1], ke, ve, dout + i * p.ds[1], attn_lse2(p.lse[stat + i]), p.delta[stat + i], i + off - je, w, ds);
                 uint64_t todo = __ballot(see);
@@ -592,15 +598,14 @@ __global__ __launch_bounds__(attn_dkv_pair<DB>() ? 512 : 256, 2) void attn_dkv_k
 #endif
 }
 
-// part [split][dk, dv][elements] -> dk, dv; eight elements a thread
+// part [split][output][elements] -> the outputs (one or two: gridDim.y), the splits in order; eight elements a thread
 template <typename T>
-__global__ __launch_bounds__(256) void attn_parts_kernel(AttnParams p) {
-    const int64_t all = (int64_t)p.B * p.Lk * p.Hk * p.D;
+__global__ __launch_bounds__(256) void attn_parts_kernel(const float* __restrict__ part, int splits, int64_t all, T* __restrict__ out0, T* __restrict__ out1) {
     const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
     if (at >= all) return;
     float x[8] = {};
-    for (int s = 0; s < p.splits; ++s) {
-        const float4* a = reinterpret_cast<const float4*>(p.part + (2 * s + blockIdx.y) * all + at);
+    for (int s = 0; s < splits; ++s) {
+        const float4* a = reinterpret_cast<const float4*>(part + (s * (int64_t)gridDim.y + blockIdx.y) * all + at);
         const float4 u = a[0], w = a[1];
         x[0] += u.x; x[1] += u.y; x[2] += u.z; x[3] += u.w;
         x[4] += w.x; x[5] += w.y; x[6] += w.z; x[7] += w.w;
@@ -608,43 +613,71 @@ __global__ __launch_bounds__(256) void attn_parts_kernel(AttnParams p) {
     typename AttnVec<T>::x8 o;
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[e] = (T)x[e];
-    *reinterpret_cast<typename AttnVec<T>::x8*>((T*)(blockIdx.y ? p.dv : p.dk) + at) = o;
+    *reinterpret_cast<typename AttnVec<T>::x8*>((blockIdx.y ? out1 : out0) + at) = o;
+}
+
+// How the gradients' work is split: parts cost a round trip through memory, so only as far as the chip has room, in runs of eight tiles at least and
+// from 24 tiles on (training step of 4096 x 2 heads x 64: 234 -> 121 us, 2 x 1500 x 4 x 64: 95 -> 83; 1100 x 1 x 64: 77 -> 82 from the launches, hence 24).
+struct AttnSplits {
+    int dq, dkv, chunks;
+};
+static AttnSplits attn_splits(const AttnParams& p) {
+    auto room = [](int64_t groups, int tiles) {
+        const int64_t s = 512 / groups;
+        return groups >= 256 || s < 2 || tiles < 24 ? 1 : (int)(s < tiles / 8 ? s : tiles / 8);
+    };
+    AttnSplits s;
+    s.dq = room((int64_t)p.B * p.Hq * cdiv(p.Lq, 128), p.nkt);
+    // dk / dv: one head of a group a workgroup where whole groups would leave workgroups for less than two rounds of the chip
+    int64_t groups = (int64_t)p.B * p.Hk * (p.Lk ? cdiv(p.Lk, 128) : 1);
+    const int heads = p.G > 1 && groups < 1024 ? p.G : 1;
+    s.chunks = room(groups * heads, p.nqt);
+    if (s.chunks > 1 && heads < p.G) s.chunks = 1;
+    s.dkv = heads * s.chunks;
+    return s;
 }
 
 template <typename T, int DB, int MODE, bool DOCS>
-static void attn_bwd_launch(AttnParams& p, int splits, hipStream_t stream) {
-    const int prep = p.maxima ? ATTN_MAXIMA : (int)(cdiv64((int64_t)p.B * p.Lq * p.Hq, 16) < 2048 ? cdiv64((int64_t)p.B * p.Lq * p.Hq, 16) : 2048);
+static void attn_bwd_launch(AttnParams& p, const AttnSplits& splits, hipStream_t stream) {
+    const int64_t q_rows = (int64_t)p.B * p.Lq * p.Hq, k_rows = (int64_t)p.B * p.Lk * p.Hk;
+    const int prep = p.maxima ? ATTN_MAXIMA : (int)(cdiv64(q_rows, 16) < 2048 ? cdiv64(q_rows, 16) : 2048);
     hipLaunchKernelGGL((attn_prep_kernel<T>), dim3(prep, p.maxima ? 2 : 1), dim3(256), 0, stream, p);
+    auto add = [&](int count, int64_t all, void* a, void* b) {
+        if (count > 1) hipLaunchKernelGGL((attn_parts_kernel<T>), dim3((unsigned)cdiv64(all, 2048), b ? 2 : 1), dim3(256), 0, stream, p.part, count, all, (T*)a, (T*)b);
+    };
     if (p.dq) {
-        p.splits = 1;
+        p.splits = splits.dq;
         p.row_blocks = cdiv(p.Lq, 128);
-        hipLaunchKernelGGL((attn_dq_kernel<T, DB, MODE, DOCS>), dim3(8 * cdiv(p.B * p.Hq * p.row_blocks, 8)), dim3(256), 0, stream, p);
+        hipLaunchKernelGGL((attn_dq_kernel<T, DB, MODE, DOCS>), dim3(8 * cdiv(p.B * p.Hq * p.splits * p.row_blocks, 8)), dim3(256), 0, stream, p);
+        add(splits.dq, q_rows * p.D, p.dq, nullptr);
     }
     if (p.dk && p.Lk > 0) {
-        p.splits = splits;
+        p.splits = splits.dkv;
+        p.chunks = splits.chunks;
         p.row_blocks = cdiv(p.Lk, 128);
         hipLaunchKernelGGL((attn_dkv_kernel<T, DB, MODE, DOCS>), dim3(8 * cdiv(p.B * p.Hk * p.splits * p.row_blocks, 8)),
                            dim3(attn_dkv_pair<DB>() ? 512 : 256), 0, stream, p);
-        if (splits > 1)
-            hipLaunchKernelGGL((attn_parts_kernel<T>), dim3((unsigned)cdiv64((int64_t)p.B * p.Lk * p.Hk * p.D, 2048), 2), dim3(256), 0, stream, p);
+        add(splits.dkv, k_rows * p.D, p.dk, p.dv);
     }
 }
 
-// floats behind the document ranges: delta, maxima (float16), parts of the heads
-static int64_t attn_bwd_floats(const AttnParams& p, int dtype, int& splits, int64_t& maxima_at, int64_t& parts_at) {
+// floats behind the document ranges: delta, maxima (float16), the larger of the two kernels' parts (one is added up before the other begins)
+static int64_t attn_bwd_floats(const AttnParams& p, int dtype, AttnSplits& splits, int64_t& maxima_at, int64_t& parts_at) {
     const int64_t ranges = (attn_range_floats(p) + 3) / 4 * 4, delta = ((int64_t)p.B * p.Hq * p.Lq + 3) / 4 * 4;
     maxima_at = ranges + delta;
     parts_at = maxima_at + (dtype == N3D_F16 ? 2 * ATTN_MAXIMA : 0);
-    // one head of a group a workgroup where whole groups would leave workgroups for less than two rounds of the chip
-    splits = p.G > 1 && (int64_t)p.B * p.Hk * cdiv(p.Lk, 128) < 1024 ? p.G : 1;
-    return parts_at + (splits > 1 ? 2 * (int64_t)splits * p.B * p.Lk * p.Hk * p.D : 0);
+    splits = attn_splits(p);
+    const int64_t dq = splits.dq > 1 ? (int64_t)splits.dq * p.B * p.Lq * p.Hq * p.D : 0;
+    const int64_t dkv = splits.dkv > 1 ? 2 * (int64_t)splits.dkv * p.B * p.Lk * p.Hk * p.D : 0;
+    return parts_at + (dq > dkv ? dq : dkv);
 }
 
 extern "C" int64_t n3d_attention_bwd_workspace(const n3d_attention_desc* d) {
     AttnParams p;
     const char* bad = attn_params(d, p);
     N3D_CHECK(!bad, "attention_bwd: %s", bad);
-    int splits;
+    if (p.B == 0 || p.Lq == 0) return 0;
+    AttnSplits splits;
     int64_t m, s;
     return 4 * attn_bwd_floats(p, d->dtype, splits, m, s);
 }
@@ -659,7 +692,7 @@ extern "C" int n3d_attention_bwd(const n3d_attention_desc* d, n3d_stream_t strea
     for (int i = 0; i < 3; ++i)
         N3D_CHECK(d->dout_strides[i] % 8 == 0 && d->dout_strides[i] >= 0 && (i != 1 || d->dout_strides[i] <= (1 << 23)), "attention_bwd: strides must be multiples of 8 elements, of tokens 2^23 at most");
     N3D_CHECK(((uintptr_t)d->dout | (uintptr_t)d->dq | (uintptr_t)d->dk | (uintptr_t)d->dv) % 16 == 0, "attention_bwd: tensors must be 16-byte aligned");
-    int splits;
+    AttnSplits splits;
     int64_t maxima_at, parts_at;
     const int64_t need = 4 * attn_bwd_floats(p, d->dtype, splits, maxima_at, parts_at);
     N3D_CHECK(d->workspace && d->workspace_bytes >= need && (uintptr_t)d->workspace % 16 == 0, "attention_bwd: a workspace of %lld bytes is needed (16-byte aligned)", (long long)need);

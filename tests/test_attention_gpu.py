@@ -143,6 +143,25 @@ def _run(dev, q, k, v, do, **kw):
     return dict(zip(('out', 'dq', 'dk', 'dv'), (out.detach(), *torch.autograd.grad(out, leaves, do.to(dev)))))
 
 
+@pytest.mark.parametrize('dtype', [F16, BF16])
+@pytest.mark.parametrize('size', [(1, 1100, 1200, 1, 1, 64), (1, 2100, 1030, 2, 1, 128), (2, 1031, 2500, 2, 2, 72), (1, 130, 4100, 2, 1, 32), (1, 4100, 70, 3, 1, 96)], ids=str)
+def test_attention_few_heads_of_long_sequences(dev, size, dtype):
+    """Few workgroups' worth of rows: the long axis is split as well, also where runs of it are empty, masked or hold NaN behind the mask."""
+    b, lq, lk, hq, hk, d = size
+    q, k, v, do = _inputs(*size, dtype, 17)
+    prefix, lengths = torch.full((b,), lk // 3, dtype=torch.int32), torch.full((b,), lk - 37, dtype=torch.int32)
+    _check(dev, q, k, v, do, what='plain')
+    _check(dev, q, k, v, do, what='causal', causal=True, prefix=prefix, softcap=8.0)
+    spoiled = k.clone()
+    spoiled[:, lk - 37:] = float('nan')
+    _check(dev, q, spoiled, v, do, what='lengths', causal=True, lengths=lengths, slopes=2.0 ** -torch.arange(1.0, hq + 1))
+    qd, kd = _docs(b, lq, 4, 5, pad=9), _docs(b, lk, 4, 6, pad=11)
+    for t, ids in ((k, kd), (v, kd), (q, qd), (do, qd)):
+        t[ids < 0] = float('nan')
+    _check(dev, q, k, v, do, what='documents', documents=qd, key_documents=kd)
+    _check(dev, q, k, v, do, what='causal documents', documents=qd, key_documents=kd, causal=True)
+
+
 def test_attention_documents_out_of_order(dev):
     """Documents need not be sorted, and queries and keys may carry different ones."""
     g = torch.Generator().manual_seed(1)
