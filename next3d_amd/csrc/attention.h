@@ -295,6 +295,13 @@ __device__ __forceinline__ void attn_store_pair(const AttnParams& p, int64_t at,
 }
 
 // ---- host: a checked descriptor as kernel parameters
+// Workgroups that share a row block's walk of `tiles` tiles, where there are `groups` row blocks of all heads: parts cost a round trip through memory and a
+// launch, so only as far as the chip has room (two workgroups a CU), in runs of eight tiles at least and from 24 tiles on.
+// (Training step of 4096 x 2 heads x 64: 234 -> 121 us, 2 x 1500 x 4 x 64: 95 -> 83; 1100 x 1 x 64, 18 tiles: 77 -> 82 from the launches, hence 24.)
+static inline int attn_room(int64_t groups, int tiles) {
+    const int64_t s = 512 / groups;
+    return groups >= 256 || tiles < 24 ? 1 : (int)(s < tiles / 8 ? s : tiles / 8);
+}
 static inline const char* attn_params(const n3d_attention_desc* d, AttnParams& p) {
     if (!d) return "null descriptor";
     if (d->B < 0 || d->Lq < 0 || d->Lk < 0) return "negative sizes";

@@ -616,22 +616,17 @@ __global__ __launch_bounds__(256) void attn_parts_kernel(const float* __restrict
     *reinterpret_cast<typename AttnVec<T>::x8*>((blockIdx.y ? out1 : out0) + at) = o;
 }
 
-// How the gradients' work is split: parts cost a round trip through memory, so only as far as the chip has room, in runs of eight tiles at least and
-// from 24 tiles on (training step of 4096 x 2 heads x 64: 234 -> 121 us, 2 x 1500 x 4 x 64: 95 -> 83; 1100 x 1 x 64: 77 -> 82 from the launches, hence 24).
+// How the gradients' work is split (attn_room)
 struct AttnSplits {
     int dq, dkv, chunks;
 };
 static AttnSplits attn_splits(const AttnParams& p) {
-    auto room = [](int64_t groups, int tiles) {
-        const int64_t s = 512 / groups;
-        return groups >= 256 || s < 2 || tiles < 24 ? 1 : (int)(s < tiles / 8 ? s : tiles / 8);
-    };
     AttnSplits s;
-    s.dq = room((int64_t)p.B * p.Hq * cdiv(p.Lq, 128), p.nkt);
+    s.dq = attn_room((int64_t)p.B * p.Hq * cdiv(p.Lq, 128), p.nkt);
     // dk / dv: one head of a group a workgroup where whole groups would leave workgroups for less than two rounds of the chip
     int64_t groups = (int64_t)p.B * p.Hk * (p.Lk ? cdiv(p.Lk, 128) : 1);
     const int heads = p.G > 1 && groups < 1024 ? p.G : 1;
-    s.chunks = room(groups * heads, p.nqt);
+    s.chunks = attn_room(groups * heads, p.nqt);
     if (s.chunks > 1 && heads < p.G) s.chunks = 1;
     s.dkv = heads * s.chunks;
     return s;

@@ -132,10 +132,11 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnParams p) {
     __shared__ __align__(16) int sdoc[2][ATTN_TILE];
     const int wave = attn_uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
     // consecutive workgroups go to different XCDs: give each XCD whole heads, so that its L2 serves their keys, and the longest rows first
-    const int total = p.B * p.Hq * p.row_blocks, per = (total + 7) / 8;
+    // (p.splits > 1: the keys in that many runs of whole tiles, joined by attn_combine_kernel)
+    const int total = p.B * p.Hq * p.row_blocks * p.splits, per = (total + 7) / 8;
     const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
     if ((int)(blockIdx.x >> 3) >= per || id >= total) return;
-    const int blk = p.row_blocks - 1 - id % p.row_blocks, bh = id / p.row_blocks, h = bh % p.Hq, b = bh / p.Hq, hk = h / p.G;
+    const int split = id % p.splits, blk = p.row_blocks - 1 - id / p.splits % p.row_blocks, bh = id / p.splits / p.row_blocks, h = bh % p.Hq, b = bh / p.Hq, hk = h / p.G;
     const int n = attn_keys(p, b), prefix = p.prefix ? p.prefix[b] : 0, q0 = blk * 128;
     const int i = q0 + 32 * wave + l31;
     const bool row_ok = i < p.Lq;
@@ -151,7 +152,8 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnParams p) {
         dhi = max(r0.y, r1.y);
     }
     AttnTiles<DOCS> tiles;
-    tiles.start(DOCS ? p.ktiles + (int64_t)b * p.nkt : nullptr, 0, (key_end + ATTN_TILE - 1) / ATTN_TILE, max(dlo, 0), dhi);
+    const int run = (p.nkt + p.splits - 1) / p.splits, run_first = split * run, run_end = min((key_end + ATTN_TILE - 1) / ATTN_TILE, run_first + run);
+    tiles.start(DOCS ? p.ktiles + (int64_t)b * p.nkt : nullptr, run_first, run_end, max(dlo, 0), dhi);
 
     typename AttnVec<T>::x8 qf[2 * DB];
     const T* q = row_ok ? (const T*)p.q + b * p.qs[0] + i * p.qs[1] + h * p.qs[2] : nullptr;
@@ -244,19 +246,35 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnParams p) {
         for (int r = 0; r < 16; ++r) nan = nan || acc[db][r] != acc[db][r];
     uint64_t redo = __ballot(nan && sum == sum && row_ok);
     redo = (redo | (redo >> 32)) & 0xffffffffu;
-    const int64_t row_at = ((int64_t)(b * (int64_t)p.Lq + i) * p.Hq + h) * p.D;
     const bool store = row_ok && !((redo >> l31) & 1);
-    attn_store_row<T, DB>((T*)p.out + row_at, acc, by, half, p.D, store);
-    if (p.rest) attn_store_row<T, DB, true>((T*)p.rest + row_at, acc, by, half, p.D, store);
-    if (p.lse && row_ok && half == 0) p.lse[((int64_t)b * p.Hq + h) * p.Lq + i] = sum == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(sum)) * ATTN_LN2;
+    const int64_t row_at = ((int64_t)(b * (int64_t)p.Lq + i) * p.Hq + h) * p.D;
+    auto part_at = [&](int row) { return (((int64_t)(b * p.Hk + hk) * p.Lq + row) * p.G + h - hk * p.G) * p.splits + split; };
+    if (p.splits > 1) {
+        const int64_t at = part_at(i);
+        attn_store_part<DB>(p.part + at * p.D, acc, 1.f, half, p.D, store);
+        if (row_ok && half == 0) {
+            p.part[p.part_ml + 2 * at] = m;
+            p.part[p.part_ml + 2 * at + 1] = sum;
+        }
+    } else {
+        attn_store_row<T, DB>((T*)p.out + row_at, acc, by, half, p.D, store);
+        if (p.rest) attn_store_row<T, DB, true>((T*)p.rest + row_at, acc, by, half, p.D, store);
+        if (p.lse && row_ok && half == 0) p.lse[((int64_t)b * p.Hq + h) * p.Lq + i] = sum == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(sum)) * ATTN_LN2;
+    }
     while (redo) {
         const int e = __builtin_ctzll(redo);
         redo &= redo - 1;
         const int ie = q0 + 32 * wave + e;
         const float me = __shfl(m, e), bye = __shfl(by, e);
         float row[2];
-        attn_exact_row<T>(p, b, ie, h, 0, n, me, lane, row);
-        attn_store_pair<T>(p, ((int64_t)(b * (int64_t)p.Lq + ie) * p.Hq + h) * p.D, row, bye, lane);
+        attn_exact_row<T>(p, b, ie, h, run_first * ATTN_TILE, min(n, (run_first + run) * ATTN_TILE), me, lane, row);
+        if (p.splits > 1) {
+            float* x = p.part + part_at(ie) * p.D;
+            if (lane < p.D) x[lane] = row[0];
+            if (lane + 64 < p.D) x[lane + 64] = row[1];
+        } else {
+            attn_store_pair<T>(p, ((int64_t)(b * (int64_t)p.Lq + ie) * p.Hq + h) * p.D, row, bye, lane);
+        }
     }
 #endif
 }
@@ -423,9 +441,13 @@ void attn_ranges(AttnParams& p, void* workspace, hipStream_t stream) {
 }
 
 // The token kernel where its rows (queries x heads of a group) fill two 32-row blocks at most; its keys go to enough workgroups to fill the chip twice.
-static bool attn_token_plan(AttnParams& p) {
+static bool attn_plan(AttnParams& p) {
     const int64_t rows = (int64_t)p.Lq * p.G;
-    if (rows > 64) return false;
+    if (rows > 64) {
+        p.row_blocks = cdiv(p.Lq, 128);
+        p.splits = attn_room((int64_t)p.B * p.Hq * p.row_blocks, p.nkt);
+        return false;
+    }
     p.row_blocks = (int)cdiv64(rows, 32);
     const int64_t groups = (int64_t)p.B * p.Hk * p.row_blocks;
     int64_t s = 512 / groups, most = cdiv64(p.Lk, 256);                 // (256 keys: two rounds of the four waves)
@@ -436,34 +458,36 @@ static bool attn_token_plan(AttnParams& p) {
 
 template <typename T, int DB, int MODE, bool DOCS>
 static hipError_t attn_fwd_launch(AttnParams& p, bool token, hipStream_t stream) {
-    if (!token) {
-        p.row_blocks = cdiv(p.Lq, 128);
-        hipLaunchKernelGGL((attn_fwd_kernel<T, DB, MODE, DOCS>), dim3(8 * cdiv(p.B * p.Hq * p.row_blocks, 8)), dim3(256), 0, stream, p);
-        return hipSuccess;
+    if (token) {
+        constexpr int lds = 4 * 4 * 32 * (DB > 2 ? 128 : 64) * 2;
+        const hipError_t e = hipFuncSetAttribute((const void*)attn_token_kernel<T, DB, MODE>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+        if (e != hipSuccess) return e;
+        hipLaunchKernelGGL((attn_token_kernel<T, DB, MODE>), dim3(p.B * p.Hk * p.row_blocks * p.splits), dim3(256), lds, stream, p);
+    } else {
+        hipLaunchKernelGGL((attn_fwd_kernel<T, DB, MODE, DOCS>), dim3(8 * cdiv(p.B * p.Hq * p.splits * p.row_blocks, 8)), dim3(256), 0, stream, p);
     }
-    constexpr int lds = 4 * 4 * 32 * (DB > 2 ? 128 : 64) * 2;
-    const hipError_t e = hipFuncSetAttribute((const void*)attn_token_kernel<T, DB, MODE>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((attn_token_kernel<T, DB, MODE>), dim3(p.B * p.Hk * p.row_blocks * p.splits), dim3(256), lds, stream, p);
     if (p.splits > 1) hipLaunchKernelGGL((attn_combine_kernel<T>), dim3((unsigned)cdiv64((int64_t)p.B * p.Hk * p.Lq * p.G, 4)), dim3(256), 0, stream, p);
     return hipSuccess;
 }
 
-static int64_t attn_fwd_floats(AttnParams& p) {
-    int64_t n = attn_range_floats(p);
-    if (attn_token_plan(p) && p.splits > 1) {
-        const int64_t parts = (int64_t)p.B * p.Hk * p.Lq * p.G * p.splits;
-        p.part_ml = parts * p.D;
-        n += parts * (p.D + 2);
-    }
-    return n;
+// floats of the workspace; parts_at: where the splits' parts lie in it (behind the document ranges)
+static int64_t attn_fwd_floats(AttnParams& p, bool& token, int64_t& parts_at) {
+    parts_at = (attn_range_floats(p) + 3) / 4 * 4;
+    token = attn_plan(p);
+    if (p.splits == 1) return attn_range_floats(p);
+    const int64_t parts = (int64_t)p.B * p.Hq * p.Lq * p.splits;
+    p.part_ml = parts * p.D;
+    return parts_at + parts * (p.D + 2);
 }
 
 extern "C" int64_t n3d_attention_workspace(const n3d_attention_desc* d) {
     AttnParams p;
     const char* bad = attn_params(d, p);
     N3D_CHECK(!bad, "attention: %s", bad);
-    return attn_fwd_floats(p) * 4;
+    if (p.B == 0 || p.Lq == 0) return 0;
+    bool token;
+    int64_t parts_at;
+    return 4 * attn_fwd_floats(p, token, parts_at);
 }
 
 extern "C" int n3d_attention(const n3d_attention_desc* d, n3d_stream_t stream_) {
@@ -472,14 +496,15 @@ extern "C" int n3d_attention(const n3d_attention_desc* d, n3d_stream_t stream_) 
     const char* bad = attn_params(d, p);
     N3D_CHECK(!bad, "attention: %s", bad);
     if (p.B == 0 || p.Lq == 0) return 0;
-    const int64_t need = attn_fwd_floats(p) * 4;
+    bool token;
+    int64_t parts_at;
+    const int64_t need = 4 * attn_fwd_floats(p, token, parts_at);
     N3D_CHECK(need == 0 || (d->workspace && d->workspace_bytes >= need && (uintptr_t)d->workspace % 16 == 0), "attention: a workspace of %lld bytes is needed (16-byte aligned)",
               (long long)need);
     const double pairs = (double)p.B * p.Hq * p.Lq * p.Lk * p.D;
     N3dProfScope prof(N3D_K_ATTENTION, stream, 4.0 * pairs, 4.0 * ((double)p.B * p.Lq * p.Hq * p.D + (double)p.B * p.Lk * p.Hk * p.D));
     attn_ranges(p, d->workspace, stream);
-    p.part = (float*)d->workspace + attn_range_floats(p);
-    const bool token = attn_token_plan(p);
+    p.part = (float*)d->workspace + parts_at;
     hipError_t e = hipSuccess;
     attn_dispatch(d->dtype, p, [&](auto* t, auto db, auto mode, auto docs) {
         e = attn_fwd_launch<std::remove_pointer_t<decltype(t)>, db.value, mode.value, docs.value>(p, token, stream);
