@@ -406,27 +406,39 @@ __global__ __launch_bounds__(256) void attn_token_kernel(AttnParams p) {
 #endif
 }
 
-// one wave a row: the splits' accumulators, in order
+// the splits' accumulators, in order: four channels a lane, 32 lanes a row (16 up to 64 channels), no lane waits for another
+__device__ __host__ __forceinline__ int attn_combine_lanes(int D) { return D > 64 ? 32 : 16; }
 template <typename T>
 __global__ __launch_bounds__(256) void attn_combine_kernel(AttnParams p) {
-    const int rows = p.Lq * p.G, lane = threadIdx.x & 63;
-    const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (w >= (int64_t)p.B * p.Hk * rows) return;
+    const int rows = p.Lq * p.G, lanes = attn_combine_lanes(p.D), d = 4 * (threadIdx.x & (lanes - 1));
+    const int64_t w = (int64_t)blockIdx.x * (256 / lanes) + threadIdx.x / lanes;
+    if (w >= (int64_t)p.B * p.Hk * rows || d >= p.D) return;
     const int r = (int)(w % rows), bh = (int)(w / rows), hk = bh % p.Hk, b = bh / p.Hk, i = r / p.G, h = hk * p.G + r - i * p.G;
-    const float* ml = p.part + p.part_ml + 2 * w * p.splits;
+    const float2* ml = reinterpret_cast<const float2*>(p.part + p.part_ml) + w * p.splits;
+    const float* a = p.part + w * p.splits * p.D + d;
     float top = -INFINITY;
-    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, ml[2 * s]);
-    float all = 0.f, x[2] = {0.f, 0.f};
+#pragma unroll 8
+    for (int s = 0; s < p.splits; ++s) top = fmaxf(top, ml[s].x);
+    float all = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
     for (int s = 0; s < p.splits; ++s) {
-        if (ml[2 * s + 1] == 0.f) continue;                             // nothing visible in this share
-        const float by = __builtin_amdgcn_exp2f(ml[2 * s] - top);
-        all += by * ml[2 * s + 1];
-        const float* a = p.part + (w * p.splits + s) * p.D;
-        if (lane < p.D) x[0] += by * a[lane];
-        if (lane + 64 < p.D) x[1] += by * a[lane + 64];
+        const float2 st = ml[s];
+        const float4 v = *reinterpret_cast<const float4*>(a + (int64_t)s * p.D);
+        const float by = st.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(st.x - top);      // (0: nothing visible in this share, whose accumulator is zero)
+        all += by * st.y;
+        x[0] += by * v.x; x[1] += by * v.y; x[2] += by * v.z; x[3] += by * v.w;
     }
-    attn_store_pair<T>(p, ((int64_t)(b * (int64_t)p.Lq + i) * p.Hq + h) * p.D, x, all == 0.f ? 0.f : 1.f / all, lane);
-    if (p.lse && lane == 0) p.lse[((int64_t)b * p.Hq + h) * p.Lq + i] = all == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(all)) * ATTN_LN2;
+    const float scale = all == 0.f ? 0.f : 1.f / all;
+    const int64_t at = ((int64_t)(b * (int64_t)p.Lq + i) * p.Hq + h) * p.D + d;
+    typename AttnVec<T>::x4 o, rest;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        o[e] = (T)(x[e] * scale);
+        rest[e] = (T)(x[e] * scale - (float)(T)(x[e] * scale));
+    }
+    *reinterpret_cast<typename AttnVec<T>::x4*>((T*)p.out + at) = o;
+    if (p.rest) *reinterpret_cast<typename AttnVec<T>::x4*>((T*)p.rest + at) = rest;
+    if (p.lse && d == 0) p.lse[((int64_t)b * p.Hq + h) * p.Lq + i] = all == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(all)) * ATTN_LN2;
 }
 
 void attn_ranges(AttnParams& p, void* workspace, hipStream_t stream) {
@@ -466,7 +478,7 @@ static hipError_t attn_fwd_launch(AttnParams& p, bool token, hipStream_t stream)
     } else {
         hipLaunchKernelGGL((attn_fwd_kernel<T, DB, MODE, DOCS>), dim3(8 * cdiv(p.B * p.Hq * p.splits * p.row_blocks, 8)), dim3(256), 0, stream, p);
     }
-    if (p.splits > 1) hipLaunchKernelGGL((attn_combine_kernel<T>), dim3((unsigned)cdiv64((int64_t)p.B * p.Hk * p.Lq * p.G, 4)), dim3(256), 0, stream, p);
+    if (p.splits > 1) hipLaunchKernelGGL((attn_combine_kernel<T>), dim3((unsigned)cdiv64((int64_t)p.B * p.Lq * p.Hq, 256 / attn_combine_lanes(p.D))), dim3(256), 0, stream, p);
     return hipSuccess;
 }
 
