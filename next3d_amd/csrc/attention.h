@@ -308,7 +308,7 @@ static inline const char* attn_params(const n3d_attention_desc* d, AttnParams& p
     if (d->dtype != N3D_F16 && d->dtype != N3D_BF16) return "float16 or bfloat16 only";
     if (d->heads_k < 1 || d->heads_q < 1 || d->heads_q % d->heads_k) return "the query heads must be a multiple of the key heads";
     if (d->D < 8 || d->D > 128 || d->D % 8) return "head sizes are multiples of 8 from 8 to 128";
-    if ((int64_t)d->B * d->heads_q * ((d->Lq > d->Lk ? d->Lq : d->Lk) / 32 + 1) >= (1 << 28)) return "too many rows for one launch";
+    if ((int64_t)d->B * d->heads_q * ((d->Lq > d->Lk ? d->Lq : d->Lk) / 32 + 1) >= (1 << 26)) return "too many rows for one launch";
     if (!(d->softcap >= 0.f && d->softcap < INFINITY) || !(d->scale > -INFINITY && d->scale < INFINITY)) return "scale and softcap must be finite, softcap not negative";
     if (d->prefix && !d->causal) return "a prefix needs causal";
     if ((!d->q_documents) != (!d->k_documents)) return "documents of the queries and of the keys, or neither";

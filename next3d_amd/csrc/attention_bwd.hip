@@ -5,7 +5,7 @@
 // queries of all its heads.  Scores are computed in both (7 products for 5) so that every sum has one owner: no atomics, the same bits every time.
 #include "attention.h"
 
-static constexpr int ATTN_MAXIMA = 256;              // workgroups (= partial maxima) of |do|, and as many of |v|
+static constexpr int ATTN_MAXIMA = 1024;             // workgroups (= partial maxima) of |do|, and as many of |v|
 // float16 has 5 exponent bits, and P ~ 1 / length and ds ~ P do v leave its range on long rows or with small gradients.  The dk / dv kernel therefore uses
 // P 2^12, and both kernels ds times a power of two taken from the largest |do| and |v| of the call, so that no ds can overflow:
 // |ds| <= |dP - delta| <= 2 D max|do| max|v|.  The accumulators undo both.  bfloat16 has float32's exponents: neither is needed.
@@ -18,19 +18,18 @@ __global__ __launch_bounds__(256) void attn_prep_kernel(AttnParams p) {
     const int lane16 = threadIdx.x & 15, D = p.D;
     float top = 0.f;
     if (blockIdx.y == 0) {
-        const int64_t rows = (int64_t)p.B * p.Lq * p.Hq;
-        for (int64_t w = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); w < rows; w += (int64_t)gridDim.x * 16) {
-            const int h = (int)(w % p.Hq);
-            const int64_t bi = w / p.Hq;
-            const int b = (int)(bi / p.Lq), i = (int)(bi - (int64_t)b * p.Lq);
+        const uint32_t rows = (uint32_t)p.B * p.Lq * p.Hq;                // (below 2^31: attn_params)
+        for (uint32_t w = blockIdx.x * 16 + (threadIdx.x >> 4); w < rows; w += gridDim.x * 16) {
+            const uint32_t bi = w / p.Hq;
+            const int h = w - bi * p.Hq, b = bi / p.Lq, i = bi - b * p.Lq;
             const int64_t stat = ((int64_t)b * p.Hq + h) * p.Lq + i;
             float s = 0.f;
             const bool live = p.lse[stat] != -INFINITY;
             if (lane16 * 8 < D) {
                 const auto x = *reinterpret_cast<const typename AttnVec<T>::x8*>((const T*)p.dout + b * p.ds[0] + i * p.ds[1] + h * p.ds[2] + lane16 * 8);
-                const auto y = *reinterpret_cast<const typename AttnVec<T>::x8*>((const T*)p.o + w * D + lane16 * 8);
+                const auto y = *reinterpret_cast<const typename AttnVec<T>::x8*>((const T*)p.o + (int64_t)w * D + lane16 * 8);
                 typename AttnVec<T>::x8 z = {};
-                if (p.rest) z = *reinterpret_cast<const typename AttnVec<T>::x8*>((const T*)p.rest + w * D + lane16 * 8);
+                if (p.rest) z = *reinterpret_cast<const typename AttnVec<T>::x8*>((const T*)p.rest + (int64_t)w * D + lane16 * 8);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     s += (float)x[e] * ((float)y[e] + (float)z[e]);
@@ -43,11 +42,10 @@ __global__ __launch_bounds__(256) void attn_prep_kernel(AttnParams p) {
             if (lane16 == 0) p.delta[stat] = s;
         }
     } else {
-        const int64_t rows = (int64_t)p.B * p.Lk * p.Hk;
-        for (int64_t w = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); w < rows; w += (int64_t)gridDim.x * 16) {
-            const int h = (int)(w % p.Hk);
-            const int64_t bj = w / p.Hk;
-            const int b = (int)(bj / p.Lk), j = (int)(bj - (int64_t)b * p.Lk);
+        const uint32_t rows = (uint32_t)p.B * p.Lk * p.Hk;
+        for (uint32_t w = blockIdx.x * 16 + (threadIdx.x >> 4); w < rows; w += gridDim.x * 16) {
+            const uint32_t bj = w / p.Hk;
+            const int h = w - bj * p.Hk, b = bj / p.Lk, j = bj - b * p.Lk;
             if (j >= attn_keys(p, b) || (p.kdoc && p.kdoc[b * p.kdoc_stride + j] < 0) || lane16 * 8 >= D) continue;
             const auto x = *reinterpret_cast<const typename AttnVec<T>::x8*>((const T*)p.v + b * p.vs[0] + j * p.vs[1] + h * p.vs[2] + lane16 * 8);
 #pragma unroll
