@@ -318,13 +318,13 @@ __global__ __launch_bounds__(attn_dkv_pair<DB>() ? 512 : 256, 2) void attn_dkv_k
     __shared__ __align__(16) int sdoc[2][ATTN_TILE];
     __shared__ __align__(16) char traded[PAIR ? 4 * 2 * 4 * 1024 : 16];   // [key group][half of the queries][w, w, d, d][lane] fragments
     const int wave = attn_uniform(threadIdx.x >> 6), keys = PAIR ? wave & 3 : wave, part = PAIR ? wave >> 2 : 0, lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
-    // p.splits: 1 (a workgroup adds up all heads of the group), or float32 parts that attn_parts_kernel adds in order: one head of the group a workgroup
-    // (G > 1), its queries in p.chunks runs of whole tiles
+    // p.splits: 1 (a workgroup adds up all heads of the group), or float32 parts that attn_parts_kernel adds in order: the heads of the group in
+    // p.splits / p.chunks equal runs, the queries in p.chunks runs of whole tiles
     const int total = p.B * p.Hk * p.splits * p.row_blocks, per = (total + 7) / 8;
     const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
     if ((int)(blockIdx.x >> 3) >= per || id >= total) return;
     const int blk = id % p.row_blocks, split = id / p.row_blocks % p.splits, bh = id / p.row_blocks / p.splits, hk = bh % p.Hk, b = bh / p.Hk;
-    const int g0 = p.splits >= p.G * p.chunks ? split / p.chunks : 0, g1 = p.splits >= p.G * p.chunks ? g0 + 1 : p.G;
+    const int heads = p.G * p.chunks / p.splits, g0 = split / p.chunks * heads, g1 = g0 + heads;
     const int n = attn_keys(p, b), prefix = p.prefix ? p.prefix[b] : 0, k0 = blk * 128, off = n - p.Lq;
     const int j = k0 + 32 * keys + l31;
     const int kdoc = DOCS && j < p.Lk ? p.kdoc[b * p.kdoc_stride + j] : 0;
@@ -621,11 +621,13 @@ struct AttnSplits {
 static AttnSplits attn_splits(const AttnParams& p) {
     AttnSplits s;
     s.dq = attn_room((int64_t)p.B * p.Hq * cdiv(p.Lq, 128), p.nkt);
-    // dk / dv: one head of a group a workgroup where whole groups would leave workgroups for less than two rounds of the chip
-    int64_t groups = (int64_t)p.B * p.Hk * (p.Lk ? cdiv(p.Lk, 128) : 1);
-    const int heads = p.G > 1 && groups < 1024 ? p.G : 1;
-    s.chunks = attn_room(groups * heads, p.nqt);
-    if (s.chunks > 1 && heads < p.G) s.chunks = 1;
+    // dk / dv: a group's heads in as many runs as fill the chip (256 workgroups beyond 96 channels, 512 up to there), or fill it twice where the diagonal
+    // or documents leave long and short ones.  Training step of 2 x 4096 x 16 heads on 4: causal x 128, 1024 -> 512 workgroups: 755 -> 727 us (half the parts);
+    // causal x 64: 467, at 512 518; no mask x 128, 512 -> 256: 1337 -> 1317; documents x 128: 492, at 256 526; documents x 64: 310, at 512 342.
+    const int64_t groups = (int64_t)p.B * p.Hk * (p.Lk ? cdiv(p.Lk, 128) : 1), fill = (p.D > 96 ? 256 : 512) * (p.causal || p.kdoc ? 2 : 1);
+    int heads = 1;
+    while (heads < p.G && (p.G % heads || groups * heads < fill)) ++heads;
+    s.chunks = heads < p.G ? 1 : attn_room(groups * heads, p.nqt);
     s.dkv = heads * s.chunks;
     return s;
 }
