@@ -33,6 +33,7 @@ struct AttnParams {
     const float* maxima;                             // partial maxima (float16 gradients), see attn_ds_scale
     int n_maxima;
     int B, Lq, Lk, Hq, Hk, G, D, nkt, nqt, causal, row_blocks;
+    const int* order;                                // [B, row blocks of queries], the longest first, or null: the last first
     int splits, chunks;                              // workgroups a row block's work is split over; of them over the long axis (dk / dv: per head)
     float scale, softcap;
 };
@@ -366,5 +367,5 @@ static inline void attn_dispatch(int dtype, const AttnParams& p, F&& f) {
 }
 
 // workspace, in floats: the document ranges come first
-static inline int64_t attn_range_floats(const AttnParams& p) { return p.kdoc ? 2 * (int64_t)p.B * (p.nkt + p.nqt) : 0; }
+static inline int64_t attn_range_floats(const AttnParams& p) { return p.kdoc ? 2 * (int64_t)p.B * (p.nkt + p.nqt) + (int64_t)p.B * cdiv(p.Lq, 128) : 0; }
 void attn_ranges(AttnParams& p, void* workspace, hipStream_t stream);      // attention_fwd.hip

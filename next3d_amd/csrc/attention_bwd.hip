@@ -132,7 +132,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnParams p) {
     const int total = p.B * p.Hq * p.row_blocks * p.splits, per = (total + 7) / 8;
     const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
     if ((int)(blockIdx.x >> 3) >= per || id >= total) return;
-    const int split = id % p.splits, blk = p.row_blocks - 1 - id / p.splits % p.row_blocks, bh = id / p.splits / p.row_blocks, h = bh % p.Hq, b = bh / p.Hq, hk = h / p.G;
+    const int split = id % p.splits, pos = id / p.splits % p.row_blocks, bh = id / p.splits / p.row_blocks, h = bh % p.Hq, b = bh / p.Hq, hk = h / p.G;
+    const int blk = DOCS && p.order ? p.order[b * p.row_blocks + pos] : p.row_blocks - 1 - pos;
     const int n = attn_keys(p, b), prefix = p.prefix ? p.prefix[b] : 0, q0 = blk * 128;
     const int i = q0 + 32 * wave + l31;
     const bool row_ok = i < p.Lq;

@@ -173,6 +173,18 @@ def test_attention_documents_out_of_order(dev):
         _check(dev, q, k, v, do, documents=torch.full_like(qd, -1), key_documents=kd)
 
 
+@pytest.mark.parametrize('causal', [False, True])
+def test_attention_many_blocks_of_uneven_documents(dev, causal):
+    """More workgroups than the chip holds at once: the blocks are taken in another order, each one once — documents in order, shuffled, one, and padding."""
+    b, n, heads, d = 3, 1300, 32, 8
+    q, k, v, do = _inputs(b, n, n, heads, heads, d, BF16, 25)
+    docs = _docs(b, n, 9, 7, pad=300)
+    docs[1] = docs[1, torch.randperm(n, generator=torch.Generator().manual_seed(3))]
+    docs[2] = 0
+    _check(dev, q, k, v, do, documents=docs, causal=causal)
+    _check(dev, q, k, v, do, documents=docs, causal=causal, lengths=torch.tensor([1300, 1000, 0], dtype=torch.int32))
+
+
 def test_attention_small_and_large_gradients_float16(dev):
     """float16 gradients of any size keep their relative accuracy (the dscores get a power of two of their own)."""
     for size in (1e-6, 1e-3, 300.0):
