@@ -31,7 +31,6 @@ struct AttnParams {
     float* part;                                     // partial results of split kernels
     int64_t part_ml;                                 // offset of their statistics in `part`
     const float* maxima;                             // partial maxima (float16 gradients), see attn_ds_scale
-    int n_maxima;
     int B, Lq, Lk, Hq, Hk, G, D, nkt, nqt, causal, row_blocks;
     const int* order;                                // [B, row blocks of queries], the longest first, or null: the last first
     int splits, chunks;                              // workgroups a row block's work is split over; of them over the long axis (dk / dv: per head)
@@ -85,7 +84,7 @@ struct AttnScore {
     float mul, cap_in, cap_out, slope;               // mul: scale log2 e;  cap_in: 2 scale log2 e / cap;  cap_out: cap log2 e;  slope: slope log2 e
     __device__ AttnScore(const AttnParams& p, int head) {
         mul = p.scale * ATTN_LOG2E;
-        cap_in = p.softcap > 0.f ? 2.f * ATTN_LOG2E * p.scale / p.softcap : 0.f;
+        cap_in = p.softcap > 0.f ? fminf(fmaxf(2.f * ATTN_LOG2E * p.scale / p.softcap, -3e38f), 3e38f) : 0.f;      // (finite: a zero stays a zero)
         cap_out = p.softcap > 0.f ? p.softcap * ATTN_LOG2E : 0.f;
         slope = p.slopes ? p.slopes[head] * ATTN_LOG2E : 0.f;
     }
@@ -309,8 +308,9 @@ static inline const char* attn_params(const n3d_attention_desc* d, AttnParams& p
     if (d->dtype != N3D_F16 && d->dtype != N3D_BF16) return "float16 or bfloat16 only";
     if (d->heads_k < 1 || d->heads_q < 1 || d->heads_q % d->heads_k) return "the query heads must be a multiple of the key heads";
     if (d->D < 8 || d->D > 128 || d->D % 8) return "head sizes are multiples of 8 from 8 to 128";
-    if ((int64_t)d->B * d->heads_q * ((d->Lq > d->Lk ? d->Lq : d->Lk) / 32 + 1) >= (1 << 26)) return "too many rows for one launch";
-    if (!(d->softcap >= 0.f && d->softcap < INFINITY) || !(d->scale > -INFINITY && d->scale < INFINITY)) return "scale and softcap must be finite, softcap not negative";
+    if ((int64_t)d->B * d->heads_q * ((d->Lq > d->Lk ? d->Lq : d->Lk) / 32 + 1) >= (1 << 28) || d->Lq > (1 << 30) || d->Lk > (1 << 30)) return "too many rows for one launch";
+    // (a capped score is off by 2^-22 of the cap: beyond 4096 that is more than the weights' own rounding)
+    if (!(fabsf(d->scale) <= 0x1p100f) || !(d->softcap == 0.f || (d->softcap >= 0x1p-100f && d->softcap <= 4096.f))) return "scale within 2^100, softcap 0 or 2^-100 to 4096";
     if (d->prefix && !d->causal) return "a prefix needs causal";
     if ((!d->q_documents) != (!d->k_documents)) return "documents of the queries and of the keys, or neither";
     const bool some = d->B > 0 && d->Lq > 0;

@@ -18,7 +18,7 @@ __global__ __launch_bounds__(256) void attn_prep_kernel(AttnParams p) {
     const int lane16 = threadIdx.x & 15, D = p.D;
     float top = 0.f;
     if (blockIdx.y == 0) {
-        const uint32_t rows = (uint32_t)p.B * p.Lq * p.Hq;                // (below 2^31: attn_params)
+        const uint32_t rows = (uint32_t)p.B * p.Lq * p.Hq;                // (below 2^31: n3d_attention_bwd)
         for (uint32_t w = blockIdx.x * 16 + (threadIdx.x >> 4); w < rows; w += gridDim.x * 16) {
             const uint32_t bi = w / p.Hq;
             const int h = w - bi * p.Hq, b = bi / p.Lq, i = bi - b * p.Lq;
@@ -684,6 +684,7 @@ extern "C" int n3d_attention_bwd(const n3d_attention_desc* d, n3d_stream_t strea
     const char* bad = attn_params(d, p);
     N3D_CHECK(!bad, "attention_bwd: %s", bad);
     N3D_CHECK(p.B > 0 && p.Lq > 0, "attention_bwd: no queries");
+    N3D_CHECK((int64_t)p.B * p.Lq * p.Hq < (1ll << 31) && (int64_t)p.B * p.Lk * p.Hk < (1ll << 31), "attention_bwd: 2^31 rows or more");
     N3D_CHECK(d->lse && d->dout && (!d->dk) == (!d->dv) && (d->dq || d->dk || p.Lk == 0), "attention_bwd: null tensor");
     for (int i = 0; i < 3; ++i)
         N3D_CHECK(d->dout_strides[i] % 8 == 0 && d->dout_strides[i] >= 0 && (i != 1 || d->dout_strides[i] <= (1 << 23)), "attention_bwd: strides must be multiples of 8 elements, of tokens 2^23 at most");

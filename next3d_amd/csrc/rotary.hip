@@ -27,13 +27,13 @@ struct RotParams {
     int64_t sb[2], sl[2], sh[2];  // element strides of batch, token and head
     int64_t pos_sb, pos_sl;       // element strides of the positions' batch (0: shared) and token
     int64_t tokens;               // B * L
-    int L, heads[2], D, P, axes, pos_type, shared, gap, tpb, sign;
+    int L, heads[2], D, P, axes, pos_type, shared, tpb, sign;
     int first[ROT_MAX_AXES + 1];  // first pair of every axis
     double log2_base;
     RotDiv by_unit, by_heads, by_len;
 };
 
-// first channel of pair p; its partner is `gap` channels on (halves), or the next channel (interleaved)
+// the axis of pair p
 __device__ __forceinline__ int rot_axis(const RotParams& r, int p) {
     int a = 0;
 #pragma unroll

@@ -80,6 +80,7 @@ variable_list once(variable_list grads, const char* op) {
     variable_list given, out;
     for (const Tensor& g : grads)
         if (g.defined()) given.push_back(g.detach().requires_grad_());
+    if (given.empty()) return grads;
     auto error = std::make_shared<torch::autograd::DelayedError>(std::string(op) + ": differentiable once only", (int64_t)given.size());
     given = (*error)(std::move(given));
     size_t at = 0;
@@ -123,7 +124,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         Tensor dx, dw, db;
         {
             Scope scope(x);
-            const Tensor x2 = rows_of(x), dy = rows_of(grads[0]);
+            const Tensor x2 = rows_of(x), dy = rows_of(grads[0].resolve_neg());
             const int64_t rows = x2.size(0), c = x2.size(1);
             if (ctx->needs_input_grad(0)) dx = dense(x);
             // (absent tensors have no edge: the bias comes right behind the weight, or behind x)
@@ -215,6 +216,8 @@ struct Rotary : torch::autograd::Function<Rotary> {
         Tensor dq = grads[0], dk = grads.size() > 1 ? grads[1] : Tensor();
         if (dq.defined() && !ctx->needs_input_grad(0)) dq = Tensor();
         if (dk.defined() && !ctx->needs_input_grad(1)) dk = Tensor();
+        if (dq.defined()) dq = dq.resolve_neg();
+        if (dk.defined()) dk = dk.resolve_neg();
         if (dq.defined() || dk.defined()) std::tie(dq, dk) = turn(dq, dk, positions, plan, true);
         return once({dq, dk, Tensor(), Tensor()}, "rotary");
     }
@@ -324,7 +327,7 @@ struct Attention : torch::autograd::Function<Attention> {
                 dv = dense(v);
             }
             if (q.numel()) {
-                call(q, k, v, m, s[3], s[5], s[4], grads[0], dq, dk, dv, scope.stream);
+                call(q, k, v, m, s[3], s[5], s[4], grads[0].resolve_neg(), dq, dk, dv, scope.stream);
             } else if (dk.defined()) {                                            // no queries: nothing flows
                 dk.zero_();
                 dv.zero_();

@@ -8,13 +8,19 @@ DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}           # N3D
 
 
 def require_tensor(op, name, t, dtypes, ndim=None):
-    """RuntimeError unless `t` is a dense tensor of one of `dtypes` (and of `ndim` dimensions)."""
-    if not isinstance(t, torch.Tensor) or t.layout != torch.strided:
+    """RuntimeError unless `t` is a dense tensor (whose memory holds its values: no lazy negation) of one of `dtypes` (and of `ndim` dimensions)."""
+    if not isinstance(t, torch.Tensor) or t.layout != torch.strided or t.is_neg():
         raise RuntimeError(f'{op}: {name} must be a (dense) tensor')
     if t.dtype not in dtypes:
         raise RuntimeError(f'{op}: {name} must be {" or ".join(str(d).replace("torch.", "") for d in dtypes)} (got {t.dtype})')
     if ndim is not None and t.ndim != ndim:
         raise RuntimeError(f'{op}: {name} must have {ndim} dimensions (got {t.ndim})')
+
+
+def require_sizes(op, *sizes):
+    """RuntimeError unless all sizes fit the kernels' 31 bits."""
+    if max(sizes) >= 1 << 31:
+        raise RuntimeError(f'{op}: a size of 2^31 or more ({max(sizes)})')
 
 
 def require_same_device(op, first, *others):

@@ -2,12 +2,10 @@
 
 Not an operator of the reference's layer; with `layer_norm` and `rotary` it makes the block of a model over w vectors, tri-plane texels or frames.  One call
 serves training (with gradients), prompts and single tokens over a cache (few queries, many keys: the keys are split over the chip)."""
-import math
-
 import torch
 
 from ... import _lib
-from ._tokens import require_same_device, require_tensor
+from ._tokens import require_same_device, require_sizes, require_tensor
 
 
 def _mask_input(name, t, shape):
@@ -21,7 +19,7 @@ def attention(q, k, v, scale=None, causal=False, prefix=None, documents=None, ke
     """softmax(scores) v for q [B, Lq, Hq, D] and k, v [B, Lk, Hk, D] (float16 or bfloat16, any strides; D a multiple of 8 up to 128; Hq a multiple of Hk,
     query head h reads key head h // (Hq // Hk)).  Returns [B, Lq, Hq, D], and with return_lse also the logarithm of each row's sum, [B, Hq, Lq] float32.
 
-    Scores: t = scale * q.k (scale defaults to D ** -0.5);  softcap > 0: t = softcap * tanh(t / softcap);  slopes [Hq] float32: t -= slope * distance.
+    Scores: t = scale * q.k (scale defaults to D ** -0.5);  softcap > 0 (to 4096): t = softcap * tanh(t / softcap), off by 2^-22 softcap;  slopes [Hq] float32: t -= slope * distance.
     lengths [B] int32: only the first n = lengths[b] keys are in use (default: all of them; the others are never read) — a cache that is filled up to
     there.  Query i stands at position i + n - Lq: the last query beside the last key; its distance to key j is |position - j|.
     causal: key j is visible up to the query's position;  prefix [B] int32 (with causal): and every key j < prefix[b].
@@ -29,8 +27,9 @@ def attention(q, k, v, scale=None, causal=False, prefix=None, documents=None, ke
     negative number belongs to none (padding).  Rows that see nothing are 0, with lse -inf, and have no gradient.  What a row does not see does not reach
     it, not even NaN or infinity.
 
-    Softmax statistics and sums are float32; weights (and in the backward pass dscores) are rounded to the inputs' type for the matrix cores.
-    Differentiable (once) in q, k and v; results and gradients are bitwise reproducible."""
+    Softmax statistics and sums are float32; weights (and in the backward pass dscores) are rounded to the inputs' type for the matrix cores.  In float16
+    the dscores of a call share one power of two, taken from its largest gradient and value: rows whose gradients are 2^-12 of the largest or smaller lose
+    digits (bfloat16's do not).  Differentiable (once) in q, k and v, not through the logarithms; results and gradients are bitwise reproducible."""
     types = (torch.float16, torch.bfloat16)
     require_tensor('attention', 'q', q, types, 4)
     for name, t in (('k', k), ('v', v)):
@@ -43,10 +42,11 @@ def attention(q, k, v, scale=None, causal=False, prefix=None, documents=None, ke
         raise RuntimeError(f'attention: {hq} query heads are not a multiple of {hk} key heads')
     if not 8 <= d <= 128 or d % 8:
         raise RuntimeError(f'attention: head sizes are multiples of 8 from 8 to 128 (got {d})')
+    require_sizes('attention', b, lq, lk, hq)
     scale = d ** -0.5 if scale is None else float(scale)
     softcap = float(softcap)
-    if not math.isfinite(scale) or not (softcap >= 0 and math.isfinite(softcap)):
-        raise RuntimeError('attention: scale and softcap must be finite numbers, softcap not negative')
+    if not abs(scale) <= 2.0 ** 100 or not (softcap == 0 or 2.0 ** -100 <= softcap <= 4096):
+        raise RuntimeError('attention: scale must be finite (within 2^100), softcap 0 (none) or between 2^-100 and 4096')
     if prefix is not None:
         if not causal:
             raise RuntimeError('attention: a prefix needs causal=True')

@@ -5,7 +5,7 @@ tri-plane texels, frames — together with `rotary` and `attention`."""
 import torch
 
 from ... import _lib
-from ._tokens import DTYPES, require_same_device, require_tensor
+from ._tokens import DTYPES, require_same_device, require_sizes, require_tensor
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
@@ -16,6 +16,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     require_tensor('layer_norm', 'x', x, DTYPES)
     if x.ndim < 1 or x.shape[-1] < 1:
         raise RuntimeError('layer_norm: x needs a last dimension of at least one channel')
+    require_sizes('layer_norm', x.shape[-1])
     for name, t in (('weight', weight), ('bias', bias)):
         if t is not None:
             require_tensor('layer_norm', name, t, (torch.float32, x.dtype), 1)

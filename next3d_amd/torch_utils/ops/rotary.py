@@ -4,7 +4,7 @@ Not an operator of the reference's layer; it turns the queries and keys of `atte
 import torch
 
 from ... import _lib
-from ._tokens import DTYPES, require_same_device, require_tensor
+from ._tokens import DTYPES, require_same_device, require_sizes, require_tensor
 
 _POSITIONS = (torch.float32, torch.int32, torch.int64)
 
@@ -25,6 +25,7 @@ def rotary(q, positions, sections, k=None, base=10000.0, pairing='interleaved', 
             raise RuntimeError(f'rotary: k {tuple(k.shape)} does not have the batch, tokens and channels of q {tuple(q.shape)}')
     require_tensor('rotary', 'positions', positions, _POSITIONS)
     b, l, _, d = q.shape
+    require_sizes('rotary', b * l)
     sections = tuple(int(s) for s in sections)
     if not 1 <= len(sections) <= 4 or any(s < 0 or s % 2 for s in sections) or not 0 < sum(sections) <= d:
         raise RuntimeError(f'rotary: sections must be 1 to 4 even numbers of channels that add up to 2..{d} (got {sections})')

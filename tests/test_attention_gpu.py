@@ -225,6 +225,82 @@ def test_attention_strides(dev):
         assert all(torch.equal(a, c) for a, c in zip(*results))
 
 
+def test_attention_offsets_beyond_32_bits(dev):
+    """One head of a cache whose tokens lie 16 KB apart: its last keys are 4.9 GB behind the first; single tokens, many queries, and the gradients."""
+    lk, d = 300000, 8
+    cache = torch.empty((2, lk, 64, 2 * 64), dtype=BF16, device=dev)
+    k, v = _randn((2, lk, 1, d), 65, BF16), _randn((2, lk, 1, d), 66, BF16)
+    cache[:, :, 63:, :d], cache[:, :, 63:, 64:64 + d] = k.to(dev), v.to(dev)
+    lengths = torch.tensor([lk, lk - 999], dtype=torch.int32)
+    for lq, train in ((1, False), (65, False), (3, True)):
+        q, do = _randn((2, lq, 1, d), 67, BF16), _randn((2, lq, 1, d), 68, BF16)
+        from next3d_amd.torch_utils.ops import attention
+        leaves = [q.to(dev).requires_grad_(train), cache[:, :, 63:, :d].detach().requires_grad_(train), cache[:, :, 63:, 64:64 + d].detach().requires_grad_(train)]
+        out = attention.attention(*leaves, causal=True, lengths=lengths.to(dev))
+        vals, tols = R.attention(q, k, v, do if train else None, causal=True, lengths=lengths)
+        got = dict(out=out)
+        if train:
+            got.update(zip(('dq', 'dk', 'dv'), torch.autograd.grad(out, leaves, do.to(dev))))
+        for name, t in got.items():
+            R.assert_within(t, vals[name], tols[name], f'{lq} {name}')
+    del cache, leaves, out, got
+    torch.cuda.empty_cache()
+
+
+def test_attention_caps_from_tiny_to_large(dev):
+    q, k, v, do = _inputs(1, 100, 100, 2, 1, 64, F16, 69)
+    q[0, 7], k[0, 9] = 0, 0                                                 # scores of exactly zero
+    for kw in (dict(softcap=2.0 ** -90), dict(softcap=2.0 ** -90, scale=1000.0), dict(softcap=4096.0), dict(softcap=0.01, causal=True, slopes=torch.tensor([0.5, 0.0]))):
+        _check(dev, q, k, v, do, what=str(sorted(kw)), **kw)
+
+
+def test_attention_one_tensor_as_query_key_and_value(dev):
+    from next3d_amd.torch_utils.ops import attention
+    x, _, _, do = _inputs(2, 77, 77, 2, 2, 64, BF16, 73)
+    leaf = x.to(dev).requires_grad_()
+    got, = torch.autograd.grad(attention.attention(leaf, leaf, leaf, causal=True), leaf, do.to(dev))
+    each = _run(dev, x, x, x, do, causal=True)
+    want = each['dq'].double() + each['dk'].double() + each['dv'].double()
+    size = each['dq'].double().abs() + each['dk'].double().abs() + each['dv'].double().abs()
+    assert bool(((got.double() - want).abs() <= 2 * 2.0 ** -8 * size).all())               # (two additions in bfloat16)
+
+
+def test_attention_lazily_negated_gradients(dev):
+    q, k, v, do = _inputs(1, 40, 40, 1, 1, 16, F16, 74)
+    plain, negated = _run(dev, q, k, v, -do), _run_neg(dev, q, k, v, do)
+    assert all(torch.equal(plain[n], negated[n]) for n in ('dq', 'dk', 'dv'))
+
+
+def _run_neg(dev, q, k, v, do):
+    from next3d_amd.torch_utils.ops import attention
+    leaves = [t.to(dev).requires_grad_() for t in (q, k, v)]
+    return dict(zip(('dq', 'dk', 'dv'), torch.autograd.grad(attention.attention(*leaves), leaves, torch._neg_view(do.to(dev)))))
+
+
+def test_attention_calls_side_by_side(dev):
+    """Calls of several forms in flight on four streams at once give what they give alone."""
+    from next3d_amd.torch_utils.ops import attention
+    work = [(_inputs(1, 900, 900, 4, 2, 64, F16, 75), dict(causal=True)), (_inputs(2, 1, 4000, 8, 2, 128, BF16, 76), dict()), (_inputs(1, 1700, 1700, 1, 1, 64, BF16, 77), dict()),
+            (_inputs(2, 500, 500, 2, 2, 72, F16, 78), dict(documents=_docs(2, 500, 4)))]
+    work = [([t.to(dev) for t in ts], _to(dev, kw)) for ts, kw in work]
+
+    def step(ts, kw):
+        leaves = [t.detach().requires_grad_() for t in ts[:3]]
+        out = attention.attention(*leaves, **kw)
+        return [out.detach(), *torch.autograd.grad(out, leaves, ts[3])]
+
+    alone = [step(*w) for w in work]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in work]
+    for _ in range(5):
+        together = []
+        for s, w in zip(streams, work):
+            with torch.cuda.stream(s):
+                together.append(step(*w))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for x, y in zip(alone, together) for a, c in zip(x, y))
+
+
 def test_attention_empty(dev):
     from next3d_amd.torch_utils.ops import attention
     for b, lq, lk in ((0, 4, 4), (2, 0, 5), (2, 5, 0)):

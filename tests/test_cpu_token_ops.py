@@ -190,3 +190,37 @@ def test_host_side_is_built_and_bound():
     assert ext is _lib.token_ext() and all(callable(getattr(ext, n)) for n in ('layer_norm', 'rotary', 'attention'))
     with pytest.raises(RuntimeError):
         ext.bind([0, 1])
+
+
+def test_token_ops_refuse_sizes_and_lazy_values():
+    from next3d_amd.torch_utils.ops.attention import attention
+    from next3d_amd.torch_utils.ops.layer_norm import layer_norm
+    from next3d_amd.torch_utils.ops.rotary import rotary
+    one = torch.zeros(1)
+    _raises('2\\^31', layer_norm, one.expand(1 << 31))
+    _raises('2\\^31', rotary, one.expand(1 << 16, 1 << 15, 1, 2), one.int().expand(1 << 15, 1), (2,))
+    half = one.half()
+    for b, l in ((1 << 31, 1), (1, 1 << 31)):
+        _raises('2\\^31', attention, half.expand(b, 1, 1, 8), half.expand(b, l, 1, 8), half.expand(b, l, 1, 8))
+    x = torch._neg_view(torch.ones(2, 8))                              # a view whose memory holds the negated values
+    _raises('dense', layer_norm, x)
+    _raises('dense', layer_norm, torch.ones(2, 8), x[0])
+    _raises('dense', rotary, x.view(1, 2, 1, 8), torch.zeros(2, 1), (8,))
+    q = torch.zeros(1, 2, 1, 8).half()
+    _raises('dense', attention, q, torch._neg_view(q), q)
+    for kw in (dict(softcap=5000.0), dict(softcap=1e-40), dict(softcap=float('nan')), dict(scale=1e38), dict(scale=-1e38)):
+        _raises('finite', attention, q, q, q, **kw)
+
+
+def test_attention_c_entries_refuse_sizes():
+    from next3d_amd import _lib
+    lib = _lib.lib()
+    base = dict(q=4096, k=4096, v=4096, out=4096, lse=4096, dout=4096, dq=4096, dk=4096, dv=4096, scale=1.0, B=1, Lq=4, Lk=300, heads_q=1, heads_k=1, D=16, dtype=1,
+                workspace=4096, workspace_bytes=1 << 60)
+    for kw, word in ((dict(Lk=(1 << 30) + 1), 'rows'), (dict(Lq=(1 << 30) + 1), 'rows'), (dict(softcap=4097.0), 'softcap'), (dict(softcap=1e-35), 'softcap'),
+                     (dict(scale=1e35), 'scale')):
+        for entry in (lib.n3d_attention, lib.n3d_attention_bwd):
+            assert entry(_lib.AttentionDesc(**dict(base, **kw)), None) != 0 and word in lib.n3d_last_error().decode(), kw
+    many = _lib.AttentionDesc(**dict(base, B=1 << 10, Lq=1 << 19, heads_q=4, heads_k=4))
+    assert lib.n3d_attention_bwd(many, None) != 0 and '2^31' in lib.n3d_last_error().decode()
+    assert lib.n3d_attention_workspace(_lib.AttentionDesc(**dict(base, B=1 << 10, Lk=1 << 15, heads_q=64, heads_k=8))) >= 0      # (a large cache, single tokens)

@@ -229,6 +229,40 @@ def test_rotary_only_one_gradient_and_differences(dev):
 
 
 
+def test_token_ops_beyond_32_bits(dev):
+    """Tensors of more than 2^31 elements: the first, a middle and the last rows."""
+    from next3d_amd.torch_utils.ops import layer_norm, rotary
+    rows, c = 2 ** 21 + 5, 1030
+    x, dy = (torch.empty((rows, c), dtype=BF16, device=dev).normal_(0.0, 1.0) for _ in range(2))
+    w = _randn((c,), 5)
+    leaf = x.requires_grad_()
+    y = layer_norm.layer_norm(leaf, w.to(dev))
+    dx, = torch.autograd.grad(y, leaf, dy)
+    some = [0, 1, rows // 2 + 1, rows - 2, rows - 1]
+    vals, tols = R.layer_norm(x.detach()[some].cpu(), w, None, 1e-5, dy[some].cpu())
+    R.assert_within(y[some], vals['y'], tols['y'], 'y')
+    R.assert_within(dx[some], vals['dx'], tols['dx'], 'dx')
+    del x, dy, leaf, y, dx
+    n = 2 ** 18 + 3
+    q = torch.empty((1, n, 64, 128), dtype=F16, device=dev).normal_(0.0, 1.0)
+    pos = torch.randint(0, 4096, (n, 3), generator=torch.Generator().manual_seed(1))
+    y = rotary.rotary(q, pos.to(dev), (32, 48, 48))
+    some = [0, n // 2, n - 1]
+    R.assert_within(y[:, some], *R.rotary(q[:, some].cpu(), pos[some], (32, 48, 48), 10000.0, 'interleaved', 'axis'), 'rotary')
+    del q, y
+    torch.cuda.empty_cache()
+
+
+def test_token_ops_lazily_negated_gradients(dev):
+    from next3d_amd.torch_utils.ops import layer_norm, rotary
+    x, pos = _randn((1, 5, 2, 16), 6).to(dev).requires_grad_(), torch.arange(5, device=dev)[:, None]
+    dy = _randn((1, 5, 2, 16), 7).to(dev)
+    for fn in (layer_norm.layer_norm, lambda t: rotary.rotary(t, pos, (16,))):
+        a, = torch.autograd.grad(fn(x), x, -dy)
+        b, = torch.autograd.grad(fn(x), x, torch._neg_view(dy))
+        assert torch.equal(a, b)
+
+
 def test_token_ops_refuse_second_derivatives(dev):
     """Under create_graph the gradients come out as ever, and differentiating them again raises."""
     from next3d_amd.torch_utils.ops import attention, layer_norm, rotary
