@@ -498,10 +498,12 @@ void attn_ranges(AttnParams& p, void* workspace, hipStream_t stream) {
     p.order = order;
 }
 
-// The token kernel where its rows (queries x heads of a group) fill two 32-row blocks at most; its keys go to enough workgroups to fill the chip twice.
+// The token kernel up to 24 queries, or where its rows (queries x heads of a group) fill two 32-row blocks at most; its keys go to enough workgroups to fill
+// the chip twice.  (Single tokens aside, against the kernel of 128 queries: 5 queries x 16 heads a group over 8192 keys 34 us against 60, 16 x 16 over 4096
+// 134 / 203, 24 x 8 over 2048 97 / 111; but 32 x 16 over 8192 39 / 37, 32 x 3 over 512 14 / 10, 100 x 1 over 4096 23 / 16.)
 static bool attn_plan(AttnParams& p) {
     const int64_t rows = (int64_t)p.Lq * p.G;
-    if (rows > 64) {
+    if (rows > 64 && p.Lq > 24) {
         p.row_blocks = cdiv(p.Lq, 128);
         p.splits = attn_room((int64_t)p.B * p.Hq * p.row_blocks, p.nkt);
         return false;

@@ -87,6 +87,15 @@ def test_attention_lengths(dev, dtype):
     _check(dev, q, k, v, do, lengths=torch.tensor([-4], dtype=torch.int32))
 
 
+@pytest.mark.parametrize('dtype', [F16, BF16])
+def test_attention_few_queries_of_large_groups(dev, dtype):
+    lengths = torch.tensor([700, 0, 333], dtype=torch.int32)
+    for lq, hq, hk, d in ((5, 32, 2, 128), (32, 6, 1, 64), (33, 6, 1, 64), (1, 71, 1, 80), (17, 12, 2, 40)):
+        q, k, v, do = _inputs(3, lq, 700, hq, hk, d, dtype, 79)
+        _check(dev, q, k, v, what=f'{lq}', causal=True, lengths=lengths, softcap=9.0)
+        _check(dev, q, k, v, do, what=f'{lq}', documents=_docs(3, lq, 3, 8), key_documents=_docs(3, 700, 3, 9))
+
+
 def test_attention_never_reads_behind_the_length(dev):
     """NaN behind the last key in use reaches nothing, and the gradients there are zero."""
     for lq in (1, 33, 200):
