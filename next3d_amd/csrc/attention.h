@@ -33,7 +33,10 @@ struct AttnParams {
     const float* maxima;                             // partial maxima (float16 gradients), see attn_ds_scale
     int B, Lq, Lk, Hq, Hk, G, D, nkt, nqt, causal, row_blocks;
     const int* order;                                // [B, row blocks of queries], the longest first, or null: the last first
-    int splits, chunks;                              // workgroups a row block's work is split over; of them over the long axis (dk / dv: per head)
+    int splits;                                      // workgroups a row block's work is split over
+    // the dk / dv kernel's own: blocks of keys, workgroups a block's work is split over, of them over the queries of a head; its parts
+    int k_blocks, k_splits, chunks, first_k;         // (first_k: where its workgroups begin in a launch of both kinds)
+    float* k_part;
     float scale, softcap;
 };
 
@@ -331,7 +334,7 @@ static inline const char* attn_params(const n3d_attention_desc* d, AttnParams& p
     p.B = d->B; p.Lq = d->Lq; p.Lk = d->Lk; p.Hq = d->heads_q; p.Hk = d->heads_k; p.G = d->heads_q / d->heads_k; p.D = d->D;
     p.nkt = cdiv(d->Lk, ATTN_TILE); p.nqt = cdiv(d->Lq, ATTN_TILE);
     p.causal = d->causal != 0; p.scale = d->scale; p.softcap = d->softcap;
-    p.splits = p.chunks = 1;
+    p.splits = p.k_splits = p.chunks = 1;
     return nullptr;
 }
 

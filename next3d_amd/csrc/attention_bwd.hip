@@ -121,17 +121,23 @@ __device__ __forceinline__ void attn_pair(const AttnParams& p, const AttnScore& 
 }
 __device__ __forceinline__ float attn_lse2(float lse) { return lse == -INFINITY ? INFINITY : lse * ATTN_LOG2E; }       // (a row that sees nothing: every weight 0)
 
-template <typename T, int DB, int MODE, bool DOCS>
-__global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnParams p) {
+template <int DB> static constexpr bool attn_dkv_pair() { return DB > 3; }      // (see attn_dkv)
+// what both kinds of workgroups keep in the LDS
+template <int DB> static constexpr int attn_row() { return DB > 2 ? 128 : 64; }
+template <int DB> static constexpr int attn_lds_bytes() { return 4 * ATTN_TILE * attn_row<DB>() * 2; }
+struct AttnRows {
+    float lse[2][ATTN_TILE], delta[2][ATTN_TILE];
+};
+
 #ifdef __HIP_DEVICE_COMPILE__                            // (hipcc drops the launch stub of a template whose body its host pass cannot read)
-    constexpr int ROW = DB > 2 ? 128 : 64, TILE_BYTES = ATTN_TILE * ROW * 2;
-    __shared__ __align__(1024) char smem[4 * TILE_BYTES];
-    __shared__ __align__(16) int sdoc[2][ATTN_TILE];
+template <typename T, int DB, int MODE, bool DOCS>
+__device__ __forceinline__ void attn_dq(const AttnParams& p, int group, char* smem, int (*sdoc)[ATTN_TILE]) {
+    constexpr int ROW = attn_row<DB>(), TILE_BYTES = ATTN_TILE * ROW * 2;
     const int wave = attn_uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
     // p.splits > 1: the keys in that many runs of whole tiles, float32 parts that attn_parts_kernel adds in order
     const int total = p.B * p.Hq * p.row_blocks * p.splits, per = (total + 7) / 8;
-    const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if ((int)(blockIdx.x >> 3) >= per || id >= total) return;
+    const int id = (group & 7) * per + (group >> 3);
+    if (group >> 3 >= per || id >= total) return;
     const int split = id % p.splits, pos = id / p.splits % p.row_blocks, bh = id / p.splits / p.row_blocks, h = bh % p.Hq, b = bh / p.Hq, hk = h / p.G;
     const int blk = DOCS && p.order ? p.order[b * p.row_blocks + pos] : p.row_blocks - 1 - pos;
     const int n = attn_keys(p, b), prefix = p.prefix ? p.prefix[b] : 0, q0 = blk * 128;
@@ -298,34 +304,28 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnParams p) {
             else ((T*)p.dq)[at + d] = (T)(x[c] * p.scale);
         }
     }
-#endif
 }
 
 // A wave owns 32 keys: their K and V as operands and their dk and dv as accumulators.  Beyond 96 channels that is more than half of a SIMD's registers, so
 // one wave a SIMD, whose vector work and products would wait for each other (537 us at 2 x 4096 x 16 heads x 128, causal with caps; two loops interleaved by
 // hand: 555).  There two waves share 32 keys (attn_dkv_pair): each takes the scores of half of a tile's queries, they trade the 16-bit weights through the
 // LDS, and each adds up half of the channels over all of the queries.
-template <int DB> static constexpr bool attn_dkv_pair() { return DB > 3; }
 template <typename T, int DB, int MODE, bool DOCS>
-__global__ __launch_bounds__(attn_dkv_pair<DB>() ? 512 : 256, 2) void attn_dkv_kernel(AttnParams p) {
-#ifdef __HIP_DEVICE_COMPILE__                            // (hipcc drops the launch stub of a template whose body its host pass cannot read)
-    constexpr int ROW = DB > 2 ? 128 : 64, TILE_BYTES = ATTN_TILE * ROW * 2;
+__device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* smem, AttnRows& rows, int (*sdoc)[ATTN_TILE], char* traded) {
+    constexpr int ROW = attn_row<DB>(), TILE_BYTES = ATTN_TILE * ROW * 2;
     constexpr float SHIFT = ATTN_P_SHIFT<T>;
     constexpr bool PAIR = attn_dkv_pair<DB>();
     constexpr int NB = PAIR ? DB / 2 : DB;                              // blocks of 32 channels a wave adds up
     typedef typename AttnVec<T>::x8 frag;
-    __shared__ __align__(1024) char smem[4 * TILE_BYTES];                 // [buffer][q, do]
-    __shared__ __align__(16) float slse[2][ATTN_TILE], sdelta[2][ATTN_TILE];
-    __shared__ __align__(16) int sdoc[2][ATTN_TILE];
-    __shared__ __align__(16) char traded[PAIR ? 4 * 2 * 4 * 1024 : 16];   // [key group][half of the queries][w, w, d, d][lane] fragments
+    // smem: [buffer][q, do];  traded (pairs): [key group][half of the queries][w, w, d, d][lane] fragments
     const int wave = attn_uniform(threadIdx.x >> 6), keys = PAIR ? wave & 3 : wave, part = PAIR ? wave >> 2 : 0, lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
-    // p.splits: 1 (a workgroup adds up all heads of the group), or float32 parts that attn_parts_kernel adds in order: the heads of the group in
-    // p.splits / p.chunks equal runs, the queries in p.chunks runs of whole tiles
-    const int total = p.B * p.Hk * p.splits * p.row_blocks, per = (total + 7) / 8;
-    const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if ((int)(blockIdx.x >> 3) >= per || id >= total) return;
-    const int blk = id % p.row_blocks, split = id / p.row_blocks % p.splits, bh = id / p.row_blocks / p.splits, hk = bh % p.Hk, b = bh / p.Hk;
-    const int heads = p.G * p.chunks / p.splits, g0 = split / p.chunks * heads, g1 = g0 + heads;
+    // p.k_splits: 1 (a workgroup adds up all heads of the group), or float32 parts that attn_parts_kernel adds in order: the heads of the group in
+    // p.k_splits / p.chunks equal runs, the queries in p.chunks runs of whole tiles
+    const int total = p.B * p.Hk * p.k_splits * p.k_blocks, per = (total + 7) / 8;
+    const int id = (group & 7) * per + (group >> 3);
+    if (group >> 3 >= per || id >= total) return;
+    const int blk = id % p.k_blocks, split = id / p.k_blocks % p.k_splits, bh = id / p.k_blocks / p.k_splits, hk = bh % p.Hk, b = bh / p.Hk;
+    const int heads = p.G * p.chunks / p.k_splits, g0 = split / p.chunks * heads, g1 = g0 + heads;
     const int n = attn_keys(p, b), prefix = p.prefix ? p.prefix[b] : 0, k0 = blk * 128, off = n - p.Lq;
     const int j = k0 + 32 * keys + l31;
     const int kdoc = DOCS && j < p.Lk ? p.kdoc[b * p.kdoc_stride + j] : 0;
@@ -386,8 +386,8 @@ __global__ __launch_bounds__(attn_dkv_pair<DB>() ? 512 : 256, 2) void attn_dkv_k
         sd.issue(attn_addr((const T*)p.dout + b * p.ds[0] + h * p.ds[2]), t, p.Lq, (int)p.ds[1], p.D, at + TILE_BYTES, wave);
     };
     auto commit = [&](int buf) {
-        if (wave == 0) slse[buf][lane] = row_next;
-        if (wave == 1) sdelta[buf][lane] = row_next;
+        if (wave == 0) rows.lse[buf][lane] = row_next;
+        if (wave == 1) rows.delta[buf][lane] = row_next;
         if (DOCS && wave == 2) sdoc[buf][lane] = __builtin_bit_cast(int, row_next);
     };
     f32x16 dk[NB] = {}, dv[NB] = {};
@@ -433,7 +433,7 @@ __global__ __launch_bounds__(attn_dkv_pair<DB>() ? 512 : 256, 2) void attn_dkv_k
             const float dist = (float)(i0 + ib + off - j);
 #pragma unroll
             for (int a = 0; a < 4; ++a) {
-                const float4 l4 = *reinterpret_cast<const float4*>(&slse[now][ib + 8 * a]), e4 = *reinterpret_cast<const float4*>(&sdelta[now][ib + 8 * a]);
+                const float4 l4 = *reinterpret_cast<const float4*>(&rows.lse[now][ib + 8 * a]), e4 = *reinterpret_cast<const float4*>(&rows.delta[now][ib + 8 * a]);
                 const float l[4] = {l4.x, l4.y, l4.z, l4.w}, de[4] = {e4.x, e4.y, e4.z, e4.w};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) attn_ds<T, MODE>(S, dP, 4 * a + e, f, ds_by, l[e], de[e], dist + (float)(8 * a + e));
@@ -536,9 +536,9 @@ __global__ __launch_bounds__(attn_dkv_pair<DB>() ? 512 : 256, 2) void attn_dkv_k
 #pragma unroll
             for (int r = 0; r < 16; ++r) dk[db][r] = dv[db][r] = 0.f;
     const int64_t row = ((int64_t)b * p.Lk + j) * p.Hk + hk, all = (int64_t)p.B * p.Lk * p.Hk;
-    if (p.splits > 1) {
-        float* pk = p.part + (2 * split * all + row) * p.D;
-        float* pv = p.part + ((2 * split + 1) * all + row) * p.D;
+    if (p.k_splits > 1) {
+        float* pk = p.k_part + (2 * split * all + row) * p.D;
+        float* pv = p.k_part + ((2 * split + 1) * all + row) * p.D;
         attn_store_part<NB>(pk + 64 * part, dk, k_by, half, p.D - 64 * part, store);
         attn_store_part<NB>(pv + 64 * part, dv, v_by, half, p.D - 64 * part, store);
     } else {
@@ -585,15 +585,48 @@ __global__ __launch_bounds__(attn_dkv_pair<DB>() ? 512 : 256, 2) void attn_dkv_k
         for (int c = 0; c < 2; ++c) {
             const int d = lane + 64 * c;
             if (d >= p.D || (PAIR && c != part)) continue;
-            if (p.splits > 1) {
-                p.part[(2 * split * all + re) * p.D + d] = xk[c] * p.scale;
-                p.part[((2 * split + 1) * all + re) * p.D + d] = xv[c];
+            if (p.k_splits > 1) {
+                p.k_part[(2 * split * all + re) * p.D + d] = xk[c] * p.scale;
+                p.k_part[((2 * split + 1) * all + re) * p.D + d] = xv[c];
             } else {
                 ((T*)p.dk)[re * p.D + d] = (T)(xk[c] * p.scale);
                 ((T*)p.dv)[re * p.D + d] = (T)xv[c];
             }
         }
     }
+}
+#endif
+
+template <typename T, int DB, int MODE, bool DOCS>
+__global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnParams p) {
+#ifdef __HIP_DEVICE_COMPILE__
+    __shared__ __align__(1024) char smem[attn_lds_bytes<DB>()];
+    __shared__ __align__(16) int sdoc[2][ATTN_TILE];
+    attn_dq<T, DB, MODE, DOCS>(p, blockIdx.x, smem, sdoc);
+#endif
+}
+template <typename T, int DB, int MODE, bool DOCS>
+__global__ __launch_bounds__(attn_dkv_pair<DB>() ? 512 : 256, 2) void attn_dkv_kernel(AttnParams p) {
+#ifdef __HIP_DEVICE_COMPILE__
+    __shared__ __align__(1024) char smem[attn_lds_bytes<DB>()];
+    __shared__ __align__(16) AttnRows rows;
+    __shared__ __align__(16) int sdoc[2][ATTN_TILE];
+    __shared__ __align__(16) char traded[attn_dkv_pair<DB>() ? 4 * 2 * 4 * 1024 : 16];
+    attn_dkv<T, DB, MODE, DOCS>(p, blockIdx.x, smem, rows, sdoc, traded);
+#endif
+}
+// Both in one launch where that is two rounds of the chip at most (1024 workgroups): small calls wait for single workgroups, and so for both kinds at once.
+// Training step of 3 x 1021 x 6 heads x 72, documents: 105 -> 91 us, 2 x 1200 x 8 heads on 2 x 72, causal with caps: 125 -> 100, 4096 x 16 x 64: 425 -> 424.
+// (Larger ones keep two launches: the dq workgroups alone need fewer registers, and more of them share a CU.)
+template <typename T, int DB, int MODE, bool DOCS>
+__global__ __launch_bounds__(256, 2) void attn_grads_kernel(AttnParams p) {
+#ifdef __HIP_DEVICE_COMPILE__
+    static_assert(!attn_dkv_pair<DB>(), "256 threads each");
+    __shared__ __align__(1024) char smem[attn_lds_bytes<DB>()];
+    __shared__ __align__(16) AttnRows rows;
+    __shared__ __align__(16) int sdoc[2][ATTN_TILE];
+    if ((int)blockIdx.x < p.first_k) attn_dq<T, DB, MODE, DOCS>(p, blockIdx.x, smem, sdoc);
+    else attn_dkv<T, DB, MODE, DOCS>(p, blockIdx.x - p.first_k, smem, rows, sdoc, nullptr);
 #endif
 }
 
@@ -616,56 +649,59 @@ __global__ __launch_bounds__(256) void attn_parts_kernel(const float* __restrict
 }
 
 // How the gradients' work is split (attn_room)
-struct AttnSplits {
-    int dq, dkv, chunks;
-};
-static AttnSplits attn_splits(const AttnParams& p) {
-    AttnSplits s;
-    s.dq = attn_room((int64_t)p.B * p.Hq * cdiv(p.Lq, 128), p.nkt);
+static void attn_bwd_split(AttnParams& p) {
+    p.row_blocks = cdiv(p.Lq, 128);
+    p.splits = attn_room((int64_t)p.B * p.Hq * p.row_blocks, p.nkt);
     // dk / dv: a group's heads in as many runs as fill the chip (256 workgroups beyond 96 channels, 512 up to there), or fill it twice where the diagonal
     // or documents leave long and short ones.  Training step of 2 x 4096 x 16 heads on 4: causal x 128, 1024 -> 512 workgroups: 755 -> 727 us (half the parts);
     // causal x 64: 467, at 512 518; no mask x 128, 512 -> 256: 1337 -> 1317; documents x 128: 492, at 256 526; documents x 64: 310, at 512 342.
-    const int64_t groups = (int64_t)p.B * p.Hk * (p.Lk ? cdiv(p.Lk, 128) : 1), fill = (p.D > 96 ? 256 : 512) * (p.causal || p.kdoc ? 2 : 1);
+    p.k_blocks = cdiv(p.Lk, 128);
+    const int64_t groups = (int64_t)p.B * p.Hk * (p.Lk ? p.k_blocks : 1), fill = (p.D > 96 ? 256 : 512) * (p.causal || p.kdoc ? 2 : 1);
     int heads = 1;
     while (heads < p.G && (p.G % heads || groups * heads < fill)) ++heads;
-    s.chunks = heads < p.G ? 1 : attn_room(groups * heads, p.nqt);
-    s.dkv = heads * s.chunks;
-    return s;
+    p.chunks = heads < p.G ? 1 : attn_room(groups * heads, p.nqt);
+    p.k_splits = heads * p.chunks;
 }
 
 template <typename T, int DB, int MODE, bool DOCS>
-static void attn_bwd_launch(AttnParams& p, const AttnSplits& splits, hipStream_t stream) {
+static void attn_bwd_launch(AttnParams& p, hipStream_t stream) {
     const int64_t q_rows = (int64_t)p.B * p.Lq * p.Hq, k_rows = (int64_t)p.B * p.Lk * p.Hk;
     const int prep = p.maxima ? ATTN_MAXIMA : (int)(cdiv64(q_rows, 16) < 2048 ? cdiv64(q_rows, 16) : 2048);
     hipLaunchKernelGGL((attn_prep_kernel<T>), dim3(prep, p.maxima ? 2 : 1), dim3(256), 0, stream, p);
-    auto add = [&](int count, int64_t all, void* a, void* b) {
-        if (count > 1) hipLaunchKernelGGL((attn_parts_kernel<T>), dim3((unsigned)cdiv64(all, 2048), b ? 2 : 1), dim3(256), 0, stream, p.part, count, all, (T*)a, (T*)b);
+    auto add = [&](const float* part, int count, int64_t all, void* a, void* b) {
+        if (count > 1) hipLaunchKernelGGL((attn_parts_kernel<T>), dim3((unsigned)cdiv64(all, 2048), b ? 2 : 1), dim3(256), 0, stream, part, count, all, (T*)a, (T*)b);
     };
-    if (p.dq) {
-        p.splits = splits.dq;
-        p.row_blocks = cdiv(p.Lq, 128);
-        hipLaunchKernelGGL((attn_dq_kernel<T, DB, MODE, DOCS>), dim3(8 * cdiv(p.B * p.Hq * p.splits * p.row_blocks, 8)), dim3(256), 0, stream, p);
-        add(splits.dq, q_rows * p.D, p.dq, nullptr);
+    const int dq = p.dq ? 8 * cdiv(p.B * p.Hq * p.splits * p.row_blocks, 8) : 0, dkv = p.dk && p.Lk > 0 ? 8 * cdiv(p.B * p.Hk * p.k_splits * p.k_blocks, 8) : 0;
+    bool both = false;
+    if constexpr (!attn_dkv_pair<DB>()) {
+        if ((both = dq && dkv && dq + dkv <= 1024)) {
+            p.first_k = dq;
+            hipLaunchKernelGGL((attn_grads_kernel<T, DB, MODE, DOCS>), dim3(dq + dkv), dim3(256), 0, stream, p);
+        }
     }
-    if (p.dk && p.Lk > 0) {
-        p.splits = splits.dkv;
-        p.chunks = splits.chunks;
-        p.row_blocks = cdiv(p.Lk, 128);
-        hipLaunchKernelGGL((attn_dkv_kernel<T, DB, MODE, DOCS>), dim3(8 * cdiv(p.B * p.Hk * p.splits * p.row_blocks, 8)),
-                           dim3(attn_dkv_pair<DB>() ? 512 : 256), 0, stream, p);
-        add(splits.dkv, k_rows * p.D, p.dk, p.dv);
+    if (dq) {
+        if (!both) hipLaunchKernelGGL((attn_dq_kernel<T, DB, MODE, DOCS>), dim3(dq), dim3(256), 0, stream, p);
+        add(p.part, p.splits, q_rows * p.D, p.dq, nullptr);
+    }
+    if (dkv) {
+        if (!both) hipLaunchKernelGGL((attn_dkv_kernel<T, DB, MODE, DOCS>), dim3(dkv), dim3(attn_dkv_pair<DB>() ? 512 : 256), 0, stream, p);
+        add(p.k_part, p.k_splits, k_rows * p.D, p.dk, p.dv);
     }
 }
 
-// floats behind the document ranges: delta, maxima (float16), the larger of the two kernels' parts (one is added up before the other begins)
-static int64_t attn_bwd_floats(const AttnParams& p, int dtype, AttnSplits& splits, int64_t& maxima_at, int64_t& parts_at) {
-    const int64_t ranges = (attn_range_floats(p) + 3) / 4 * 4, delta = ((int64_t)p.B * p.Hq * p.Lq + 3) / 4 * 4;
-    maxima_at = ranges + delta;
-    parts_at = maxima_at + (dtype == N3D_F16 ? 2 * ATTN_MAXIMA : 0);
-    splits = attn_splits(p);
-    const int64_t dq = splits.dq > 1 ? (int64_t)splits.dq * p.B * p.Lq * p.Hq * p.D : 0;
-    const int64_t dkv = splits.dkv > 1 ? 2 * (int64_t)splits.dkv * p.B * p.Lk * p.Hk * p.D : 0;
-    return parts_at + (dq > dkv ? dq : dkv);
+// Where the workspace's parts lie, in floats: document ranges and order, delta, maxima (float16), parts of dq, parts of dk and dv, the end
+struct AttnBwdSpace {
+    int64_t delta, maxima, part, k_part, end;
+};
+static AttnBwdSpace attn_bwd_plan(AttnParams& p, int dtype) {
+    attn_bwd_split(p);
+    AttnBwdSpace at;
+    at.delta = (attn_range_floats(p) + 3) / 4 * 4;
+    at.maxima = at.delta + ((int64_t)p.B * p.Hq * p.Lq + 3) / 4 * 4;
+    at.part = at.maxima + (dtype == N3D_F16 ? 2 * ATTN_MAXIMA : 0);
+    at.k_part = at.part + (p.splits > 1 ? (int64_t)p.splits * p.B * p.Lq * p.Hq * p.D : 0);
+    at.end = at.k_part + (p.k_splits > 1 ? 2 * (int64_t)p.k_splits * p.B * p.Lk * p.Hk * p.D : 0);
+    return at;
 }
 
 extern "C" int64_t n3d_attention_bwd_workspace(const n3d_attention_desc* d) {
@@ -673,9 +709,7 @@ extern "C" int64_t n3d_attention_bwd_workspace(const n3d_attention_desc* d) {
     const char* bad = attn_params(d, p);
     N3D_CHECK(!bad, "attention_bwd: %s", bad);
     if (p.B == 0 || p.Lq == 0) return 0;
-    AttnSplits splits;
-    int64_t m, s;
-    return 4 * attn_bwd_floats(p, d->dtype, splits, m, s);
+    return 4 * attn_bwd_plan(p, d->dtype).end;
 }
 
 extern "C" int n3d_attention_bwd(const n3d_attention_desc* d, n3d_stream_t stream_) {
@@ -689,20 +723,20 @@ extern "C" int n3d_attention_bwd(const n3d_attention_desc* d, n3d_stream_t strea
     for (int i = 0; i < 3; ++i)
         N3D_CHECK(d->dout_strides[i] % 8 == 0 && d->dout_strides[i] >= 0 && (i != 1 || d->dout_strides[i] <= (1 << 23)), "attention_bwd: strides must be multiples of 8 elements, of tokens 2^23 at most");
     N3D_CHECK(((uintptr_t)d->dout | (uintptr_t)d->dq | (uintptr_t)d->dk | (uintptr_t)d->dv) % 16 == 0, "attention_bwd: tensors must be 16-byte aligned");
-    AttnSplits splits;
-    int64_t maxima_at, parts_at;
-    const int64_t need = 4 * attn_bwd_floats(p, d->dtype, splits, maxima_at, parts_at);
+    const AttnBwdSpace at = attn_bwd_plan(p, d->dtype);
+    const int64_t need = 4 * at.end;
     N3D_CHECK(d->workspace && d->workspace_bytes >= need && (uintptr_t)d->workspace % 16 == 0, "attention_bwd: a workspace of %lld bytes is needed (16-byte aligned)", (long long)need);
     float* ws = (float*)d->workspace;
     p.dout = d->dout; p.dq = d->dq; p.dk = d->dk; p.dv = d->dv;
-    p.delta = ws + (attn_range_floats(p) + 3) / 4 * 4;
-    p.maxima = d->dtype == N3D_F16 ? ws + maxima_at : nullptr;
-    p.part = ws + parts_at;
+    p.delta = ws + at.delta;
+    p.maxima = d->dtype == N3D_F16 ? ws + at.maxima : nullptr;
+    p.part = ws + at.part;
+    p.k_part = ws + at.k_part;
     const double pairs = (double)p.B * p.Hq * p.Lq * p.Lk * p.D;
     N3dProfScope prof(N3D_K_ATTENTION, stream, 10.0 * pairs, 8.0 * ((double)p.B * p.Lq * p.Hq * p.D + (double)p.B * p.Lk * p.Hk * p.D));
     attn_ranges(p, ws, stream);
     attn_dispatch(d->dtype, p, [&](auto* t, auto db, auto mode, auto docs) {
-        attn_bwd_launch<std::remove_pointer_t<decltype(t)>, db.value, mode.value, docs.value>(p, splits, stream);
+        attn_bwd_launch<std::remove_pointer_t<decltype(t)>, db.value, mode.value, docs.value>(p, stream);
     });
     N3D_LAUNCH_CHECK();
     return 0;
