@@ -341,33 +341,31 @@ static inline const char* attn_params(const n3d_attention_desc* d, AttnParams& p
 // How a score comes out of the raw product: a positive multiple of it; any multiple and a distance; a cap; a cap and a distance.  Each is straight code of
 // its own in the kernels: values that pass through a branch in place cost a register copy each, and no product is scheduled across it.
 enum { ATTN_PLAIN = 0, ATTN_BIAS = 1, ATTN_CAP = 2, ATTN_CAP_BIAS = 3 };
-// f(element type, 32-channel blocks, mode, documents)
+// f(32-channel blocks, mode, documents), as integral constants
 template <typename F>
-static inline void attn_dispatch(int dtype, const AttnParams& p, F&& f) {
-    auto doc = [&](auto* t, auto db, auto mode) {
-        if (p.kdoc) f(t, db, mode, std::true_type());
-        else f(t, db, mode, std::false_type());
+static inline void attn_forms(const AttnParams& p, F&& f) {
+    auto doc = [&](auto db, auto mode) {
+        if (p.kdoc) f(db, mode, std::true_type());
+        else f(db, mode, std::false_type());
     };
-    auto form = [&](auto* t, auto db) {
+    auto form = [&](auto db) {
         if (p.softcap > 0.f) {
-            if (p.slopes) doc(t, db, std::integral_constant<int, ATTN_CAP_BIAS>());
-            else doc(t, db, std::integral_constant<int, ATTN_CAP>());
+            if (p.slopes) doc(db, std::integral_constant<int, ATTN_CAP_BIAS>());
+            else doc(db, std::integral_constant<int, ATTN_CAP>());
         } else {
-            if (p.slopes || !(p.scale > 0.f)) doc(t, db, std::integral_constant<int, ATTN_BIAS>());
-            else doc(t, db, std::integral_constant<int, ATTN_PLAIN>());
+            if (p.slopes || !(p.scale > 0.f)) doc(db, std::integral_constant<int, ATTN_BIAS>());
+            else doc(db, std::integral_constant<int, ATTN_PLAIN>());
         }
     };
-    auto typed = [&](auto* t) {
-        switch (cdiv(p.D, 32)) {
-            case 1: form(t, std::integral_constant<int, 1>()); break;
-            case 2: form(t, std::integral_constant<int, 2>()); break;
-            case 3: form(t, std::integral_constant<int, 3>()); break;
-            default: form(t, std::integral_constant<int, 4>()); break;
-        }
-    };
-    if (dtype == N3D_F16) typed((_Float16*)nullptr);
-    else typed((__bf16*)nullptr);
+    switch (cdiv(p.D, 32)) {
+        case 1: form(std::integral_constant<int, 1>()); break;
+        case 2: form(std::integral_constant<int, 2>()); break;
+        case 3: form(std::integral_constant<int, 3>()); break;
+        default: form(std::integral_constant<int, 4>()); break;
+    }
 }
+
+static constexpr int ATTN_MAXIMA = 1024;             // partial maxima of |do|, and as many of |v| (attn_prep_kernel: its workgroups)
 
 // workspace, in floats: the document ranges come first
 static inline int64_t attn_range_floats(const AttnParams& p) { return p.kdoc ? 2 * (int64_t)p.B * (p.nkt + p.nqt) + (int64_t)p.B * cdiv(p.Lq, 128) : 0; }

@@ -1,0 +1,680 @@
+// Attention, backward (attention.h):  P = exp2(u - lse),  dP = do v^T,  delta = sum(do o),  dt = P (dP - delta),  ds = dt (1 - tanh^2),
+//   dq = scale ds k,   dk = scale ds^T q,   dv = P^T do,   dk and dv summed over the query heads of a key head.
+// attn_prep_kernel: delta, and for float16 the largest |do| and |v| (attn_ds_scale).
+// attn_dq_kernel: a workgroup owns 128 queries of a head and walks the keys;  attn_dkv_kernel: a workgroup owns 128 keys of a key head and walks the
+// queries of all its heads.  Scores are computed in both (7 products for 5) so that every sum has one owner: no atomics, the same bits every time.
+#pragma once
+#include "attention.h"
+
+// float16 has 5 exponent bits, and P ~ 1 / length and ds ~ P do v leave its range on long rows or with small gradients.  The dk / dv kernel therefore uses
+// P 2^12, and both kernels ds times a power of two taken from the largest |do| and |v| of the call, so that no ds can overflow:
+// |ds| <= |dP - delta| <= 2 D max|do| max|v|.  The accumulators undo both.  bfloat16 has float32's exponents: neither is needed.
+template <typename T> static constexpr float ATTN_P_SHIFT = std::is_same<T, _Float16>::value ? 12.f : 0.f;
+
+template <typename T>
+__global__ __launch_bounds__(256) void attn_prep_kernel(AttnParams p) {
+    // 16 lanes a row, 8 channels a lane
+    const int lane16 = threadIdx.x & 15, D = p.D;
+    float top = 0.f;
+    if (blockIdx.y == 0) {
+        const uint32_t rows = (uint32_t)p.B * p.Lq * p.Hq;                // (below 2^31: n3d_attention_bwd)
+        for (uint32_t w = blockIdx.x * 16 + (threadIdx.x >> 4); w < rows; w += gridDim.x * 16) {
+            const uint32_t bi = w / p.Hq;
+            const int h = w - bi * p.Hq, b = bi / p.Lq, i = bi - b * p.Lq;
+            const int64_t stat = ((int64_t)b * p.Hq + h) * p.Lq + i;
+            float s = 0.f;
+            const bool live = p.lse[stat] != -INFINITY;
+            if (lane16 * 8 < D) {
+                const auto x = *reinterpret_cast<const typename AttnVec<T>::x8*>((const T*)p.dout + b * p.ds[0] + i * p.ds[1] + h * p.ds[2] + lane16 * 8);
+                const auto y = *reinterpret_cast<const typename AttnVec<T>::x8*>((const T*)p.o + (int64_t)w * D + lane16 * 8);
+                typename AttnVec<T>::x8 z = {};
+                if (p.rest) z = *reinterpret_cast<const typename AttnVec<T>::x8*>((const T*)p.rest + (int64_t)w * D + lane16 * 8);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    s += (float)x[e] * ((float)y[e] + (float)z[e]);
+                    const float a = fabsf((float)x[e]);
+                    if (live && a < INFINITY) top = fmaxf(top, a);
+                }
+            }
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o);
+            if (lane16 == 0) p.delta[stat] = s;
+        }
+    } else {
+        const uint32_t rows = (uint32_t)p.B * p.Lk * p.Hk;
+        for (uint32_t w = blockIdx.x * 16 + (threadIdx.x >> 4); w < rows; w += gridDim.x * 16) {
+            const uint32_t bj = w / p.Hk;
+            const int h = w - bj * p.Hk, b = bj / p.Lk, j = bj - b * p.Lk;
+            if (j >= attn_keys(p, b) || (p.kdoc && p.kdoc[b * p.kdoc_stride + j] < 0) || lane16 * 8 >= D) continue;
+            const auto x = *reinterpret_cast<const typename AttnVec<T>::x8*>((const T*)p.v + b * p.vs[0] + j * p.vs[1] + h * p.vs[2] + lane16 * 8);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float a = fabsf((float)x[e]);
+                if (a < INFINITY) top = fmaxf(top, a);
+            }
+        }
+    }
+    if (!p.maxima) return;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    __shared__ float tops[4];
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) ((float*)p.maxima)[blockIdx.y * ATTN_MAXIMA + blockIdx.x] = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+}
+
+// the exponent of ds's factor (0 without maxima); every wave computes it for itself
+__device__ __forceinline__ int attn_ds_scale(const AttnParams& p, int lane) {
+    if (!p.maxima) return 0;
+    float a = 0.f, c = 0.f;
+#pragma unroll
+    for (int i = 0; i < ATTN_MAXIMA / 64; ++i) {
+        a = fmaxf(a, p.maxima[i * 64 + lane]);
+        c = fmaxf(c, p.maxima[ATTN_MAXIMA + i * 64 + lane]);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        a = fmaxf(a, __shfl_xor(a, o));
+        c = fmaxf(c, __shfl_xor(c, o));
+    }
+    if (a == 0.f || c == 0.f) return 0;
+    // 2 D <= 2^8 and a < 2^(ilogb a + 1): ds 2^e < 2^15
+    const int e = 15 - 8 - (ilogbf(a) + 1) - (ilogbf(c) + 1);
+    return attn_uniform(e);
+}
+
+// Raw score and dP of one element -> P 2^shift and ds 2^e (ds_by 1 where T needs no scaling: no multiplication then)
+template <typename T, int MODE>
+__device__ __forceinline__ void attn_ds(f32x16& S, f32x16& dP, int r, const AttnScore& f, float ds_by, float lse2, float delta, float dist) {
+    float u, d = dP[r] - delta;
+    if constexpr (MODE == ATTN_CAP || MODE == ATTN_CAP_BIAS) {
+        const float x = f.cap_r(S[r]);
+        u = f.capped(x, lse2);
+        d *= __builtin_fmaf(-x, x, x);                       // a quarter of 1 - tanh^2: attn_ds_unit
+    } else {
+        u = __builtin_fmaf(S[r], f.mul, -lse2);
+    }
+    if constexpr (MODE == ATTN_BIAS || MODE == ATTN_CAP_BIAS) u -= f.slope * fabsf(dist);
+    S[r] = __builtin_amdgcn_exp2f(u);
+    if constexpr (ATTN_P_SHIFT<T> != 0.f) d *= ds_by;
+    dP[r] = S[r] * d;
+}
+template <int MODE> static constexpr float attn_ds_unit() { return MODE == ATTN_CAP || MODE == ATTN_CAP_BIAS ? 4.f : 1.f; }
+
+template <typename T>
+__device__ __forceinline__ void attn_pack(const f32x16& x, typename AttnVec<T>::x8 (&out)[2]) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) out[c][e] = (T)x[8 * c + e];
+}
+
+// P and ds / scale of one (query, key) pair, plain arithmetic
+template <typename T>
+__device__ __forceinline__ void attn_pair(const AttnParams& p, const AttnScore& f, const T* q, const T* k, const T* v, const T* dout, float lse2, float delta, int dist,
+                                          float& w, float& ds) {
+    const float s = attn_dot<T>(q, k, p.D);
+    const float x = f.cap_out > 0.f ? f.cap_r(s) : 0.5f;
+    w = __builtin_amdgcn_exp2f(attn_score(f, s, dist) - lse2);
+    ds = w * (attn_dot<T>(dout, v, p.D) - delta) * 4.f * (x - x * x);
+}
+__device__ __forceinline__ float attn_lse2(float lse) { return lse == -INFINITY ? INFINITY : lse * ATTN_LOG2E; }       // (a row that sees nothing: every weight 0)
+
+template <int DB> static constexpr bool attn_dkv_pair() { return DB > 3; }      // (see attn_dkv)
+// what both kinds of workgroups keep in the LDS
+template <int DB> static constexpr int attn_row() { return DB > 2 ? 128 : 64; }
+template <int DB> static constexpr int attn_lds_bytes() { return 4 * ATTN_TILE * attn_row<DB>() * 2; }
+struct AttnRows {
+    float lse[2][ATTN_TILE], delta[2][ATTN_TILE];
+};
+
+#ifdef __HIP_DEVICE_COMPILE__                            // (hipcc drops the launch stub of a template whose body its host pass cannot read)
+template <typename T, int DB, int MODE, bool DOCS>
+__device__ __forceinline__ void attn_dq(const AttnParams& p, int group, char* smem, int (*sdoc)[ATTN_TILE]) {
+    constexpr int ROW = attn_row<DB>(), TILE_BYTES = ATTN_TILE * ROW * 2;
+    const int wave = attn_uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
+    // p.splits > 1: the keys in that many runs of whole tiles, float32 parts that attn_parts_kernel adds in order
+    const int total = p.B * p.Hq * p.row_blocks * p.splits, per = (total + 7) / 8;
+    const int id = (group & 7) * per + (group >> 3);
+    if (group >> 3 >= per || id >= total) return;
+    const int split = id % p.splits, pos = id / p.splits % p.row_blocks, bh = id / p.splits / p.row_blocks, h = bh % p.Hq, b = bh / p.Hq, hk = h / p.G;
+    const int blk = DOCS && p.order ? p.order[b * p.row_blocks + pos] : p.row_blocks - 1 - pos;
+    const int n = attn_keys(p, b), prefix = p.prefix ? p.prefix[b] : 0, q0 = blk * 128;
+    const int i = q0 + 32 * wave + l31;
+    const bool row_ok = i < p.Lq;
+    const int qdoc = DOCS && row_ok ? p.qdoc[b * p.qdoc_stride + i] : 0;
+    const int lim = !row_ok || qdoc < 0 ? -1 : attn_limit(p, i, n, prefix);
+    const int lim_last = attn_limit(p, min(q0 + 32 * wave + 31, p.Lq - 1), n, prefix);
+    const int key_end = attn_limit(p, min(q0 + 127, p.Lq - 1), n, prefix) + 1;
+    int dlo = 0, dhi = 0;
+    if constexpr (DOCS) {
+        const int2* r = p.qtiles + (int64_t)b * p.nqt + 2 * blk;
+        const int2 r0 = r[0], r1 = 2 * blk + 1 < p.nqt ? r[1] : r[0];
+        dlo = min(r0.x, r1.x);
+        dhi = max(r0.y, r1.y);
+    }
+    AttnTiles<DOCS> tiles;
+    const int run = (p.nkt + p.splits - 1) / p.splits, run_first = split * run, run_end = min((key_end + ATTN_TILE - 1) / ATTN_TILE, run_first + run);
+    tiles.start(DOCS ? p.ktiles + (int64_t)b * p.nkt : nullptr, run_first, run_end, max(dlo, 0), dhi);
+    typename AttnVec<T>::x8 qf[2 * DB], df[2 * DB];
+    const T* q = row_ok ? (const T*)p.q + b * p.qs[0] + i * p.qs[1] + h * p.qs[2] : nullptr;
+    const T* dout = row_ok ? (const T*)p.dout + b * p.ds[0] + i * p.ds[1] + h * p.ds[2] : nullptr;
+#pragma unroll
+    for (int c = 0; c < 2 * DB; ++c) {
+        qf[c] = attn_lane_frag<T>(q, 2 * c + half, p.D);
+        df[c] = attn_lane_frag<T>(dout, 2 * c + half, p.D);
+    }
+    const int64_t stat = ((int64_t)b * p.Hq + h) * p.Lq + i;
+    const float lse2 = row_ok ? attn_lse2(p.lse[stat]) : INFINITY, delta = row_ok ? p.delta[stat] : 0.f;
+    const T* k = (const T*)p.k + b * p.ks[0] + hk * p.ks[2];
+    const T* v = (const T*)p.v + b * p.vs[0] + hk * p.vs[2];
+    const int* kdoc = DOCS ? p.kdoc + b * p.kdoc_stride : nullptr;
+    const AttnScore f(p, h);
+    const int ds_exp = attn_ds_scale(p, lane);
+    const float ds_by = ldexpf(1.f, ds_exp);
+    AttnStage<ROW, ATTN_TILE, 4> sk, sv;
+    sk.setup(wave, lane, p.ks[1], p.D);
+    sv.setup(wave, lane, p.vs[1], p.D);
+    f32x16 acc[DB] = {};
+    const uint64_t k_at = attn_addr(k), v_at = attn_addr(v);
+    const int k_row = (int)p.ks[1], v_row = (int)p.vs[1];
+    const AttnLane<ROW> at_lane(lane);
+    const uint32_t lds = attn_lds(smem);
+    int doc_next = 0;                                                   // of the tile being staged: loaded ahead of its pieces, written behind the products
+    auto stage = [&](int t, int buf) {
+        const uint32_t at = lds + buf * 2 * TILE_BYTES;
+        if (DOCS && wave == 0) doc_next = kdoc[min(t * ATTN_TILE + lane, p.Lk - 1)];
+        sk.issue(k_at, t, n, k_row, p.D, at, wave);
+        sv.issue(v_at, t, n, v_row, p.D, at + TILE_BYTES, wave);
+    };
+    int t = tiles.next(lane), buf = 0;
+    if (t >= 0) stage(t, 0);
+    if (DOCS && wave == 0) sdoc[0][lane] = doc_next;
+    // every key of tile t visible to every query of the workgroup
+    const int full_end = DOCS && dlo != dhi ? 0 : attn_limit(p, q0, n, prefix) + 1;
+    auto full = [&] { return (t + 1) * ATTN_TILE <= full_end && (!DOCS || ((tiles.low == dlo) & (tiles.high == dlo))); };
+    auto visit = [&](auto mask) {
+        const int j0 = t * ATTN_TILE, now = buf;
+        attn_sync();
+        t = tiles.next(lane);
+        buf ^= 1;
+        if (t >= 0) stage(t, buf);
+        if (!mask.value || j0 <= lim_last) {
+            const uint32_t k_lds = at_lane.rows(lds + now * 2 * TILE_BYTES), v_lds = at_lane.rows(lds + now * 2 * TILE_BYTES + TILE_BYTES);
+            const uint32_t kc_lds = at_lane.cols(lds + now * 2 * TILE_BYTES);
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                typename AttnVec<T>::x8 kf[2 * DB], vf[2 * DB], cf[DB][2], d[2];
+#pragma unroll
+                for (int c = 0; c < 2 * DB; ++c) kf[c] = attn_row_frag<T, ROW>(k_lds, kb, c);
+                // (values behind the first products where registers are short: half of the keys' are free again by then)
+                constexpr int FIRST = DB > 2 ? DB : 0;
+                f32x16 S = {}, dP = {};
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int c = 0; c < FIRST; ++c) S = attn_mfma(kf[c], qf[c], S);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int c = 0; c < 2 * DB; ++c) vf[c] = attn_row_frag<T, ROW>(v_lds, kb, c);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int c = FIRST; c < 2 * DB; ++c) S = attn_mfma(kf[c], qf[c], S);
+#pragma unroll
+                for (int c = 0; c < 2 * DB; ++c) dP = attn_mfma(vf[c], df[c], dP);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int db = 0; db < DB; ++db)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) cf[db][c] = attn_col_frag<T, ROW>(kc_lds, 2 * kb + c, db);
+                __builtin_amdgcn_sched_barrier(0);
+                const int jb = j0 + 32 * kb + 4 * half;
+                const float dist = (float)(i + n - p.Lq - jb);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) attn_ds<T, MODE>(S, dP, r, f, ds_by, lse2, delta, dist - (float)(8 * (r >> 2) + (r & 3)));
+                if constexpr (mask.value) {
+                    const int last = lim - jb;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) dP[r] = 8 * (r >> 2) + (r & 3) <= last ? dP[r] : 0.f;
+                    if constexpr (DOCS)
+#pragma unroll
+                        for (int a = 0; a < 4; ++a) {
+                            const int4 o = *reinterpret_cast<const int4*>(&sdoc[now][32 * kb + 8 * a + 4 * half]);
+                            dP[4 * a] = o.x == qdoc ? dP[4 * a] : 0.f;
+                            dP[4 * a + 1] = o.y == qdoc ? dP[4 * a + 1] : 0.f;
+                            dP[4 * a + 2] = o.z == qdoc ? dP[4 * a + 2] : 0.f;
+                            dP[4 * a + 3] = o.w == qdoc ? dP[4 * a + 3] : 0.f;
+                        }
+                }
+                attn_pack<T>(dP, d);
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) acc[db] = attn_mfma(cf[db][c], d[c], acc[db]);
+            }
+        }
+        if (DOCS && wave == 0) sdoc[buf][lane] = doc_next;
+    };
+    while (t >= 0) {
+        while (t >= 0 && full()) visit(std::false_type());
+        while (t >= 0 && !full()) visit(std::true_type());
+    }
+    bool nan = false;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) nan = nan || acc[db][r] != acc[db][r];
+    uint64_t redo = __ballot(nan && row_ok && lse2 == lse2);
+    redo = (redo | (redo >> 32)) & 0xffffffffu;
+    const float by = ldexpf(p.scale * attn_ds_unit<MODE>(), -ds_exp);
+    const int64_t row_at = ((int64_t)(b * (int64_t)p.Lq + i) * p.Hq + h) * p.D, all = (int64_t)p.B * p.Lq * p.Hq * p.D;
+    const bool store = row_ok && !((redo >> l31) & 1);
+    if (p.splits > 1) attn_store_part<DB>(p.part + split * all + row_at, acc, by, half, p.D, store);
+    else attn_store_row<T, DB>((T*)p.dq + row_at, acc, by, half, p.D, store);
+    while (redo) {                                                      // a NaN behind the mask may have come in through 0 * NaN: these rows key by key
+        const int e = __builtin_ctzll(redo);
+        redo &= redo - 1;
+        const int ie = q0 + 32 * wave + e, lime = __shfl(lim, e), doce = __shfl(qdoc, e);
+        const float le = __shfl(lse2, e), de = __shfl(delta, e);
+        const T* qe = (const T*)p.q + b * p.qs[0] + ie * p.qs[1] + h * p.qs[2];
+        const T* doe = (const T*)p.dout + b * p.ds[0] + ie * p.ds[1] + h * p.ds[2];
+        float x[2] = {0.f, 0.f};
+        const int last = min(lime, run_end * ATTN_TILE - 1);
+        for (int j0 = run_first * ATTN_TILE; j0 <= last; j0 += 64) {
+            const int j = j0 + lane;
+            const bool see = j <= last && attn_visible(p, b, j, lime, doce);
+            float w, ds = 0.f;
+            if (see) attn_pair<T>(p, f, qe, k + j * p.ks[1], v + j * p.vs[1], doe, le, de, ie + n - p.Lq - j, w, ds);
+            uint64_t todo = __ballot(see);
+            while (todo) {
+                const int s = __builtin_ctzll(todo);
+                todo &= todo - 1;
+                const float d = __shfl(ds, s);
+                const T* kj = k + (int64_t)(j0 + s) * p.ks[1];
+                if (lane < p.D) x[0] += d * (float)kj[lane];
+                if (lane + 64 < p.D) x[1] += d * (float)kj[lane + 64];
+            }
+        }
+        const int64_t at = ((int64_t)(b * (int64_t)p.Lq + ie) * p.Hq + h) * p.D;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int d = lane + 64 * c;
+            if (d >= p.D) continue;
+            if (p.splits > 1) p.part[split * all + at + d] = x[c] * p.scale;
+            else ((T*)p.dq)[at + d] = (T)(x[c] * p.scale);
+        }
+    }
+}
+
+// A wave owns 32 keys: their K and V as operands and their dk and dv as accumulators.  Beyond 96 channels that is more than half of a SIMD's registers, so
+// one wave a SIMD, whose vector work and products would wait for each other (537 us at 2 x 4096 x 16 heads x 128, causal with caps; two loops interleaved by
+// hand: 555).  There two waves share 32 keys (attn_dkv_pair): each takes the scores of half of a tile's queries, they trade the 16-bit weights through the
+// LDS, and each adds up half of the channels over all of the queries.
+template <typename T, int DB, int MODE, bool DOCS>
+__device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* smem, AttnRows& rows, int (*sdoc)[ATTN_TILE], char* traded) {
+    constexpr int ROW = attn_row<DB>(), TILE_BYTES = ATTN_TILE * ROW * 2;
+    constexpr float SHIFT = ATTN_P_SHIFT<T>;
+    constexpr bool PAIR = attn_dkv_pair<DB>();
+    constexpr int NB = PAIR ? DB / 2 : DB;                              // blocks of 32 channels a wave adds up
+    typedef typename AttnVec<T>::x8 frag;
+    // smem: [buffer][q, do];  traded (pairs): [key group][half of the queries][w, w, d, d][lane] fragments
+    const int wave = attn_uniform(threadIdx.x >> 6), keys = PAIR ? wave & 3 : wave, part = PAIR ? wave >> 2 : 0, lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
+    // p.k_splits: 1 (a workgroup adds up all heads of the group), or float32 parts that attn_parts_kernel adds in order: the heads of the group in
+    // p.k_splits / p.chunks equal runs, the queries in p.chunks runs of whole tiles
+    const int total = p.B * p.Hk * p.k_splits * p.k_blocks, per = (total + 7) / 8;
+    const int id = (group & 7) * per + (group >> 3);
+    if (group >> 3 >= per || id >= total) return;
+    const int blk = id % p.k_blocks, split = id / p.k_blocks % p.k_splits, bh = id / p.k_blocks / p.k_splits, hk = bh % p.Hk, b = bh / p.Hk;
+    const int heads = p.G * p.chunks / p.k_splits, g0 = split / p.chunks * heads, g1 = g0 + heads;
+    const int n = attn_keys(p, b), prefix = p.prefix ? p.prefix[b] : 0, k0 = blk * 128, off = n - p.Lq;
+    const int j = k0 + 32 * keys + l31;
+    const int kdoc = DOCS && j < p.Lk ? p.kdoc[b * p.kdoc_stride + j] : 0;
+    const bool key_ok = j < n && kdoc >= 0;
+    // first query that sees key x
+    auto first_query = [&](int x) { return !p.causal || x < prefix ? 0 : max(x - off, 0); };
+    const int qmin = key_ok ? first_query(j) : 0x7fffffff;
+    const int wave_first = first_query(k0 + 32 * keys);
+    const bool wave_on = k0 + 32 * keys < n;
+    int dlo = 0, dhi = 0;
+    if constexpr (DOCS) {
+        const int2* r = p.ktiles + (int64_t)b * p.nkt + 2 * blk;
+        const int2 r0 = r[0], r1 = 2 * blk + 1 < p.nkt ? r[1] : r[0];
+        dlo = min(r0.x, r1.x);
+        dhi = max(r0.y, r1.y);
+    }
+    const int2* ranges = DOCS ? p.qtiles + (int64_t)b * p.nqt : nullptr;
+    const int run = (p.nqt + p.chunks - 1) / p.chunks, run_first = split % p.chunks * run, run_end = min(p.nqt, run_first + run);
+    const int t_first = max(first_query(k0) / ATTN_TILE, run_first), t_end = k0 < n ? run_end : 0;
+    AttnTiles<DOCS> tiles;
+    int g = g0;
+    tiles.start(ranges, t_first, t_end, max(dlo, 0), dhi);
+    auto next = [&](int& gn) {
+        int t = tiles.next(lane);
+        while (t < 0 && gn + 1 < g1) {
+            ++gn;
+            tiles.start(ranges, t_first, t_end, max(dlo, 0), dhi);
+            t = tiles.next(lane);
+        }
+        return t;
+    };
+    frag kf[2 * DB], vf[2 * DB];
+    const T* k = j < n ? (const T*)p.k + b * p.ks[0] + j * p.ks[1] + hk * p.ks[2] : nullptr;
+    const T* v = j < n ? (const T*)p.v + b * p.vs[0] + j * p.vs[1] + hk * p.vs[2] : nullptr;
+#pragma unroll
+    for (int c = 0; c < 2 * DB; ++c) {
+        kf[c] = attn_lane_frag<T>(k, 2 * c + half, p.D);
+        vf[c] = attn_lane_frag<T>(v, 2 * c + half, p.D);
+    }
+    AttnStage<ROW, ATTN_TILE, PAIR ? 8 : 4> sq, sd;
+    sq.setup(wave, lane, p.qs[1], p.D);
+    sd.setup(wave, lane, p.ds[1], p.D);
+    const int ds_exp = attn_ds_scale(p, lane);
+    const float ds_by = ldexpf(1.f, ds_exp - (int)SHIFT);
+    const AttnLane<ROW> at_lane(lane);
+    const uint32_t lds = attn_lds(smem);
+    float row_next = 0.f;
+    auto stage = [&](int t, int gt, int buf) {
+        const int h = hk * p.G + gt, i0 = t * ATTN_TILE;
+        const uint32_t at = lds + buf * 2 * TILE_BYTES;
+        // the rows' statistics: loaded ahead of the pieces (one of the three a wave), written to the LDS behind the products of the tile before
+        const int i = i0 + lane;
+        const int64_t stat = ((int64_t)b * p.Hq + h) * p.Lq + i;
+        if (wave == 0) row_next = i < p.Lq ? attn_lse2(p.lse[stat]) - SHIFT : INFINITY;            // (queries behind the last: every weight 0)
+        if (wave == 1) row_next = i < p.Lq ? p.delta[stat] : 0.f;
+        if (DOCS && wave == 2) row_next = __builtin_bit_cast(float, i < p.Lq ? p.qdoc[b * p.qdoc_stride + i] : -1);
+        sq.issue(attn_addr((const T*)p.q + b * p.qs[0] + h * p.qs[2]), t, p.Lq, (int)p.qs[1], p.D, at, wave);
+        sd.issue(attn_addr((const T*)p.dout + b * p.ds[0] + h * p.ds[2]), t, p.Lq, (int)p.ds[1], p.D, at + TILE_BYTES, wave);
+    };
+    auto commit = [&](int buf) {
+        if (wave == 0) rows.lse[buf][lane] = row_next;
+        if (wave == 1) rows.delta[buf][lane] = row_next;
+        if (DOCS && wave == 2) sdoc[buf][lane] = __builtin_bit_cast(int, row_next);
+    };
+    f32x16 dk[NB] = {}, dv[NB] = {};
+    AttnScore f(p, hk * p.G);
+    int t = next(g), buf = 0;
+    if (t >= 0) stage(t, g, 0);
+    commit(0);
+    // every query of tile t sees every key of the workgroup (but those behind the last, whose lanes are not stored)
+    const int full_first = DOCS && dlo != dhi ? 0x7fffffff : first_query(min(k0 + 127, n - 1));
+    auto full = [&] { return t * ATTN_TILE >= full_first && (!DOCS || ((tiles.low == dlo) & (tiles.high == dlo))); };
+    auto visit = [&](auto mask) {
+        const int i0 = t * ATTN_TILE, now = buf;
+        const float slope = MODE != ATTN_PLAIN && p.slopes ? p.slopes[hk * p.G + g] * ATTN_LOG2E : 0.f;
+        attn_sync();
+        t = next(g);
+        buf ^= 1;
+        if (t >= 0) stage(t, g, buf);
+        const bool on = wave_on && (!mask.value || i0 + ATTN_TILE - 1 >= wave_first);
+        f.slope = slope;
+        constexpr int BLOCK = 32 * ROW * 2;                             // bytes of half a tile
+        const uint32_t tile = lds + now * 2 * TILE_BYTES;
+        // weights and dscores of the 32 queries of half a tile as second operands
+        auto weights = [&](int qb, frag (&w)[2], frag (&d)[2]) {
+            const uint32_t q_lds = at_lane.rows(tile + qb * BLOCK), d_lds = at_lane.rows(tile + TILE_BYTES + qb * BLOCK);
+            frag qf[2 * DB], df[2 * DB];
+            constexpr int FIRST = DB > 2 ? DB : 0;                      // (as in attn_dq_kernel)
+            f32x16 S = {}, dP = {};
+#pragma unroll
+            for (int c = 0; c < 2 * DB; ++c) qf[c] = attn_row_frag<T, ROW>(q_lds, 0, c);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int c = 0; c < FIRST; ++c) S = attn_mfma(qf[c], kf[c], S);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int c = 0; c < 2 * DB; ++c) df[c] = attn_row_frag<T, ROW>(d_lds, 0, c);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int c = FIRST; c < 2 * DB; ++c) S = attn_mfma(qf[c], kf[c], S);
+#pragma unroll
+            for (int c = 0; c < 2 * DB; ++c) dP = attn_mfma(df[c], vf[c], dP);
+            __builtin_amdgcn_sched_barrier(0);
+            const int ib = 32 * qb + 4 * half;
+            const float dist = (float)(i0 + ib + off - j);
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+                const float4 l4 = *reinterpret_cast<const float4*>(&rows.lse[now][ib + 8 * a]), e4 = *reinterpret_cast<const float4*>(&rows.delta[now][ib + 8 * a]);
+                const float l[4] = {l4.x, l4.y, l4.z, l4.w}, de[4] = {e4.x, e4.y, e4.z, e4.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) attn_ds<T, MODE>(S, dP, 4 * a + e, f, ds_by, l[e], de[e], dist + (float)(8 * a + e));
+            }
+            if constexpr (mask.value) {
+                const int first = qmin - i0 - ib;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const bool see = 8 * (r >> 2) + (r & 3) >= first;
+                    S[r] = see ? S[r] : 0.f;
+                    dP[r] = see ? dP[r] : 0.f;
+                }
+                if constexpr (DOCS)
+#pragma unroll
+                    for (int a = 0; a < 4; ++a) {
+                        const int4 o4 = *reinterpret_cast<const int4*>(&sdoc[now][ib + 8 * a]);
+                        const int o[4] = {o4.x, o4.y, o4.z, o4.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const bool see = o[e] == kdoc;
+                            S[4 * a + e] = see ? S[4 * a + e] : 0.f;
+                            dP[4 * a + e] = see ? dP[4 * a + e] : 0.f;
+                        }
+                    }
+            }
+            attn_pack<T>(S, w);
+            attn_pack<T>(dP, d);
+        };
+        // first operands of half a tile, this wave's channels
+        auto columns = [&](int qb, frag (&qc)[NB][2], frag (&dc)[NB][2]) {
+            const uint32_t qc_lds = at_lane.cols(tile + qb * BLOCK) ^ (part << 7), dc_lds = at_lane.cols(tile + TILE_BYTES + qb * BLOCK) ^ (part << 7);
+#pragma unroll
+            for (int db = 0; db < NB; ++db)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    dc[db][c] = attn_col_frag<T, ROW>(dc_lds, c, db);
+                    qc[db][c] = attn_col_frag<T, ROW>(qc_lds, c, db);
+                }
+        };
+        auto products = [&](const frag (&w)[2], const frag (&d)[2], const frag (&qc)[NB][2], const frag (&dc)[NB][2]) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int db = 0; db < NB; ++db) {
+                    dv[db] = attn_mfma(dc[db][c], w[c], dv[db]);
+                    dk[db] = attn_mfma(qc[db][c], d[c], dk[db]);
+                }
+        };
+        if constexpr (PAIR) {
+            frag w[2], d[2], qc[NB][2], dc[NB][2];
+            frag* mine = reinterpret_cast<frag*>(traded) + (keys * 2 + part) * 4 * 64 + lane;
+            const frag* theirs = reinterpret_cast<const frag*>(traded) + (keys * 2 + (part ^ 1)) * 4 * 64 + lane;
+            if (on) {
+                weights(part, w, d);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    mine[c * 64] = w[c];
+                    mine[(2 + c) * 64] = d[c];
+                }
+                columns(part, qc, dc);
+                products(w, d, qc, dc);
+            }
+            attn_traded();
+            if (on) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    w[c] = theirs[c * 64];
+                    d[c] = theirs[(2 + c) * 64];
+                }
+                columns(part ^ 1, qc, dc);
+                products(w, d, qc, dc);
+            }
+        } else if (on) {
+#pragma unroll
+            for (int qb = 0; qb < 2; ++qb) {
+                frag w[2], d[2], qc[NB][2], dc[NB][2];
+                weights(qb, w, d);
+                columns(qb, qc, dc);
+                products(w, d, qc, dc);
+            }
+        }
+        commit(buf);
+    };
+    while (t >= 0) {
+        while (t >= 0 && full()) visit(std::false_type());
+        while (t >= 0 && !full()) visit(std::true_type());
+    }
+    bool nan = false;
+#pragma unroll
+    for (int db = 0; db < NB; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) nan = nan || dk[db][r] != dk[db][r] || dv[db][r] != dv[db][r];
+    uint64_t redo = __ballot(nan && key_ok);
+    redo = (redo | (redo >> 32)) & 0xffffffffu;
+    const float k_by = ldexpf(p.scale * attn_ds_unit<MODE>(), -ds_exp), v_by = ldexpf(1.f, -(int)SHIFT);
+    const bool store = j < p.Lk && !((redo >> l31) & 1);
+    if (!key_ok)                                                        // keys that nobody sees (their lanes held something else)
+#pragma unroll
+        for (int db = 0; db < NB; ++db)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dk[db][r] = dv[db][r] = 0.f;
+    const int64_t row = ((int64_t)b * p.Lk + j) * p.Hk + hk, all = (int64_t)p.B * p.Lk * p.Hk;
+    if (p.k_splits > 1) {
+        float* pk = p.k_part + (2 * split * all + row) * p.D;
+        float* pv = p.k_part + ((2 * split + 1) * all + row) * p.D;
+        attn_store_part<NB>(pk + 64 * part, dk, k_by, half, p.D - 64 * part, store);
+        attn_store_part<NB>(pv + 64 * part, dv, v_by, half, p.D - 64 * part, store);
+    } else {
+        attn_store_row<T, NB>((T*)p.dk + row * p.D + 64 * part, dk, k_by, half, p.D - 64 * part, store);
+        attn_store_row<T, NB>((T*)p.dv + row * p.D + 64 * part, dv, v_by, half, p.D - 64 * part, store);
+    }
+    while (redo) {
+        const int e = __builtin_ctzll(redo);
+        redo &= redo - 1;
+        const int je = k0 + 32 * keys + e, doce = __shfl(kdoc, e);
+        const T* ke = (const T*)p.k + b * p.ks[0] + je * p.ks[1] + hk * p.ks[2];
+        const T* ve = (const T*)p.v + b * p.vs[0] + je * p.vs[1] + hk * p.vs[2];
+        float xk[2] = {0.f, 0.f}, xv[2] = {0.f, 0.f};
+        for (int ge = g0; ge < g1; ++ge) {
+            const int h = hk * p.G + ge;
+            const AttnScore f(p, h);
+            const T* q = (const T*)p.q + b * p.qs[0] + h * p.qs[2];
+            const T* dout = (const T*)p.dout + b * p.ds[0] + h * p.ds[2];
+            const int64_t stat = ((int64_t)b * p.Hq + h) * p.Lq;
+            const int end = min(p.Lq, run_end * ATTN_TILE);
+            for (int i0 = max(first_query(je), run_first * ATTN_TILE); i0 < end; i0 += 64) {
+                const int i = i0 + lane;
+                const bool see = i < end && (!p.kdoc || p.qdoc[b * p.qdoc_stride + i] == doce);
+                float w = 0.f, ds = 0.f;
+                if (see) attn_pair<T>(p, f, q + i * p.qs[1], ke, ve, dout + i * p.ds[1], attn_lse2(p.lse[stat + i]), p.delta[stat + i], i + off - je, w, ds);
+                uint64_t todo = __ballot(see);
+                while (todo) {
+                    const int s = __builtin_ctzll(todo);
+                    todo &= todo - 1;
+                    const float we = __shfl(w, s), de = __shfl(ds, s);
+                    const T* qi = q + (int64_t)(i0 + s) * p.qs[1];
+                    const T* di = dout + (int64_t)(i0 + s) * p.ds[1];
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+                        if (lane + 64 * c < p.D) {
+                            xk[c] += de * (float)qi[lane + 64 * c];
+                            xv[c] += we * (float)di[lane + 64 * c];
+                        }
+                }
+            }
+        }
+        const int64_t re = ((int64_t)b * p.Lk + je) * p.Hk + hk;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int d = lane + 64 * c;
+            if (d >= p.D || (PAIR && c != part)) continue;
+            if (p.k_splits > 1) {
+                p.k_part[(2 * split * all + re) * p.D + d] = xk[c] * p.scale;
+                p.k_part[((2 * split + 1) * all + re) * p.D + d] = xv[c];
+            } else {
+                ((T*)p.dk)[re * p.D + d] = (T)(xk[c] * p.scale);
+                ((T*)p.dv)[re * p.D + d] = (T)xv[c];
+            }
+        }
+    }
+}
+#endif
+
+template <typename T, int DB, int MODE, bool DOCS>
+__global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnParams p) {
+#ifdef __HIP_DEVICE_COMPILE__
+    __shared__ __align__(1024) char smem[attn_lds_bytes<DB>()];
+    __shared__ __align__(16) int sdoc[2][ATTN_TILE];
+    attn_dq<T, DB, MODE, DOCS>(p, blockIdx.x, smem, sdoc);
+#endif
+}
+template <typename T, int DB, int MODE, bool DOCS>
+__global__ __launch_bounds__(attn_dkv_pair<DB>() ? 512 : 256, 2) void attn_dkv_kernel(AttnParams p) {
+#ifdef __HIP_DEVICE_COMPILE__
+    __shared__ __align__(1024) char smem[attn_lds_bytes<DB>()];
+    __shared__ __align__(16) AttnRows rows;
+    __shared__ __align__(16) int sdoc[2][ATTN_TILE];
+    __shared__ __align__(16) char traded[attn_dkv_pair<DB>() ? 4 * 2 * 4 * 1024 : 16];
+    attn_dkv<T, DB, MODE, DOCS>(p, blockIdx.x, smem, rows, sdoc, traded);
+#endif
+}
+// Both in one launch where that is two rounds of the chip at most (1024 workgroups): small calls wait for single workgroups, and so for both kinds at once.
+// Training step of 3 x 1021 x 6 heads x 72, documents: 105 -> 91 us, 2 x 1200 x 8 heads on 2 x 72, causal with caps: 125 -> 100, 4096 x 16 x 64: 425 -> 424.
+// (Larger ones keep two launches: the dq workgroups alone need fewer registers, and more of them share a CU.)
+template <typename T, int DB, int MODE, bool DOCS>
+__global__ __launch_bounds__(256, 2) void attn_grads_kernel(AttnParams p) {
+#ifdef __HIP_DEVICE_COMPILE__
+    static_assert(!attn_dkv_pair<DB>(), "256 threads each");
+    __shared__ __align__(1024) char smem[attn_lds_bytes<DB>()];
+    __shared__ __align__(16) AttnRows rows;
+    __shared__ __align__(16) int sdoc[2][ATTN_TILE];
+    if ((int)blockIdx.x < p.first_k) attn_dq<T, DB, MODE, DOCS>(p, blockIdx.x, smem, sdoc);
+    else attn_dkv<T, DB, MODE, DOCS>(p, blockIdx.x - p.first_k, smem, rows, sdoc, nullptr);
+#endif
+}
+
+// part [split][output][elements] -> the outputs (one or two: gridDim.y), the splits in order; eight elements a thread
+template <typename T>
+__global__ __launch_bounds__(256) void attn_parts_kernel(const float* __restrict__ part, int splits, int64_t all, T* __restrict__ out0, T* __restrict__ out1) {
+    const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+    if (at >= all) return;
+    float x[8] = {};
+    for (int s = 0; s < splits; ++s) {
+        const float4* a = reinterpret_cast<const float4*>(part + (s * (int64_t)gridDim.y + blockIdx.y) * all + at);
+        const float4 u = a[0], w = a[1];
+        x[0] += u.x; x[1] += u.y; x[2] += u.z; x[3] += u.w;
+        x[4] += w.x; x[5] += w.y; x[6] += w.z; x[7] += w.w;
+    }
+    typename AttnVec<T>::x8 o;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] = (T)x[e];
+    *reinterpret_cast<typename AttnVec<T>::x8*>((blockIdx.y ? out1 : out0) + at) = o;
+}
+
+template <typename T, int DB, int MODE, bool DOCS>
+static void attn_bwd_launch(AttnParams& p, hipStream_t stream) {
+    const int64_t q_rows = (int64_t)p.B * p.Lq * p.Hq, k_rows = (int64_t)p.B * p.Lk * p.Hk;
+    const int prep = p.maxima ? ATTN_MAXIMA : (int)(cdiv64(q_rows, 16) < 2048 ? cdiv64(q_rows, 16) : 2048);
+    hipLaunchKernelGGL((attn_prep_kernel<T>), dim3(prep, p.maxima ? 2 : 1), dim3(256), 0, stream, p);
+    auto add = [&](const float* part, int count, int64_t all, void* a, void* b) {
+        if (count > 1) hipLaunchKernelGGL((attn_parts_kernel<T>), dim3((unsigned)cdiv64(all, 2048), b ? 2 : 1), dim3(256), 0, stream, part, count, all, (T*)a, (T*)b);
+    };
+    const int dq = p.dq ? 8 * cdiv(p.B * p.Hq * p.splits * p.row_blocks, 8) : 0, dkv = p.dk && p.Lk > 0 ? 8 * cdiv(p.B * p.Hk * p.k_splits * p.k_blocks, 8) : 0;
+    bool both = false;
+    if constexpr (!attn_dkv_pair<DB>()) {
+        if ((both = dq && dkv && dq + dkv <= 1024)) {
+            p.first_k = dq;
+            hipLaunchKernelGGL((attn_grads_kernel<T, DB, MODE, DOCS>), dim3(dq + dkv), dim3(256), 0, stream, p);
+        }
+    }
+    if (dq) {
+        if (!both) hipLaunchKernelGGL((attn_dq_kernel<T, DB, MODE, DOCS>), dim3(dq), dim3(256), 0, stream, p);
+        add(p.part, p.splits, q_rows * p.D, p.dq, nullptr);
+    }
+    if (dkv) {
+        if (!both) hipLaunchKernelGGL((attn_dkv_kernel<T, DB, MODE, DOCS>), dim3(dkv), dim3(attn_dkv_pair<DB>() ? 512 : 256), 0, stream, p);
+        add(p.k_part, p.k_splits, k_rows * p.D, p.dk, p.dv);
+    }
+}
+
+// the kernels of one element type, each in a file of its own (they take two minutes to compile)
+template <typename T>
+static void attn_bwd_typed(AttnParams& p, hipStream_t stream) {
+    attn_forms(p, [&](auto db, auto mode, auto docs) { attn_bwd_launch<T, db.value, mode.value, docs.value>(p, stream); });
+}

@@ -566,9 +566,8 @@ extern "C" int n3d_attention(const n3d_attention_desc* d, n3d_stream_t stream_) 
     if (!token) attn_ranges(p, d->workspace, stream);
     p.part = (float*)d->workspace + parts_at;
     hipError_t e = hipSuccess;
-    attn_dispatch(d->dtype, p, [&](auto* t, auto db, auto mode, auto docs) {
-        e = attn_fwd_launch<std::remove_pointer_t<decltype(t)>, db.value, mode.value, docs.value>(p, token, stream);
-    });
+    if (d->dtype == N3D_F16) attn_forms(p, [&](auto db, auto mode, auto docs) { e = attn_fwd_launch<_Float16, db.value, mode.value, docs.value>(p, token, stream); });
+    else attn_forms(p, [&](auto db, auto mode, auto docs) { e = attn_fwd_launch<__bf16, db.value, mode.value, docs.value>(p, token, stream); });
     N3D_CHECK(e == hipSuccess, "attention: %s", hipGetErrorString(e));
     N3D_LAUNCH_CHECK();
     return 0;
