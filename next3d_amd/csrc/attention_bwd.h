@@ -188,11 +188,12 @@ __device__ __forceinline__ void attn_dq(const AttnParams& p, int group, char* sm
         sv.issue(v_at, t, n, v_row, p.D, at + TILE_BYTES, wave);
     };
     int t = tiles.next(lane), buf = 0;
+    const bool fine = tiles.few();
     if (t >= 0) stage(t, 0);
     if (DOCS && wave == 0) sdoc[0][lane] = doc_next;
     // every key of tile t visible to every query of the workgroup
     const int full_end = DOCS && dlo != dhi ? 0 : attn_limit(p, q0, n, prefix) + 1;
-    auto full = [&] { return (t + 1) * ATTN_TILE <= full_end && (!DOCS || ((tiles.low == dlo) & (tiles.high == dlo))); };
+    auto full = [&] { return !fine && (t + 1) * ATTN_TILE <= full_end && (!DOCS || ((tiles.low == dlo) & (tiles.high == dlo))); };
     auto visit = [&](auto mask) {
         const int j0 = t * ATTN_TILE, now = buf;
         attn_sync();
@@ -250,6 +251,13 @@ __device__ __forceinline__ void attn_dq(const AttnParams& p, int group, char* sm
                 for (int c = 0; c < 2; ++c)
 #pragma unroll
                     for (int db = 0; db < DB; ++db) acc[db] = attn_mfma(cf[db][c], d[c], acc[db]);
+                if (mask.value && (DB < 4 || !DOCS) && fine)            // (attn_left_over, where registers are left for it)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const typename AttnVec<T>::x8 left = attn_left_over<T>(dP, d[c], c);
+#pragma unroll
+                        for (int db = 0; db < DB; ++db) acc[db] = attn_mfma(cf[db][c], left, acc[db]);
+                    }
             }
         }
         if (DOCS && wave == 0) sdoc[buf][lane] = doc_next;
@@ -315,6 +323,7 @@ __device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* s
     constexpr float SHIFT = ATTN_P_SHIFT<T>;
     constexpr bool PAIR = attn_dkv_pair<DB>();
     constexpr int NB = PAIR ? DB / 2 : DB;                              // blocks of 32 channels a wave adds up
+    constexpr bool LEFT = !PAIR && (DB < 3 || !DOCS);                   // attn_left_over, where registers are left for it
     typedef typename AttnVec<T>::x8 frag;
     // smem: [buffer][q, do];  traded (pairs): [key group][half of the queries][w, w, d, d][lane] fragments
     const int wave = attn_uniform(threadIdx.x >> 6), keys = PAIR ? wave & 3 : wave, part = PAIR ? wave >> 2 : 0, lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
@@ -392,11 +401,12 @@ __device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* s
     f32x16 dk[NB] = {}, dv[NB] = {};
     AttnScore f(p, hk * p.G);
     int t = next(g), buf = 0;
+    const bool fine = tiles.few();
     if (t >= 0) stage(t, g, 0);
     commit(0);
     // every query of tile t sees every key of the workgroup (but those behind the last, whose lanes are not stored)
     const int full_first = DOCS && dlo != dhi ? 0x7fffffff : first_query(min(k0 + 127, n - 1));
-    auto full = [&] { return t * ATTN_TILE >= full_first && (!DOCS || ((tiles.low == dlo) & (tiles.high == dlo))); };
+    auto full = [&] { return !fine && t * ATTN_TILE >= full_first && (!DOCS || ((tiles.low == dlo) & (tiles.high == dlo))); };
     auto visit = [&](auto mask) {
         const int i0 = t * ATTN_TILE, now = buf;
         const float slope = MODE != ATTN_PLAIN && p.slopes ? p.slopes[hk * p.G + g] * ATTN_LOG2E : 0.f;
@@ -409,7 +419,7 @@ __device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* s
         constexpr int BLOCK = 32 * ROW * 2;                             // bytes of half a tile
         const uint32_t tile = lds + now * 2 * TILE_BYTES;
         // weights and dscores of the 32 queries of half a tile as second operands
-        auto weights = [&](int qb, frag (&w)[2], frag (&d)[2]) {
+        auto weights = [&](int qb, frag (&w)[2], frag (&d)[2], frag (&left)[2]) {
             const uint32_t q_lds = at_lane.rows(tile + qb * BLOCK), d_lds = at_lane.rows(tile + TILE_BYTES + qb * BLOCK);
             frag qf[2 * DB], df[2 * DB];
             constexpr int FIRST = DB > 2 ? DB : 0;                      // (as in attn_dq_kernel)
@@ -460,6 +470,9 @@ __device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* s
             }
             attn_pack<T>(S, w);
             attn_pack<T>(dP, d);
+            if (mask.value && LEFT && fine)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) left[c] = attn_left_over<T>(dP, d[c], c);
         };
         // first operands of half a tile, this wave's channels
         auto columns = [&](int qb, frag (&qc)[NB][2], frag (&dc)[NB][2]) {
@@ -482,11 +495,11 @@ __device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* s
                 }
         };
         if constexpr (PAIR) {
-            frag w[2], d[2], qc[NB][2], dc[NB][2];
+            frag w[2], d[2], none[2], qc[NB][2], dc[NB][2];
             frag* mine = reinterpret_cast<frag*>(traded) + (keys * 2 + part) * 4 * 64 + lane;
             const frag* theirs = reinterpret_cast<const frag*>(traded) + (keys * 2 + (part ^ 1)) * 4 * 64 + lane;
             if (on) {
-                weights(part, w, d);
+                weights(part, w, d, none);
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     mine[c * 64] = w[c];
@@ -508,10 +521,15 @@ __device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* s
         } else if (on) {
 #pragma unroll
             for (int qb = 0; qb < 2; ++qb) {
-                frag w[2], d[2], qc[NB][2], dc[NB][2];
-                weights(qb, w, d);
+                frag w[2], d[2], left[2], qc[NB][2], dc[NB][2];
+                weights(qb, w, d, left);
                 columns(qb, qc, dc);
                 products(w, d, qc, dc);
+                if (mask.value && LEFT && fine)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int db = 0; db < NB; ++db) dk[db] = attn_mfma(qc[db][c], left[c], dk[db]);
             }
         }
         commit(buf);

@@ -221,11 +221,12 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnParams p) {
         sv.issue(v_at, t, n, v_row, p.D, lds + buf * 2 * TILE_BYTES + TILE_BYTES, wave);
     };
     int t = tiles.next(lane), buf = 0;
+    const bool fine = p.rest && tiles.few();
     if (t >= 0) stage(t, 0);
     if (DOCS && wave == 0) sdoc[0][lane] = doc_next;
     // every key of tile t visible to every query of the workgroup
     const int full_end = DOCS && dlo != dhi ? 0 : attn_limit(p, q0, n, prefix) + 1;
-    auto full = [&] { return (t + 1) * ATTN_TILE <= full_end && (!DOCS || ((tiles.low == dlo) & (tiles.high == dlo))); };
+    auto full = [&] { return !fine && (t + 1) * ATTN_TILE <= full_end && (!DOCS || ((tiles.low == dlo) & (tiles.high == dlo))); };
     auto visit = [&](auto mask) {
         const int j0 = t * ATTN_TILE, now = buf;
         attn_sync();
@@ -270,6 +271,17 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnParams p) {
                 for (int c = 0; c < 2; ++c)
 #pragma unroll
                     for (int db = 0; db < DB; ++db) acc[db] = attn_mfma(vf[db][kb][c], P[kb][c], acc[db]);
+            if constexpr (mask.value)
+                if (fine) {                                             // (attn_left_over)
+#pragma unroll
+                    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const typename AttnVec<T>::x8 left = attn_left_over<T>(S[kb], P[kb][c], c);
+#pragma unroll
+                            for (int db = 0; db < DB; ++db) acc[db] = attn_mfma(vf[db][kb][c], left, acc[db]);
+                        }
+                }
         }
         if (DOCS && wave == 0) sdoc[buf][lane] = doc_next;
     };
@@ -382,6 +394,13 @@ __global__ __launch_bounds__(256) void attn_token_kernel(AttnParams p) {
         for (int db = 0; db < DB; ++db)
 #pragma unroll
             for (int c = 0; c < 2; ++c) acc[db] = attn_mfma(attn_col_frag<T, ROW>(v_lds, c, db), P[0][c], acc[db]);
+        if (p.rest && lim_last < ATTN_FEW * ATTN_TILE)         // (attn_left_over)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const typename AttnVec<T>::x8 left = attn_left_over<T>(S[0], P[0][c], c);
+#pragma unroll
+                for (int db = 0; db < DB; ++db) acc[db] = attn_mfma(attn_col_frag<T, ROW>(v_lds, c, db), left, acc[db]);
+            }
         if (kdoc && lane < KEYS) sdoc[wave][buf ^ 1][lane] = doc_next;
     }
     // join the four waves: common maximum, then the accumulators through the LDS, one [32 rows][32 * DB + 1] float image a wave
