@@ -357,15 +357,18 @@ __global__ __launch_bounds__(1024) void ln_reduce_kernel(const float* __restrict
 }
 
 // Lanes per row and vectors per lane of a row of `nv` 16-byte vectors; f(LPR, K) as integral constants; false: a long row.
+// Two vectors a lane halve the shuffles, but a wave is kept to one row, or a workgroup of 256 to one, as long as its loads are enough.  Training step of
+// bfloat16 rows, against half / twice the lanes: 64 channels 247 us (4 x 2: 271), 256: 234 (32 x 1: 245), 512: 234 (64 x 1: 245), 1024: 228 (256 x 1: 411),
+// 2048: 247 (64 x 4: 333), 4096: 243 (512 x 1: 268), each of 1.2e8 elements.
 template <typename F>
 static bool ln_plan(int64_t nv, F&& f) {
 #define LN_CASE(limit, lpr, k) \
     if (nv <= (limit)) { f(std::integral_constant<int, lpr>(), std::integral_constant<int, k>()); return true; }
     LN_CASE(4, 4, 1)
     LN_CASE(8, 8, 1)
-    LN_CASE(16, 16, 1)
-    LN_CASE(32, 32, 1)
-    LN_CASE(64, 64, 1)
+    LN_CASE(16, 8, 2)
+    LN_CASE(32, 16, 2)
+    LN_CASE(64, 32, 2)
     LN_CASE(128, 64, 2)
     LN_CASE(256, 256, 1)
     LN_CASE(512, 256, 2)
@@ -375,10 +378,17 @@ static bool ln_plan(int64_t nv, F&& f) {
     return false;
 }
 
+// Workgroups of the backward pass, and rows of its partial column sums: 262144 threads in all.  16384 x 4096 bfloat16: 142 us with 1024 workgroups of 256, 183
+// with half and 157 with twice as many (a part is written and read again for every workgroup); 4000 x 8192: 101 with 512 of 512, 112 with 1024.
 static int ln_parts(int64_t rows, int64_t C, int dtype) {
     const int64_t nv = cdiv64(C, dtype == N3D_F32 ? 4 : 8);
     int64_t n = 0;
-    if (ln_plan(nv, [&](auto lpr, auto) { n = cdiv64(rows, ln_threads(lpr.value) / lpr.value); })) return (int)(n < 1024 ? n : 1024);
+    int64_t most = 0;
+    if (ln_plan(nv, [&](auto lpr, auto) {
+            n = cdiv64(rows, ln_threads(lpr.value) / lpr.value);
+            most = 1024 * 256 / ln_threads(lpr.value);
+        }))
+        return (int)(n < most ? n : most);
     return (int)(rows < 64 ? rows : 64);
 }
 
