@@ -211,7 +211,8 @@ __device__ __forceinline__ void attn_dq(const AttnParams& p, int group, char* sm
                 typename AttnVec<T>::x8 kf[2 * DB], vf[2 * DB], cf[DB][2], d[2];
 #pragma unroll
                 for (int c = 0; c < 2 * DB; ++c) kf[c] = attn_row_frag<T, ROW>(k_lds, kb, c);
-                // (values behind the first products where registers are short: half of the keys' are free again by then)
+                // (values behind the first products where registers are short: half of the keys' are free again by then.  Training step of 2 x 4096 x 16
+                // heads on 4 x 128, causal with caps: 929 us, with all ahead 939; documents 506 / 520)
                 constexpr int FIRST = DB > 2 ? DB : 0;
                 f32x16 S = {}, dP = {};
                 __builtin_amdgcn_sched_barrier(0);

@@ -239,9 +239,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnParams p) {
         if (t >= 0) stage(t, buf);
         if (!mask.value || j0 <= lim_last) {
             const uint32_t k_lds = at_lane.rows(lds + now * 2 * TILE_BYTES), v_lds = at_lane.cols(lds + now * 2 * TILE_BYTES + TILE_BYTES);
-            // every fragment is on its way before the first product that needs one: keys ahead of the scores, values (their first half, where registers
-            // are short) ahead of the softmax
-            constexpr int AHEAD = DB > 2 ? 1 : 2;
+            // every fragment is on its way before the first product that needs one: keys ahead of the scores, values ahead of the softmax
             typename AttnVec<T>::x8 kf[2][2 * DB], vf[DB][2][2], P[2][2];
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
@@ -257,17 +255,11 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnParams p) {
 #pragma unroll
             for (int db = 0; db < DB; ++db)
 #pragma unroll
-                for (int kb = 0; kb < AHEAD; ++kb)
+                for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                     for (int c = 0; c < 2; ++c) vf[db][kb][c] = attn_col_frag<T, ROW>(v_lds, 2 * kb + c, db);
             __builtin_amdgcn_sched_barrier(0);
             attn_softmax_form<T, 2, DB, MODE, mask.value>(S, P, acc, m, sum, f, lim, i + n - p.Lq, j0, half, DOCS ? sdoc[now] : nullptr, qdoc);
-#pragma unroll
-            for (int kb = AHEAD; kb < 2; ++kb)
-#pragma unroll
-                for (int c = 0; c < 2; ++c)
-#pragma unroll
-                    for (int db = 0; db < DB; ++db) vf[db][kb][c] = attn_col_frag<T, ROW>(v_lds, 2 * kb + c, db);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
