@@ -422,8 +422,19 @@ __device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* s
         f.slope = slope;
         constexpr int BLOCK = 32 * ROW * 2;                             // bytes of half a tile
         const uint32_t tile = lds + now * 2 * TILE_BYTES;
+        // first operands of half a tile, this wave's channels
+        auto columns = [&](int qb, frag (&qc)[NB][2], frag (&dc)[NB][2]) {
+            const uint32_t qc_lds = at_lane.cols(tile + qb * BLOCK) ^ (part << 7), dc_lds = at_lane.cols(tile + TILE_BYTES + qb * BLOCK) ^ (part << 7);
+#pragma unroll
+            for (int db = 0; db < NB; ++db)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    dc[db][c] = attn_col_frag<T, ROW>(dc_lds, c, db);
+                    qc[db][c] = attn_col_frag<T, ROW>(qc_lds, c, db);
+                }
+        };
         // weights and dscores of the 32 queries of half a tile as second operands
-        auto weights = [&](int qb, frag (&w)[2], frag (&d)[2], frag (&left)[2]) {
+        auto weights = [&](int qb, frag (&w)[2], frag (&d)[2], frag (&left)[2], auto&& ahead) {
             const uint32_t q_lds = at_lane.rows(tile + qb * BLOCK), d_lds = at_lane.rows(tile + TILE_BYTES + qb * BLOCK);
             frag qf[2 * DB], df[2 * DB];
             constexpr int FIRST = DB > 2 ? DB : 0;                      // (as in attn_dq_kernel)
@@ -441,6 +452,8 @@ __device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* s
             for (int c = FIRST; c < 2 * DB; ++c) S = attn_mfma(qf[c], kf[c], S);
 #pragma unroll
             for (int c = 0; c < 2 * DB; ++c) dP = attn_mfma(df[c], vf[c], dP);
+            __builtin_amdgcn_sched_barrier(0);
+            ahead();
             __builtin_amdgcn_sched_barrier(0);
             const int ib = 32 * qb + 4 * half;
             const float dist = (float)(i0 + ib + off - j);
@@ -478,17 +491,6 @@ __device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* s
 #pragma unroll
                 for (int c = 0; c < 2; ++c) left[c] = attn_left_over<T>(dP, d[c], c);
         };
-        // first operands of half a tile, this wave's channels
-        auto columns = [&](int qb, frag (&qc)[NB][2], frag (&dc)[NB][2]) {
-            const uint32_t qc_lds = at_lane.cols(tile + qb * BLOCK) ^ (part << 7), dc_lds = at_lane.cols(tile + TILE_BYTES + qb * BLOCK) ^ (part << 7);
-#pragma unroll
-            for (int db = 0; db < NB; ++db)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    dc[db][c] = attn_col_frag<T, ROW>(dc_lds, c, db);
-                    qc[db][c] = attn_col_frag<T, ROW>(qc_lds, c, db);
-                }
-        };
         auto products = [&](const frag (&w)[2], const frag (&d)[2], const frag (&qc)[NB][2], const frag (&dc)[NB][2]) {
 #pragma unroll
             for (int c = 0; c < 2; ++c)
@@ -503,14 +505,16 @@ __device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* s
             frag* mine = reinterpret_cast<frag*>(traded) + (keys * 2 + part) * 4 * 64 + lane;
             const frag* theirs = reinterpret_cast<const frag*>(traded) + (keys * 2 + (part ^ 1)) * 4 * 64 + lane;
             if (on) {
-                weights(part, w, d, none);
+                // (the products' fragments are on their way during the vector work, and the other half's during the wait: 932 -> 911 us for a training step of
+                // 2 x 4096 x 16 heads on 4 x 128, causal with caps.  The unpaired form lets two workgroups overlap instead: 458 us at x 64, with this 473)
+                weights(part, w, d, none, [&] { columns(part, qc, dc); });
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     mine[c * 64] = w[c];
                     mine[(2 + c) * 64] = d[c];
                 }
-                columns(part, qc, dc);
                 products(w, d, qc, dc);
+                columns(part ^ 1, qc, dc);
             }
             attn_traded();
             if (on) {
@@ -519,14 +523,13 @@ __device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* s
                     w[c] = theirs[c * 64];
                     d[c] = theirs[(2 + c) * 64];
                 }
-                columns(part ^ 1, qc, dc);
                 products(w, d, qc, dc);
             }
         } else if (on) {
 #pragma unroll
             for (int qb = 0; qb < 2; ++qb) {
                 frag w[2], d[2], left[2], qc[NB][2], dc[NB][2];
-                weights(qb, w, d, left);
+                weights(qb, w, d, left, [] {});
                 columns(qb, qc, dc);
                 products(w, d, qc, dc);
                 if (mask.value && LEFT && fine)
