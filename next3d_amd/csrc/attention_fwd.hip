@@ -12,7 +12,7 @@
 
 // lowest and highest document of every ATTN_TILE tokens
 __global__ __launch_bounds__(256) void attn_ranges_kernel(const int* __restrict__ doc, int64_t stride, int L, int tiles, int2* __restrict__ out) {
-    const int t = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, b = blockIdx.y;
+    const int groups = (tiles + 3) / 4, b = blockIdx.x / groups, t = (blockIdx.x - b * groups) * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (t >= tiles) return;
     const int j = t * ATTN_TILE + lane;
     const int d = doc[b * stride + (j < L ? j : L - 1)];
@@ -501,9 +501,9 @@ void attn_ranges(AttnParams& p, void* workspace, hipStream_t stream) {
     if (!p.kdoc) return;
     int2* kt = (int2*)workspace;
     int2* qt = kt + (int64_t)p.B * p.nkt;
-    if (p.nkt) hipLaunchKernelGGL(attn_ranges_kernel, dim3(cdiv(p.nkt, 4), p.B), dim3(256), 0, stream, p.kdoc, p.kdoc_stride, p.Lk, p.nkt, kt);
+    if (p.nkt) hipLaunchKernelGGL(attn_ranges_kernel, dim3(cdiv(p.nkt, 4) * p.B), dim3(256), 0, stream, p.kdoc, p.kdoc_stride, p.Lk, p.nkt, kt);
     if (p.qdoc == p.kdoc && p.qdoc_stride == p.kdoc_stride && p.Lq == p.Lk) qt = kt;
-    else hipLaunchKernelGGL(attn_ranges_kernel, dim3(cdiv(p.nqt, 4), p.B), dim3(256), 0, stream, p.qdoc, p.qdoc_stride, p.Lq, p.nqt, qt);
+    else hipLaunchKernelGGL(attn_ranges_kernel, dim3(cdiv(p.nqt, 4) * p.B), dim3(256), 0, stream, p.qdoc, p.qdoc_stride, p.Lq, p.nqt, qt);
     p.ktiles = kt;
     p.qtiles = qt;
     p.row_blocks = cdiv(p.Lq, 128);

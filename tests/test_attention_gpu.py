@@ -389,6 +389,42 @@ def test_attention_reproducible_on_another_stream_and_in_graphs(dev):
                 assert all(torch.equal(a, c) for a, c in zip(want, out))
 
 
+def test_attention_many_short_sequences(dev):
+    """More sequences than a launch's second dimension holds, with documents."""
+    b, n = 70000, 6
+    q, k, v, do = _inputs(b, n, n, 1, 1, 8, BF16, 82)
+    docs = torch.tensor([0, 0, 1, 1, 1, -1], dtype=torch.int32).repeat(b, 1)
+    _check(dev, q, k, v, do, documents=docs, causal=True)
+
+
+def test_attention_split_and_ordered_calls_in_graphs(dev):
+    """Calls whose work is split over the long axis, or taken in the order of the documents' lengths, replayed beside eager ones."""
+    from next3d_amd.torch_utils.ops import attention
+    for size, kw in (((1, 1700, 1700, 2, 1, 64), dict(causal=True)), ((2, 1100, 1100, 64, 64, 8), dict(documents=_docs(2, 1100, 7, 4, pad=100)))):
+        q, k, v, do = (t.to(dev) for t in _inputs(*size, F16, 83))
+        kw = _to(dev, kw)
+
+        def step():
+            leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+            out = attention.attention(*leaves, **kw)
+            return [out.detach(), *torch.autograd.grad(out, leaves, do)]
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        for seed in range(3):
+            q.copy_(_randn(tuple(q.shape), 84 + seed, F16))
+            want = [t.clone() for t in step()]
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, c) for a, c in zip(want, out))
+
+
 def test_token_block(dev):
     """The three operators as a block uses them — normalise, project, turn, attend, add — forward and gradients, against the same block in float64."""
     from next3d_amd.torch_utils.ops import attention, layer_norm, rotary
