@@ -9,7 +9,7 @@ objs=""
 for src in next3d_amd/csrc/*.hip; do
   b=$(basename ${src%.hip})
   extra=""; [ "$b" = raster ] && extra="-ffp-contract=off"
-  /opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -DN3D_TUNING $extra "$@" -c $src -o tools/probe/tuning_obj/$b.o &
+  /opt/rocm/bin/hipcc -O3 -std=c++17 -Xclang -target-feature -Xclang -packed-fp32-ops -fPIC --offload-arch=gfx950 -DN3D_TUNING $extra "$@" -c $src -o tools/probe/tuning_obj/$b.o &
   objs="$objs tools/probe/tuning_obj/$b.o"
 done
 wait

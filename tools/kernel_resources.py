@@ -3,7 +3,7 @@
 import re, subprocess, sys
 src = sys.argv[1]
 extra = sys.argv[2:]
-r = subprocess.run(['/opt/rocm/bin/hipcc', '-O3', '-std=c++17', '-fPIC', '--offload-arch=gfx950',
+r = subprocess.run(['/opt/rocm/bin/hipcc', '-O3', '-std=c++17', '-fPIC', '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops', '--offload-arch=gfx950',
                     '-Rpass-analysis=kernel-resource-usage', '-c', src, '-o', '/dev/null'] + extra, capture_output=True, text=True)
 cur = None
 rows = {}
