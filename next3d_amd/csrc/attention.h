@@ -26,7 +26,7 @@ struct AttnParams {
     const int *prefix, *lengths, *qdoc, *kdoc;
     int64_t qdoc_stride, kdoc_stride;
     const float* slopes;
-    const int2 *ktiles, *qtiles;                     // lowest and highest document of every ATTN_TILE keys / queries, [B][nkt] / [B][nqt]
+    const int2 *ktiles, *qtiles;                     // lowest and highest document of every ATTN_TILE keys / queries, [B][nkt] / [B][nqt] (attn_ranges_kernel)
     float* delta;                                    // [B][Hq][Lq]
     float* part;                                     // partial results of split kernels
     int64_t part_ml;                                 // offset of their statistics in `part`

@@ -150,11 +150,13 @@ __device__ __forceinline__ void attn_dq(const AttnParams& p, int group, char* sm
     const int lim_last = attn_limit(p, min(q0 + 32 * wave + 31, p.Lq - 1), n, prefix);
     const int key_end = attn_limit(p, min(q0 + 127, p.Lq - 1), n, prefix) + 1;
     int dlo = 0, dhi = 0;
+    bool one = true;
     if constexpr (DOCS) {
         const int2* r = p.qtiles + (int64_t)b * p.nqt + 2 * blk;
         const int2 r0 = r[0], r1 = 2 * blk + 1 < p.nqt ? r[1] : r[0];
         dlo = min(r0.x, r1.x);
         dhi = max(r0.y, r1.y);
+        one = r0.x == r0.y && r1.x == r1.y && r0.x == r1.x;
     }
     AttnTiles<DOCS> tiles;
     const int run = (p.nkt + p.splits - 1) / p.splits, run_first = split * run, run_end = min((key_end + ATTN_TILE - 1) / ATTN_TILE, run_first + run);
@@ -195,7 +197,7 @@ __device__ __forceinline__ void attn_dq(const AttnParams& p, int group, char* sm
     if (t >= 0) stage(t, 0);
     if (DOCS && wave == 0) sdoc[0][lane] = doc_next;
     // every key of tile t visible to every query of the workgroup
-    const int full_end = DOCS && dlo != dhi ? 0 : attn_limit(p, q0, n, prefix) + 1;
+    const int full_end = DOCS && !one ? 0 : attn_limit(p, q0, n, prefix) + 1;
     auto full = [&] { return !fine && (t + 1) * ATTN_TILE <= full_end && (!DOCS || ((tiles.low == dlo) & (tiles.high == dlo))); };
     auto visit = [&](auto mask) {
         const int j0 = t * ATTN_TILE, now = buf;
@@ -348,11 +350,13 @@ __device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* s
     const int wave_first = first_query(k0 + 32 * keys);
     const bool wave_on = k0 + 32 * keys < n;
     int dlo = 0, dhi = 0;
+    bool one = true;
     if constexpr (DOCS) {
         const int2* r = p.ktiles + (int64_t)b * p.nkt + 2 * blk;
         const int2 r0 = r[0], r1 = 2 * blk + 1 < p.nkt ? r[1] : r[0];
         dlo = min(r0.x, r1.x);
         dhi = max(r0.y, r1.y);
+        one = r0.x == r0.y && r1.x == r1.y && r0.x == r1.x;
     }
     const int2* ranges = DOCS ? p.qtiles + (int64_t)b * p.nqt : nullptr;
     const int run = (p.nqt + p.chunks - 1) / p.chunks, run_first = split % p.chunks * run, run_end = min(p.nqt, run_first + run);
@@ -409,7 +413,7 @@ __device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* s
     if (t >= 0) stage(t, g, 0);
     commit(0);
     // every query of tile t sees every key of the workgroup (but those behind the last, whose lanes are not stored)
-    const int full_first = DOCS && dlo != dhi ? 0x7fffffff : first_query(min(k0 + 127, n - 1));
+    const int full_first = DOCS && !one ? 0x7fffffff : first_query(min(k0 + 127, n - 1));
     auto full = [&] { return !fine && t * ATTN_TILE >= full_first && (!DOCS || ((tiles.low == dlo) & (tiles.high == dlo))); };
     auto visit = [&](auto mask) {
         const int i0 = t * ATTN_TILE, now = buf;

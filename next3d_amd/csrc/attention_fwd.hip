@@ -10,18 +10,20 @@
 //   148 + 5 us, 5.3 TB/s (a large copy: 4.9): bound by memory.
 #include "attention.h"
 
-// lowest and highest document of every ATTN_TILE tokens
+// Lowest and highest document of every ATTN_TILE tokens.  Tokens of no document do not count (none at all: an empty range that meets no other), but a tile
+// that holds some of them must not pass for one of a single document: its range gets one document more.
 __global__ __launch_bounds__(256) void attn_ranges_kernel(const int* __restrict__ doc, int64_t stride, int L, int tiles, int2* __restrict__ out) {
     const int groups = (tiles + 3) / 4, b = blockIdx.x / groups, t = (blockIdx.x - b * groups) * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (t >= tiles) return;
     const int j = t * ATTN_TILE + lane;
     const int d = doc[b * stride + (j < L ? j : L - 1)];
-    int lo = d, hi = d;
+    int lo = d < 0 ? 0x7fffffff : d, hi = d < 0 ? -1 : d;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
         lo = min(lo, __shfl_xor(lo, o));
         hi = max(hi, __shfl_xor(hi, o));
     }
+    if (__ballot(d < 0) && lo == hi) --lo;
     if (lane == 0) out[(int64_t)b * tiles + t] = make_int2(lo, hi);
 }
 
@@ -190,11 +192,13 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnParams p) {
     const int lim_last = attn_limit(p, min(q0 + 32 * wave + 31, p.Lq - 1), n, prefix);
     const int key_end = attn_limit(p, min(q0 + 127, p.Lq - 1), n, prefix) + 1;
     int dlo = 0, dhi = 0;
+    bool one = true;                                                            // one document, and every query in it
     if constexpr (DOCS) {                                                       // documents of this workgroup's queries: two ranges of ATTN_TILE queries
         const int2* r = p.qtiles + (int64_t)b * p.nqt + 2 * blk;
         const int2 r0 = r[0], r1 = 2 * blk + 1 < p.nqt ? r[1] : r[0];
         dlo = min(r0.x, r1.x);
         dhi = max(r0.y, r1.y);
+        one = r0.x == r0.y && r1.x == r1.y && r0.x == r1.x;
     }
     AttnTiles<DOCS> tiles;
     const int run = (p.nkt + p.splits - 1) / p.splits, run_first = split * run, run_end = min((key_end + ATTN_TILE - 1) / ATTN_TILE, run_first + run);
@@ -229,7 +233,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnParams p) {
     if (t >= 0) stage(t, 0);
     if (DOCS && wave == 0) sdoc[0][lane] = doc_next;
     // every key of tile t visible to every query of the workgroup
-    const int full_end = DOCS && dlo != dhi ? 0 : attn_limit(p, q0, n, prefix) + 1;
+    const int full_end = DOCS && !one ? 0 : attn_limit(p, q0, n, prefix) + 1;
     auto full = [&] { return !fine && (t + 1) * ATTN_TILE <= full_end && (!DOCS || ((tiles.low == dlo) & (tiles.high == dlo))); };
     auto visit = [&](auto mask) {
         const int j0 = t * ATTN_TILE, now = buf;

@@ -194,6 +194,19 @@ def test_attention_many_blocks_of_uneven_documents(dev, causal):
     _check(dev, q, k, v, do, documents=docs, causal=causal, lengths=torch.tensor([1300, 1000, 0], dtype=torch.int32))
 
 
+@pytest.mark.parametrize('lengths', [(64, 64, 128), (128, 128), (300, 20), (1, 255), (130, 0, 62)], ids=str)
+def test_attention_padding_beside_a_single_document(dev, lengths):
+    """Tiles and blocks that hold one document and padding in every arrangement: whole tiles of either, and tiles shared by both."""
+    n, d = sum(lengths), 64
+    for pattern in range(2 ** len(lengths)):
+        ids = torch.cat([torch.full((l,), 3 if pattern >> i & 1 else -5, dtype=torch.int32) for i, l in enumerate(lengths)])[None]
+        q, k, v, do = _inputs(1, n, n, 2, 1, d, BF16, 26)
+        for t in (q, k, v, do):
+            t[ids < 0] = float('nan')
+        _check(dev, q, k, v, do, what=f'{pattern}', documents=ids)
+        _check(dev, q, k, v, do, what=f'{pattern} causal', documents=ids, causal=True)
+
+
 def test_attention_small_and_large_gradients_float16(dev):
     """float16 gradients of any size keep their relative accuracy (the dscores get a power of two of their own)."""
     for size in (1e-6, 1e-3, 300.0):
