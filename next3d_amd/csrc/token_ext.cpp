@@ -5,6 +5,7 @@
 #include <ATen/ATen.h>
 
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/AutogradState.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
@@ -67,6 +68,15 @@ int code(const Tensor& t) { return t.scalar_type() == at::kHalf ? N3D_F16 : t.sc
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor get(const Opt& t) { return t ? *t : Tensor(); }
 Tensor dense(const Tensor& like) { return at::empty(like.sizes(), like.options().memory_format(c10::MemoryFormat::Contiguous)); }
+// What a call of the library cannot serve, and would answer wrongly without a word: a tangent would be dropped.
+void refuse(const char* op, std::initializer_list<const Tensor*> ts) {
+    const std::string name = op;
+    const bool tangents = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+    for (const Tensor* t : ts) {
+        if (!t->defined()) continue;
+        if (tangents && t->_fw_grad(0).defined()) throw std::runtime_error(name + ": no forward-mode derivative");
+    }
+}
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
     if (!at::GradMode::is_enabled()) return false;
     for (const Tensor* t : ts)
@@ -147,6 +157,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 
 Tensor layer_norm(const Tensor& x, const Opt& weight, const Opt& bias, double eps) {
     Tensor w = get(weight), b = get(bias);
+    refuse("layer_norm", {&x, &w, &b});
     if (w.defined()) w = w.contiguous();
     if (b.defined()) b = b.contiguous();
     if (wants_grad({&x, &w, &b})) return LayerNorm::apply(x, w.defined() ? Opt(w) : Opt(), b.defined() ? Opt(b) : Opt(), eps);
@@ -224,7 +235,9 @@ struct Rotary : torch::autograd::Function<Rotary> {
 };
 
 std::tuple<Tensor, Opt> rotary(const Tensor& q, const Opt& k, const Tensor& positions, const std::vector<int64_t>& sections, double base, bool interleaved, bool shared) {
-    const Tensor k_ = get(k), pos = positions.stride(-1) == 1 ? positions : positions.contiguous();
+    const Tensor k_ = get(k);
+    refuse("rotary", {&q, &k_, &positions});
+    const Tensor pos = positions.stride(-1) == 1 ? positions : positions.contiguous();
     const RotaryPlan plan = {sections, base, interleaved, shared};
     if (wants_grad({&q, &k_})) {
         variable_list y = Rotary::apply(q, k, pos, plan);
@@ -342,6 +355,7 @@ struct Attention : torch::autograd::Function<Attention> {
 std::tuple<Tensor, Opt> attention(const Tensor& q, const Tensor& k, const Tensor& v, double scale, bool causal, const Opt& prefix, const Opt& documents,
                                   const Opt& key_documents, const Opt& lengths, double softcap, const Opt& slopes, bool want_lse) {
     const Attention::Masks m = {get(prefix), get(documents), get(key_documents), get(lengths), get(slopes), scale, softcap, causal};
+    refuse("attention", {&q, &k, &v, &m.prefix, &m.documents, &m.key_documents, &m.lengths, &m.slopes});
     if (wants_grad({&q, &k, &v})) {
         variable_list r = Attention::apply(q, k, v, m);
         return {r[0], r[1]};

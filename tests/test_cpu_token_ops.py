@@ -224,3 +224,24 @@ def test_attention_c_entries_refuse_sizes():
     many = _lib.AttentionDesc(**dict(base, B=1 << 10, Lq=1 << 19, heads_q=4, heads_k=4))
     assert lib.n3d_attention_bwd(many, None) != 0 and '2^31' in lib.n3d_last_error().decode()
     assert lib.n3d_attention_workspace(_lib.AttentionDesc(**dict(base, B=1 << 10, Lk=1 << 15, heads_q=64, heads_k=8))) >= 0      # (a large cache, single tokens)
+
+
+def _host_side_calls():
+    """Each operator's call of the C++ host side (no device check in front of it) and its floating-point arguments."""
+    from next3d_amd import _lib
+    ext = _lib.token_ext()
+    pos, q, q16 = torch.zeros(3, 1), torch.ones(1, 3, 2, 8), torch.ones(1, 3, 2, 8).half()
+    return (('layer_norm', lambda x, w, b: ext.layer_norm(x, w, b, 1e-5), [torch.ones(3, 8), torch.ones(8), torch.ones(8)]),
+            ('rotary', lambda q, k, p: ext.rotary(q, k, p, (8,), 1e4, True, False)[0], [q, q, pos]),
+            ('attention', lambda q, k, v, s: ext.attention(q, k, v, 1.0, False, None, None, None, None, 0.0, s, False)[0], [q16, q16, q16, torch.ones(2)]))
+
+
+@pytest.mark.parametrize('op', [0, 1, 2])
+def test_forward_mode_derivatives_are_refused(op):
+    """A tangent on any argument: refused, not dropped."""
+    import torch.autograd.forward_ad as fwd
+    name, call, args = _host_side_calls()[op]
+    for which in range(len(args)):
+        with fwd.dual_level():
+            duals = [fwd.make_dual(t, torch.ones_like(t)) if i == which else t for i, t in enumerate(args)]
+            _raises(f'{name}: no forward-mode', call, *duals)

@@ -275,3 +275,21 @@ def test_token_ops_refuse_second_derivatives(dev):
         assert all(torch.equal(a, b) for a, b in zip(plain, graph))
         with pytest.raises(RuntimeError, match='differentiable once'):
             graph[0].float().square().sum().backward()
+
+
+def test_token_ops_refuse_what_cannot_see_into_them(dev):
+    """Forward-mode derivatives and functional transforms raise through the public functions; none returns a result without a derivative."""
+    import torch.autograd.forward_ad as fwd
+    from next3d_amd.torch_utils.ops import attention, layer_norm, rotary
+    q = torch.ones(1, 3, 2, 8, dtype=torch.float16, device=dev)
+    pos = torch.zeros(3, 1, device=dev)
+    for call, x in ((layer_norm.layer_norm, torch.ones(3, 8, device=dev)), (lambda t: rotary.rotary(t, pos, (8,)), q), (lambda t: attention.attention(t, q, q), q)):
+        with fwd.dual_level():
+            with pytest.raises(RuntimeError, match='forward-mode'):
+                call(fwd.make_dual(x, x))
+            with torch.no_grad(), pytest.raises(RuntimeError, match='forward-mode'):
+                call(fwd.make_dual(x, x))
+        for transform in (lambda: torch.vmap(call)(x[None]), lambda: torch.func.jvp(call, (x,), (x,)), lambda: torch.func.grad(lambda t: call(t).sum())(x)):
+            with pytest.raises(RuntimeError):
+                transform()
+        assert call(x).shape == x.shape
