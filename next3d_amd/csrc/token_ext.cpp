@@ -6,8 +6,10 @@
 
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/AutogradState.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <stdexcept>
@@ -68,9 +70,12 @@ int code(const Tensor& t) { return t.scalar_type() == at::kHalf ? N3D_F16 : t.sc
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor get(const Opt& t) { return t ? *t : Tensor(); }
 Tensor dense(const Tensor& like) { return at::empty(like.sizes(), like.options().memory_format(c10::MemoryFormat::Contiguous)); }
-// What a call of the library cannot serve, and would answer wrongly without a word: a tangent would be dropped.
+// What a call of the library cannot serve, and would answer wrongly without a word: a tracer would record the empty output and not the kernel that fills it,
+// a tangent would be dropped.
 void refuse(const char* op, std::initializer_list<const Tensor*> ts) {
     const std::string name = op;
+    if (torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY))
+        throw std::runtime_error(name + ": cannot be traced");
     const bool tangents = c10::AutogradState::get_tls_state().get_fw_grad_mode();
     for (const Tensor* t : ts) {
         if (!t->defined()) continue;

@@ -1,5 +1,5 @@
 """What the token operators (layer_norm, rotary, attention) share: element types and argument checks.  Buffers, launches and autograd nodes are in
-csrc/token_ext.cpp, which also refuses the calls that forward-mode derivatives make: they do not see into the library."""
+csrc/token_ext.cpp, which also refuses the calls that torch's tracers and forward-mode derivatives make: neither sees into the library."""
 import torch
 
 from ... import _lib

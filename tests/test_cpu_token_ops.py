@@ -245,3 +245,12 @@ def test_forward_mode_derivatives_are_refused(op):
         with fwd.dual_level():
             duals = [fwd.make_dual(t, torch.ones_like(t)) if i == which else t for i, t in enumerate(args)]
             _raises(f'{name}: no forward-mode', call, *duals)
+
+
+@pytest.mark.parametrize('op', [0, 1, 2])
+def test_tracing_is_refused(op):
+    """A tracer sees an empty tensor and not what fills it: refused, not recorded."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    name, call, args = _host_side_calls()[op]
+    _raises(f'{name}: cannot be traced', torch.jit.trace, call, tuple(args))
+    _raises(f'{name}: cannot be traced', make_fx(call), *args)

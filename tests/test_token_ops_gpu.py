@@ -278,7 +278,7 @@ def test_token_ops_refuse_second_derivatives(dev):
 
 
 def test_token_ops_refuse_what_cannot_see_into_them(dev):
-    """Forward-mode derivatives and functional transforms raise through the public functions; none returns a result without a derivative."""
+    """Forward-mode derivatives, tracers and functional transforms raise through the public functions; none returns a result without a derivative."""
     import torch.autograd.forward_ad as fwd
     from next3d_amd.torch_utils.ops import attention, layer_norm, rotary
     q = torch.ones(1, 3, 2, 8, dtype=torch.float16, device=dev)
@@ -289,6 +289,8 @@ def test_token_ops_refuse_what_cannot_see_into_them(dev):
                 call(fwd.make_dual(x, x))
             with torch.no_grad(), pytest.raises(RuntimeError, match='forward-mode'):
                 call(fwd.make_dual(x, x))
+        with pytest.raises(RuntimeError, match='traced'):
+            torch.jit.trace(call, (x,))
         for transform in (lambda: torch.vmap(call)(x[None]), lambda: torch.func.jvp(call, (x,), (x,)), lambda: torch.func.grad(lambda t: call(t).sum())(x)):
             with pytest.raises(RuntimeError):
                 transform()
