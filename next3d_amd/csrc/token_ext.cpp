@@ -71,7 +71,7 @@ void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 Tensor get(const Opt& t) { return t ? *t : Tensor(); }
 Tensor dense(const Tensor& like) { return at::empty(like.sizes(), like.options().memory_format(c10::MemoryFormat::Contiguous)); }
 // What a call of the library cannot serve, and would answer wrongly without a word: a tracer would record the empty output and not the kernel that fills it,
-// a tangent would be dropped.
+// a tangent would be dropped, a tensor that holds no memory would pass for an absent one.
 void refuse(const char* op, std::initializer_list<const Tensor*> ts) {
     const std::string name = op;
     if (torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY))
@@ -80,6 +80,7 @@ void refuse(const char* op, std::initializer_list<const Tensor*> ts) {
     for (const Tensor* t : ts) {
         if (!t->defined()) continue;
         if (tangents && t->_fw_grad(0).defined()) throw std::runtime_error(name + ": no forward-mode derivative");
+        if (t->numel() && !t->const_data_ptr()) throw std::runtime_error(name + ": a tensor without memory of its own");
     }
 }
 bool wants_grad(std::initializer_list<const Tensor*> ts) {

@@ -254,3 +254,20 @@ def test_tracing_is_refused(op):
     name, call, args = _host_side_calls()[op]
     _raises(f'{name}: cannot be traced', torch.jit.trace, call, tuple(args))
     _raises(f'{name}: cannot be traced', make_fx(call), *args)
+
+
+@pytest.mark.parametrize('op', [0, 1, 2])
+def test_tensors_without_memory_are_refused(op):
+    """A wrapping tensor holds no memory itself: refused, not taken for an absent argument."""
+    class Wrapper(torch.Tensor):
+        @staticmethod
+        def __new__(cls, t):
+            return torch.Tensor._make_wrapper_subclass(cls, t.shape, dtype=t.dtype, device=t.device)
+
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            return func(*(torch.zeros(a.shape, dtype=a.dtype) if isinstance(a, cls) else a for a in args), **(kwargs or {}))
+
+    name, call, args = _host_side_calls()[op]
+    for which in range(len(args)):
+        _raises(f'{name}: a tensor without memory', call, *(Wrapper(t) if i == which else t for i, t in enumerate(args)))
