@@ -184,10 +184,10 @@ __device__ __forceinline__ typename AttnVec<T>::x8 attn_lane_frag(const T* p, in
     return p && chunk * 8 < D ? *reinterpret_cast<const typename AttnVec<T>::x8*>(p + chunk * 8) : z;
 }
 
-// Eight values of x that `rounded` holds in 16 bits: what the rounding left over.  Where gradients are wanted, workgroups that walk ATTN_FEW tiles or fewer
-// take a second product with it: rows of a few keys have nothing to average the roundings out (22 causal queries: float16 dq / dk off by 3.4e-4 of their
-// norm without it, 2.0e-4 with it, plain float32 arithmetic 2.0e-4).  (Such workgroups take every tile as one with a mask, which the code of the others
-// is spared.)  In every masked tile of long documents it would cost 26 % of the forward pass (2 x 4096 x 16 heads x 64: 73 -> 92 us) and gain little.
+// Eight values of x that `rounded` holds in 16 bits: what the rounding left over.  Workgroups that walk ATTN_FEW tiles or fewer take a second product with
+// it, whether or not gradients are wanted (the same call gives the same bits in both): rows of a few keys have nothing to average the roundings out (22
+// causal queries: float16 dq / dk off by 3.4e-4 of their norm without it, 2.0e-4 with it, plain float32 arithmetic 2.0e-4).  (Such workgroups take every
+// tile as one with a mask, which the code of the others is spared.)  In every masked tile of long documents it would cost 26 % of the forward pass (2 x 4096 x 16 heads x 64: 73 -> 92 us) and gain little.
 static constexpr int ATTN_FEW = 4;
 template <typename T>
 __device__ __forceinline__ typename AttnVec<T>::x8 attn_left_over(const f32x16& x, typename AttnVec<T>::x8 rounded, int c) {
@@ -227,8 +227,17 @@ struct AttnTiles {
     __device__ __forceinline__ void start(const int2* r, int first, int stop, int dlo, int dhi) {
         ranges = r; t = first; end = stop; lo = dlo; hi = dhi; bits = 0; base = first - 64;
     }
-    // behind the first next(): ATTN_FEW tiles at most (with documents: of the first 64 that were looked at)
-    __device__ __forceinline__ bool few() const { return DOCS ? __popcll(bits) < ATTN_FEW : end - t < ATTN_FEW; }
+    // behind the first next(): ATTN_FEW tiles at most (with documents: of the first 128 ranges from where the first such tile lies)
+    __device__ __forceinline__ bool few(int lane) const {
+        if constexpr (!DOCS) return end - t < ATTN_FEW;
+        int more = __popcll(bits);
+        if (more < ATTN_FEW && base + 64 < end) {
+            const int i = base + 64 + lane;
+            const int2 r = i < end ? ranges[i] : make_int2(1, 0);
+            more += __popcll(__ballot((i < end) & (r.y >= lo) & (r.x <= hi)));
+        }
+        return more < ATTN_FEW;
+    }
     // the next tile or -1
     __device__ __forceinline__ int next(int lane) {
         if constexpr (!DOCS) return t < end ? t++ : -1;

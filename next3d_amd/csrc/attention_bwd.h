@@ -193,7 +193,7 @@ __device__ __forceinline__ void attn_dq(const AttnParams& p, int group, char* sm
         sv.issue(v_at, t, n, v_row, p.D, at + TILE_BYTES, wave);
     };
     int t = tiles.next(lane), buf = 0;
-    const bool fine = tiles.few();
+    const bool fine = tiles.few(lane);
     if (t >= 0) stage(t, 0);
     if (DOCS && wave == 0) sdoc[0][lane] = doc_next;
     // every key of tile t visible to every query of the workgroup
@@ -409,7 +409,7 @@ __device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* s
     f32x16 dk[NB] = {}, dv[NB] = {};
     AttnScore f(p, hk * p.G);
     int t = next(g), buf = 0;
-    const bool fine = tiles.few();
+    const bool fine = tiles.few(lane);
     if (t >= 0) stage(t, g, 0);
     commit(0);
     // every query of tile t sees every key of the workgroup (but those behind the last, whose lanes are not stored)

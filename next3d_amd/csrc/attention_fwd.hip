@@ -229,7 +229,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnParams p) {
         sv.issue(v_at, t, n, v_row, p.D, lds + buf * 2 * TILE_BYTES + TILE_BYTES, wave);
     };
     int t = tiles.next(lane), buf = 0;
-    const bool fine = p.rest && tiles.few();
+    const bool fine = tiles.few(lane);
     if (t >= 0) stage(t, 0);
     if (DOCS && wave == 0) sdoc[0][lane] = doc_next;
     // every key of tile t visible to every query of the workgroup
@@ -394,7 +394,7 @@ __global__ __launch_bounds__(256) void attn_token_kernel(AttnParams p) {
         for (int db = 0; db < DB; ++db)
 #pragma unroll
             for (int c = 0; c < 2; ++c) acc[db] = attn_mfma(attn_col_frag<T, ROW>(v_lds, c, db), P[0][c], acc[db]);
-        if (p.rest && lim_last < ATTN_FEW * ATTN_TILE)         // (attn_left_over)
+        if (lim_last < ATTN_FEW * ATTN_TILE)         // (attn_left_over)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const typename AttnVec<T>::x8 left = attn_left_over<T>(S[0], P[0][c], c);

@@ -482,3 +482,34 @@ def test_token_block(dev):
     for name, a, ref, roundings in zip(('out', 'x', 'weight', 'bias', 'proj'), got, want, (6, 12, 12, 12, 12)):
         err = float((a.detach().cpu().double() - ref.detach()).abs().max())
         assert err <= roundings * 2.0 ** -11 * float(ref.detach().abs().max()) * 2, (name, err, float(ref.detach().abs().max()))
+
+
+@pytest.mark.parametrize('dtype', [F16, BF16])
+def test_attention_same_bits_with_and_without_gradients(dev, dtype):
+    """Short calls, single tokens, documents and long rows: inference gives the bits that a recorded call (and a checkpoint's second pass) gives."""
+    from next3d_amd.torch_utils.ops import attention
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32)
+    for size, kw in (((2, 7, 77, 8, 8, 64), dict(causal=True, slopes=2.0 ** -torch.arange(1.0, 9))), ((3, 1, 190, 8, 2, 128), dict(lengths=i32(1, 64, 190))),
+                     ((2, 1, 3000, 8, 2, 128), dict(causal=True)), ((2, 150, 150, 2, 2, 72), dict(causal=True)), ((1, 200, 256, 4, 1, 128), dict(softcap=5.0)),
+                     ((2, 700, 700, 2, 1, 64), dict(documents=_docs(2, 700, 6, 3, pad=50), causal=True)), ((1, 600, 600, 2, 2, 32), dict())):
+        q, k, v, _ = (t.to(dev) for t in _inputs(*size, dtype, 101))
+        kw = _to(dev, kw)
+        plain = attention.attention(q, k, v, return_lse=True, **kw)
+        with torch.no_grad():
+            quiet = attention.attention(*(t.detach().requires_grad_() for t in (q, k, v)), return_lse=True, **kw)
+        recorded = attention.attention(*(t.detach().requires_grad_() for t in (q, k, v)), return_lse=True, **kw)
+        assert recorded[0].requires_grad and not quiet[0].requires_grad
+        for a, c, e in zip(plain, quiet, recorded):
+            assert torch.equal(a, c) and torch.equal(a, e), size
+
+
+def test_attention_document_that_begins_at_the_end_of_64_tiles(dev):
+    """A long document whose first tiles are the last of the 64 ranges that are looked at together, and one that ends right behind them."""
+    n = 5200
+    ids = torch.zeros(1, n, dtype=torch.int32)
+    ids[0, 4000:] = 1
+    ids[0, 4200:4220] = 2
+    q, k, v, do = _inputs(1, n, n, 1, 1, 16, F16, 102)
+    _check(dev, q, k, v, do, documents=ids)
+    ids[0, 4150:] = -1
+    _check(dev, q, k, v, do, documents=ids, causal=True)
