@@ -513,3 +513,19 @@ def test_attention_document_that_begins_at_the_end_of_64_tiles(dev):
     _check(dev, q, k, v, do, documents=ids)
     ids[0, 4150:] = -1
     _check(dev, q, k, v, do, documents=ids, causal=True)
+
+
+@pytest.mark.parametrize('dtype', [F16, BF16])
+def test_attention_of_few_queries_is_rounded_once(dev, dtype):
+    """Few queries over a cache: the weights keep what their rounding left over, so results are off by their own rounding and second-order terms only."""
+    from next3d_amd.torch_utils.ops import attention
+    for size, kw in (((2, 1, 3000, 8, 2, 128), dict()), ((1, 5, 900, 4, 1, 64), dict(causal=True)), ((2, 1, 70, 2, 2, 80), dict())):
+        q, k, v, _ = _inputs(*size, dtype, 103)
+        out = attention.attention(q.to(dev), k.to(dev), v.to(dev), **kw).cpu().double()
+        vals, tols = R.attention(q, k, v, **kw)
+        mean = R.attention(q, k, v.abs(), **kw)[0]['out']                       # sum of weight |v|
+        exact, u = vals['out'], R.HALF[dtype]
+        first = u * (mean + exact.abs())                                        # the two roundings that the bound counts for every call ...
+        inner = tols['out'] - first + 2 * u * u * mean                          # ... here the rounding of a left-over, and what is float32
+        own = (exact.to(dtype).double() - exact).abs()                          # the exact result's own rounding; the nearest of exact + e is within own + 2 e
+        assert bool(((out - exact).abs() <= own + 2 * inner).all()), size
