@@ -30,7 +30,6 @@ struct AttnParams {
     float* delta;                                    // [B][Hq][Lq]
     float* part;                                     // partial results of split kernels
     int64_t part_ml;                                 // offset of their statistics in `part`
-    const float* maxima;                             // partial maxima (float16 gradients), see attn_ds_scale
     int B, Lq, Lk, Hq, Hk, G, D, nkt, nqt, causal, row_blocks;
     const int* order;                                // [B, row blocks of queries], the longest first, or null: the last first
     int splits;                                      // workgroups a row block's work is split over
@@ -388,8 +387,6 @@ static inline void attn_forms(const AttnParams& p, F&& f) {
         default: form(std::integral_constant<int, 4>()); break;
     }
 }
-
-static constexpr int ATTN_MAXIMA = 1024;             // partial maxima of |do|, and as many of |v| (attn_prep_kernel: its workgroups)
 
 // workspace, in floats: the document ranges come first
 static inline int64_t attn_range_floats(const AttnParams& p) { return p.kdoc ? 2 * (int64_t)p.B * (p.nkt + p.nqt) + (int64_t)p.B * cdiv(p.Lq, 128) : 0; }

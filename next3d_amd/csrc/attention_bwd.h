@@ -1,6 +1,6 @@
 // Attention, backward (attention.h):  P = exp2(u - lse),  dP = do v^T,  delta = sum(do o),  dt = P (dP - delta),  ds = dt (1 - tanh^2),
 //   dq = scale ds k,   dk = scale ds^T q,   dv = P^T do,   dk and dv summed over the query heads of a key head.
-// attn_prep_kernel: delta, and for float16 the largest |do| and |v| (attn_ds_scale).
+// attn_prep_kernel: delta.
 // attn_dq_kernel: a workgroup owns 128 queries of a head and walks the keys;  attn_dkv_kernel: a workgroup owns 128 keys of a key head and walks the
 // queries of all its heads.  Scores are computed in both (7 products for 5) so that every sum has one owner: no atomics, the same bits every time.
 // Measured, 4096 x 16 heads x 128 bfloat16 without a mask: prep 10 us, dq 183 us (1.13 PFLOP/s of its three products), dk / dv 286 to 306 us (0.90 to 0.96 of
@@ -9,85 +9,72 @@
 #pragma once
 #include "attention.h"
 
-// float16 has 5 exponent bits, and P ~ 1 / length and ds ~ P do v leave its range on long rows or with small gradients.  The dk / dv kernel therefore uses
-// P 2^12, and both kernels ds times a power of two taken from the largest |do| and |v| of the call, so that no ds can overflow:
-// |ds| <= |dP - delta| <= 2 D max|do| max|v|.  The accumulators undo both.  bfloat16 has float32's exponents: neither is needed.
+// float16 has 5 exponent bits, and P ~ 1 / length and ds ~ P do v leave its range on long rows or with small gradients (bfloat16 has float32's exponents).
+// The dk / dv kernel therefore uses P 2^12, and both kernels ds 2^e with an e of the lane's own — a query's in dq, a key's in dk / dv — found like the running
+// maximum of a softmax: e begins high, and where a visible ds 2^e reaches 2 it is lowered until the largest is 1/4 to 1/2, and the accumulators with it.  So
+// dscores of any size are rounded by half a step of their own, or, below 2^-12 of the lane's largest, by 2^-23 of that; what a lane does not see has no say.
 template <typename T> static constexpr float ATTN_P_SHIFT = std::is_same<T, _Float16>::value ? 12.f : 0.f;
+static constexpr int ATTN_DS_EXP = 64;                        // (|P dP| < 2^41 in float16: 2^64 of it is a float32)
 
 template <typename T>
 __global__ __launch_bounds__(256) void attn_prep_kernel(AttnParams p) {
     // 16 lanes a row, 8 channels a lane
     const int lane16 = threadIdx.x & 15, D = p.D;
-    float top = 0.f;
-    if (blockIdx.y == 0) {
-        const uint32_t rows = (uint32_t)p.B * p.Lq * p.Hq;                // (below 2^31: n3d_attention_bwd)
-        for (uint32_t w = blockIdx.x * 16 + (threadIdx.x >> 4); w < rows; w += gridDim.x * 16) {
-            const uint32_t bi = w / p.Hq;
-            const int h = w - bi * p.Hq, b = bi / p.Lq, i = bi - b * p.Lq;
-            const int64_t stat = ((int64_t)b * p.Hq + h) * p.Lq + i;
-            float s = 0.f;
-            const bool live = p.lse[stat] != -INFINITY;
-            if (lane16 * 8 < D) {
-                const auto x = *reinterpret_cast<const typename AttnVec<T>::x8*>((const T*)p.dout + b * p.ds[0] + i * p.ds[1] + h * p.ds[2] + lane16 * 8);
-                const auto y = *reinterpret_cast<const typename AttnVec<T>::x8*>((const T*)p.o + (int64_t)w * D + lane16 * 8);
-                typename AttnVec<T>::x8 z = {};
-                if (p.rest) z = *reinterpret_cast<const typename AttnVec<T>::x8*>((const T*)p.rest + (int64_t)w * D + lane16 * 8);
+    const uint32_t rows = (uint32_t)p.B * p.Lq * p.Hq;                    // (below 2^31: n3d_attention_bwd)
+    for (uint32_t w = blockIdx.x * 16 + (threadIdx.x >> 4); w < rows; w += gridDim.x * 16) {
+        const uint32_t bi = w / p.Hq;
+        const int h = w - bi * p.Hq, b = bi / p.Lq, i = bi - b * p.Lq;
+        float s = 0.f;
+        if (lane16 * 8 < D) {
+            const auto x = *reinterpret_cast<const typename AttnVec<T>::x8*>((const T*)p.dout + b * p.ds[0] + i * p.ds[1] + h * p.ds[2] + lane16 * 8);
+            const auto y = *reinterpret_cast<const typename AttnVec<T>::x8*>((const T*)p.o + (int64_t)w * D + lane16 * 8);
+            typename AttnVec<T>::x8 z = {};
+            if (p.rest) z = *reinterpret_cast<const typename AttnVec<T>::x8*>((const T*)p.rest + (int64_t)w * D + lane16 * 8);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    s += (float)x[e] * ((float)y[e] + (float)z[e]);
-                    const float a = fabsf((float)x[e]);
-                    if (live && a < INFINITY) top = fmaxf(top, a);
-                }
-            }
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o);
-            if (lane16 == 0) p.delta[stat] = s;
+            for (int e = 0; e < 8; ++e) s += (float)x[e] * ((float)y[e] + (float)z[e]);
         }
-    } else {
-        const uint32_t rows = (uint32_t)p.B * p.Lk * p.Hk;
-        for (uint32_t w = blockIdx.x * 16 + (threadIdx.x >> 4); w < rows; w += gridDim.x * 16) {
-            const uint32_t bj = w / p.Hk;
-            const int h = w - bj * p.Hk, b = bj / p.Lk, j = bj - b * p.Lk;
-            if (j >= attn_keys(p, b) || (p.kdoc && p.kdoc[b * p.kdoc_stride + j] < 0) || lane16 * 8 >= D) continue;
-            const auto x = *reinterpret_cast<const typename AttnVec<T>::x8*>((const T*)p.v + b * p.vs[0] + j * p.vs[1] + h * p.vs[2] + lane16 * 8);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float a = fabsf((float)x[e]);
-                if (a < INFINITY) top = fmaxf(top, a);
-            }
-        }
+        for (int o = 8; o > 0; o >>= 1) s += __shfl_xor(s, o);
+        if (lane16 == 0) p.delta[((int64_t)b * p.Hq + h) * p.Lq + i] = s;
     }
-    if (!p.maxima) return;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    __shared__ float tops[4];
-    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
-    __syncthreads();
-    if (threadIdx.x == 0) ((float*)p.maxima)[blockIdx.y * ATTN_MAXIMA + blockIdx.x] = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
 }
 
-// the exponent of ds's factor (0 without maxima); every wave computes it for itself
-__device__ __forceinline__ int attn_ds_scale(const AttnParams& p, int lane) {
-    if (!p.maxima) return 0;
-    float a = 0.f, c = 0.f;
+template <typename T>
+__device__ __forceinline__ void attn_pack(const f32x16& x, typename AttnVec<T>::x8 (&out)[2]) {
 #pragma unroll
-    for (int i = 0; i < ATTN_MAXIMA / 64; ++i) {
-        a = fmaxf(a, p.maxima[i * 64 + lane]);
-        c = fmaxf(c, p.maxima[ATTN_MAXIMA + i * 64 + lane]);
-    }
+    for (int c = 0; c < 2; ++c)
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        a = fmaxf(a, __shfl_xor(a, o));
-        c = fmaxf(c, __shfl_xor(c, o));
-    }
-    if (a == 0.f || c == 0.f) return 0;
-    // 2 D <= 2^8 and a < 2^(ilogb a + 1): ds 2^e < 2^15
-    const int e = 15 - 8 - (ilogbf(a) + 1) - (ilogbf(c) + 1);
-    return attn_uniform(e);
+        for (int e = 0; e < 8; ++e) out[c][e] = (T)x[8 * c + e];
 }
 
-// Raw score and dP of one element -> P 2^shift and ds 2^e (ds_by 1 where T needs no scaling: no multiplication then)
-template <typename T, int MODE>
+// This wave's 32 x 32 block of ds 2^e, to be rounded to float16: where a column's largest reaches 2, e falls, and the block and the column's accumulators with
+// it.  (Infinities and NaN pass: the result is one of them.)  2 is the number from which on the first bit of a float's exponent is set: a block without such a
+// column pays for eight or's and a ballot.  (Against one exponent for the whole call, training steps of 2 x 4096 causal, 16 heads on 4 x 32, 64, 128: 409 ->
+// 415, 513 -> 511, 781 -> 791 us; looking at the 16 maxima instead: 449, 523, 799.)
+template <int NB>
+__device__ __forceinline__ void attn_fit(f32x16& ds, int& e, f32x16 (&acc)[NB]) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) bits |= __builtin_bit_cast(uint32_t, (float)ds[r]);
+    if (__ballot((bits & 0x40000000u) != 0)) {
+        float top = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(ds[r]));
+        top = attn_half_max(top);                                         // (a column's queries or keys are in both halves)
+        const int by = (top >= 2.f) & (top < INFINITY) ? ilogbf(top) + 2 : 0;
+        const float shrink = ldexpf(1.f, -by);
+        e -= by;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) ds[r] *= shrink;
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][r] *= shrink;
+    }
+}
+
+// Raw score and dP of one element -> P 2^shift (in lse2) and, times ds_by, ds (SCALED false: ds_by is 1)
+template <int MODE, bool SCALED>
 __device__ __forceinline__ void attn_ds(f32x16& S, f32x16& dP, int r, const AttnScore& f, float ds_by, float lse2, float delta, float dist) {
     float u, d = dP[r] - delta;
     if constexpr (MODE == ATTN_CAP || MODE == ATTN_CAP_BIAS) {
@@ -99,18 +86,10 @@ __device__ __forceinline__ void attn_ds(f32x16& S, f32x16& dP, int r, const Attn
     }
     if constexpr (MODE == ATTN_BIAS || MODE == ATTN_CAP_BIAS) u -= f.slope * fabsf(dist);
     S[r] = __builtin_amdgcn_exp2f(u);
-    if constexpr (ATTN_P_SHIFT<T> != 0.f) d *= ds_by;
+    if constexpr (SCALED) d *= ds_by;
     dP[r] = S[r] * d;
 }
 template <int MODE> static constexpr float attn_ds_unit() { return MODE == ATTN_CAP || MODE == ATTN_CAP_BIAS ? 4.f : 1.f; }
-
-template <typename T>
-__device__ __forceinline__ void attn_pack(const f32x16& x, typename AttnVec<T>::x8 (&out)[2]) {
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) out[c][e] = (T)x[8 * c + e];
-}
 
 // P and ds / scale of one (query, key) pair, plain arithmetic
 template <typename T>
@@ -175,8 +154,8 @@ __device__ __forceinline__ void attn_dq(const AttnParams& p, int group, char* sm
     const T* v = (const T*)p.v + b * p.vs[0] + hk * p.vs[2];
     const int* kdoc = DOCS ? p.kdoc + b * p.kdoc_stride : nullptr;
     const AttnScore f(p, h);
-    const int ds_exp = attn_ds_scale(p, lane);
-    const float ds_by = ldexpf(1.f, ds_exp);
+    constexpr bool FIT = ATTN_P_SHIFT<T> != 0.f;
+    int ds_exp = FIT ? ATTN_DS_EXP : 0;                                 // (2^e in the weights: a lane's column is one query)
     AttnStage<ROW, ATTN_TILE, 4> sk, sv;
     sk.setup(wave, lane, p.ks[1], p.D);
     sv.setup(wave, lane, p.vs[1], p.D);
@@ -235,9 +214,9 @@ __device__ __forceinline__ void attn_dq(const AttnParams& p, int group, char* sm
                     for (int c = 0; c < 2; ++c) cf[db][c] = attn_col_frag<T, ROW>(kc_lds, 2 * kb + c, db);
                 __builtin_amdgcn_sched_barrier(0);
                 const int jb = j0 + 32 * kb + 4 * half;
-                const float dist = (float)(i + n - p.Lq - jb);
+                const float dist = (float)(i + n - p.Lq - jb), less = FIT ? lse2 - (float)ds_exp : lse2;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) attn_ds<T, MODE>(S, dP, r, f, ds_by, lse2, delta, dist - (float)(8 * (r >> 2) + (r & 3)));
+                for (int r = 0; r < 16; ++r) attn_ds<MODE, false>(S, dP, r, f, 1.f, less, delta, dist - (float)(8 * (r >> 2) + (r & 3)));
                 if constexpr (mask.value) {
                     const int last = lim - jb;
 #pragma unroll
@@ -252,6 +231,7 @@ __device__ __forceinline__ void attn_dq(const AttnParams& p, int group, char* sm
                             dP[4 * a + 3] = o.w == qdoc ? dP[4 * a + 3] : 0.f;
                         }
                 }
+                if constexpr (FIT) attn_fit(dP, ds_exp, acc);
                 attn_pack<T>(dP, d);
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
@@ -324,14 +304,14 @@ __device__ __forceinline__ void attn_dq(const AttnParams& p, int group, char* sm
 // hand: 555).  There two waves share 32 keys (attn_dkv_pair): each takes the scores of half of a tile's queries, they trade the 16-bit weights through the
 // LDS, and each adds up half of the channels over all of the queries.
 template <typename T, int DB, int MODE, bool DOCS>
-__device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* smem, AttnRows& rows, int (*sdoc)[ATTN_TILE], char* traded) {
+__device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* smem, AttnRows& rows, int (*sdoc)[ATTN_TILE], char* traded, int (*exps)[64]) {
     constexpr int ROW = attn_row<DB>(), TILE_BYTES = ATTN_TILE * ROW * 2;
     constexpr float SHIFT = ATTN_P_SHIFT<T>;
-    constexpr bool PAIR = attn_dkv_pair<DB>();
+    constexpr bool PAIR = attn_dkv_pair<DB>(), FIT = SHIFT != 0.f;
     constexpr int NB = PAIR ? DB / 2 : DB;                              // blocks of 32 channels a wave adds up
     constexpr bool LEFT = !PAIR && (DB < 3 || !DOCS);                   // attn_left_over, where registers are left for it
     typedef typename AttnVec<T>::x8 frag;
-    // smem: [buffer][q, do];  traded (pairs): [key group][half of the queries][w, w, d, d][lane] fragments
+    // smem: [buffer][q, do];  traded (pairs): [key group][half of the queries][w, w, d, d][lane] fragments;  exps: [key group][half][lane], their ds_exp
     const int wave = attn_uniform(threadIdx.x >> 6), keys = PAIR ? wave & 3 : wave, part = PAIR ? wave >> 2 : 0, lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
     // p.k_splits: 1 (a workgroup adds up all heads of the group), or float32 parts that attn_parts_kernel adds in order: the heads of the group in
     // p.k_splits / p.chunks equal runs, the queries in p.chunks runs of whole tiles
@@ -384,8 +364,7 @@ __device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* s
     AttnStage<ROW, ATTN_TILE, PAIR ? 8 : 4> sq, sd;
     sq.setup(wave, lane, p.qs[1], p.D);
     sd.setup(wave, lane, p.ds[1], p.D);
-    const int ds_exp = attn_ds_scale(p, lane);
-    const float ds_by = ldexpf(1.f, ds_exp - (int)SHIFT);
+    int ds_exp = FIT ? ATTN_DS_EXP : 0;                                 // (a lane's column is one key; the two waves of a pair keep theirs alike)
     const AttnLane<ROW> at_lane(lane);
     const uint32_t lds = attn_lds(smem);
     float row_next = 0.f;
@@ -460,13 +439,13 @@ __device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* s
             ahead();
             __builtin_amdgcn_sched_barrier(0);
             const int ib = 32 * qb + 4 * half;
-            const float dist = (float)(i0 + ib + off - j);
+            const float dist = (float)(i0 + ib + off - j), ds_by = FIT ? ldexpf(1.f, ds_exp - (int)SHIFT) : 1.f;
 #pragma unroll
             for (int a = 0; a < 4; ++a) {
                 const float4 l4 = *reinterpret_cast<const float4*>(&rows.lse[now][ib + 8 * a]), e4 = *reinterpret_cast<const float4*>(&rows.delta[now][ib + 8 * a]);
                 const float l[4] = {l4.x, l4.y, l4.z, l4.w}, de[4] = {e4.x, e4.y, e4.z, e4.w};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) attn_ds<T, MODE>(S, dP, 4 * a + e, f, ds_by, l[e], de[e], dist + (float)(8 * a + e));
+                for (int e = 0; e < 4; ++e) attn_ds<MODE, FIT>(S, dP, 4 * a + e, f, ds_by, l[e], de[e], dist + (float)(8 * a + e));
             }
             if constexpr (mask.value) {
                 const int first = qmin - i0 - ib;
@@ -489,6 +468,7 @@ __device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* s
                         }
                     }
             }
+            if constexpr (FIT) attn_fit(dP, ds_exp, dk);
             attn_pack<T>(S, w);
             attn_pack<T>(dP, d);
             if (mask.value && LEFT && fine)
@@ -517,6 +497,7 @@ __device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* s
                     mine[c * 64] = w[c];
                     mine[(2 + c) * 64] = d[c];
                 }
+                if constexpr (FIT) exps[keys * 2 + part][lane] = ds_exp;
                 products(w, d, qc, dc);
                 columns(part ^ 1, qc, dc);
             }
@@ -526,6 +507,21 @@ __device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* s
                 for (int c = 0; c < 2; ++c) {
                     w[c] = theirs[c * 64];
                     d[c] = theirs[(2 + c) * 64];
+                }
+                if constexpr (FIT) {                                    // the lower of the two exponents for both
+                    const int other = exps[keys * 2 + (part ^ 1)][lane], low = min(ds_exp, other);
+                    if (__ballot(other != ds_exp)) {
+                        const float by = ldexpf(1.f, low - ds_exp), their = ldexpf(1.f, low - other);
+                        ds_exp = low;
+#pragma unroll
+                        for (int db = 0; db < NB; ++db)
+#pragma unroll
+                            for (int r = 0; r < 16; ++r) dk[db][r] *= by;
+#pragma unroll
+                        for (int c = 0; c < 2; ++c)
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) d[c][e] = (T)((float)d[c][e] * their);
+                    }
                 }
                 products(w, d, qc, dc);
             }
@@ -640,7 +636,8 @@ __global__ __launch_bounds__(attn_dkv_pair<DB>() ? 512 : 256, 2) void attn_dkv_k
     __shared__ __align__(16) AttnRows rows;
     __shared__ __align__(16) int sdoc[2][ATTN_TILE];
     __shared__ __align__(16) char traded[attn_dkv_pair<DB>() ? 4 * 2 * 4 * 1024 : 16];
-    attn_dkv<T, DB, MODE, DOCS>(p, blockIdx.x, smem, rows, sdoc, traded);
+    __shared__ int exps[attn_dkv_pair<DB>() && ATTN_P_SHIFT<T> != 0.f ? 8 : 1][64];
+    attn_dkv<T, DB, MODE, DOCS>(p, blockIdx.x, smem, rows, sdoc, traded, exps);
 #endif
 }
 // Both in one launch where that is two rounds of the chip at most (1024 workgroups): small calls wait for single workgroups, and so for both kinds at once.
@@ -654,7 +651,7 @@ __global__ __launch_bounds__(256, 2) void attn_grads_kernel(AttnParams p) {
     __shared__ __align__(16) AttnRows rows;
     __shared__ __align__(16) int sdoc[2][ATTN_TILE];
     if ((int)blockIdx.x < p.first_k) attn_dq<T, DB, MODE, DOCS>(p, blockIdx.x, smem, sdoc);
-    else attn_dkv<T, DB, MODE, DOCS>(p, blockIdx.x - p.first_k, smem, rows, sdoc, nullptr);
+    else attn_dkv<T, DB, MODE, DOCS>(p, blockIdx.x - p.first_k, smem, rows, sdoc, nullptr, nullptr);
 #endif
 }
 
@@ -679,8 +676,7 @@ __global__ __launch_bounds__(256) void attn_parts_kernel(const float* __restrict
 template <typename T, int DB, int MODE, bool DOCS>
 static void attn_bwd_launch(AttnParams& p, hipStream_t stream) {
     const int64_t q_rows = (int64_t)p.B * p.Lq * p.Hq, k_rows = (int64_t)p.B * p.Lk * p.Hk;
-    const int prep = p.maxima ? ATTN_MAXIMA : (int)(cdiv64(q_rows, 16) < 2048 ? cdiv64(q_rows, 16) : 2048);
-    hipLaunchKernelGGL((attn_prep_kernel<T>), dim3(prep, p.maxima ? 2 : 1), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((attn_prep_kernel<T>), dim3((unsigned)(cdiv64(q_rows, 16) < 2048 ? cdiv64(q_rows, 16) : 2048)), dim3(256), 0, stream, p);
     auto add = [&](const float* part, int count, int64_t all, void* a, void* b) {
         if (count > 1) hipLaunchKernelGGL((attn_parts_kernel<T>), dim3((unsigned)cdiv64(all, 2048), b ? 2 : 1), dim3(256), 0, stream, part, count, all, (T*)a, (T*)b);
     };

@@ -19,16 +19,15 @@ static void attn_bwd_split(AttnParams& p) {
     p.k_splits = heads * p.chunks;
 }
 
-// Where the workspace's parts lie, in floats: document ranges and order, delta, maxima (float16), parts of dq, parts of dk and dv, the end
+// Where the workspace's parts lie, in floats: document ranges and order, delta, parts of dq, parts of dk and dv, the end
 struct AttnBwdSpace {
-    int64_t delta, maxima, part, k_part, end;
+    int64_t delta, part, k_part, end;
 };
-static AttnBwdSpace attn_bwd_plan(AttnParams& p, int dtype) {
+static AttnBwdSpace attn_bwd_plan(AttnParams& p) {
     attn_bwd_split(p);
     AttnBwdSpace at;
     at.delta = (attn_range_floats(p) + 3) / 4 * 4;
-    at.maxima = at.delta + ((int64_t)p.B * p.Hq * p.Lq + 3) / 4 * 4;
-    at.part = at.maxima + (dtype == N3D_F16 ? 2 * ATTN_MAXIMA : 0);
+    at.part = at.delta + ((int64_t)p.B * p.Hq * p.Lq + 3) / 4 * 4;
     at.k_part = at.part + (p.splits > 1 ? (int64_t)p.splits * p.B * p.Lq * p.Hq * p.D : 0);
     at.end = at.k_part + (p.k_splits > 1 ? 2 * (int64_t)p.k_splits * p.B * p.Lk * p.Hk * p.D : 0);
     return at;
@@ -39,7 +38,7 @@ extern "C" int64_t n3d_attention_bwd_workspace(const n3d_attention_desc* d) {
     const char* bad = attn_params(d, p);
     N3D_CHECK(!bad, "attention_bwd: %s", bad);
     if (p.B == 0 || p.Lq == 0) return 0;
-    return 4 * attn_bwd_plan(p, d->dtype).end;
+    return 4 * attn_bwd_plan(p).end;
 }
 
 extern "C" int n3d_attention_bwd(const n3d_attention_desc* d, n3d_stream_t stream_) {
@@ -53,13 +52,12 @@ extern "C" int n3d_attention_bwd(const n3d_attention_desc* d, n3d_stream_t strea
     for (int i = 0; i < 3; ++i)
         N3D_CHECK(d->dout_strides[i] % 8 == 0 && d->dout_strides[i] >= 0 && (i != 1 || d->dout_strides[i] <= (1 << 23)), "attention_bwd: strides must be multiples of 8 elements, of tokens 2^23 at most");
     N3D_CHECK(((uintptr_t)d->dout | (uintptr_t)d->dq | (uintptr_t)d->dk | (uintptr_t)d->dv) % 16 == 0, "attention_bwd: tensors must be 16-byte aligned");
-    const AttnBwdSpace at = attn_bwd_plan(p, d->dtype);
+    const AttnBwdSpace at = attn_bwd_plan(p);
     const int64_t need = 4 * at.end;
     N3D_CHECK(d->workspace && d->workspace_bytes >= need && (uintptr_t)d->workspace % 16 == 0, "attention_bwd: a workspace of %lld bytes is needed (16-byte aligned)", (long long)need);
     float* ws = (float*)d->workspace;
     p.dout = d->dout; p.dq = d->dq; p.dk = d->dk; p.dv = d->dv;
     p.delta = ws + at.delta;
-    p.maxima = d->dtype == N3D_F16 ? ws + at.maxima : nullptr;
     p.part = ws + at.part;
     p.k_part = ws + at.k_part;
     const double pairs = (double)p.B * p.Hq * p.Lq * p.Lk * p.D;

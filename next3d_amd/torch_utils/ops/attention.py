@@ -27,9 +27,8 @@ def attention(q, k, v, scale=None, causal=False, prefix=None, documents=None, ke
     negative number belongs to none (padding).  Rows that see nothing are 0, with lse -inf, and have no gradient.  What a row does not see does not reach
     it, not even NaN or infinity.
 
-    Softmax statistics and sums are float32; weights (and in the backward pass dscores) are rounded to the inputs' type for the matrix cores.  In float16
-    the dscores of a call share one power of two, taken from its largest gradient and value: rows whose gradients are 2^-12 of the largest or smaller lose
-    digits (bfloat16's do not).  Differentiable (once) in q, k and v, not through the logarithms; results and gradients are bitwise reproducible."""
+    Softmax statistics and sums are float32; weights (and in the backward pass dscores) are rounded to the inputs' type for the matrix cores.  float16
+    dscores take a power of two of each query's own (of each key's own for dk), so gradients of any size keep their digits.  Differentiable (once) in q, k and v, not through the logarithms; results and gradients are bitwise reproducible."""
     types = (torch.float16, torch.bfloat16)
     require_tensor('attention', 'q', q, types, 4)
     for name, t in (('k', k), ('v', v)):

@@ -529,3 +529,66 @@ def test_attention_of_few_queries_is_rounded_once(dev, dtype):
         inner = tols['out'] - first + 2 * u * u * mean                          # ... here the rounding of a left-over, and what is float32
         own = (exact.to(dtype).double() - exact).abs()                          # the exact result's own rounding; the nearest of exact + e is within own + 2 e
         assert bool(((out - exact).abs() <= own + 2 * inner).all()), size
+
+
+def _gradients64(q, k, v, do, see):
+    """dq, dk [L, D] of one head in float64, and the expected squared error of each row from rounding every dscore to float16 (half a step, 2^-11 of it at
+    most, is uniform: a third of the square) and the result once."""
+    q, k, v, do = (t.double() for t in (q, k, v, do))
+    scale = q.shape[1] ** -0.5
+    p = torch.softmax((q @ k.t() * scale).masked_fill(~see, float('-inf')), 1)
+    dp = do @ v.t()
+    ds = p * (dp - (p * dp).sum(1, keepdim=True)) * scale
+    dq, dk = ds @ k, ds.t() @ q
+    third = 2.0 ** -22 / 3
+    row = lambda ds, x, g: third * (ds.square() @ x.square().sum(1) + g.square().sum(1)) + g.shape[1] * 2.0 ** -50          # (2^-25: half a step near zero)
+    return dq, dk, row(ds, k, dq), row(ds.t(), q, dk)
+
+
+@pytest.mark.parametrize('d', [64, 128])
+@pytest.mark.parametrize('causal', [False, True])
+def test_attention_float16_gradients_of_different_sizes(dev, causal, d):
+    """Rows whose gradients are 2^-6 .. 2^-12 of the largest, beside it and in another document, keep their digits: the errors' norms are within twice what the
+    roundings of the dscores and of the results make (they are thousands of independent ones)."""
+    n = 4096
+    q, k, v, do = _inputs(1, n, n, 1, 1, d, F16, 111)
+    sizes = torch.tensor([8.0, 2.0, -2.0, -4.0]).exp2()
+    which = torch.arange(n) % 4
+    ids = (torch.arange(n) >= 1800).to(torch.int32)[None]
+    see = torch.ones(n, n, dtype=torch.bool)
+    see = see.tril() if causal else see
+    for what, size, docs in (('rows', sizes[which], None), ('documents', sizes[3 * ids[0].long()], ids)):
+        g = (do.float() * size[None, :, None, None]).to(F16)
+        got = _run(dev, q, k, v, g, causal=causal, documents=docs)
+        seen = see if docs is None else see & (ids[0][:, None] == ids[0][None])
+        dq, dk, e_dq, e_dk = _gradients64(q[0, :, 0], k[0, :, 0], v[0, :, 0], g[0, :, 0], seen)
+        for s in sizes.unique():
+            rows = size == s
+            if not bool(rows.any()):
+                continue
+            pairs = [('dq', dq, e_dq)] + ([('dk', dk, e_dk)] if docs is not None else [])
+            for name, want, var in pairs:
+                err = float((got[name][0, :, 0].cpu().double() - want)[rows].norm())
+                assert err <= 2 * float(var[rows].sum()) ** 0.5 + 1e-5 * float(want[rows].norm()), (what, name, float(s), err, float(want[rows].norm()))
+
+
+def test_attention_float16_gradients_do_not_depend_on_what_is_not_seen(dev):
+    """Large gradients and values of another sequence, of another document or behind the diagonal change no bit of a row's gradients."""
+    n = 1500
+    for d in (64, 128):
+        q, k, v, do = _inputs(2, n, n, 2, 1, d, F16, 112)
+        ids = (torch.arange(n) >= 700).to(torch.int32).repeat(2, 1)
+        lo, hi = slice(0, 700), slice(700, n)
+        for kw, spoil, keep in ((dict(), (0, slice(0, n)), (1, slice(0, n))), (dict(documents=ids), (slice(0, 2), hi), (slice(0, 2), lo)),
+                                (dict(documents=ids, causal=True), (slice(0, 2), lo), (slice(0, 2), hi))):
+            plain = _run(dev, q, k, v, do, **kw)
+            big_v, big_do = v.clone(), do.clone()
+            big_v[spoil][..., 3] = 60000.0
+            big_do[spoil][..., 5] = 30000.0
+            got = _run(dev, q, k, big_v, big_do, **kw)
+            for name in ('out', 'dq', 'dk', 'dv'):
+                assert torch.equal(got[name][keep], plain[name][keep]), (d, sorted(kw), name)
+        big_v = v.clone()
+        big_v[:, hi] *= 10000.0
+        plain, got = _run(dev, q, k, v, do, causal=True), _run(dev, q, k, big_v, do, causal=True)
+        assert all(torch.equal(got[name][:, lo], plain[name][:, lo]) for name in ('out', 'dq'))
