@@ -255,24 +255,94 @@ struct AttnTiles {
     }
 };
 
-// visible to a scalar pass over single keys (the repair of rows that a masked NaN or infinity has reached through 0 * NaN in a matrix product)
-__device__ __forceinline__ bool attn_visible(const AttnParams& p, int b, int j, int lim, int qdoc) {
-    return j <= lim && (!p.kdoc || (qdoc >= 0 && p.kdoc[b * p.kdoc_stride + j] == qdoc));
-}
-template <typename T>
-__device__ __forceinline__ float attn_dot(const T* a, const T* c, int D) {
-    float s = 0.f;
-    for (int d = 0; d < D; d += 8) {
-        const auto x = *reinterpret_cast<const typename AttnVec<T>::x8*>(a + d), y = *reinterpret_cast<const typename AttnVec<T>::x8*>(c + d);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) s += (float)x[e] * (float)y[e];
-    }
-    return s;
-}
-// base-2 score of raw product s at distance `dist`
-__device__ __forceinline__ float attn_score(const AttnScore& f, float s, int dist) {
+// base-2 score of raw product s at distance `dist`, in any form
+__device__ __forceinline__ float attn_score(const AttnScore& f, float s, float dist) {
     const float u = f.cap_out > 0.f ? f.capped(f.cap_r(s), 0.f) : s * f.mul;
-    return u - f.slope * fabsf((float)dist);
+    return u - f.slope * fabsf(dist);
+}
+
+// ---- infinities and NaN.  A masked weight is zero, but zero times them is NaN in a matrix product.  Where an accumulator ends as NaN, the workgroup's waves
+// take their sums again, each its own 32 columns through its own LDS (attn_out_again, attn_dq_again, attn_dkv_again).  They walk three times, with the products'
+// first operands changed in the LDS: ones where a tile holds NaN or infinities of one sign, and ones for the visible pairs as second operands, say what reaches
+// a sum; then zeros in their places.  The functions are not inlined (inside the kernels they cost these their registers) and serve every form of the scores;
+// a call pays one barrier for them; a training step of 4096 x 4 heads on 2, causal, in which one key of v is NaN takes 9 (64 channels) to 19 (128) times as long.
+enum { ATTN_FINITE = 0, ATTN_PLUS = 1, ATTN_MINUS = -1, ATTN_EITHER = 2 };      // what is left of a tile: finite values; ones at NaN and +inf, -inf, both
+template <typename T> struct AttnBits;
+template <> struct AttnBits<_Float16> { static constexpr short INF = 0x7c00, ONE = 0x3c00; };
+template <> struct AttnBits<__bf16> { static constexpr short INF = 0x7f80, ONE = 0x3f80; };
+typedef short attn_s16x8 __attribute__((ext_vector_type(8)));
+template <typename T, int BYTES>
+__device__ __forceinline__ void attn_change(uint32_t tile, int lane, int kind) {
+    typedef __attribute__((address_space(3))) attn_s16x8* ptr;
+#pragma unroll 1
+    for (int at = lane * 16; at < BYTES; at += 1024) {
+        attn_s16x8 v = *(ptr)(uintptr_t)(tile + at);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int size = v[e] & 0x7fff;
+            const bool hit = size > AttnBits<T>::INF || (size == AttnBits<T>::INF && (kind == ATTN_EITHER || (v[e] < 0) == (kind == ATTN_MINUS)));
+            if (kind == ATTN_FINITE) v[e] = size >= AttnBits<T>::INF ? (short)0 : v[e];
+            else v[e] = hit ? AttnBits<T>::ONE : (short)0;
+        }
+        *(ptr)(uintptr_t)(tile + at) = v;
+    }
+}
+// ones at the registers of `seen`
+template <typename T>
+__device__ __forceinline__ void attn_ones(uint32_t seen, typename AttnVec<T>::x8 (&out)[2]) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        attn_s16x8 v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = seen >> (8 * c + e) & 1 ? AttnBits<T>::ONE : (short)0;
+        out[c] = __builtin_bit_cast(typename AttnVec<T>::x8, v);
+    }
+}
+// a bit for every accumulator that counted something, and what that adds to the sums of another walk
+template <int N> struct AttnMarks {
+    uint32_t bits[(N + 1) / 2];
+    __device__ __forceinline__ void take(const f32x16 (&count)[N]) {
+#pragma unroll
+        for (int i = 0; i < (N + 1) / 2; ++i) bits[i] = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) bits[i >> 1] |= count[i][r] > 0.f ? 1u << ((i & 1) * 16 + r) : 0u;
+    }
+    __device__ __forceinline__ void add(f32x16 (&acc)[N], float x) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][r] += bits[i >> 1] >> ((i & 1) * 16 + r) & 1 ? x : 0.f;
+    }
+};
+// the parameters of the running kernel, where a function that is not inlined finds them (a copy on the stack would be scratch memory of every lane)
+typedef const __attribute__((address_space(4))) AttnParams* attn_args;
+__device__ __forceinline__ attn_args attn_kernel_args() { return (attn_args)__builtin_amdgcn_kernarg_segment_ptr(); }
+template <int N>
+__device__ __forceinline__ void attn_clear(f32x16 (&acc)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = f32x16{};
+}
+// does any wave of the workgroup say yes?  (`said`: one word a wave; all of them are behind their last tile then)
+template <int WAVES>
+__device__ __forceinline__ bool attn_any(bool yes, int wave, uint32_t (&said)[WAVES]) {
+    const uint64_t mine = __ballot(yes);
+    if ((threadIdx.x & 63) == 0) said[wave] = mine != 0;
+    __syncthreads();
+    uint32_t all = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) all |= said[w];
+    return __builtin_expect(attn_uniform(all) != 0, 0);
+}
+template <int N>
+__device__ __forceinline__ bool attn_has_nan(const f32x16 (&acc)[N]) {
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) nan = nan || acc[i][r] != acc[i][r];
+    return nan;
 }
 
 // a row's 32 * DB channels spread over lanes l31 and l31 + 32 -> 16-byte stores (the halves trade their 8-byte runs).  REST: what the rounding left over

@@ -61,7 +61,7 @@ __device__ __forceinline__ void attn_fit(f32x16& ds, int& e, f32x16 (&acc)[NB]) 
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(ds[r]));
         top = attn_half_max(top);                                         // (a column's queries or keys are in both halves)
-        const int by = (top >= 2.f) & (top < INFINITY) ? ilogbf(top) + 2 : 0;
+        const int by = top >= 2.f && top < INFINITY ? ilogbf(top) + 2 : 0;
         const float shrink = ldexpf(1.f, -by);
         e -= by;
 #pragma unroll
@@ -91,18 +91,12 @@ __device__ __forceinline__ void attn_ds(f32x16& S, f32x16& dP, int r, const Attn
 }
 template <int MODE> static constexpr float attn_ds_unit() { return MODE == ATTN_CAP || MODE == ATTN_CAP_BIAS ? 4.f : 1.f; }
 
-// P and ds / scale of one (query, key) pair, plain arithmetic
-template <typename T>
-__device__ __forceinline__ void attn_pair(const AttnParams& p, const AttnScore& f, const T* q, const T* k, const T* v, const T* dout, float lse2, float delta, int dist,
-                                          float& w, float& ds) {
-    const float s = attn_dot<T>(q, k, p.D);
-    const float x = f.cap_out > 0.f ? f.cap_r(s) : 0.5f;
-    w = __builtin_amdgcn_exp2f(attn_score(f, s, dist) - lse2);
-    ds = w * (attn_dot<T>(dout, v, p.D) - delta) * 4.f * (x - x * x);
-}
 __device__ __forceinline__ float attn_lse2(float lse) { return lse == -INFINITY ? INFINITY : lse * ATTN_LOG2E; }       // (a row that sees nothing: every weight 0)
 
 template <int DB> static constexpr bool attn_dkv_pair() { return DB > 3; }      // (see attn_dkv)
+// waves a SIMD that the registers of these kernels, and of what they call, leave room for (256 threads; pairs: one workgroup of 512 a CU)
+template <int DB, bool DOCS> static constexpr int attn_dq_waves() { return DB < 2 || (DB < 3 && !DOCS) ? 3 : 2; }
+template <int DB> static constexpr int attn_dkv_waves() { return DB < 2 ? 3 : 2; }
 // what both kinds of workgroups keep in the LDS
 template <int DB> static constexpr int attn_row() { return DB > 2 ? 128 : 64; }
 template <int DB> static constexpr int attn_lds_bytes() { return 4 * ATTN_TILE * attn_row<DB>() * 2; }
@@ -111,8 +105,210 @@ struct AttnRows {
 };
 
 #ifdef __HIP_DEVICE_COMPILE__                            // (hipcc drops the launch stub of a template whose body its host pass cannot read)
-template <typename T, int DB, int MODE, bool DOCS>
-__device__ __forceinline__ void attn_dq(const AttnParams& p, int group, char* smem, int (*sdoc)[ATTN_TILE]) {
+// P 2^shift (in lse2) and ds 2^e / scale (in ds_by) of one pair from its raw products, in any form of the scores
+__device__ __forceinline__ void attn_pair(const AttnScore& f, float s, float dp, float lse2, float delta, float ds_by, float dist, float& w, float& ds) {
+    const float x = f.cap_out > 0.f ? f.cap_r(s) : 0.5f;
+    w = __builtin_amdgcn_exp2f(attn_score(f, s, dist) - lse2);
+    ds = w * ((dp - delta) * ds_by * 4.f * __builtin_fmaf(-x, x, x));
+}
+template <typename T, int DB>
+__device__ __forceinline__ void attn_dq_store(const AttnParams& p, const f32x16 (&acc)[DB], float unit, int ds_exp, int b, int i, int h, int split, int half, bool row_ok) {
+    const float by = ldexpf(p.scale * unit, -ds_exp);
+    const int64_t row_at = ((int64_t)(b * (int64_t)p.Lq + i) * p.Hq + h) * p.D, all = (int64_t)p.B * p.Lq * p.Hq * p.D;
+    if (p.splits > 1) attn_store_part<DB>(p.part + split * all + row_at, acc, by, half, p.D, row_ok);
+    else attn_store_row<T, DB>((T*)p.dq + row_at, acc, by, half, p.D, row_ok);
+}
+// NB blocks of channels from 64 part on
+template <typename T, int NB>
+__device__ __forceinline__ void attn_dkv_store(const AttnParams& p, const f32x16 (&dk)[NB], const f32x16 (&dv)[NB], float unit, int ds_exp, int b, int j, int hk, int split, int part, int half, bool store) {
+    const float k_by = ldexpf(p.scale * unit, -ds_exp), v_by = ldexpf(1.f, -(int)ATTN_P_SHIFT<T>);
+    const int64_t row = ((int64_t)b * p.Lk + j) * p.Hk + hk, all = (int64_t)p.B * p.Lk * p.Hk;
+    if (p.k_splits > 1) {
+        float* pk = p.k_part + (2 * split * all + row) * p.D;
+        float* pv = p.k_part + ((2 * split + 1) * all + row) * p.D;
+        attn_store_part<NB>(pk + 64 * part, dk, k_by, half, p.D - 64 * part, store);
+        attn_store_part<NB>(pv + 64 * part, dv, v_by, half, p.D - 64 * part, store);
+    } else {
+        attn_store_row<T, NB>((T*)p.dk + row * p.D + 64 * part, dk, k_by, half, p.D - 64 * part, store);
+        attn_store_row<T, NB>((T*)p.dv + row * p.D + 64 * part, dv, v_by, half, p.D - 64 * part, store);
+    }
+}
+// A wave's sums once more (attention.h: infinities and NaN).  WAVES (a SIMD's) keeps the copies of kernels with different registers apart.
+// dq of 32 queries over the keys [first, end)
+template <typename T, int DB, int WAVES>
+static __device__ __attribute__((noinline)) void attn_dq_again(attn_args args, int b, int i, int h, bool row_ok, int split, int first, int end, uint32_t lds) {
+    constexpr int ROW = attn_row<DB>(), KEYS = 32, BYTES = KEYS * ROW * 2;
+    constexpr bool FIT = ATTN_P_SHIFT<T> != 0.f;
+    const AttnParams p = *args;
+    const int lane = threadIdx.x & 63, half = lane >> 5, hk = attn_uniform(h / p.G);
+    const int n = attn_keys(p, b), at = i + n - p.Lq;
+    const int qdoc = p.kdoc && row_ok ? p.qdoc[b * p.qdoc_stride + i] : 0;
+    const int lim = !row_ok || qdoc < 0 ? -1 : attn_limit(p, i, n, p.prefix ? p.prefix[b] : 0);
+    const T* q = row_ok ? (const T*)p.q + b * p.qs[0] + i * p.qs[1] + h * p.qs[2] : nullptr;
+    const T* dout = row_ok ? (const T*)p.dout + b * p.ds[0] + i * p.ds[1] + h * p.ds[2] : nullptr;
+    const int64_t stat = ((int64_t)b * p.Hq + h) * p.Lq + i;
+    const float lse2 = row_ok ? attn_lse2(p.lse[stat]) : INFINITY, delta = row_ok ? p.delta[stat] : 0.f;
+    const uint64_t k = attn_addr((const T*)p.k + b * p.ks[0] + hk * p.ks[2]), v = attn_addr((const T*)p.v + b * p.vs[0] + hk * p.vs[2]);
+    const AttnScore f(p, h);
+    AttnStage<ROW, KEYS, 1> sk, sv;
+    sk.setup(0, lane, p.ks[1], p.D);
+    sv.setup(0, lane, p.vs[1], p.D);
+    const AttnLane<ROW> at_lane(lane);
+    struct {
+        f32x16 dk[DB];
+        int ds_exp;
+    } g;
+    AttnMarks<DB> either;                                               // (an infinity of a key too: its pair's score is not finite then, and ds 0 or NaN)
+#pragma unroll 1
+    for (int walk = 0; walk < 2; ++walk) {
+        const int kind = walk == 0 ? ATTN_EITHER : ATTN_FINITE;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) g.dk[db] = f32x16{};
+        g.ds_exp = FIT ? ATTN_DS_EXP : 0;
+#pragma unroll 1
+        for (int j0 = first; j0 < end; j0 += KEYS) {
+            uint32_t seen = 0;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int j = j0 + 4 * half + 8 * (r >> 2) + (r & 3);
+                if (j <= lim && (!p.kdoc || p.kdoc[b * p.kdoc_stride + j] == qdoc)) seen |= 1u << r;
+            }
+            if (!__ballot(seen != 0)) continue;
+            attn_landed();                                              // (the LDS reads of the tile before)
+            sk.issue(k, j0 / KEYS, n, (int)p.ks[1], p.D, lds, 0);
+            sv.issue(v, j0 / KEYS, n, (int)p.vs[1], p.D, lds + BYTES, 0);
+            attn_landed();
+            typename AttnVec<T>::x8 d[2];
+            if (kind == ATTN_FINITE) {
+                const uint32_t k_lds = at_lane.rows(lds), v_lds = at_lane.rows(lds + BYTES);
+                f32x16 S = {}, dP = {};
+#pragma unroll
+                for (int c = 0; c < 2 * DB; ++c) S = attn_mfma(attn_row_frag<T, ROW>(k_lds, 0, c), attn_lane_frag<T>(q, 2 * c + half, p.D), S);
+#pragma unroll
+                for (int c = 0; c < 2 * DB; ++c) dP = attn_mfma(attn_row_frag<T, ROW>(v_lds, 0, c), attn_lane_frag<T>(dout, 2 * c + half, p.D), dP);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    float w, ds;
+                    attn_pair(f, S[r], dP[r], lse2 - (float)g.ds_exp, delta, 1.f, (float)(at - (j0 + 4 * half + 8 * (r >> 2) + (r & 3))), w, ds);
+                    dP[r] = seen >> r & 1 ? ds : 0.f;
+                }
+                if constexpr (FIT) attn_fit(dP, g.ds_exp, g.dk);
+                attn_pack<T>(dP, d);
+            } else {
+                attn_ones<T>(seen, d);
+            }
+            attn_landed();
+            attn_change<T, BYTES>(lds, lane, kind);
+            attn_landed();
+            const uint32_t kc_lds = at_lane.cols(lds);
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) g.dk[db] = attn_mfma(attn_col_frag<T, ROW>(kc_lds, c, db), d[c], g.dk[db]);
+        }
+        if (walk == 0) either.take(g.dk);
+    }
+    either.add(g.dk, NAN);
+    attn_dq_store<T, DB>(p, g.dk, 1.f, g.ds_exp, b, i, h, split, half, row_ok);
+}
+// dk and dv of 32 keys, NB blocks of channels from 32 NB part on, over the queries [first, end) of the heads [g0, g1) of their group
+template <typename T, int DB, int NB, int WAVES>
+static __device__ __attribute__((noinline)) void attn_dkv_again(attn_args args, int b, int hk, int j, int kdoc, int split, int g0, int g1, int first, int end, int part, uint32_t lds) {
+    constexpr int ROW = attn_row<DB>(), ROWS = 32, BYTES = ROWS * ROW * 2;
+    constexpr float SHIFT = ATTN_P_SHIFT<T>;
+    constexpr bool FIT = SHIFT != 0.f;
+    const AttnParams p = *args;
+    const int lane = threadIdx.x & 63, half = lane >> 5, n = attn_keys(p, b), off = n - p.Lq;
+    const bool key_ok = j < n && kdoc >= 0;
+    const int qmin = !key_ok ? 0x7fffffff : !p.causal || j < (p.prefix ? p.prefix[b] : 0) ? 0 : max(j - off, 0);
+    const T* k = j < n ? (const T*)p.k + b * p.ks[0] + j * p.ks[1] + hk * p.ks[2] : nullptr;
+    const T* v = j < n ? (const T*)p.v + b * p.vs[0] + j * p.vs[1] + hk * p.vs[2] : nullptr;
+    AttnStage<ROW, ROWS, 1> sq, sd;
+    sq.setup(0, lane, p.qs[1], p.D);
+    sd.setup(0, lane, p.ds[1], p.D);
+    const AttnLane<ROW> at_lane(lane);
+    struct {
+        f32x16 dk[NB], dv[NB];
+        int ds_exp;
+    } g;
+    AttnMarks<NB> either, plus, minus;                                  // (an infinity of a query: as a key's in attn_dq_again)
+#pragma unroll 1
+    for (int walk = 0; walk < 3; ++walk) {
+        const int kind = walk == 0 ? ATTN_PLUS : walk == 1 ? ATTN_MINUS : ATTN_FINITE;
+#pragma unroll
+        for (int db = 0; db < NB; ++db) g.dk[db] = g.dv[db] = f32x16{};
+        g.ds_exp = FIT ? ATTN_DS_EXP : 0;
+#pragma unroll 1
+        for (int gh = g0; gh < g1; ++gh) {
+            const int h = hk * p.G + gh;
+            const AttnScore f(p, h);
+            const uint64_t q = attn_addr((const T*)p.q + b * p.qs[0] + h * p.qs[2]), dout = attn_addr((const T*)p.dout + b * p.ds[0] + h * p.ds[2]);
+            const int64_t stat = ((int64_t)b * p.Hq + h) * p.Lq;
+#pragma unroll 1
+            for (int i0 = first; i0 < end; i0 += ROWS) {
+                uint32_t seen = 0;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int i = i0 + 4 * half + 8 * (r >> 2) + (r & 3);
+                    if (i >= qmin && i < p.Lq && (!p.kdoc || p.qdoc[b * p.qdoc_stride + i] == kdoc)) seen |= 1u << r;
+                }
+                if (!__ballot(seen != 0)) continue;
+                attn_landed();                                          // (the LDS reads of the tile before)
+                sq.issue(q, i0 / ROWS, p.Lq, (int)p.qs[1], p.D, lds, 0);
+                sd.issue(dout, i0 / ROWS, p.Lq, (int)p.ds[1], p.D, lds + BYTES, 0);
+                attn_landed();
+                typename AttnVec<T>::x8 w[2], d[2];
+                if (kind == ATTN_FINITE) {
+                    const uint32_t q_lds = at_lane.rows(lds), d_lds = at_lane.rows(lds + BYTES);
+                    f32x16 S = {}, dP = {};
+#pragma unroll
+                    for (int c = 0; c < 2 * DB; ++c) S = attn_mfma(attn_row_frag<T, ROW>(q_lds, 0, c), attn_lane_frag<T>(k, 2 * c + half, p.D), S);
+#pragma unroll
+                    for (int c = 0; c < 2 * DB; ++c) dP = attn_mfma(attn_row_frag<T, ROW>(d_lds, 0, c), attn_lane_frag<T>(v, 2 * c + half, p.D), dP);
+                    const float ds_by = FIT ? ldexpf(1.f, g.ds_exp - (int)SHIFT) : 1.f;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int i = i0 + 4 * half + 8 * (r >> 2) + (r & 3), row = min(i, p.Lq - 1);
+                        float weight, ds;
+                        attn_pair(f, S[r], dP[r], attn_lse2(p.lse[stat + row]) - SHIFT, p.delta[stat + row], ds_by, (float)(i + off - j), weight, ds);
+                        S[r] = seen >> r & 1 ? weight : 0.f;
+                        dP[r] = seen >> r & 1 ? ds : 0.f;
+                    }
+                    if constexpr (FIT) attn_fit(dP, g.ds_exp, g.dk);
+                    attn_pack<T>(S, w);
+                    attn_pack<T>(dP, d);
+                } else {
+                    attn_ones<T>(seen, w);
+                    attn_ones<T>(seen, d);
+                }
+                attn_landed();
+                attn_change<T, BYTES>(lds, lane, kind == ATTN_FINITE ? ATTN_FINITE : ATTN_EITHER);
+                attn_change<T, BYTES>(lds + BYTES, lane, kind);
+                attn_landed();
+                const uint32_t qc_lds = at_lane.cols(lds) ^ (part << 7), dc_lds = at_lane.cols(lds + BYTES) ^ (part << 7);
+#pragma unroll
+                for (int db = 0; db < NB; ++db)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        g.dv[db] = attn_mfma(attn_col_frag<T, ROW>(dc_lds, c, db), w[c], g.dv[db]);
+                        g.dk[db] = attn_mfma(attn_col_frag<T, ROW>(qc_lds, c, db), d[c], g.dk[db]);
+                    }
+            }
+        }
+        if (walk == 0) {
+            either.take(g.dk);
+            plus.take(g.dv);
+        }
+        if (walk == 1) minus.take(g.dv);
+    }
+    either.add(g.dk, NAN);
+    plus.add(g.dv, INFINITY);
+    minus.add(g.dv, -INFINITY);
+    attn_dkv_store<T, NB>(p, g.dk, g.dv, 1.f, g.ds_exp, b, j, hk, split, part, half, j < p.Lk);
+}
+
+template <typename T, int DB, int MODE, bool DOCS, int WAVES>
+__device__ __forceinline__ void attn_dq(const AttnParams& p, int group, char* smem, int (*sdoc)[ATTN_TILE], uint32_t (&said)[4]) {
     constexpr int ROW = attn_row<DB>(), TILE_BYTES = ATTN_TILE * ROW * 2;
     const int wave = attn_uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
     // p.splits > 1: the keys in that many runs of whole tiles, float32 parts that attn_parts_kernel adds in order
@@ -252,59 +448,22 @@ __device__ __forceinline__ void attn_dq(const AttnParams& p, int group, char* sm
         while (t >= 0 && full()) visit(std::false_type());
         while (t >= 0 && !full()) visit(std::true_type());
     }
-    bool nan = false;
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) nan = nan || acc[db][r] != acc[db][r];
-    uint64_t redo = __ballot(nan && row_ok && lse2 == lse2);
-    redo = (redo | (redo >> 32)) & 0xffffffffu;
-    const float by = ldexpf(p.scale * attn_ds_unit<MODE>(), -ds_exp);
-    const int64_t row_at = ((int64_t)(b * (int64_t)p.Lq + i) * p.Hq + h) * p.D, all = (int64_t)p.B * p.Lq * p.Hq * p.D;
-    const bool store = row_ok && !((redo >> l31) & 1);
-    if (p.splits > 1) attn_store_part<DB>(p.part + split * all + row_at, acc, by, half, p.D, store);
-    else attn_store_row<T, DB>((T*)p.dq + row_at, acc, by, half, p.D, store);
-    while (redo) {                                                      // a NaN behind the mask may have come in through 0 * NaN: these rows key by key
-        const int e = __builtin_ctzll(redo);
-        redo &= redo - 1;
-        const int ie = q0 + 32 * wave + e, lime = __shfl(lim, e), doce = __shfl(qdoc, e);
-        const float le = __shfl(lse2, e), de = __shfl(delta, e);
-        const T* qe = (const T*)p.q + b * p.qs[0] + ie * p.qs[1] + h * p.qs[2];
-        const T* doe = (const T*)p.dout + b * p.ds[0] + ie * p.ds[1] + h * p.ds[2];
-        float x[2] = {0.f, 0.f};
-        const int last = min(lime, run_end * ATTN_TILE - 1);
-        for (int j0 = run_first * ATTN_TILE; j0 <= last; j0 += 64) {
-            const int j = j0 + lane;
-            const bool see = j <= last && attn_visible(p, b, j, lime, doce);
-            float w, ds = 0.f;
-            if (see) attn_pair<T>(p, f, qe, k + j * p.ks[1], v + j * p.vs[1], doe, le, de, ie + n - p.Lq - j, w, ds);
-            uint64_t todo = __ballot(see);
-            while (todo) {
-                const int s = __builtin_ctzll(todo);
-                todo &= todo - 1;
-                const float d = __shfl(ds, s);
-                const T* kj = k + (int64_t)(j0 + s) * p.ks[1];
-                if (lane < p.D) x[0] += d * (float)kj[lane];
-                if (lane + 64 < p.D) x[1] += d * (float)kj[lane + 64];
-            }
-        }
-        const int64_t at = ((int64_t)(b * (int64_t)p.Lq + ie) * p.Hq + h) * p.D;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const int d = lane + 64 * c;
-            if (d >= p.D) continue;
-            if (p.splits > 1) p.part[split * all + at + d] = x[c] * p.scale;
-            else ((T*)p.dq)[at + d] = (T)(x[c] * p.scale);
-        }
+    bool store = row_ok;
+    if (attn_any(attn_has_nan(acc) && row_ok && lse2 == lse2, wave, said)) {
+        attn_dq_again<T, DB, WAVES>(attn_kernel_args(), b, i, h, row_ok, split, run_first * ATTN_TILE, min(key_end, run_end * ATTN_TILE), lds + wave * TILE_BYTES);
+        attn_clear(acc);                                                // (stored there; a return would keep the sums across the call)
+        store = false;
     }
+    attn_dq_store<T, DB>(p, acc, attn_ds_unit<MODE>(), ds_exp, b, i, h, split, half, store);
 }
 
 // A wave owns 32 keys: their K and V as operands and their dk and dv as accumulators.  Beyond 96 channels that is more than half of a SIMD's registers, so
 // one wave a SIMD, whose vector work and products would wait for each other (537 us at 2 x 4096 x 16 heads x 128, causal with caps; two loops interleaved by
 // hand: 555).  There two waves share 32 keys (attn_dkv_pair): each takes the scores of half of a tile's queries, they trade the 16-bit weights through the
 // LDS, and each adds up half of the channels over all of the queries.
-template <typename T, int DB, int MODE, bool DOCS>
-__device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* smem, AttnRows& rows, int (*sdoc)[ATTN_TILE], char* traded, int (*exps)[64]) {
+template <typename T, int DB, int MODE, bool DOCS, int WAVES>
+__device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* smem, AttnRows& rows, int (*sdoc)[ATTN_TILE], uint32_t (&said)[attn_dkv_pair<DB>() ? 8 : 4],
+                                         char* traded, int (*exps)[64]) {
     constexpr int ROW = attn_row<DB>(), TILE_BYTES = ATTN_TILE * ROW * 2;
     constexpr float SHIFT = ATTN_P_SHIFT<T>;
     constexpr bool PAIR = attn_dkv_pair<DB>(), FIT = SHIFT != 0.f;
@@ -545,113 +704,61 @@ __device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* s
         while (t >= 0 && full()) visit(std::false_type());
         while (t >= 0 && !full()) visit(std::true_type());
     }
-    bool nan = false;
-#pragma unroll
-    for (int db = 0; db < NB; ++db)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) nan = nan || dk[db][r] != dk[db][r] || dv[db][r] != dv[db][r];
-    uint64_t redo = __ballot(nan && key_ok);
-    redo = (redo | (redo >> 32)) & 0xffffffffu;
-    const float k_by = ldexpf(p.scale * attn_ds_unit<MODE>(), -ds_exp), v_by = ldexpf(1.f, -(int)SHIFT);
-    const bool store = j < p.Lk && !((redo >> l31) & 1);
+    bool store = j < p.Lk;
+    if (attn_any((attn_has_nan(dk) || attn_has_nan(dv)) && key_ok, wave, said)) {
+        const int first = max(first_query(k0) / ATTN_TILE, run_first) * ATTN_TILE, end = min(t_end * ATTN_TILE, p.Lq);
+#pragma unroll 1
+        for (int turn = 0; turn < (PAIR ? 2 : 1); ++turn) {             // (two waves of a pair share their half of a buffer: one after the other)
+            if (turn == part) attn_dkv_again<T, DB, NB, WAVES>(attn_kernel_args(), b, hk, j, kdoc, split, g0, g1, first, end, part, lds + keys * TILE_BYTES);
+            if (PAIR) __syncthreads();
+        }
+        attn_clear(dk);
+        attn_clear(dv);
+        store = false;
+    }
     if (!key_ok)                                                        // keys that nobody sees (their lanes held something else)
 #pragma unroll
         for (int db = 0; db < NB; ++db)
 #pragma unroll
             for (int r = 0; r < 16; ++r) dk[db][r] = dv[db][r] = 0.f;
-    const int64_t row = ((int64_t)b * p.Lk + j) * p.Hk + hk, all = (int64_t)p.B * p.Lk * p.Hk;
-    if (p.k_splits > 1) {
-        float* pk = p.k_part + (2 * split * all + row) * p.D;
-        float* pv = p.k_part + ((2 * split + 1) * all + row) * p.D;
-        attn_store_part<NB>(pk + 64 * part, dk, k_by, half, p.D - 64 * part, store);
-        attn_store_part<NB>(pv + 64 * part, dv, v_by, half, p.D - 64 * part, store);
-    } else {
-        attn_store_row<T, NB>((T*)p.dk + row * p.D + 64 * part, dk, k_by, half, p.D - 64 * part, store);
-        attn_store_row<T, NB>((T*)p.dv + row * p.D + 64 * part, dv, v_by, half, p.D - 64 * part, store);
-    }
-    while (redo) {
-        const int e = __builtin_ctzll(redo);
-        redo &= redo - 1;
-        const int je = k0 + 32 * keys + e, doce = __shfl(kdoc, e);
-        const T* ke = (const T*)p.k + b * p.ks[0] + je * p.ks[1] + hk * p.ks[2];
-        const T* ve = (const T*)p.v + b * p.vs[0] + je * p.vs[1] + hk * p.vs[2];
-        float xk[2] = {0.f, 0.f}, xv[2] = {0.f, 0.f};
-        for (int ge = g0; ge < g1; ++ge) {
-            const int h = hk * p.G + ge;
-            const AttnScore f(p, h);
-            const T* q = (const T*)p.q + b * p.qs[0] + h * p.qs[2];
-            const T* dout = (const T*)p.dout + b * p.ds[0] + h * p.ds[2];
-            const int64_t stat = ((int64_t)b * p.Hq + h) * p.Lq;
-            const int end = min(p.Lq, run_end * ATTN_TILE);
-            for (int i0 = max(first_query(je), run_first * ATTN_TILE); i0 < end; i0 += 64) {
-                const int i = i0 + lane;
-                const bool see = i < end && (!p.kdoc || p.qdoc[b * p.qdoc_stride + i] == doce);
-                float w = 0.f, ds = 0.f;
-                if (see) attn_pair<T>(p, f, q + i * p.qs[1], ke, ve, dout + i * p.ds[1], attn_lse2(p.lse[stat + i]), p.delta[stat + i], i + off - je, w, ds);
-                uint64_t todo = __ballot(see);
-                while (todo) {
-                    const int s = __builtin_ctzll(todo);
-                    todo &= todo - 1;
-                    const float we = __shfl(w, s), de = __shfl(ds, s);
-                    const T* qi = q + (int64_t)(i0 + s) * p.qs[1];
-                    const T* di = dout + (int64_t)(i0 + s) * p.ds[1];
-#pragma unroll
-                    for (int c = 0; c < 2; ++c)
-                        if (lane + 64 * c < p.D) {
-                            xk[c] += de * (float)qi[lane + 64 * c];
-                            xv[c] += we * (float)di[lane + 64 * c];
-                        }
-                }
-            }
-        }
-        const int64_t re = ((int64_t)b * p.Lk + je) * p.Hk + hk;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const int d = lane + 64 * c;
-            if (d >= p.D || (PAIR && c != part)) continue;
-            if (p.k_splits > 1) {
-                p.k_part[(2 * split * all + re) * p.D + d] = xk[c] * p.scale;
-                p.k_part[((2 * split + 1) * all + re) * p.D + d] = xv[c];
-            } else {
-                ((T*)p.dk)[re * p.D + d] = (T)(xk[c] * p.scale);
-                ((T*)p.dv)[re * p.D + d] = (T)xv[c];
-            }
-        }
-    }
+    attn_dkv_store<T, NB>(p, dk, dv, attn_ds_unit<MODE>(), ds_exp, b, j, hk, split, part, half, store);
 }
 #endif
 
 template <typename T, int DB, int MODE, bool DOCS>
-__global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnParams p) {
+__global__ __launch_bounds__(256, (attn_dq_waves<DB, DOCS>())) void attn_dq_kernel(AttnParams p) {
 #ifdef __HIP_DEVICE_COMPILE__
     __shared__ __align__(1024) char smem[attn_lds_bytes<DB>()];
     __shared__ __align__(16) int sdoc[2][ATTN_TILE];
-    attn_dq<T, DB, MODE, DOCS>(p, blockIdx.x, smem, sdoc);
+    __shared__ uint32_t said[4];
+    attn_dq<T, DB, MODE, DOCS, attn_dq_waves<DB, DOCS>()>(p, blockIdx.x, smem, sdoc, said);
 #endif
 }
 template <typename T, int DB, int MODE, bool DOCS>
-__global__ __launch_bounds__(attn_dkv_pair<DB>() ? 512 : 256, 2) void attn_dkv_kernel(AttnParams p) {
+__global__ __launch_bounds__(attn_dkv_pair<DB>() ? 512 : 256, attn_dkv_waves<DB>()) void attn_dkv_kernel(AttnParams p) {
 #ifdef __HIP_DEVICE_COMPILE__
     __shared__ __align__(1024) char smem[attn_lds_bytes<DB>()];
     __shared__ __align__(16) AttnRows rows;
     __shared__ __align__(16) int sdoc[2][ATTN_TILE];
     __shared__ __align__(16) char traded[attn_dkv_pair<DB>() ? 4 * 2 * 4 * 1024 : 16];
     __shared__ int exps[attn_dkv_pair<DB>() && ATTN_P_SHIFT<T> != 0.f ? 8 : 1][64];
-    attn_dkv<T, DB, MODE, DOCS>(p, blockIdx.x, smem, rows, sdoc, traded, exps);
+    __shared__ uint32_t said[attn_dkv_pair<DB>() ? 8 : 4];
+    attn_dkv<T, DB, MODE, DOCS, attn_dkv_waves<DB>()>(p, blockIdx.x, smem, rows, sdoc, said, traded, exps);
 #endif
 }
 // Both in one launch where that is two rounds of the chip at most (1024 workgroups): small calls wait for single workgroups, and so for both kinds at once.
 // Training step of 3 x 1021 x 6 heads x 72, documents: 105 -> 91 us, 2 x 1200 x 8 heads on 2 x 72, causal with caps: 125 -> 100, 4096 x 16 x 64: 425 -> 424.
 // (Larger ones keep two launches: the dq workgroups alone need fewer registers, and more of them share a CU.)
 template <typename T, int DB, int MODE, bool DOCS>
-__global__ __launch_bounds__(256, 2) void attn_grads_kernel(AttnParams p) {
+__global__ __launch_bounds__(256, attn_dkv_waves<DB>()) void attn_grads_kernel(AttnParams p) {
 #ifdef __HIP_DEVICE_COMPILE__
     static_assert(!attn_dkv_pair<DB>(), "256 threads each");
     __shared__ __align__(1024) char smem[attn_lds_bytes<DB>()];
     __shared__ __align__(16) AttnRows rows;
     __shared__ __align__(16) int sdoc[2][ATTN_TILE];
-    if ((int)blockIdx.x < p.first_k) attn_dq<T, DB, MODE, DOCS>(p, blockIdx.x, smem, sdoc);
-    else attn_dkv<T, DB, MODE, DOCS>(p, blockIdx.x - p.first_k, smem, rows, sdoc, nullptr, nullptr);
+    __shared__ uint32_t said[4];
+    if ((int)blockIdx.x < p.first_k) attn_dq<T, DB, MODE, DOCS, attn_dkv_waves<DB>()>(p, blockIdx.x, smem, sdoc, said);
+    else attn_dkv<T, DB, MODE, DOCS, attn_dkv_waves<DB>()>(p, blockIdx.x - p.first_k, smem, rows, sdoc, said, nullptr, nullptr);
 #endif
 }
 

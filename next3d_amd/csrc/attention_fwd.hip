@@ -67,34 +67,6 @@ __global__ __launch_bounds__(1024) void attn_order_kernel(AttnParams p, int* __r
     if (mine && seg == 0) order[b * p.row_blocks + ranks[i]] = i;
 }
 
-// accumulator [DB] of one row += sum over visible keys j in [k0, k1) of exp2(u - m) v_j, one wave, plain arithmetic: acc[e] belongs to channel lane + 64 e
-template <typename T>
-__device__ void attn_exact_row(const AttnParams& p, int b, int i, int h, int k0, int k1, float m, int lane, float (&acc)[2]) {
-    const AttnScore f(p, h);
-    const int hk = h / p.G, n = attn_keys(p, b), lim = attn_limit(p, i, n, p.prefix ? p.prefix[b] : 0);
-    const int qdoc = p.kdoc ? p.qdoc[b * p.qdoc_stride + i] : 0;
-    const T* q = (const T*)p.q + b * p.qs[0] + i * p.qs[1] + h * p.qs[2];
-    const T* k = (const T*)p.k + b * p.ks[0] + hk * p.ks[2];
-    const T* v = (const T*)p.v + b * p.vs[0] + hk * p.vs[2];
-    acc[0] = acc[1] = 0.f;
-    const int end = min(k1, lim + 1);
-    for (int j0 = k0; j0 < end; j0 += 64) {
-        const int j = j0 + lane;
-        const bool see = j < end && attn_visible(p, b, j, lim, qdoc);
-        float w = 0.f;
-        if (see) w = __builtin_amdgcn_exp2f(attn_score(f, attn_dot<T>(q, k + j * p.ks[1], p.D), i + n - p.Lq - j) - m);
-        uint64_t todo = __ballot(see);
-        while (todo) {
-            const int e = __builtin_ctzll(todo);
-            todo &= todo - 1;
-            const float we = __shfl(w, e);
-            const T* vj = v + (int64_t)(j0 + e) * p.vs[1];
-            if (lane < p.D) acc[0] += we * (float)vj[lane];
-            if (lane + 64 < p.D) acc[1] += we * (float)vj[lane + 64];
-        }
-    }
-}
-
 // One wave's softmax step over the 32 queries of its lanes: S (raw products of KB blocks of 32 keys) -> P as second operands; rescales acc, sum and m.
 // MASK: not every key of the tile is visible to every query.
 template <typename T, int KB, int DB, int MODE, bool MASK>
@@ -170,12 +142,137 @@ __device__ __forceinline__ void attn_softmax_step(f32x16 (&S)[KB], typename Attn
     else attn_softmax_form<T, KB, DB, MODE, true>(S, P, acc, m, sum, f, lim, at, j0, half, docs, qdoc);
 }
 
+// The sums of one wave's 32 rows (query i and head h are the lane's own) over the keys [first, end), 32 at a time, `step` apart
+template <int DB> struct AttnSums {
+    f32x16 acc[DB];
+    float m, sum;
+};
+template <typename T, int DB>
+__device__ __forceinline__ void attn_fwd_store(const AttnParams& p, const f32x16 (&acc)[DB], float m, float sum, int b, int i, int h, int split, int half, bool row_ok) {
+    if (p.splits > 1) {
+        const int hk = h / p.G;
+        const int64_t at = (((int64_t)(b * p.Hk + hk) * p.Lq + i) * p.G + h - hk * p.G) * p.splits + split;
+        attn_store_part<DB>(p.part + at * p.D, acc, 1.f, half, p.D, row_ok);
+        if (row_ok && half == 0) {
+            p.part[p.part_ml + 2 * at] = m;
+            p.part[p.part_ml + 2 * at + 1] = sum;
+        }
+    } else {
+        const float by = sum == 0.f ? 0.f : 1.f / sum;
+        const int64_t row_at = ((int64_t)(b * (int64_t)p.Lq + i) * p.Hq + h) * p.D;
+        attn_store_row<T, DB>((T*)p.out + row_at, acc, by, half, p.D, row_ok);
+        if (p.rest) attn_store_row<T, DB, true>((T*)p.rest + row_at, acc, by, half, p.D, row_ok);
+        if (p.lse && row_ok && half == 0) p.lse[((int64_t)b * p.Hq + h) * p.Lq + i] = sum == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(sum)) * ATTN_LN2;
+    }
+}
+#ifdef __HIP_DEVICE_COMPILE__
+template <typename T, int DB>
+static __device__ __forceinline__ AttnSums<DB> attn_sums_again(attn_args args, int b, int i, int h, bool row_ok, int first, int end, int step, uint32_t lds, bool fine) {
+    constexpr int ROW = DB > 2 ? 128 : 64, KEYS = 32, BYTES = KEYS * ROW * 2;
+    const AttnParams p = *args;
+    const int lane = threadIdx.x & 63, half = lane >> 5, hk = attn_uniform(h / p.G);
+    const int n = attn_keys(p, b), at = i + n - p.Lq;
+    const int qdoc = p.kdoc && row_ok ? p.qdoc[b * p.qdoc_stride + i] : 0;
+    const int lim = !row_ok || qdoc < 0 ? -1 : attn_limit(p, i, n, p.prefix ? p.prefix[b] : 0);
+    const T* q = row_ok ? (const T*)p.q + b * p.qs[0] + i * p.qs[1] + h * p.qs[2] : nullptr;
+    const uint64_t k = attn_addr((const T*)p.k + b * p.ks[0] + hk * p.ks[2]), v = attn_addr((const T*)p.v + b * p.vs[0] + hk * p.vs[2]);
+    const AttnScore f(p, row_ok ? h : 0);
+    AttnStage<ROW, KEYS, 1> sk, sv;
+    sk.setup(0, lane, p.ks[1], p.D);
+    sv.setup(0, lane, p.vs[1], p.D);
+    const AttnLane<ROW> at_lane(lane);
+    AttnSums<DB> s;
+    AttnMarks<DB> plus, minus;
+#pragma unroll 1
+    for (int walk = 0; walk < 3; ++walk) {
+        const int kind = walk == 0 ? ATTN_PLUS : walk == 1 ? ATTN_MINUS : ATTN_FINITE;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) s.acc[db] = f32x16{};
+        s.m = -INFINITY;
+        s.sum = 0.f;
+#pragma unroll 1
+        for (int j0 = first; j0 < end; j0 += step) {
+            uint32_t seen = 0;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int j = j0 + 4 * half + 8 * (r >> 2) + (r & 3);
+                if (j <= lim && (!p.kdoc || p.kdoc[b * p.kdoc_stride + j] == qdoc)) seen |= 1u << r;
+            }
+            if (!__ballot(seen != 0)) continue;
+            attn_landed();                                              // (the LDS reads of the tile before)
+            sk.issue(k, j0 / KEYS, n, (int)p.ks[1], p.D, lds, 0);
+            sv.issue(v, j0 / KEYS, n, (int)p.vs[1], p.D, lds + BYTES, 0);
+            attn_landed();
+            attn_change<T, BYTES>(lds + BYTES, lane, kind);
+            attn_landed();
+            const uint32_t k_lds = at_lane.rows(lds), v_lds = at_lane.cols(lds + BYTES);
+            f32x16 S = {};
+            typename AttnVec<T>::x8 P[2];
+            if (kind == ATTN_FINITE) {
+#pragma unroll
+                for (int c = 0; c < 2 * DB; ++c) S = attn_mfma(attn_row_frag<T, ROW>(k_lds, 0, c), attn_lane_frag<T>(q, 2 * c + half, p.D), S);
+                float top = -INFINITY;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    S[r] = seen >> r & 1 ? attn_score(f, S[r], (float)(at - (j0 + 4 * half + 8 * (r >> 2) + (r & 3)))) : -INFINITY;
+                    top = fmaxf(top, S[r]);
+                }
+                const float now = fmaxf(s.m, attn_half_max(top)), shrink = now == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(s.m - now);
+                s.m = now;
+                s.sum *= shrink;
+#pragma unroll
+                for (int db = 0; db < DB; ++db)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s.acc[db][r] *= shrink;
+                const float sub = now == -INFINITY ? 0.f : now;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    S[r] = __builtin_amdgcn_exp2f(S[r] - sub);
+                    s.sum += S[r];
+                }
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) P[c][e] = (T)S[8 * c + e];
+            } else {
+                attn_ones<T>(seen, P);
+            }
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const auto vf = attn_col_frag<T, ROW>(v_lds, c, db);
+                    s.acc[db] = attn_mfma(vf, P[c], s.acc[db]);
+                    if (fine && kind == ATTN_FINITE) s.acc[db] = attn_mfma(vf, attn_left_over<T>(S, P[c], c), s.acc[db]);
+                }
+        }
+        if (walk == 0) plus.take(s.acc);
+        if (walk == 1) minus.take(s.acc);
+    }
+    plus.add(s.acc, INFINITY);
+    minus.add(s.acc, -INFINITY);
+    s.sum = attn_half_sum(s.sum);
+    return s;
+}
+template <typename T, int DB>
+static __device__ __attribute__((noinline)) AttnSums<DB> attn_out_again(attn_args args, int b, int i, int h, bool row_ok, int first, int end, int step, uint32_t lds) {
+    return attn_sums_again<T, DB>(args, b, i, h, row_ok, first, end, step, lds, true);
+}
+template <typename T, int DB>
+static __device__ __attribute__((noinline)) void attn_rows_again(attn_args args, int b, int i, int h, bool row_ok, int split, int first, int end, uint32_t lds, bool fine) {
+    const AttnSums<DB> s = attn_sums_again<T, DB>(args, b, i, h, row_ok, first, end, 32, lds, fine);
+    const AttnParams p = *args;
+    attn_fwd_store<T, DB>(p, s.acc, s.m, s.sum, b, i, h, split, (threadIdx.x & 63) >> 5, row_ok);
+}
+#endif
+
 template <typename T, int DB, int MODE, bool DOCS>
-__global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnParams p) {
+__global__ __launch_bounds__(256, DB < 3 ? 3 : 2) void attn_fwd_kernel(AttnParams p) {
 #ifdef __HIP_DEVICE_COMPILE__                            // (hipcc drops the launch stub of a template whose body its host pass cannot read)
     constexpr int ROW = DB > 2 ? 128 : 64, TILE_BYTES = ATTN_TILE * ROW * 2;
     __shared__ __align__(1024) char smem[4 * TILE_BYTES];                 // [buffer][k, v]
     __shared__ __align__(16) int sdoc[2][ATTN_TILE];
+    __shared__ uint32_t said[4];
     const int wave = attn_uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
     // consecutive workgroups go to different XCDs: give each XCD whole heads, so that its L2 serves their keys, and the longest rows first
     // (p.splits > 1: the keys in that many runs of whole tiles, joined by attn_combine_kernel)
@@ -291,50 +388,19 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnParams p) {
         while (t >= 0 && !full()) visit(std::true_type());
     }
     sum = attn_half_sum(sum);
-    const float by = sum == 0.f ? 0.f : 1.f / sum;
-    bool nan = false;
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) nan = nan || acc[db][r] != acc[db][r];
-    uint64_t redo = __ballot(nan && sum == sum && row_ok);
-    redo = (redo | (redo >> 32)) & 0xffffffffu;
-    const bool store = row_ok && !((redo >> l31) & 1);
-    const int64_t row_at = ((int64_t)(b * (int64_t)p.Lq + i) * p.Hq + h) * p.D;
-    auto part_at = [&](int row) { return (((int64_t)(b * p.Hk + hk) * p.Lq + row) * p.G + h - hk * p.G) * p.splits + split; };
-    if (p.splits > 1) {
-        const int64_t at = part_at(i);
-        attn_store_part<DB>(p.part + at * p.D, acc, 1.f, half, p.D, store);
-        if (row_ok && half == 0) {
-            p.part[p.part_ml + 2 * at] = m;
-            p.part[p.part_ml + 2 * at + 1] = sum;
-        }
-    } else {
-        attn_store_row<T, DB>((T*)p.out + row_at, acc, by, half, p.D, store);
-        if (p.rest) attn_store_row<T, DB, true>((T*)p.rest + row_at, acc, by, half, p.D, store);
-        if (p.lse && row_ok && half == 0) p.lse[((int64_t)b * p.Hq + h) * p.Lq + i] = sum == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(sum)) * ATTN_LN2;
+    bool store = row_ok;
+    if (attn_any(attn_has_nan(acc) && sum == sum && row_ok, wave, said)) {
+        attn_rows_again<T, DB>(attn_kernel_args(), b, i, h, row_ok, split, run_first * ATTN_TILE, min(key_end, run_end * ATTN_TILE), lds + wave * TILE_BYTES, fine);
+        attn_clear(acc);                                                // (stored there; a return would keep the sums across the call)
+        store = false;
     }
-    while (redo) {
-        const int e = __builtin_ctzll(redo);
-        redo &= redo - 1;
-        const int ie = q0 + 32 * wave + e;
-        const float me = __shfl(m, e), bye = __shfl(by, e);
-        float row[2];
-        attn_exact_row<T>(p, b, ie, h, run_first * ATTN_TILE, min(n, (run_first + run) * ATTN_TILE), me, lane, row);
-        if (p.splits > 1) {
-            float* x = p.part + part_at(ie) * p.D;
-            if (lane < p.D) x[lane] = row[0];
-            if (lane + 64 < p.D) x[lane + 64] = row[1];
-        } else {
-            attn_store_pair<T>(p, ((int64_t)(b * (int64_t)p.Lq + ie) * p.Hq + h) * p.D, row, bye, lane);
-        }
-    }
+    attn_fwd_store<T, DB>(p, acc, m, sum, b, i, h, split, half, store);
 #endif
 }
 
 // ---- few queries: rows r = query * G + head of the group, 32 a workgroup
 template <typename T, int DB, int MODE>
-__global__ __launch_bounds__(256) void attn_token_kernel(AttnParams p) {
+__global__ __launch_bounds__(256, DB < 3 ? 3 : 2) void attn_token_kernel(AttnParams p) {
 #ifdef __HIP_DEVICE_COMPILE__                            // (hipcc drops the launch stub of a template whose body its host pass cannot read)
     constexpr int ROW = DB > 2 ? 128 : 64, KEYS = 32, TILE_BYTES = KEYS * ROW * 2, WAVES = 4;
     extern __shared__ __align__(1024) char smem[];                        // [wave][buffer][k, v], then the waves' results
@@ -406,7 +472,15 @@ __global__ __launch_bounds__(256) void attn_token_kernel(AttnParams p) {
     }
     // join the four waves: common maximum, then the accumulators through the LDS, one [32 rows][32 * DB + 1] float image a wave
     constexpr int PITCH = 32 * DB + 1;
+    __shared__ uint32_t said[WAVES];
     sum = attn_half_sum(sum);
+    if (attn_any(attn_has_nan(acc) && sum == sum && row_ok, wave, said)) {
+        const AttnSums<DB> s = attn_out_again<T, DB>(attn_kernel_args(), b, i, h, row_ok, k0 + wave * KEYS, k1, WAVES * KEYS, lds);
+#pragma unroll
+        for (int db = 0; db < DB; ++db) acc[db] = s.acc[db];
+        m = s.m;
+        sum = s.sum;
+    }
     if (half == 0) {
         sm[wave][l31] = m;
         ssum[wave][l31] = sum;
@@ -419,38 +493,23 @@ __global__ __launch_bounds__(256) void attn_token_kernel(AttnParams p) {
     for (int w = 0; w < WAVES; ++w) all += ssum[w][l31] == 0.f ? 0.f : ssum[w][l31] * __builtin_amdgcn_exp2f(sm[w][l31] - top);
     const float shrink = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
     float* img = reinterpret_cast<float*>(smem) + wave * 32 * PITCH;
-    bool nan = false;
 #pragma unroll
     for (int db = 0; db < DB; ++db)
 #pragma unroll
-        for (int rr = 0; rr < 16; ++rr) {
-            const float x = m == -INFINITY ? 0.f : acc[db][rr] * shrink;
-            nan = nan || x != x;
-            img[l31 * PITCH + 32 * db + 8 * (rr >> 2) + 4 * half + (rr & 3)] = x;
-        }
-    __shared__ uint32_t bad[WAVES];
-    uint64_t any = __ballot(nan && all == all && row_ok);
-    if (lane == 0) bad[wave] = (uint32_t)(any | (any >> 32));
+        for (int rr = 0; rr < 16; ++rr) img[l31 * PITCH + 32 * db + 8 * (rr >> 2) + 4 * half + (rr & 3)] = m == -INFINITY ? 0.f : acc[db][rr] * shrink;
     __syncthreads();
-    const uint32_t redo = bad[0] | bad[1] | bad[2] | bad[3];
     const bool direct = p.splits == 1;
     for (int e = wave * 8; e < wave * 8 + 8; ++e) {                     // eight rows a wave
         const int re = blk * 32 + e;
         if (re >= rows) break;
         const int ie = re / p.G, he = hk * p.G + re - ie * p.G;
         const float te = __shfl(top, e), ae = __shfl(all, e);
-        float x[2];
-        if ((redo >> e) & 1) {
-            attn_exact_row<T>(p, b, ie, he, k0, k1, te, lane, x);
-        } else {
+        float x[2] = {0.f, 0.f};
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                x[c] = 0.f;
-                if (lane + 64 * c < 32 * DB)
+        for (int c = 0; c < 2; ++c)
+            if (lane + 64 * c < 32 * DB)
 #pragma unroll
-                    for (int w = 0; w < WAVES; ++w) x[c] += reinterpret_cast<float*>(smem)[(w * 32 + e) * PITCH + lane + 64 * c];
-            }
-        }
+                for (int w = 0; w < WAVES; ++w) x[c] += reinterpret_cast<float*>(smem)[(w * 32 + e) * PITCH + lane + 64 * c];
         if (direct) {
             attn_store_pair<T>(p, ((int64_t)(b * (int64_t)p.Lq + ie) * p.Hq + he) * p.D, x, ae == 0.f ? 0.f : 1.f / ae, lane);
             if (p.lse && lane == 0) p.lse[((int64_t)b * p.Hq + he) * p.Lq + ie] = ae == 0.f ? -INFINITY : (te + __builtin_amdgcn_logf(ae)) * ATTN_LN2;

@@ -592,3 +592,102 @@ def test_attention_float16_gradients_do_not_depend_on_what_is_not_seen(dev):
         big_v[:, hi] *= 10000.0
         plain, got = _run(dev, q, k, v, do, causal=True), _run(dev, q, k, big_v, do, causal=True)
         assert all(torch.equal(got[name][:, lo], plain[name][:, lo]) for name in ('out', 'dq'))
+
+
+def _classes64(q, k, v, do, see):
+    """out, dq, dk, dv [L, D] of one head in float64 with every sum over the visible pairs only, so that infinities and NaN are those of the formula."""
+    q, k, v, do = (t.double() for t in (q, k, v, do))
+    scale = q.shape[1] ** -0.5
+    pick = lambda keep, t: torch.where(keep, t, torch.zeros_like(t))
+    t = (q[:, None] * k[None]).sum(2) * scale
+    p = torch.softmax(t.masked_fill(~see, float('-inf')), 1)
+    p = pick(see & see.any(1, keepdim=True), p)
+    out = pick(see[..., None], p[..., None] * v[None]).sum(1)
+    dp = (do[:, None] * v[None]).sum(2)
+    ds = pick(see, p * (dp - (do * out).sum(1, keepdim=True)) * scale)
+    return dict(out=out, dq=pick(see[..., None], ds[..., None] * k[None]).sum(1), dk=pick(see[..., None], ds[..., None] * q[:, None]).sum(0),
+                dv=pick(see[..., None], p[..., None] * do[:, None]).sum(0))
+
+
+@pytest.mark.parametrize('dtype', [F16, BF16])
+@pytest.mark.parametrize('d', [16, 40, 72, 128])
+def test_attention_visible_and_masked_nonfinite(dev, d, dtype):
+    """Infinities and NaN in one tensor, some visible and some not: out and dv are the infinity or NaN of the formula where it has one, gradients are finite
+    exactly where the formula's are, and everything finite is within the bounds of the call without them."""
+    n = 150
+    inf, nan = float('inf'), float('nan')
+    docs = torch.zeros(1, n, dtype=torch.int32)
+    docs[:, 60:], docs[:, 130:] = 1, -1
+    i = torch.arange(n)
+    for causal in (True, False):
+        see = (docs[0][:, None] == docs[0][None]) & (docs[0] >= 0)[:, None]
+        if causal:
+            see = see & (i[:, None] >= i[None])
+        for name in ('v', 'do', 'k', 'q'):
+            ts = dict(zip(('q', 'k', 'v', 'do'), _inputs(1, n, n, 1, 1, d, dtype, 121)))
+            clean = {key: t.clone() for key, t in ts.items()}
+            for row, channel, x in ((20, 3, inf), (33, 5, -inf), (40, 3, inf), (41, 7, inf), (45, 7, -inf), (70, 9, nan), (100, 2, inf), (135, 4, nan), (140, 3, -inf)):
+                if name in ('q', 'k') and row not in (41, 100, 135, 140):
+                    continue
+                ts[name][0, row, 0, channel] = x
+                clean[name][0, row, 0, channel] = 0
+            got = _run(dev, ts['q'], ts['k'], ts['v'], ts['do'], documents=docs, causal=causal)
+            want = _classes64(*(ts[key][0, :, 0] for key in ('q', 'k', 'v', 'do')), see)
+            vals, tols = R.attention(clean['q'], clean['k'], clean['v'], clean['do'], documents=docs, causal=causal)
+            for key, w in want.items():
+                g, what = got[key][0, :, 0].cpu(), (causal, name, key)
+                finite = torch.isfinite(w)
+                assert torch.equal(torch.isfinite(g), finite), what
+                if (name, key) in (('v', 'out'), ('do', 'dv')):
+                    assert torch.equal(g.isnan(), w.isnan()) and torch.equal(g[g.isinf()].double(), w[w.isinf()]), what
+                keep = finite
+                if name == 'k':                                             # (a score of -inf takes its key out of a row, which the call without it keeps)
+                    rows = see[:, [41, 100]].any(1)
+                    keep = finite & ~(rows if key in ('out', 'dq') else see[rows].any(0))[:, None]
+                R.assert_within(g[keep], vals[key][0, :, 0][keep], tols[key][0, :, 0][keep], str(what))
+
+
+@pytest.mark.parametrize('lq', [1, 6])
+def test_attention_visible_nonfinite_in_a_cache(dev, lq):
+    """Few queries over a cache: the infinities of the keys in use, beside NaN in keys of another document."""
+    n, d = 700, 64
+    q, k, v, _ = _inputs(1, lq, n, 1, 1, d, F16, 122)
+    kd, qd = (torch.arange(n) % 3 == 0).to(torch.int32)[None], torch.ones(1, lq, dtype=torch.int32)
+    clean = v.clone()
+    for row, channel, x in ((3, 1, float('inf')), (300, 2, -float('inf')), (6, 5, float('inf')), (333, 5, -float('inf')), (699, 9, float('nan')), (4, 1, float('nan')), (5, 30, float('inf'))):
+        v[0, row, 0, channel], clean[0, row, 0, channel] = x, 0
+    from next3d_amd.torch_utils.ops import attention
+    out = attention.attention(q.to(dev), k.to(dev), v.to(dev), documents=qd.to(dev), key_documents=kd.to(dev)).cpu()[0, :, 0]
+    vals, tols = R.attention(q, k, clean, documents=qd, key_documents=kd)
+    for channel, x in ((1, float('inf')), (2, -float('inf'))):
+        assert bool((out[:, channel] == x).all())
+    assert bool(out[:, [5, 9]].isnan().all())
+    rest = [c for c in range(d) if c not in (1, 2, 5, 9)]
+    R.assert_within(out[:, rest], vals['out'][0, :, 0][:, rest], tols['out'][0, :, 0][:, rest])
+
+
+@pytest.mark.parametrize('d', [64, 128])
+def test_attention_overflowed_step_takes_a_few_times_as_long(dev, d):
+    """One infinity in the gradient, as a loss scale too large makes it, or a row of NaN: the call repeats its sums; it does not walk them key by key."""
+    q, k, v, do = (t.to(dev) for t in _inputs(1, 4096, 4096, 4, 2, d, F16, 123))
+
+    def time(q, k, v, do):
+        best = float('inf')
+        for _ in range(4):
+            leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+            begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            begin.record()
+            torch.autograd.grad(attention.attention(*leaves, causal=True), leaves, do)
+            end.record()
+            end.synchronize()
+            best = min(best, begin.elapsed_time(end))
+        return best
+
+    from next3d_amd.torch_utils.ops import attention
+    usual = time(q, k, v, do)
+    spoiled = do.clone()
+    spoiled[0, 4000, 1, 3] = float('inf')
+    late = v.clone()
+    late[0, 10] = float('nan')
+    for which, t in (('do', time(q, k, v, spoiled)), ('v', time(q, k, late, do))):
+        assert t < 40 * usual, (which, usual, t)
