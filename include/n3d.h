@@ -525,6 +525,8 @@ int n3d_rotary(const n3d_rotary_desc* desc, n3d_stream_t stream);
  *   visible: j < n; causal: j <= position or j < prefix[b] (prefix [B] int32 or NULL); documents (int32, [B, Lq] / [B, Lk] with the given batch strides,
  *   both or neither NULL): equal and not negative.
  * A row that sees nothing gives out 0 and lse -inf.  Keys behind n are not read.  float32 softmax and accumulation.
+ * Refused: 2^24 blocks of rows (128 queries of a head; up to 24 queries, 32 of the queries and heads of a key head) or more; half of that in the backward pass
+ * beyond 96 channels.
  * workspace: n3d_attention_workspace(desc) bytes (-1: refused, see n3d_last_error), 16-byte aligned; nothing in it outlives the call. */
 typedef struct {
     const void *q, *k, *v;

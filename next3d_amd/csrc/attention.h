@@ -398,6 +398,8 @@ static inline int attn_room(int64_t groups, int tiles) {
     const int64_t s = 512 / groups;
     return groups >= 256 || tiles < 24 ? 1 : (int)(s < tiles / 8 ? s : tiles / 8);
 }
+// workgroups of the kernels whose workgroups share the XCDs evenly (attn_fwd_kernel)
+static inline int64_t attn_even(int64_t workgroups) { return cdiv64(workgroups, 8) * 8; }
 static inline const char* attn_params(const n3d_attention_desc* d, AttnParams& p) {
     if (!d) return "null descriptor";
     if (d->B < 0 || d->Lq < 0 || d->Lk < 0) return "negative sizes";
@@ -459,5 +461,7 @@ static inline void attn_forms(const AttnParams& p, F&& f) {
 }
 
 // workspace, in floats: the document ranges come first
+// do the launches of attn_ranges fit? (the order of the blocks is left out where its own does not)
+static inline bool attn_ranges_fit(const AttnParams& p) { return !p.kdoc || n3d_grid_fits((int64_t)p.B * cdiv(p.nkt > p.nqt ? p.nkt : p.nqt, 4), 256); }
 static inline int64_t attn_range_floats(const AttnParams& p) { return p.kdoc ? 2 * (int64_t)p.B * (p.nkt + p.nqt) + (int64_t)p.B * cdiv(p.Lq, 128) : 0; }
 void attn_ranges(AttnParams& p, void* workspace, hipStream_t stream);      // attention_fwd.hip

@@ -787,7 +787,8 @@ static void attn_bwd_launch(AttnParams& p, hipStream_t stream) {
     auto add = [&](const float* part, int count, int64_t all, void* a, void* b) {
         if (count > 1) hipLaunchKernelGGL((attn_parts_kernel<T>), dim3((unsigned)cdiv64(all, 2048), b ? 2 : 1), dim3(256), 0, stream, part, count, all, (T*)a, (T*)b);
     };
-    const int dq = p.dq ? 8 * cdiv(p.B * p.Hq * p.splits * p.row_blocks, 8) : 0, dkv = p.dk && p.Lk > 0 ? 8 * cdiv(p.B * p.Hk * p.k_splits * p.k_blocks, 8) : 0;
+    const unsigned dq = p.dq ? attn_even((int64_t)p.B * p.Hq * p.splits * p.row_blocks) : 0;
+    const unsigned dkv = p.dk && p.Lk > 0 ? attn_even((int64_t)p.B * p.Hk * p.k_splits * p.k_blocks) : 0;
     bool both = false;
     if constexpr (!attn_dkv_pair<DB>()) {
         if ((both = dq && dkv && dq + dkv <= 1024)) {

@@ -33,12 +33,20 @@ static AttnBwdSpace attn_bwd_plan(AttnParams& p) {
     return at;
 }
 
+// (pairs of waves in dk / dv beyond 96 channels: 512 threads)
+static bool attn_bwd_fits(const AttnParams& p) {
+    return n3d_grid_fits(attn_even((int64_t)p.B * p.Hq * p.splits * p.row_blocks), 256) && attn_ranges_fit(p) &&
+           n3d_grid_fits(attn_even((int64_t)p.B * p.Hk * p.k_splits * p.k_blocks), p.D > 96 ? 512 : 256);
+}
+
 extern "C" int64_t n3d_attention_bwd_workspace(const n3d_attention_desc* d) {
     AttnParams p;
     const char* bad = attn_params(d, p);
     N3D_CHECK(!bad, "attention_bwd: %s", bad);
     if (p.B == 0 || p.Lq == 0) return 0;
-    return 4 * attn_bwd_plan(p).end;
+    const int64_t need = 4 * attn_bwd_plan(p).end;
+    N3D_CHECK(attn_bwd_fits(p), "attention_bwd: too many rows for one launch");
+    return need;
 }
 
 extern "C" int n3d_attention_bwd(const n3d_attention_desc* d, n3d_stream_t stream_) {
@@ -54,6 +62,7 @@ extern "C" int n3d_attention_bwd(const n3d_attention_desc* d, n3d_stream_t strea
     N3D_CHECK(((uintptr_t)d->dout | (uintptr_t)d->dq | (uintptr_t)d->dk | (uintptr_t)d->dv) % 16 == 0, "attention_bwd: tensors must be 16-byte aligned");
     const AttnBwdSpace at = attn_bwd_plan(p);
     const int64_t need = 4 * at.end;
+    N3D_CHECK(attn_bwd_fits(p), "attention_bwd: too many rows for one launch");
     N3D_CHECK(d->workspace && d->workspace_bytes >= need && (uintptr_t)d->workspace % 16 == 0, "attention_bwd: a workspace of %lld bytes is needed (16-byte aligned)", (long long)need);
     float* ws = (float*)d->workspace;
     p.dout = d->dout; p.dq = d->dq; p.dk = d->dk; p.dv = d->dv;

@@ -571,7 +571,7 @@ void attn_ranges(AttnParams& p, void* workspace, hipStream_t stream) {
     p.ktiles = kt;
     p.qtiles = qt;
     p.row_blocks = cdiv(p.Lq, 128);
-    if (p.nkt > ATTN_ORDER_TILES || p.row_blocks > ATTN_ORDER_BLOCKS || (int64_t)p.B * p.Hq * p.row_blocks <= 1024) return;
+    if (p.nkt > ATTN_ORDER_TILES || p.row_blocks > ATTN_ORDER_BLOCKS || (int64_t)p.B * p.Hq * p.row_blocks <= 1024 || !n3d_grid_fits(p.B, 1024)) return;
     int* order = (int*)(kt + (int64_t)p.B * (p.nkt + p.nqt));
     hipLaunchKernelGGL(attn_order_kernel, dim3(p.B), dim3(1024), 0, stream, p, order);
     p.order = order;
@@ -604,7 +604,7 @@ static hipError_t attn_fwd_launch(AttnParams& p, bool token, hipStream_t stream)
         if (e != hipSuccess) return e;
         hipLaunchKernelGGL((attn_token_kernel<T, DB, MODE>), dim3(p.B * p.Hk * p.row_blocks * p.splits), dim3(256), lds, stream, p);
     } else {
-        hipLaunchKernelGGL((attn_fwd_kernel<T, DB, MODE, DOCS>), dim3(8 * cdiv(p.B * p.Hq * p.splits * p.row_blocks, 8)), dim3(256), 0, stream, p);
+        hipLaunchKernelGGL((attn_fwd_kernel<T, DB, MODE, DOCS>), dim3((unsigned)attn_even((int64_t)p.B * p.Hq * p.splits * p.row_blocks)), dim3(256), 0, stream, p);
     }
     if (p.splits > 1) hipLaunchKernelGGL((attn_combine_kernel<T>), dim3((unsigned)cdiv64((int64_t)p.B * p.Lq * p.Hq, 256 / attn_combine_lanes(p.D))), dim3(256), 0, stream, p);
     return hipSuccess;
@@ -620,6 +620,11 @@ static int64_t attn_fwd_floats(AttnParams& p, bool& token, int64_t& parts_at) {
     return parts_at + parts * (p.D + 2);
 }
 
+static bool attn_fwd_fits(const AttnParams& p, bool token) {
+    const int64_t groups = (int64_t)p.B * p.row_blocks * p.splits;
+    return token ? n3d_grid_fits(groups * p.Hk, 256) : n3d_grid_fits(attn_even(groups * p.Hq), 256) && attn_ranges_fit(p);
+}
+
 extern "C" int64_t n3d_attention_workspace(const n3d_attention_desc* d) {
     AttnParams p;
     const char* bad = attn_params(d, p);
@@ -627,7 +632,9 @@ extern "C" int64_t n3d_attention_workspace(const n3d_attention_desc* d) {
     if (p.B == 0 || p.Lq == 0) return 0;
     bool token;
     int64_t parts_at;
-    return 4 * attn_fwd_floats(p, token, parts_at);
+    const int64_t need = 4 * attn_fwd_floats(p, token, parts_at);
+    N3D_CHECK(attn_fwd_fits(p, token), "attention: too many rows for one launch");
+    return need;
 }
 
 extern "C" int n3d_attention(const n3d_attention_desc* d, n3d_stream_t stream_) {
@@ -639,6 +646,7 @@ extern "C" int n3d_attention(const n3d_attention_desc* d, n3d_stream_t stream_) 
     bool token;
     int64_t parts_at;
     const int64_t need = 4 * attn_fwd_floats(p, token, parts_at);
+    N3D_CHECK(attn_fwd_fits(p, token), "attention: too many rows for one launch");
     N3D_CHECK(need == 0 || (d->workspace && d->workspace_bytes >= need && (uintptr_t)d->workspace % 16 == 0), "attention: a workspace of %lld bytes is needed (16-byte aligned)",
               (long long)need);
     const double pairs = (double)p.B * p.Hq * p.Lq * p.Lk * p.D;

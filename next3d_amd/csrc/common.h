@@ -39,6 +39,8 @@ static inline int n3d_tune(const char* name, int dflt) { const char* e = getenv(
 static inline int n3d_tune(const char*, int dflt) { return dflt; }
 #endif
 
+// HIP launches fewer than 2^32 threads in a grid's dimension
+static inline bool n3d_grid_fits(int64_t workgroups, int threads) { return workgroups * threads < (1ll << 32); }
 static inline int64_t cdiv64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 static inline int cdiv(int a, int b) { return (a + b - 1) / b; }
 

@@ -271,3 +271,21 @@ def test_tensors_without_memory_are_refused(op):
     name, call, args = _host_side_calls()[op]
     for which in range(len(args)):
         _raises(f'{name}: a tensor without memory', call, *(Wrapper(t) if i == which else t for i, t in enumerate(args)))
+
+
+def test_attention_c_entries_refuse_launches_of_2_to_the_32_threads():
+    """HIP refuses such a launch; the library refuses the call before it enqueues anything.  One sequence fewer passes the same check."""
+    from next3d_amd import _lib
+    lib = _lib.lib()
+    base = dict(q=4096, k=4096, v=4096, out=4096, lse=4096, dout=4096, dq=4096, dk=4096, dv=4096, scale=1.0, Lq=100, Lk=100, D=8, dtype=1)
+    for kw, entries in ((dict(B=1 << 20, heads_q=16, heads_k=16), 'fb'), (dict(B=1 << 24, Lq=1, Lk=1, heads_q=1, heads_k=1), 'fb'), (dict(B=1 << 22, Lq=1, heads_q=16, heads_k=4), 'f'),
+                        (dict(B=1 << 19, Lq=1, Lk=1000, heads_q=4, heads_k=4, D=8), 'b'), (dict(B=1 << 19, Lk=200, heads_q=8, heads_k=8, D=128), 'b')):
+        for which in entries:
+            entry, size = (lib.n3d_attention, lib.n3d_attention_workspace) if which == 'f' else (lib.n3d_attention_bwd, lib.n3d_attention_bwd_workspace)
+            d = _lib.AttentionDesc(**dict(base, workspace=4096, workspace_bytes=1 << 60, **kw))
+            assert entry(d, None) != 0 and 'one launch' in lib.n3d_last_error().decode(), (kw, which, lib.n3d_last_error())
+            assert size(d) == -1 and 'one launch' in lib.n3d_last_error().decode()
+            d.B -= 8
+            assert size(d) >= 0, (kw, which)
+    docs = _lib.AttentionDesc(**dict(base, B=1 << 23, Lq=1, Lk=300, heads_q=1, heads_k=1, q_documents=4096, k_documents=4096))
+    assert lib.n3d_attention_bwd_workspace(docs) == -1 and 'one launch' in lib.n3d_last_error().decode()
