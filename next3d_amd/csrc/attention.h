@@ -71,6 +71,7 @@ __device__ __forceinline__ int attn_keys(const AttnParams& p, int b) {
     const int n = p.lengths ? p.lengths[b] : p.Lk;
     return n < 0 ? 0 : n < p.Lk ? n : p.Lk;
 }
+__device__ __forceinline__ int attn_prefix(const AttnParams& p, int b) { return p.prefix ? max(p.prefix[b], 0) : 0; }
 __device__ __forceinline__ int attn_limit(const AttnParams& p, int i, int n, int prefix) {
     int lim = n - 1;
     if (p.causal) {

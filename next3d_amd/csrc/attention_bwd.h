@@ -143,7 +143,7 @@ static __device__ __attribute__((noinline)) void attn_dq_again(attn_args args, i
     const int lane = threadIdx.x & 63, half = lane >> 5, hk = attn_uniform(h / p.G);
     const int n = attn_keys(p, b), at = i + n - p.Lq;
     const int qdoc = p.kdoc && row_ok ? p.qdoc[b * p.qdoc_stride + i] : 0;
-    const int lim = !row_ok || qdoc < 0 ? -1 : attn_limit(p, i, n, p.prefix ? p.prefix[b] : 0);
+    const int lim = !row_ok || qdoc < 0 ? -1 : attn_limit(p, i, n, attn_prefix(p, b));
     const T* q = row_ok ? (const T*)p.q + b * p.qs[0] + i * p.qs[1] + h * p.qs[2] : nullptr;
     const T* dout = row_ok ? (const T*)p.dout + b * p.ds[0] + i * p.ds[1] + h * p.ds[2] : nullptr;
     const int64_t stat = ((int64_t)b * p.Hq + h) * p.Lq + i;
@@ -220,7 +220,7 @@ static __device__ __attribute__((noinline)) void attn_dkv_again(attn_args args, 
     const AttnParams p = *args;
     const int lane = threadIdx.x & 63, half = lane >> 5, n = attn_keys(p, b), off = n - p.Lq;
     const bool key_ok = j < n && kdoc >= 0;
-    const int qmin = !key_ok ? 0x7fffffff : !p.causal || j < (p.prefix ? p.prefix[b] : 0) ? 0 : max(j - off, 0);
+    const int qmin = !key_ok ? 0x7fffffff : !p.causal || j < attn_prefix(p, b) ? 0 : max(j - off, 0);
     const T* k = j < n ? (const T*)p.k + b * p.ks[0] + j * p.ks[1] + hk * p.ks[2] : nullptr;
     const T* v = j < n ? (const T*)p.v + b * p.vs[0] + j * p.vs[1] + hk * p.vs[2] : nullptr;
     AttnStage<ROW, ROWS, 1> sq, sd;
@@ -317,7 +317,7 @@ __device__ __forceinline__ void attn_dq(const AttnParams& p, int group, char* sm
     if (group >> 3 >= per || id >= total) return;
     const int split = id % p.splits, pos = id / p.splits % p.row_blocks, bh = id / p.splits / p.row_blocks, h = bh % p.Hq, b = bh / p.Hq, hk = h / p.G;
     const int blk = DOCS && p.order ? p.order[b * p.row_blocks + pos] : p.row_blocks - 1 - pos;
-    const int n = attn_keys(p, b), prefix = p.prefix ? p.prefix[b] : 0, q0 = blk * 128;
+    const int n = attn_keys(p, b), prefix = attn_prefix(p, b), q0 = blk * 128;
     const int i = q0 + 32 * wave + l31;
     const bool row_ok = i < p.Lq;
     const int qdoc = DOCS && row_ok ? p.qdoc[b * p.qdoc_stride + i] : 0;
@@ -479,7 +479,7 @@ __device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* s
     if (group >> 3 >= per || id >= total) return;
     const int blk = id % p.k_blocks, split = id / p.k_blocks % p.k_splits, bh = id / p.k_blocks / p.k_splits, hk = bh % p.Hk, b = bh / p.Hk;
     const int heads = p.G * p.chunks / p.k_splits, g0 = split / p.chunks * heads, g1 = g0 + heads;
-    const int n = attn_keys(p, b), prefix = p.prefix ? p.prefix[b] : 0, k0 = blk * 128, off = n - p.Lq;
+    const int n = attn_keys(p, b), prefix = attn_prefix(p, b), k0 = blk * 128, off = n - p.Lq;
     const int j = k0 + 32 * keys + l31;
     const int kdoc = DOCS && j < p.Lk ? p.kdoc[b * p.kdoc_stride + j] : 0;
     const bool key_ok = j < n && kdoc >= 0;

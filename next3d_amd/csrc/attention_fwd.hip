@@ -34,7 +34,7 @@ static constexpr int ATTN_ORDER_TILES = 1024, ATTN_ORDER_BLOCKS = 512;
 __global__ __launch_bounds__(1024) void attn_order_kernel(AttnParams p, int* __restrict__ order) {
     __shared__ int2 tiles[ATTN_ORDER_TILES];
     __shared__ int counts[ATTN_ORDER_BLOCKS], ranks[ATTN_ORDER_BLOCKS];
-    const int b = blockIdx.x, n = attn_keys(p, b), prefix = p.prefix ? p.prefix[b] : 0;
+    const int b = blockIdx.x, n = attn_keys(p, b), prefix = attn_prefix(p, b);
     const int log = max(6, 32 - __builtin_clz(p.row_blocks - 1 | 1)), i = threadIdx.x & ((1 << log) - 1), seg = threadIdx.x >> log, segs = 1024 >> log;
     const bool mine = i < p.row_blocks;
     int lo = 1, hi = 0, end = 0;
@@ -173,7 +173,7 @@ static __device__ __forceinline__ AttnSums<DB> attn_sums_again(attn_args args, i
     const int lane = threadIdx.x & 63, half = lane >> 5, hk = attn_uniform(h / p.G);
     const int n = attn_keys(p, b), at = i + n - p.Lq;
     const int qdoc = p.kdoc && row_ok ? p.qdoc[b * p.qdoc_stride + i] : 0;
-    const int lim = !row_ok || qdoc < 0 ? -1 : attn_limit(p, i, n, p.prefix ? p.prefix[b] : 0);
+    const int lim = !row_ok || qdoc < 0 ? -1 : attn_limit(p, i, n, attn_prefix(p, b));
     const T* q = row_ok ? (const T*)p.q + b * p.qs[0] + i * p.qs[1] + h * p.qs[2] : nullptr;
     const uint64_t k = attn_addr((const T*)p.k + b * p.ks[0] + hk * p.ks[2]), v = attn_addr((const T*)p.v + b * p.vs[0] + hk * p.vs[2]);
     const AttnScore f(p, row_ok ? h : 0);
@@ -281,7 +281,7 @@ __global__ __launch_bounds__(256, DB < 3 ? 3 : 2) void attn_fwd_kernel(AttnParam
     if ((int)(blockIdx.x >> 3) >= per || id >= total) return;
     const int split = id % p.splits, pos = id / p.splits % p.row_blocks, bh = id / p.splits / p.row_blocks, h = bh % p.Hq, b = bh / p.Hq, hk = h / p.G;
     const int blk = DOCS && p.order ? p.order[b * p.row_blocks + pos] : p.row_blocks - 1 - pos;
-    const int n = attn_keys(p, b), prefix = p.prefix ? p.prefix[b] : 0, q0 = blk * 128;
+    const int n = attn_keys(p, b), prefix = attn_prefix(p, b), q0 = blk * 128;
     const int i = q0 + 32 * wave + l31;
     const bool row_ok = i < p.Lq;
     const int qdoc = DOCS && row_ok ? p.qdoc[b * p.qdoc_stride + i] : 0;
@@ -409,7 +409,7 @@ __global__ __launch_bounds__(256, DB < 3 ? 3 : 2) void attn_token_kernel(AttnPar
     const int wave = attn_uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
     const int split = blockIdx.x % p.splits, blk = blockIdx.x / p.splits % p.row_blocks, bh = blockIdx.x / (p.splits * p.row_blocks);
     const int hk = bh % p.Hk, b = bh / p.Hk, rows = p.Lq * p.G;
-    const int n = attn_keys(p, b), prefix = p.prefix ? p.prefix[b] : 0;
+    const int n = attn_keys(p, b), prefix = attn_prefix(p, b);
     const int r = blk * 32 + l31, i = r / p.G, h = hk * p.G + r - i * p.G;
     const bool row_ok = r < rows;
     const int qdoc = p.kdoc && row_ok ? p.qdoc[b * p.qdoc_stride + i] : 0;

@@ -691,3 +691,11 @@ def test_attention_overflowed_step_takes_a_few_times_as_long(dev, d):
     late[0, 10] = float('nan')
     for which, t in (('do', time(q, k, v, spoiled)), ('v', time(q, k, late, do))):
         assert t < 40 * usual, (which, usual, t)
+
+
+def test_attention_prefix_below_zero(dev):
+    """A prefix of less than nothing is none, down to the lowest number."""
+    q, k, v, do = _inputs(4, 90, 90, 2, 1, 64, BF16, 131)
+    prefix = torch.tensor([-2 ** 31, -2 ** 31 + 1, -1, 2 ** 31 - 1], dtype=torch.int32)
+    _check(dev, q, k, v, do, causal=True, prefix=prefix)
+    _check(dev, q[:, :1], k, v, causal=True, prefix=prefix, lengths=torch.tensor([90, 3, 60, 90], dtype=torch.int32))
