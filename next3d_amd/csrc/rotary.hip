@@ -190,6 +190,7 @@ extern "C" int n3d_rotary(const n3d_rotary_desc* d, n3d_stream_t stream_) {
     if (tpb > tokens / 1024) tpb = tokens / 1024;
     if (tpb > ROT_MAX_TABLE / r.P) tpb = ROT_MAX_TABLE / r.P;
     r.tpb = tpb < 1 ? 1 : (int)tpb;
+    N3D_CHECK(n3d_grid_fits(cdiv64(tokens, r.tpb), ROT_THREADS), "rotary: too many tokens for one launch");
     const double esize = d->dtype == N3D_F32 ? 4.0 : 2.0;
     N3dProfScope prof(N3D_K_ROTARY, stream, 3.0 * tokens * heads * d->D, 2.0 * esize * tokens * heads * d->D);
     token_dispatch(d->dtype, [&](auto* t) {

@@ -289,3 +289,12 @@ def test_attention_c_entries_refuse_launches_of_2_to_the_32_threads():
             assert size(d) >= 0, (kw, which)
     docs = _lib.AttentionDesc(**dict(base, B=1 << 23, Lq=1, Lk=300, heads_q=1, heads_k=1, q_documents=4096, k_documents=4096))
     assert lib.n3d_attention_bwd_workspace(docs) == -1 and 'one launch' in lib.n3d_last_error().decode()
+
+
+def test_rotary_refuses_launches_of_2_to_the_32_threads():
+    """Eight tokens a workgroup of 256 where a token has 256 pairs: 2^27 tokens are 2^24 workgroups."""
+    from next3d_amd import _lib
+    lib = _lib.lib()
+    d = _lib.RotaryDesc(q=4096, positions=4096, out_q=4096, pos_token_stride=1, base=1e4, B=1 << 12, L=1 << 15, heads_q=1, D=512, axes=1, dtype=0)
+    d.sections[0] = 512
+    assert lib.n3d_rotary(d, None) != 0 and 'one launch' in lib.n3d_last_error().decode()
