@@ -340,21 +340,24 @@ __global__ __launch_bounds__(256) void ln_cols_big_kernel(LnParams p) {
 template <typename TW>
 __global__ __launch_bounds__(1024) void ln_reduce_kernel(const float* __restrict__ ws, int parts, int64_t C, TW* __restrict__ dw, TW* __restrict__ db) {
     __shared__ float acc[32][33];
-    const int64_t c = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
     const int g = threadIdx.x >> 5;
-    float s = 0.f;
-    if (c < 2 * C) {
+    for (int64_t c0 = (int64_t)blockIdx.x * 32; c0 < 2 * C; c0 += (int64_t)gridDim.x * 32) {
+        const int64_t c = c0 + (threadIdx.x & 31);
+        float s = 0.f;
+        if (c < 2 * C) {
 #pragma unroll 8
-        for (int r = g; r < parts; r += 32) s += ws[(int64_t)r * 2 * C + c];
-    }
-    acc[g][threadIdx.x & 31] = s;
-    __syncthreads();
-    if (g == 0 && c < 2 * C) {
-        float t = 0.f;
+            for (int r = g; r < parts; r += 32) s += ws[(int64_t)r * 2 * C + c];
+        }
+        acc[g][threadIdx.x & 31] = s;
+        __syncthreads();
+        if (g == 0 && c < 2 * C) {
+            float t = 0.f;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) t += acc[i][threadIdx.x & 31];
-        TW* d = c < C ? dw : db;
-        if (d) d[c < C ? c : c - C] = (TW)t;
+            for (int i = 0; i < 32; ++i) t += acc[i][threadIdx.x & 31];
+            TW* d = c < C ? dw : db;
+            if (d) d[c < C ? c : c - C] = (TW)t;
+        }
+        __syncthreads();
     }
 }
 
@@ -455,9 +458,10 @@ extern "C" int n3d_layer_norm_bwd(const void* dy, const void* x, const void* w, 
     });
     N3D_LAUNCH_CHECK();
     if (cols) {
+        const int64_t blocks = cdiv64(2 * (int64_t)C, 32), most = 1 << 20;          // (2^32 threads are more than a launch can have)
         token_dispatch(w_dtype, [&](auto* t) {
             using TW = std::remove_pointer_t<decltype(t)>;
-            hipLaunchKernelGGL((ln_reduce_kernel<TW>), dim3((unsigned)cdiv64(2 * (int64_t)C, 32)), dim3(1024), 0, stream, workspace, parts, (int64_t)C, (TW*)dw, (TW*)db);
+            hipLaunchKernelGGL((ln_reduce_kernel<TW>), dim3((unsigned)(blocks < most ? blocks : most)), dim3(1024), 0, stream, workspace, parts, (int64_t)C, (TW*)dw, (TW*)db);
         });
         N3D_LAUNCH_CHECK();
     }

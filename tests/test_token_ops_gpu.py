@@ -295,3 +295,21 @@ def test_token_ops_refuse_what_cannot_see_into_them(dev):
             with pytest.raises(RuntimeError):
                 transform()
         assert call(x).shape == x.shape
+
+
+def test_layer_norm_gradients_of_very_long_rows(dev):
+    """More channels than a launch of the column sums has threads for."""
+    from next3d_amd.torch_utils.ops import layer_norm
+    c = (1 << 26) + 5
+    g = torch.Generator(device=dev).manual_seed(7)
+    x, dy = (torch.randn((2, c), generator=g, device=dev).half() for _ in range(2))
+    w, b = torch.ones(c, device=dev).requires_grad_(), torch.zeros(c, device=dev).requires_grad_()
+    dw, db = torch.autograd.grad(layer_norm.layer_norm(x, w, b), (w, b), dy)
+    xd, dyd = x.double(), dy.double()
+    xc = xd - xd.mean(1, keepdim=True)
+    xh = xc / (xc.square().mean(1, keepdim=True) + 1e-5).sqrt()
+    chain = (c / 1024 + 80) * R.U32                                        # a thread adds c / 1024 terms one after the other; the mean's terms are |x| ~ 1 on average
+    assert bool(((db.double() - dyd.sum(0)).abs() <= 4 * R.U32 * dyd.abs().sum(0)).all())
+    assert bool(((dw.double() - (dyd * xh).sum(0)).abs() <= (dyd.abs() * (1 + xh.abs()) * 2 * chain).sum(0)).all())
+    del x, dy, xd, dyd, xc, xh, dw, db, w, b
+    torch.cuda.empty_cache()
