@@ -1,6 +1,8 @@
 """rotary — rotary positions with several axes (time, height, width) for tokens of images and videos, on libn3d.so (csrc/rotary.hip).
 
 Not an operator of the reference's layer; it turns the queries and keys of `attention`."""
+import operator
+
 import torch
 
 from ... import _lib
@@ -26,7 +28,10 @@ def rotary(q, positions, sections, k=None, base=10000.0, pairing='interleaved', 
     require_tensor('rotary', 'positions', positions, _POSITIONS)
     b, l, _, d = q.shape
     require_sizes('rotary', b * l)
-    sections = tuple(int(s) for s in sections)
+    try:
+        sections = tuple(operator.index(s) for s in sections)
+    except TypeError:
+        raise RuntimeError(f'rotary: sections must be whole numbers (got {sections!r})') from None
     if not 1 <= len(sections) <= 4 or any(s < 0 or s % 2 for s in sections) or not 0 < sum(sections) <= d:
         raise RuntimeError(f'rotary: sections must be 1 to 4 even numbers of channels that add up to 2..{d} (got {sections})')
     if d > 1024:

@@ -298,3 +298,11 @@ def test_rotary_refuses_launches_of_2_to_the_32_threads():
     d = _lib.RotaryDesc(q=4096, positions=4096, out_q=4096, pos_token_stride=1, base=1e4, B=1 << 12, L=1 << 15, heads_q=1, D=512, axes=1, dtype=0)
     d.sections[0] = 512
     assert lib.n3d_rotary(d, None) != 0 and 'one launch' in lib.n3d_last_error().decode()
+
+
+def test_rotary_refuses_sections_that_are_no_whole_numbers():
+    from next3d_amd.torch_utils.ops.rotary import rotary
+    q, pos = torch.zeros(2, 5, 3, 16), torch.zeros(5, 2, dtype=torch.int32)
+    for sections in ((8.0, 8.0), (8.9, 7.9), ('8', 8), 16):
+        _raises('whole numbers', rotary, q, pos, sections)
+    _raises('HIP device only', rotary, q, pos, torch.tensor([8, 8]))
