@@ -107,10 +107,12 @@ __device__ __forceinline__ int attn_swizzle(int row) {
 
 // One piece: 16 bytes a lane from voff of the buffer to lds + 16 lane (zeros beyond the range).  In asm because the compiler, which sees LDS behind the
 // builtin, would wait for every piece in flight before the next LDS read of any buffer.  It has no register result; attn_sync / attn_landed wait for it, and
-// the compiler's own vmcnt waits, which do not count it, can only be longer than needed (loads return in order).  (m0 has no other use in these kernels.)
+// the compiler's own vmcnt waits, which do not count it, can only be longer than needed (loads return in order).  Nor does it keep, in asm, the five wait states between a
+// vector instruction that writes a scalar register (a readfirstlane, the reload of a spilled descriptor) and a memory instruction that reads it: the move and
+// the s_nop are five.  (m0, which the compiler reserves and a clobber list may not name, has no other use in these kernels.)
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void attn_piece(i32x4 rsrc, int voff, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(lds), "v"(voff), "s"(rsrc) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(lds), "v"(voff), "s"(rsrc) : "memory");
 }
 
 // Staging by LDS-DMA: a piece is 1 KB = 64 lanes x 16 bytes; wave w of W takes pieces w, w + W, ...  Rows behind the last and channels behind D are beyond

@@ -306,3 +306,44 @@ def test_rotary_refuses_sections_that_are_no_whole_numbers():
     for sections in ((8.0, 8.0), (8.9, 7.9), ('8', 8), 16):
         _raises('whole numbers', rotary, q, pos, sections)
     _raises('HIP device only', rotary, q, pos, torch.tensor([8, 8]))
+
+
+def test_tile_pieces_wait_for_their_descriptor(tmp_path):
+    """A memory instruction may read a scalar register five wait states after a vector instruction wrote it; inside asm nobody but the asm sees to that."""
+    import re
+    from next3d_amd import build
+    src, out = tmp_path / 'piece.hip', tmp_path / 'piece.s'
+    src.write_text('''#include "attention.h"
+__global__ void piece(const int* p, float* out) {
+    __shared__ __align__(1024) float tile[4096];
+    const int x = p[threadIdx.x], y = p[threadIdx.x + 64];
+    for (int i = 0; i < 4; ++i) {
+        const i32x4 r = {attn_uniform(x + i), attn_uniform(y) & 0xffff, attn_uniform(x ^ y), 0x00020000};
+        attn_piece(r, x, attn_uniform(attn_lds(tile) + i * 1024));
+        attn_piece(r, y, attn_uniform(attn_lds(tile) + y));
+    }
+    attn_sync();
+    out[threadIdx.x] = tile[threadIdx.x];
+}
+''')
+    subprocess.run([build.HIPCC, *build.CFLAGS, '-w', '-I', build.CSRC, '--cuda-device-only', '-S', str(src), '-o', str(out)], check=True, capture_output=True)
+
+    def scalars(text):
+        m = re.fullmatch(r's\[(\d+):(\d+)\]|s(\d+)', text)
+        return set() if not m else {int(m.group(3))} if m.group(3) else set(range(int(m.group(1)), int(m.group(2)) + 1))
+
+    at, written, pieces, vector_writes = 0, {}, 0, 0
+    for line in out.read_text().splitlines():
+        m = re.match(r'\s+([a-z]\w+)\s*([^;]*)', line)
+        if not m:
+            continue
+        op, args = m.group(1), [a.strip() for a in m.group(2).split(',')]
+        at += 1 + (int(args[0]) if op == 's_nop' else 0)
+        if op.startswith('v_') or op.startswith('s_'):
+            for r in scalars(args[0]):
+                written[r] = at if op.startswith('v_') else -1000
+                vector_writes += op == 'v_readfirstlane_b32'
+        if op == 'buffer_load_dwordx4' and 'lds' in line:
+            pieces += 1
+            assert all(at - written.get(r, -1000) - 1 >= 5 for r in scalars(args[1])), line
+    assert pieces == 8 and vector_writes >= 2
