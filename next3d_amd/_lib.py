@@ -192,6 +192,9 @@ def token_ext():
             from . import _token_ext as ext
         except ImportError as e:
             raise RuntimeError(f'{_HERE}/_token_ext.so cannot be loaded ({e}): build it with `python -m next3d_amd.build`') from e
+        if ext.torch_version != torch.__version__:
+            raise RuntimeError(f'{_HERE}/_token_ext.so was built against torch {ext.torch_version}, this is {torch.__version__}: build it again with '
+                               '`python -m next3d_amd.build`')
         names = ('n3d_last_error', 'n3d_layer_norm', 'n3d_layer_norm_bwd_workspace', 'n3d_layer_norm_bwd', 'n3d_rotary', 'n3d_attention_workspace',
                  'n3d_attention', 'n3d_attention_bwd_workspace', 'n3d_attention_bwd')
         ext.bind([ctypes.cast(getattr(handle, name), c_void_p).value for name in names])

@@ -35,8 +35,22 @@ def _stale(target, deps):
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+def _other_command(target, cmd):
+    """Was `target` built by another command (other flags, another torch)?  Every object has the command that made it beside it."""
+    try:
+        with open(target + '.cmd') as f:
+            return f.read() != ' '.join(cmd)
+    except FileNotFoundError:
+        return True
+
+
+def _note_command(target, cmd):
+    with open(target + '.cmd', 'w') as f:
+        f.write(' '.join(cmd))
+
+
 def _ext_commands():
-    """Compile and link commands of _token_ext.so: host code only, linked against the torch that will load it."""
+    """Compile and link commands of _token_ext.so: host code only, linked against the torch that will load it, whose version is part of them."""
     import sysconfig
 
     import torch
@@ -44,7 +58,7 @@ def _ext_commands():
     src, obj = os.path.join(CSRC, 'token_ext.cpp'), os.path.join(OBJ, 'token_ext.o')
     includes = [os.path.join(root, 'include'), os.path.join(root, 'include', 'torch', 'csrc', 'api', 'include'), '/opt/rocm/include',
                 sysconfig.get_paths()['include']]
-    compile_ = ['g++', '-O2', '-std=c++17', '-fPIC', '-Wall', '-D__HIP_PLATFORM_AMD__=1', '-DUSE_ROCM=1',
+    compile_ = ['g++', '-O2', '-std=c++17', '-fPIC', '-Wall', '-D__HIP_PLATFORM_AMD__=1', '-DUSE_ROCM=1', f'-DN3D_TORCH="{torch.__version__}"',
                 f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}']
     compile_ += [a for i in includes for a in ('-isystem', i)] + ['-c', src, '-o', obj]
     link = ['g++', '-shared', '-fPIC', '-o', EXT, obj, '-L' + os.path.join(root, 'lib'), '-ltorch_python', '-ltorch', '-ltorch_cpu', '-ltorch_hip', '-lc10', '-lc10_hip']
@@ -58,12 +72,13 @@ def build(force=False, verbose=True):
     jobs = []
     for src in _sources():
         obj = os.path.join(OBJ, src.replace('.hip', '.o'))
-        if force or _stale(obj, [os.path.join(CSRC, src)] + headers):
-            jobs.append([HIPCC] + CFLAGS + PER_FILE.get(src, []) + ['-c', os.path.join(CSRC, src), '-o', obj])
+        cmd = [HIPCC] + CFLAGS + PER_FILE.get(src, []) + ['-c', os.path.join(CSRC, src), '-o', obj]
+        if force or _stale(obj, [os.path.join(CSRC, src)] + headers) or _other_command(obj, cmd):
+            jobs.append((obj, cmd))
 
     ext_src, ext_obj, ext_compile, ext_link = _ext_commands()
-    if force or _stale(ext_obj, [ext_src, os.path.join(HERE, '..', 'include', 'n3d.h')]):
-        jobs.insert(0, ext_compile)                    # (the longest job first)
+    if force or _stale(ext_obj, [ext_src, os.path.join(HERE, '..', 'include', 'n3d.h')]) or _other_command(ext_obj, ext_compile):
+        jobs.insert(0, (ext_obj, ext_compile))         # (the longest job first)
 
     def run(cmd):
         if verbose:
@@ -75,8 +90,12 @@ def build(force=False, verbose=True):
         if verbose and said.strip():
             print(said, file=sys.stderr)
 
+    def make(job):
+        run(job[1])
+        _note_command(*job)
+
     with ThreadPoolExecutor(max_workers=min(8, max(1, len(jobs)))) as ex:
-        list(ex.map(run, jobs))
+        list(ex.map(make, jobs))
     objs = [os.path.join(OBJ, s.replace('.hip', '.o')) for s in _sources()]
     if force or _stale(LIB, objs):
         run([HIPCC, '-shared', '-fPIC', f'--offload-arch={ARCH}', '-Wl,--no-undefined', '-o', LIB] + objs)

@@ -373,6 +373,7 @@ std::tuple<Tensor, Opt> attention(const Tensor& q, const Tensor& k, const Tensor
 }  // namespace
 
 PYBIND11_MODULE(_token_ext, m) {
+    m.attr("torch_version") = N3D_TORCH;                    // of the headers that this was compiled against
     m.def("bind", &bind);
     m.def("layer_norm", &layer_norm);
     m.def("rotary", &rotary);

@@ -347,3 +347,22 @@ __global__ void piece(const int* p, float* out) {
             pieces += 1
             assert all(at - written.get(r, -1000) - 1 >= 5 for r in scalars(args[1])), line
     assert pieces == 8 and vector_writes >= 2
+
+
+def test_host_side_belongs_to_one_torch(monkeypatch):
+    """Loaded under another torch than it was built against, it is refused; under that torch the build's command is another one."""
+    from next3d_amd import _lib, build
+    assert _lib.token_ext().torch_version == torch.__version__
+    command = build._ext_commands()[2]
+    monkeypatch.setattr(torch, '__version__', '1.0.0')
+    assert build._ext_commands()[2] != command
+    monkeypatch.setattr(_lib, '_token_ext', None)
+    _raises('built against torch', _lib.token_ext)
+
+
+def test_objects_are_made_again_by_another_command(tmp_path):
+    from next3d_amd import build
+    obj = str(tmp_path / 'x.o')
+    assert build._other_command(obj, ['hipcc', '-O3'])
+    build._note_command(obj, ['hipcc', '-O3'])
+    assert not build._other_command(obj, ['hipcc', '-O3']) and build._other_command(obj, ['hipcc', '-O2'])
