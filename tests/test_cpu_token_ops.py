@@ -366,3 +366,12 @@ def test_objects_are_made_again_by_another_command(tmp_path):
     assert build._other_command(obj, ['hipcc', '-O3'])
     build._note_command(obj, ['hipcc', '-O3'])
     assert not build._other_command(obj, ['hipcc', '-O3']) and build._other_command(obj, ['hipcc', '-O2'])
+
+
+def test_the_build_entry_compiles_every_time(monkeypatch):
+    import __graft_entry__ as entry
+    from next3d_amd import build
+    asked = []
+    monkeypatch.setattr(build, 'build', lambda force=False, verbose=True: asked.append(force) or build.LIB)
+    entry.build()
+    assert asked == [True]
