@@ -4,7 +4,8 @@
 // The gradient is the same kernel with -sin.  HBM-bound: q and k of a token are one launch, read once and written once; the cosines and sines of a
 // workgroup's tokens are computed once into the LDS and serve every head of q and k.  The angle is taken in 64 bits and reduced to a fraction of a
 // turn there — in 32 bits the angle of position 100000 is off by 0.004 — and the cosine and sine of that fraction are float32.
-// Measured: q and k of 32768 tokens x 16 heads x 128 channels each, bfloat16, 113 us (4.7 TB/s; a large copy reaches 4.9); a single token of 8 sequences 3.9 us.
+// Measured (medians of 60 launches): q and k of 32768 tokens x 16 heads x 128 channels each, bfloat16, 117 us (4.6 TB/s; a large copy reaches 4.9); a single
+// token of 8 sequences 4.0 us.
 #include "token_vec.h"
 
 static constexpr int ROT_THREADS = 256, ROT_MAX_AXES = 4, ROT_MAX_TABLE = 2048;
@@ -183,8 +184,8 @@ extern "C" int n3d_rotary(const n3d_rotary_desc* d, n3d_stream_t stream_) {
     }
     const int units = r.P / w + cdiv(rest, d->interleaved ? 2 * w : w);
     r.by_unit = rot_div(units); r.by_heads = rot_div(heads); r.by_len = rot_div(d->L);
-    // tokens a workgroup: four rounds of its threads over the channels and a full round over the angles, as long as 1024 workgroups remain (16 rounds: the
-    // 113 us above become 121; one round, or 256 to 4096 workgroups, are as fast where many tokens come, but then a workgroup's angles fill no round)
+    // tokens a workgroup: four rounds of its threads over the channels and a full round over the angles, as long as 1024 workgroups remain (16 rounds: 121 us
+    // instead of 113 for the call above, in one run; one round, or 256 to 4096 workgroups, are as fast where many tokens come, but then a workgroup's angles fill no round)
     int64_t tpb = cdiv64(4 * ROT_THREADS, (int64_t)heads * units);
     if (tpb < cdiv(ROT_THREADS, r.P)) tpb = cdiv(ROT_THREADS, r.P);
     if (tpb > tokens / 1024) tpb = tokens / 1024;

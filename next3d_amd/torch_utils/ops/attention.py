@@ -28,7 +28,8 @@ def attention(q, k, v, scale=None, causal=False, prefix=None, documents=None, ke
     it, not even NaN or infinity.
 
     Softmax statistics and sums are float32; weights (and in the backward pass dscores) are rounded to the inputs' type for the matrix cores.  float16
-    dscores take a power of two of each query's own (of each key's own for dk), so gradients of any size keep their digits.  Differentiable (once) in q, k and v, not through the logarithms; results and gradients are bitwise reproducible."""
+    dscores take a power of two of each query's own (of each key's own for dk), so gradients of any size keep their digits.  Differentiable (once) in q, k and v, not through the logarithms; results and gradients are bitwise reproducible, results also
+    with and without gradients being recorded.  Refused: 2^24 blocks of rows (128 queries of a head, or 32 queries and heads where there are few) or more."""
     types = (torch.float16, torch.bfloat16)
     require_tensor('attention', 'q', q, types, 4)
     for name, t in (('k', k), ('v', v)):
