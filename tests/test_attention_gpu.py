@@ -699,3 +699,51 @@ def test_attention_prefix_below_zero(dev):
     prefix = torch.tensor([-2 ** 31, -2 ** 31 + 1, -1, 2 ** 31 - 1], dtype=torch.int32)
     _check(dev, q, k, v, do, causal=True, prefix=prefix)
     _check(dev, q[:, :1], k, v, causal=True, prefix=prefix, lengths=torch.tensor([90, 3, 60, 90], dtype=torch.int32))
+
+
+def test_attention_repeated_sums_in_graphs_and_side_by_side(dev):
+    """Calls that take their sums again — NaN in padding, an infinity in the gradient, a NaN key — captured, replayed, and in flight on several streams at once."""
+    from next3d_amd.torch_utils.ops import attention
+    work = []
+    for size, dtype, kw in (((2, 300, 300, 4, 2, 128), F16, dict(causal=True)), ((1, 500, 500, 2, 2, 64), BF16, dict(documents=_docs(1, 500, 3, 5, pad=90))),
+                            ((1, 1700, 1700, 1, 1, 64), F16, dict(causal=True)), ((3, 2, 900, 8, 2, 128), F16, dict(lengths=torch.tensor([900, 0, 444], dtype=torch.int32)))):
+        q, k, v, do = _inputs(*size, dtype, 141)
+        do[0, size[1] // 2, 0, 3] = float('inf')
+        v[0, 40, 0] = float('nan')
+        if 'documents' in kw:
+            for t in (q, k, v, do):
+                t[kw['documents'] < 0] = float('nan')
+        work.append(([t.to(dev) for t in (q, k, v, do)], _to(dev, kw)))
+
+    def step(ts, kw):
+        leaves = [t.detach().requires_grad_() for t in ts[:3]]
+        out = attention.attention(*leaves, **kw)
+        return [out.detach(), *torch.autograd.grad(out, leaves, ts[3])]
+
+    same = lambda x, y: all(torch.equal(a.nan_to_num(7.0, 8.0, 9.0), c.nan_to_num(7.0, 8.0, 9.0)) and torch.equal(a.isnan(), c.isnan()) for a, c in zip(x, y))
+    alone = [step(*w) for w in work]
+    assert all(bool(x[0].isnan().any()) and bool(torch.isfinite(x[0]).any()) for x in alone)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in work]
+    for _ in range(3):
+        together = []
+        for s, w in zip(streams, work):
+            with torch.cuda.stream(s):
+                together.append(step(*w))
+        torch.cuda.synchronize()
+        assert all(same(x, y) for x, y in zip(alone, together))
+    graphs = []
+    for w in work:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step(*w)
+        graphs.append((g, out))
+    for _ in range(3):
+        for s, (g, _) in zip(streams, graphs):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                g.replay()
+        again = [step(*w) for w in work]
+        torch.cuda.synchronize()
+        assert all(same(x, y) for x, y in zip(alone, again))
+        assert all(same(x, out) for x, (_, out) in zip(alone, graphs))
