@@ -433,7 +433,7 @@ __device__ __forceinline__ void attn_dq(const AttnParams& p, int group, char* sm
                 for (int c = 0; c < 2; ++c)
 #pragma unroll
                     for (int db = 0; db < DB; ++db) acc[db] = attn_mfma(cf[db][c], d[c], acc[db]);
-                if (mask.value && (DB < 4 || !DOCS) && fine)            // (attn_left_over, where registers are left for it)
+                if (mask.value && fine)                                 // (attn_left_over)
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         const typename AttnVec<T>::x8 left = attn_left_over<T>(dP, d[c], c);
@@ -468,7 +468,6 @@ __device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* s
     constexpr float SHIFT = ATTN_P_SHIFT<T>;
     constexpr bool PAIR = attn_dkv_pair<DB>(), FIT = SHIFT != 0.f;
     constexpr int NB = PAIR ? DB / 2 : DB;                              // blocks of 32 channels a wave adds up
-    constexpr bool LEFT = !PAIR && (DB < 3 || !DOCS);                   // attn_left_over, where registers are left for it
     typedef typename AttnVec<T>::x8 frag;
     // smem: [buffer][q, do];  traded (pairs): [key group][half of the queries][w, w, d, d][lane] fragments;  exps: [key group][half][lane], their ds_exp
     const int wave = attn_uniform(threadIdx.x >> 6), keys = PAIR ? wave & 3 : wave, part = PAIR ? wave >> 2 : 0, lane = threadIdx.x & 63, l31 = lane & 31, half = lane >> 5;
@@ -576,7 +575,7 @@ __device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* s
                 }
         };
         // weights and dscores of the 32 queries of half a tile as second operands
-        auto weights = [&](int qb, frag (&w)[2], frag (&d)[2], frag (&left)[2], auto&& ahead) {
+        auto weights = [&](int qb, frag (&w)[2], frag (&d)[2], frag (&w_left)[2], frag (&d_left)[2], auto&& ahead) {
             const uint32_t q_lds = at_lane.rows(tile + qb * BLOCK), d_lds = at_lane.rows(tile + TILE_BYTES + qb * BLOCK);
             frag qf[2 * DB], df[2 * DB];
             constexpr int FIRST = DB > 2 ? DB : 0;                      // (as in attn_dq_kernel)
@@ -630,9 +629,12 @@ __device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* s
             if constexpr (FIT) attn_fit(dP, ds_exp, dk);
             attn_pack<T>(S, w);
             attn_pack<T>(dP, d);
-            if (mask.value && LEFT && fine)
+            if (mask.value && fine)                                     // (attn_left_over)
 #pragma unroll
-                for (int c = 0; c < 2; ++c) left[c] = attn_left_over<T>(dP, d[c], c);
+                for (int c = 0; c < 2; ++c) {
+                    w_left[c] = attn_left_over<T>(S, w[c], c);
+                    d_left[c] = attn_left_over<T>(dP, d[c], c);
+                }
         };
         auto products = [&](const frag (&w)[2], const frag (&d)[2], const frag (&qc)[NB][2], const frag (&dc)[NB][2]) {
 #pragma unroll
@@ -644,13 +646,13 @@ __device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* s
                 }
         };
         if constexpr (PAIR) {
-            frag w[2], d[2], none[2], qc[NB][2], dc[NB][2];
+            frag w[2], d[2], w_left[2], d_left[2], qc[NB][2], dc[NB][2];
             frag* mine = reinterpret_cast<frag*>(traded) + (keys * 2 + part) * 4 * 64 + lane;
             const frag* theirs = reinterpret_cast<const frag*>(traded) + (keys * 2 + (part ^ 1)) * 4 * 64 + lane;
             if (on) {
                 // (the products' fragments are on their way during the vector work, and the other half's during the wait: 932 -> 911 us for a training step of
                 // 2 x 4096 x 16 heads on 4 x 128, causal with caps.  The unpaired form lets two workgroups overlap instead: 458 us at x 64, with this 473)
-                weights(part, w, d, none, [&] { columns(part, qc, dc); });
+                weights(part, w, d, w_left, d_left, [&] { columns(part, qc, dc); });
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     mine[c * 64] = w[c];
@@ -658,6 +660,7 @@ __device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* s
                 }
                 if constexpr (FIT) exps[keys * 2 + part][lane] = ds_exp;
                 products(w, d, qc, dc);
+                if (mask.value && fine) products(w_left, d_left, qc, dc);
                 columns(part ^ 1, qc, dc);
             }
             attn_traded();
@@ -679,23 +682,41 @@ __device__ __forceinline__ void attn_dkv(const AttnParams& p, int group, char* s
 #pragma unroll
                         for (int c = 0; c < 2; ++c)
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) d[c][e] = (T)((float)d[c][e] * their);
+                            for (int e = 0; e < 8; ++e) {
+                                d[c][e] = (T)((float)d[c][e] * their);
+                                if (mask.value && fine) d_left[c][e] = (T)((float)d_left[c][e] * by);
+                            }
                     }
                 }
                 products(w, d, qc, dc);
             }
+            if (mask.value && fine) {                                   // (the same for all waves of the workgroup)
+                attn_traded();
+                if (on) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        mine[c * 64] = w_left[c];
+                        mine[(2 + c) * 64] = d_left[c];
+                    }
+                }
+                attn_traded();
+                if (on) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        w[c] = theirs[c * 64];
+                        d[c] = theirs[(2 + c) * 64];
+                    }
+                    products(w, d, qc, dc);
+                }
+            }
         } else if (on) {
 #pragma unroll
             for (int qb = 0; qb < 2; ++qb) {
-                frag w[2], d[2], left[2], qc[NB][2], dc[NB][2];
-                weights(qb, w, d, left, [] {});
+                frag w[2], d[2], w_left[2], d_left[2], qc[NB][2], dc[NB][2];
+                weights(qb, w, d, w_left, d_left, [] {});
                 columns(qb, qc, dc);
                 products(w, d, qc, dc);
-                if (mask.value && LEFT && fine)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c)
-#pragma unroll
-                        for (int db = 0; db < NB; ++db) dk[db] = attn_mfma(qc[db][c], left[c], dk[db]);
+                if (mask.value && fine) products(w_left, d_left, qc, dc);
             }
         }
         commit(buf);

@@ -747,3 +747,20 @@ def test_attention_repeated_sums_in_graphs_and_side_by_side(dev):
         torch.cuda.synchronize()
         assert all(same(x, y) for x, y in zip(alone, again))
         assert all(same(x, out) for x, (_, out) in zip(alone, graphs))
+
+
+@pytest.mark.parametrize('dtype', [F16, BF16])
+@pytest.mark.parametrize('d', [32, 64, 72, 96, 128])
+def test_attention_short_walks_are_rounded_once(dev, d, dtype):
+    """Up to four tiles: weights and dscores keep what their rounding left over, forward and backward, with documents and without, so the errors' norms are those
+    of rounding the exact results once; what is left (float32 sums, roundings of left-overs) is below a tenth of that."""
+    slopes = torch.tensor([0.1, 0.02])
+    for n, kw in ((60, dict(causal=True)), (190, dict(documents=_docs(1, 190, 3, 151, pad=11))), (255, dict(causal=True, slopes=slopes)),
+                  (240, dict(documents=_docs(1, 240, 2, 152), causal=True, softcap=8.0)), (19, dict(softcap=5.0))):
+        q, k, v, do = _inputs(1, n, n, 2, 1, d, dtype, 153)
+        got = _run(dev, q, k, v, do, **kw)
+        vals, _ = R.attention(q, k, v, do, **kw)
+        for name in ('out', 'dq', 'dk', 'dv'):
+            exact = vals[name]
+            err, once = float((got[name].cpu().double() - exact).norm()), float((exact.to(dtype).double() - exact).norm())
+            assert err <= 1.1 * once, (n, sorted(kw), name, err / once)
