@@ -187,9 +187,10 @@ __device__ __forceinline__ typename AttnVec<T>::x8 attn_lane_frag(const T* p, in
 }
 
 // Eight values of x that `rounded` holds in 16 bits: what the rounding left over.  The single-token kernel, and workgroups of the others that walk ATTN_FEW
-// tiles or fewer, take a second product with it, of the weights and of the dscores, whether or not gradients are wanted (the same call gives the same bits in both): rows of a few keys have nothing to average the roundings out (22
-// causal queries: float16 dq / dk off by 3.4e-4 of their norm without it, 2.0e-4 with it, plain float32 arithmetic 2.0e-4).  (Such workgroups take every
-// tile as one with a mask, which the code of the others is spared.)  In every masked tile of long documents it would cost 26 % of the forward pass (2 x 4096 x 16 heads x 64: 73 -> 92 us) and gain little.
+// tiles or fewer, take a second product with it, of the weights and of the dscores, whether or not gradients are wanted (the same call gives the same bits in
+// both): rows of a few keys have nothing to average the roundings out (22 causal queries: float16 dq / dk off by 3.4e-4 of their norm without it, 2.0e-4 with
+// it, plain float32 arithmetic 2.0e-4).  Such workgroups take every tile as one with a mask, which the code of the others is spared.  In every masked tile of
+// long documents it would cost 26 % of the forward pass (2 x 4096 x 16 heads x 64: 73 -> 92 us) and gain little.
 static constexpr int ATTN_FEW = 4;
 template <typename T>
 __device__ __forceinline__ typename AttnVec<T>::x8 attn_left_over(const f32x16& x, typename AttnVec<T>::x8 rounded, int c) {
