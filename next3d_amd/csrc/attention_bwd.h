@@ -3,8 +3,8 @@
 // attn_prep_kernel: delta.
 // attn_dq_kernel: a workgroup owns 128 queries of a head and walks the keys;  attn_dkv_kernel: a workgroup owns 128 keys of a key head and walks the
 // queries of all its heads.  Scores are computed in both (7 products for 5) so that every sum has one owner: no atomics, the same bits every time.
-// Measured, 4096 x 16 heads x 128 bfloat16 without a mask, medians of 60 launches: prep 10 us, dq 201 us (1.02 PFLOP/s of its three products), dk / dv 333 us
-// (0.83 of its four); x 64 float16: 7 us and 338 us for both.  The matrix pipe is busy for 58 % (dq) and 40 % (dk / dv, whose waves also trade weights and
+// Measured, 4096 x 16 heads x 128 bfloat16 without a mask, medians of 60 launches: prep 10 us, dq 188 us (1.10 PFLOP/s of its three products), dk / dv 301 us
+// (0.91 of its four); x 64 float16: 7 us and 314 us for both.  The matrix pipe is busy for 58 % (dq) and 42 % (dk / dv, whose waves also trade weights and
 // wait for each other twice a tile); the rest is the same vector work as in the forward pass, here without a running maximum.
 #pragma once
 #include "attention.h"

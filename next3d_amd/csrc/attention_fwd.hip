@@ -2,13 +2,13 @@
 // attn_fwd_kernel: a workgroup owns 128 queries of one head, a wave 32 of them; tiles of 64 keys pass through the LDS once, double-buffered by LDS-DMA, with
 //   the running maximum and sum of every query in its lane.  The accumulators are rescaled only when a maximum grows by more than 2^8 since they were last
 //   (at every growth: 4096 x 16 heads x 64 88 us instead of 84, in one run).  Measured, without a mask, 4096 x 16 heads, medians of 60 launches: x 128 bfloat16
-//   152 us = 0.90 PFLOP/s (a large matrix product of the library: 1.20), x 64 float16 98 us = 0.70 PFLOP/s.  The matrix pipe is busy for half of the time;
+//   143 us = 0.96 PFLOP/s (a large matrix product of the library: 1.20), x 64 float16 92 us = 0.75 PFLOP/s.  The matrix pipe is busy for half of the time;
 //   the exponentials, maxima and roundings between the two products share the issue slots with it, two waves a SIMD taking turns, and bound it, most of all
 //   at 64 channels.
 // attn_token_kernel: few queries over many keys.  The rows of a wave are (query, head) pairs that share a key head, so a key is read once for all of
 //   them; every wave walks its own tiles of 32 keys through its own LDS (no barriers), the keys are split over `splits` workgroups, and
 //   attn_combine_kernel joins their (maximum, sum, accumulator).  Measured: 16 single tokens of 32 heads on 8 over caches of up to 16384 keys x 128, 802 MB:
-//   151 + 6 us, 5.3 TB/s (a large copy: 4.9): bound by memory.
+//   149 + 6 us, 5.4 TB/s (a large copy: 4.9): bound by memory.
 #include "attention.h"
 
 // Lowest and highest document of every ATTN_TILE tokens.  Tokens of no document do not count (none at all: an empty range that meets no other), but a tile

@@ -4,8 +4,8 @@
 //   backward  g = dy * w,  xh = (x - mean) * rstd:   dx = rstd * (g - mean(g) - xh * mean(g * xh)),  dw = sum_rows dy * xh,  db = sum_rows dy
 // HBM-bound: a row is read once into registers (LPR lanes hold it, K vectors of 16 bytes each), both statistics are taken from the registers — the
 // variance from centred values, so a large common offset costs no digits — and the result is written once.  All sums are float32.
-// Measured (medians of 60 launches): 16384 x 4096 bfloat16 forward 59 us (4.6 TB/s; a large copy reaches 4.9), backward 91 + 7 us for the parts' sum (4.4);
-// 786432 x 32 float16 20 (5.0) and 28 + 4 us (5.4); 5003 x 1001 float32 12 and 15 + 4.4 us; 112 x 512 float32 3.3 us.  Bound by memory, below some 20 MB by
+// Measured (medians of 60 launches): 16384 x 4096 bfloat16 forward 56 us (4.8 TB/s; a large copy reaches 4.9), backward 90 + 7 us for the parts' sum (4.5);
+// 786432 x 32 float16 20 (5.0) and 28 + 4 us (5.4); 5003 x 1001 float32 12 and 15 + 4.4 us; 112 x 512 float32 3.4 us.  Bound by memory, below some 20 MB by
 // the launches.
 // dw / db: a thread keeps the same columns for every row it visits and adds them up in registers; the workgroup's sums go to `ws` as one row and a
 // second launch adds the rows in index order.  No atomics: the same call gives the same bits.

@@ -4,7 +4,7 @@
 // The gradient is the same kernel with -sin.  HBM-bound: q and k of a token are one launch, read once and written once; the cosines and sines of a
 // workgroup's tokens are computed once into the LDS and serve every head of q and k.  The angle is taken in 64 bits and reduced to a fraction of a
 // turn there — in 32 bits the angle of position 100000 is off by 0.004 — and the cosine and sine of that fraction are float32.
-// Measured (medians of 60 launches): q and k of 32768 tokens x 16 heads x 128 channels each, bfloat16, 117 us (4.6 TB/s; a large copy reaches 4.9); a single
+// Measured (medians of 60 launches): q and k of 32768 tokens x 16 heads x 128 channels each, bfloat16, 116 us (4.6 TB/s; a large copy reaches 4.9); a single
 // token of 8 sequences 4.0 us.
 #include "token_vec.h"
 
